@@ -92,6 +92,9 @@ int64_t b200kv_workspace_bytes(const b200kv_config* cfg);
 int b200kv_seq_new(b200kv_cache* cache, int32_t* seq_out);
 int b200kv_seq_free(b200kv_cache* cache, int32_t seq);
 
+/* b200kv_seq_free for a batch in one call; all sequences are checked first, on KO none has been freed. */
+int b200kv_seq_free_many(b200kv_cache* cache, int32_t n_seqs, const int32_t* seqs);
+
 /* Cached length of a sequence: what OpState::resolve_symbols binds the past-length symbol to
  * (transformers/src/ops/dyn_kv_cache.rs:153-156).  Returns -1 on error. */
 int64_t b200kv_seq_len(b200kv_cache* cache, int32_t seq);
@@ -215,6 +218,29 @@ int b200kv_truncate_many(b200kv_cache* cache, int32_t n_seqs, const int32_t* seq
  * device, gpu/src/ops/dyn_kv_cache.rs:136-168). */
 int b200kv_fork(b200kv_cache* cache, int32_t seq, int32_t* new_seq_out, void* stream);
 
+/* n new sequences that go on where their parents are (n continuations of one prompt, the beams of a search, drafts):
+ * new_seqs_out[i] starts with the tokens of seqs[i], which may appear more than once.  The full pages of a parent are
+ * shared, not copied -- every page counts the sequences that hold it and goes back to the pool with the last of them --
+ * and only a partly filled last page is copied, one page of the pool per new sequence.  Parent and children are
+ * independent from then on: append, truncate, trim, free, fork and attention on one of them leave the others as they
+ * are.  (Where two sequences were truncated into a page they still share, the next append of either copies that page
+ * first: it then needs one page more than the tokens it adds.)  A trimmed parent gives trimmed children.  On KO nothing
+ * has changed.  Not for the KIVI formats.  The reference clones a state whole (gpu/src/ops/dyn_kv_cache.rs:136-168, the
+ * counterpart of b200kv_fork). */
+int b200kv_fork_shared(b200kv_cache* cache, int32_t n, const int32_t* seqs, int32_t* new_seqs_out, void* stream);
+
+/* Decode attention of a batch whose sequences share their beginning (b200kv_fork_shared): what b200kv_attend with
+ * n_new = 1 gives, up to the order of its sums, but the pages that neighbours of the batch share are read once for all of
+ * them.  Neighbours: sequences of one prompt stand next to each other in `seqs`; a batch may hold several prompts, and
+ * sequences that share nothing.  q, out: [n_seqs, n_q_heads, 1, D].
+ * cos / sin (both or none): ApplyRope folded into the query load, as in b200kv_attend_rope.  scratch (may be null): the
+ * result as the quantised activation of a W4A8 GEMM, as in b200kv_attend_q40; `out` may then be null.
+ * Batches of more than 256 sequences are served 256 at a time, and without sharing where `scratch` is given.  Not for the
+ * KIVI formats. */
+int b200kv_attend_shared(b200kv_cache* cache, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q,
+                         const int64_t q_strides[3], const void* cos, const void* sin, int64_t rope_stride, void* out,
+                         const int64_t out_strides[3], void* scratch, int32_t dtype, float scale, void* stream);
+
 /* Device status word: 0 unless a kernel recorded a problem (page index out of range, a bounded wait
  * that expired).  Synchronises the stream.  Returns KO and sets the message if the word is non-zero. */
 int b200kv_check(b200kv_cache* cache, void* stream);
@@ -319,7 +345,7 @@ int b200kv_cast(const void* src, int64_t src_stride, int32_t src_dtype, void* ds
  * CUDA event pair on the caller's stream (what tract-cuda's TractCudaStream does for its profiler,
  * cuda/src/context.rs:364-453).  b200kv_profile_read waits for the recorded launches, returns up to
  * max_records (kernel id, milliseconds) pairs in launch order and clears the log.  Kernel ids:
- * 0 page-table update, 1 append, 2 decode, 3 split combine, 4 export, 5 generic sdpa, 6 prefill.
+ * 0 page-table update, 1 append, 2 decode, 3 split combine, 4 export, 5 generic sdpa, 6 prefill, 7 page sharing, 8 attention over shared pages.
  * `enable` is a bit set: bit 0 turns the timing on; bit 1 (a test hook) routes decode attention through the
  * CUDA-core kernel even where the tensor-core kernel applies (KIVI caches: through export + the generic kernel), so
  * the two can be checked against each other; bit 2 (a test hook) keeps KIVI decode attention on its CUDA-core

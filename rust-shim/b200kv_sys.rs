@@ -59,6 +59,7 @@ extern "C" {
     pub fn b200kv_destroy(cache: *mut b200kv_cache) -> c_int;
     pub fn b200kv_seq_new(cache: *mut b200kv_cache, seq_out: *mut i32) -> c_int;
     pub fn b200kv_seq_free(cache: *mut b200kv_cache, seq: i32) -> c_int;
+    pub fn b200kv_seq_free_many(cache: *mut b200kv_cache, n_seqs: i32, seqs: *const i32) -> c_int;
     pub fn b200kv_seq_len(cache: *mut b200kv_cache, seq: i32) -> i64;
     pub fn b200kv_free_pages(cache: *mut b200kv_cache) -> i64;
     pub fn b200kv_page_bytes(cache: *mut b200kv_cache) -> i64;
@@ -130,6 +131,14 @@ extern "C" {
     pub fn b200kv_truncate(cache: *mut b200kv_cache, seq: i32, len: i64) -> c_int;
     pub fn b200kv_truncate_many(cache: *mut b200kv_cache, n_seqs: i32, seqs: *const i32, lens: *const i64) -> c_int;
     pub fn b200kv_fork(cache: *mut b200kv_cache, seq: i32, new_seq_out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn b200kv_fork_shared(
+        cache: *mut b200kv_cache, n: i32, seqs: *const i32, new_seqs_out: *mut i32, stream: *mut c_void,
+    ) -> c_int;
+    pub fn b200kv_attend_shared(
+        cache: *mut b200kv_cache, n_seqs: i32, seqs: *const i32, n_q_heads: i32,
+        q: *const c_void, q_strides: *const i64, cos: *const c_void, sin: *const c_void, rope_stride: i64,
+        out: *mut c_void, out_strides: *const i64, scratch: *mut c_void, dtype: i32, scale: c_float, stream: *mut c_void,
+    ) -> c_int;
     pub fn b200kv_check(cache: *mut b200kv_cache, stream: *mut c_void) -> c_int;
     pub fn b200kv_profile(cache: *mut b200kv_cache, enable: i32) -> c_int;
     pub fn b200kv_profile_read(

@@ -28,8 +28,9 @@ EXPORTS = [
     "b200kv_rms_norm", "b200kv_silu_mul", "b200kv_add", "b200kv_argmax", "b200kv_gather_rows", "b200kv_cast",
     "b200kv_attend_window", "b200kv_trim", "b200kv_attend_rope", "b200kv_attend_q40", "b200kv_append_attend", "b200kv_q40_quantize", "b200kv_q40_gemm_quantized", "b200kv_q40_gemm_quantized_as",
     "b200kv_q40_silu_mul_quantize", "b200kv_q40_add_rms_norm_quantize", "b200kv_workspace_bytes", "b200kv_truncate_many", "b200kv_sdpa_check",
+    "b200kv_fork_shared", "b200kv_seq_free_many", "b200kv_attend_shared",
 ]
-KERNEL_NAMES = {0: "table_scatter", 1: "append", 2: "decode", 3: "combine", 4: "export", 5: "sdpa_dense", 6: "prefill"}
+KERNEL_NAMES = {0: "table_scatter", 1: "append", 2: "decode", 3: "combine", 4: "export", 5: "sdpa_dense", 6: "prefill", 7: "share", 8: "prefix"}
 
 
 class B200KvError(RuntimeError):
@@ -88,6 +89,9 @@ def lib():
         L.b200kv_attend_q40.argtypes = [vp, i32, i32p, i32, vp, i64p, vp, vp, i64, vp, i64p, vp, i32, C.c_float, vp]
         L.b200kv_attend_window.argtypes = [vp, i32, i32p, i32, vp, i64p, vp, i64p, i32, C.c_float, i64, vp]
         L.b200kv_trim.argtypes = [vp, i32, i64]
+        L.b200kv_fork_shared.argtypes = [vp, i32, i32p, i32p, vp]
+        L.b200kv_seq_free_many.argtypes = [vp, i32, i32p]
+        L.b200kv_attend_shared.argtypes = [vp, i32, i32p, i32, vp, i64p, vp, vp, i64, vp, i64p, vp, i32, C.c_float, vp]
         _lib = L
     return _lib
 
@@ -157,6 +161,10 @@ class KvCache:
 
     def free_seq(self, seq):
         _ck(lib().b200kv_seq_free(self._h, seq))
+
+    def free_seqs(self, seqs):
+        """free_seq() for a batch in one call: every sequence is checked before any is freed."""
+        _ck(lib().b200kv_seq_free_many(self._h, len(seqs), _ids(seqs)))
 
     def seq_len(self, seq) -> int:
         n = lib().b200kv_seq_len(self._h, seq)
@@ -350,6 +358,57 @@ class KvCache:
         s = C.c_int32()
         _ck(lib().b200kv_fork(self._h, seq, C.byref(s), _stream()))
         return s.value
+
+    def fork_shared(self, seqs) -> list:
+        """One new sequence for each entry of `seqs` (which may repeat): it starts with that sequence's tokens, shares its full
+        pages and gets a copy of the partly filled last one."""
+        n = len(seqs)
+        out = (C.c_int32 * max(n, 1))()
+        _ck(lib().b200kv_fork_shared(self._h, n, _ids(seqs), out, _stream()))
+        return list(out[:n])
+
+    def attend_shared(self, seqs, q, cos=None, sin=None, scratch=None, scale=None, out=None):
+        """Decode attention (q: [n_seqs, Hq, 1, D]) in which the pages that neighbours of the batch share (fork_shared) are
+        read once for all of them.  cos / sin: ApplyRope of the query, as in attend_rope.  scratch: the result also as the
+        quantised activation of a Q40Linear, as in attend_q40 (`out` stays unwritten then unless it is given)."""
+        import torch
+
+        assert q.dim() == 4 and q.shape[0] == len(seqs) and q.shape[2] == 1 and q.shape[3] == self.head_dim
+        stride = 0
+        if cos is not None:
+            cos, sin = cos.reshape(len(seqs), -1), sin.reshape(len(seqs), -1)
+            assert cos.dtype == q.dtype and sin.dtype == q.dtype and cos.stride(1) == 1 and sin.stride(1) == 1
+            assert cos.stride(0) == sin.stride(0) and cos.shape[1] == q.shape[3]
+            stride = cos.stride(0)
+        if scratch is not None:
+            assert scratch.numel() >= Q40Linear.scratch_bytes(q.shape[1] * q.shape[3], len(seqs))
+        elif out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        assert out is None or (out.shape == q.shape and out.dtype == q.dtype)
+        _ck(lib().b200kv_attend_shared(self._h, len(seqs), _ids(seqs), q.shape[1], q.data_ptr(), _strides(q, 3),
+                                       cos.data_ptr() if cos is not None else None, sin.data_ptr() if sin is not None else None, stride,
+                                       out.data_ptr() if out is not None else None, _strides(out, 3) if out is not None else None,
+                                       scratch.data_ptr() if scratch is not None else None, _dtype_code(q), float(scale or 0.0), _stream()))
+        return out
+
+    def prepared_attend_shared(self, seqs, q, out, scale=None):
+        """A zero-argument callable that runs attend_shared(seqs, q, out=out) with every argument marshalled once, here (see
+        prepared_step).  The tensors must stay alive and in place; the current CUDA stream is looked up at every call."""
+        import torch
+
+        assert q.dim() == 4 and q.shape[0] == len(seqs) and q.shape[2] == 1 and q.shape[3] == self.head_dim
+        assert out.shape == q.shape and out.dtype == q.dtype
+        L, h, n, ids = lib(), self._h, len(seqs), _ids(seqs)
+        qs, os_, qp, op = _strides(q, 3), _strides(out, 3), C.c_void_p(q.data_ptr()), C.c_void_p(out.data_ptr())
+        hq, dt, sc = int(q.shape[1]), _dtype_code(q), C.c_float(scale or 0.0)
+        keep = (q, out, self)
+
+        def call(_keep=keep):
+            st = torch.cuda.current_stream().cuda_stream
+            if L.b200kv_attend_shared(h, n, ids, hq, qp, qs, None, None, 0, op, os_, None, dt, sc, st) != 0:
+                raise B200KvError(L.b200kv_last_error().decode())
+
+        return call
 
     def check(self):
         _ck(lib().b200kv_check(self._h, _stream()))

@@ -425,8 +425,7 @@ static int alloc_pages(b200kv_cache* c, SeqState& s, int64_t new_len, std::vecto
     if (need - have > (int64_t)c->free_pages.size())
         return fail("page pool exhausted: need %lld more pages, %zu free", (long long)(need - have), c->free_pages.size());
     for (int64_t i = have; i < need; i++) {
-        int32_t pg = c->free_pages.back();
-        c->free_pages.pop_back();
+        const int32_t pg = page_take(c);
         s.pages.push_back(pg);
         upd.push_back((int32_t)((int64_t)row * c->max_pages_per_seq + i));
         upd.push_back(pg);
@@ -531,6 +530,7 @@ int b200kv_create(const b200kv_config* cfg, b200kv_cache** out) {
         return cleanup(fail("cannot allocate the page tables"));
     if (cudaMalloc(&c->d_status, sizeof(int)) != cudaSuccess || cudaMemset(c->d_status, 0, sizeof(int)) != cudaSuccess)
         return cleanup(fail("cannot allocate the status word"));
+    c->page_refs.assign(c->n_pages, 0);
     c->free_pages.resize(c->n_pages);
     for (int64_t i = 0; i < c->n_pages; i++) c->free_pages[i] = (int32_t)(c->n_pages - 1 - i);
     // descriptor slots: the largest descriptor is a decode work list (64 splits per sequence at most)
@@ -593,11 +593,17 @@ int b200kv_seq_free(b200kv_cache* c, int32_t seq) {
     if (!c || seq < 0 || seq >= (int)c->seqs.size() || !c->seqs[seq].live) return fail("sequence %d is not live", seq);
     SeqState& s = c->seqs[seq];
     for (int32_t pg : s.pages)
-        if (pg >= 0) c->free_pages.push_back(pg);  // trimmed entries are -1
+        if (pg >= 0) page_drop(c, pg);  // trimmed entries are -1
     s.pages.clear();
     s.len = 0;
     s.start = 0;
     s.live = false;
+    return B200KV_OK;
+}
+
+int b200kv_seq_free_many(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs) {
+    if (validate_seqs(c, n_seqs, seqs) != B200KV_OK) return B200KV_KO;
+    for (int i = 0; i < n_seqs; i++) b200kv_seq_free(c, seqs[i]);
     return B200KV_OK;
 }
 
@@ -638,18 +644,38 @@ static int append_impl(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int
     // host bookkeeping first, committed only if everything can be enqueued
     std::vector<int32_t> upd;
     std::vector<size_t> old_pages(n_seqs);
+    // A partly filled last page that another sequence holds too (both were truncated into a page they share) is copied
+    // before it is written: its entry here, in the order of the sequences.
+    std::vector<PageCopy> moved;
     auto rollback = [&](int upto) {
         for (int i = 0; i < upto; i++) {
             SeqState& s = c->seqs[seqs[i]];
             while (s.pages.size() > old_pages[i]) {
-                c->free_pages.push_back(s.pages.back());
+                page_drop(c, s.pages.back());
                 s.pages.pop_back();
             }
+            for (const PageCopy& m : moved)
+                if (!s.pages.empty() && s.pages.back() == m.dst) {
+                    page_share(c, m.src);
+                    page_drop(c, m.dst);
+                    s.pages.back() = m.src;
+                }
         }
+        moved.clear();
     };
     for (int i = 0; i < n_seqs; i++) {
         SeqState& s = c->seqs[seqs[i]];
         old_pages[i] = s.pages.size();
+        if (s.len % PAGE_TOKENS && !fmt_is_kivi(c->L.fmt) && c->page_refs[s.pages.back()] > 1) {
+            if (c->free_pages.empty()) {
+                rollback(i + 1);
+                return fail("page pool exhausted: sequence %d needs a page of its own to go on in a page it shares", seqs[i]);
+            }
+            const int32_t old = s.pages.back(), pg = page_take(c);
+            moved.push_back({old, pg, (int32_t)((int64_t)seqs[i] * c->max_pages_per_seq + (int64_t)s.pages.size() - 1), (int32_t)(s.len % PAGE_TOKENS)});
+            page_drop(c, old);
+            s.pages.back() = pg;
+        }
         if (alloc_pages(c, s, s.len + n_new, upd, seqs[i]) != B200KV_OK) {
             rollback(i + 1);
             return B200KV_KO;
@@ -692,6 +718,14 @@ static int append_impl(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int
             rollback(n_seqs);
             return B200KV_KO;
         }
+    }
+    if (!moved.empty()) {  // nothing can be refused from here on: the copies only read what stays as it is
+        if (launch_page_copies(c, moved.data(), (int)moved.size(), stream) != B200KV_OK) {
+            if (slot >= 0) staging_release(c, slot, stream);
+            rollback(n_seqs);
+            return B200KV_KO;
+        }
+        moved.clear();  // the sequences keep their own copies whatever happens next: the same tokens
     }
     if (!upd.empty() && fmt_is_kivi(c->L.fmt)) {  // the KIVI kernels read the table; the others take new pages from the descriptor
         int n = (int)(upd.size() / 2);
@@ -800,7 +834,7 @@ int b200kv_truncate(b200kv_cache* c, int32_t seq, int64_t len) {
         return fail("a KIVI cache cannot be truncated (blocks are frozen once quantised; the reference has no truncate either)");
     size_t keep = (size_t)((len + PAGE_TOKENS - 1) / PAGE_TOKENS);
     while (s.pages.size() > keep) {
-        c->free_pages.push_back(s.pages.back());
+        page_drop(c, s.pages.back());
         s.pages.pop_back();
     }
     s.len = len;
@@ -833,7 +867,7 @@ int b200kv_trim(b200kv_cache* c, int32_t seq, int64_t keep_last) {
     const int64_t start = std::max<int64_t>(s.start, s.len - keep_last);
     for (int64_t pgi = s.start / PAGE_TOKENS; pgi < start / PAGE_TOKENS; pgi++)
         if (s.pages[(size_t)pgi] >= 0) {
-            c->free_pages.push_back(s.pages[(size_t)pgi]);
+            page_drop(c, s.pages[(size_t)pgi]);
             s.pages[(size_t)pgi] = -1;
         }
     s.start = start;

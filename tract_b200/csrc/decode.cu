@@ -435,15 +435,10 @@ int launch_combine(const DecodeParams& p, const int32_t* batch_info, void* out, 
 //     runs stay long.
 // (2) Many sequences: 16 CTAs per SM over the run, so that the tail is short; small launches fill one round with up
 //     to 8 pages per split instead of one page per CTA.
-int64_t decode_pages_per_split(const b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int64_t window, bool use_mma, int nz) {
+int64_t pages_per_split(const b200kv_cache* c, const int64_t* pages, int n_seqs, bool use_mma, int nz) {
     const int Hkv = c->L.Hkv;
-    auto pages_of = [&](int i) {
-        const SeqState& s = c->seqs[seqs[i]];
-        const int64_t first = std::max<int64_t>(s.start, window > 0 ? s.len - window : 0);
-        return (s.len + PAGE_TOKENS - 1) / PAGE_TOKENS - first / PAGE_TOKENS;
-    };
     int64_t total_pages = 0, max_pages = 1;
-    for (int i = 0; i < n_seqs; i++) total_pages += pages_of(i), max_pages = std::max<int64_t>(max_pages, pages_of(i));
+    for (int i = 0; i < n_seqs; i++) total_pages += pages[i], max_pages = std::max<int64_t>(max_pages, pages[i]);
     const int64_t work = total_pages * Hkv * nz, target_ctas = 148 * 16, one_wave = 148 * 3;
     int64_t chunk = std::max<int64_t>((work + target_ctas - 1) / target_ctas, std::min<int64_t>((work + one_wave - 1) / one_wave, 8));
     int resident;
@@ -463,12 +458,21 @@ int64_t decode_pages_per_split(const b200kv_cache* c, int32_t n_seqs, const int3
         int64_t cand = std::max<int64_t>(1, work / slots);
         for (; cand < max_pages; cand += std::max<int64_t>(1, cand / 32)) {  // the count falls as cand grows; at max_pages it is one CTA per pair
             int64_t n = 0;
-            for (int i = 0; i < n_seqs; i++) n += std::min<int64_t>(MAX_SPLITS, (pages_of(i) + cand - 1) / cand);
+            for (int i = 0; i < n_seqs; i++) n += std::min<int64_t>(MAX_SPLITS, (pages[i] + cand - 1) / cand);
             if (n * Hkv * nz <= slots) break;
         }
         chunk = std::min(cand, max_pages);
     }
     return std::max<int64_t>(chunk, 1);
+}
+int64_t decode_pages_per_split(const b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int64_t window, bool use_mma, int nz) {
+    std::vector<int64_t> pages((size_t)n_seqs);
+    for (int i = 0; i < n_seqs; i++) {
+        const SeqState& s = c->seqs[seqs[i]];
+        const int64_t first = std::max<int64_t>(s.start, window > 0 ? s.len - window : 0);
+        pages[i] = (s.len + PAGE_TOKENS - 1) / PAGE_TOKENS - first / PAGE_TOKENS;
+    }
+    return pages_per_split(c, pages.data(), n_seqs, use_mma, nz);
 }
 
 int launch_decode(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q,

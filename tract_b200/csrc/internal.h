@@ -74,6 +74,7 @@ struct b200kv_cache {
     int32_t* d_table = nullptr;  // [max_seqs][max_pages_per_seq] page ids
     int* d_status = nullptr;
     std::vector<int32_t> free_pages;
+    std::vector<int32_t> page_refs;  // sequences that hold each page (b200kv_fork_shared): it goes back to the pool with the last of them
     std::vector<b200kv::SeqState> seqs;
     b200kv::Staging st;
     uint8_t* ws = nullptr;  // split-KV partials: allocated once at create, never grown
@@ -105,8 +106,28 @@ int64_t workspace_records(const b200kv_config& cfg);
 
 int validate_seqs(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs);
 
+// Pages of the pool: taken with one holder, shared by adding holders, back in the free list when the last holder lets go.
+inline int32_t page_take(b200kv_cache* c) {
+    const int32_t pg = c->free_pages.back();
+    c->free_pages.pop_back();
+    c->page_refs[pg] = 1;
+    return pg;
+}
+inline void page_share(b200kv_cache* c, int32_t pg) { c->page_refs[pg]++; }
+inline void page_drop(b200kv_cache* c, int32_t pg) {
+    if (--c->page_refs[pg] == 0) c->free_pages.push_back(pg);
+}
+
+// share.cu: a partly filled page of a sequence moves to a page of its own before it is written
+struct PageCopy {
+    int32_t src, dst;    // page ids
+    int32_t table_at;    // page-table index that takes dst
+    int32_t n_tokens;    // filled slots of the page
+};
+int launch_page_copies(b200kv_cache* c, const PageCopy* copies, int n, cudaStream_t stream);
+
 // Kernel ids reported by b200kv_profile_read.
-enum { K_SCATTER = 0, K_APPEND = 1, K_DECODE = 2, K_COMBINE = 3, K_EXPORT = 4, K_DENSE = 5, K_PREFILL = 6 };
+enum { K_SCATTER = 0, K_APPEND = 1, K_DECODE = 2, K_COMBINE = 3, K_EXPORT = 4, K_DENSE = 5, K_PREFILL = 6, K_SHARE = 7, K_PREFIX = 8 };
 
 // Brackets the launches made during its lifetime with an event pair when profiling is on.
 struct ProfScope {
@@ -135,6 +156,8 @@ struct QueryRope {  // what a decode call may fold in at its two ends
     int64_t stride_b;  // elements
     void* act_scratch; // the result also (or only) as the quantised activation of a W4A8 GEMM, or null
 };
+// pages of each sequence that a call walks -> pages per run
+int64_t pages_per_split(const b200kv_cache* c, const int64_t* pages, int n_seqs, bool use_mma, int nz);
 int64_t decode_pages_per_split(const b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int64_t window, bool use_mma, int nz);
 int launch_decode(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q,
                   const int64_t* q_strides, void* out, const int64_t* out_strides, int32_t dtype, float scale,

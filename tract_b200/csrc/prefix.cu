@@ -1,0 +1,830 @@
+// b200kv_attend_shared: decode attention of a batch whose sequences begin with the same pages (b200kv_fork_shared).
+//
+// b200kv_attend streams the pages of every sequence for that sequence alone, so the beginning that n sequences share is read
+// n times.  Here the rows of all of them -- sequence x query head of the kv head's group -- meet each shared page once:
+//   m, l, O  of a row over the shared pages     prefix_tc_kernel (tcgen05) or prefix_simt_kernel, split along the pages
+//   m, l, O  of a row over its own pages        the decode kernels, starting behind the shared pages
+//   out = sum_k e^(m_k - m) O_k / sum_k e^(m_k - m) l_k,   m = max m_k      combine_shared_kernel
+// Semantics of each row: transformers/src/ops/flash_sdpa.rs:239-341 with one query.  The reference has no counterpart of the
+// sharing itself: its states are cloned whole (gpu/src/ops/dyn_kv_cache.rs:136-168).
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <vector>
+
+#include "attn_convert.cuh"
+#include "decode_common.h"
+#include "q40_common.cuh"
+
+namespace b200kv {
+
+// One run of batch entries that share their first n_pages pages.
+struct PrefixGroup {
+    int32_t trow;       // page-table row of one of them
+    int32_t n_pages;    // shared pages, all of them full
+    int32_t b0, n_seqs; // batch entries b0 .. b0 + n_seqs - 1
+    int32_t tiles;      // row tiles (of one CTA) that cover n_seqs * G rows
+    int32_t splits;     // runs of pages
+    int32_t cta0;       // first CTA (x) of the group: cta0 + split * tiles + tile
+    int32_t base;       // first partial record: base + (split * Hkv + kvh) * n_seqs * G + row
+};
+constexpr int PREFIX_GROUPS = INLINE_BATCH / 2;
+struct PrefixBatch {
+    int32_t n;
+    int32_t pad[3];
+    PrefixGroup g[PREFIX_GROUPS];
+};
+struct PrefixParams {
+    DecodeParams d;  // q, rotary embedding, pool, table, workspace: as the decode kernels get them
+    int32_t chunk_bytes;
+    float skip_fraction;
+};
+
+__device__ inline PrefixGroup prefix_group_of(const PrefixBatch& pb, int cta) {
+    int lo = 0, hi = pb.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pb.g[mid].cta0 <= cta) lo = mid;
+        else hi = mid - 1;
+    }
+    return pb.g[lo];
+}
+// pages [first, first + count) of split k
+__device__ inline void prefix_run(const PrefixGroup& g, int k, int* first, int* count) {
+    const int base = g.n_pages / g.splits, rem = g.n_pages % g.splits;
+    *first = k * base + min(k, rem);
+    *count = base + (k < rem ? 1 : 0);
+}
+
+constexpr int XM = 128;            // rows of a tile
+constexpr int X_SM_THREADS = 128;  // softmax threads per tile: one per row
+constexpr int X_XCHG = 8;          // per tile and page parity: one flag per softmax warp (does the page need its remainder product)
+// f16 weights skip the remainder product of a page once sqrt(64) x the largest weight of the page is below this fraction of
+// the running sum, for every row of the tile (see prefill_tc.cu)
+constexpr float X_SKIP_FRACTION = 0.125f;
+enum { PSRC_PAGES16 = 0, PSRC_Q8 = 1, PSRC_Q4 = 2 };
+
+template <int NQ, int D, int SRC>
+struct XGeo {
+    static constexpr bool RAW = SRC != PSRC_PAGES16;   // block-quantised pages: converter warps rebuild the operand tiles
+    static constexpr int FT = RAW ? 128 : 32;          // converter threads, or the copy warp
+    static constexpr int PLANES = D / 64;
+    static constexpr int CHUNK = PAGE_TOKENS * D * 2;  // one operand tile: 64 keys
+    static constexpr int QBYTES = XM * D * 2;
+    static constexpr int KPARTS = RAW ? 2 : 1;         // K as value + remainder where it was rounded
+    static constexpr int KSTAGE = KPARTS * CHUNK;
+    static constexpr int RESIDENT = (NQ == 1 && !RAW) ? 2 : 1;  // CTAs per SM
+    static constexpr int NK = RAW ? 2 : (NQ == 2 ? 4 : (D == 64 ? 4 : 2));
+    static constexpr int NV = RAW ? 3 : (NQ == 2 ? 5 : (D == 64 ? 4 : 2));
+    static constexpr int NR = RAW ? 2 : 1;
+    static constexpr int RAW_STAGE = RAW ? 2 * (PAGE_TOKENS * D + PAGE_TOKENS * (D / 32) * 2) : 0;
+    static constexpr int THREADS = NQ * X_SM_THREADS + 32 * NQ + FT;
+    static constexpr int N_BARS = 2 * NK + 2 * NV + 6 * NQ + 2 * NR;
+    static constexpr uint32_t COL_S = D, COLS_PER_TILE = 256;  // TMEM: O in columns 0 .. D-1, the two S buffers behind it
+    static constexpr size_t SMEM = (size_t)NQ * QBYTES + (size_t)NK * KSTAGE + (size_t)NV * CHUNK + (size_t)NR * RAW_STAGE + N_BARS * 8 + 32 +
+                                   NQ * 2 * X_XCHG * 4;
+    static_assert(COL_S + 128 <= COLS_PER_TILE && NQ * COLS_PER_TILE * RESIDENT <= 512, "TMEM columns of an SM");
+    static_assert(RESIDENT * (SMEM + 1024) <= 228 * 1024 && SMEM <= 227 * 1024, "shared memory of an SM");
+};
+
+// The shared pages against every row that sees them, on the 5th-generation tensor cores.
+//   S = Q K^T   M = 128 rows (sequence, head of the group), N = 64 keys of a page, operands in shared memory
+//   P = 2^(scale log2e S - m)   one thread per row, m raised only when exceeded by 2^8, l = sum P
+//   O += P V    A = P from TMEM, B = V as it lies in the page
+// The pipeline -- S double-buffered in TMEM, P over the S it came from, rings of K and V tiles, bounded waits -- is the one
+// of prefill_tc.cu and attn_tc.cu; there are no masks (every row sees every shared page whole), the rows come from different
+// sequences, and the result is the run's partial (m, l, O) in f32 for the combine pass.
+// Bound: a page and kv head is 32 KB of f16 (1340 cycles of an SM's share of HBM at the copy rate); its products for 128 rows
+// take 640 to 900 cycles of the tensor pipe.  Up to 128 rows one tile per CTA and two CTAs per SM (16-bit pages), so that one
+// CTA's softmax runs under the other's products; more rows go two tiles to a CTA, which read each staged page twice.
+template <int NQ, int D, int SRC>
+__global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::RESIDENT)
+    prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
+    using GEO = XGeo<NQ, D, SRC>;
+    constexpr int NK = GEO::NK, NV = GEO::NV, NR = GEO::NR, CHUNK = GEO::CHUNK, QBYTES = GEO::QBYTES, PLANES = GEO::PLANES;
+    constexpr int KSTAGE = GEO::KSTAGE, KPARTS = GEO::KPARTS, FT = GEO::FT;
+    constexpr bool RAW = GEO::RAW;  // converted pages: f16 operands whatever the query type
+    constexpr uint32_t COL_O = 0, COL_S = GEO::COL_S, COLS_PER_TILE = GEO::COLS_PER_TILE;
+    constexpr int FILL_ARRIVALS = RAW ? FT / 32 : 1;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* q_s = smem;                                    // [NQ][PLANES][128 rows][128 B], swizzled
+    uint8_t* k_ring = smem + NQ * QBYTES;                   // NK K stages of KPARTS tiles
+    uint8_t* v_ring = k_ring + NK * KSTAGE;                 // NV V tiles
+    uint8_t* raw_ring = v_ring + NV * CHUNK;                // NR raw chunk pairs
+    uint64_t* full_k = (uint64_t*)(raw_ring + NR * GEO::RAW_STAGE);  // [NK] the tile is complete
+    uint64_t* full_v = full_k + NK;                         // [NV]
+    uint64_t* free_k = full_v + NV;                         // [NK] every tile's Q.K^T on the stage has completed
+    uint64_t* free_v = free_k + NK;                         // [NV] every tile's P.V on the stage has completed
+    uint64_t* bar_s = free_v + NV;                          // [NQ][2] S buffer written
+    uint64_t* bar_p = bar_s + 2 * NQ;                       // [NQ][2] P written by the softmax warps
+    uint64_t* bar_o = bar_p + 2 * NQ;                       // [NQ][2] P.V of page j completed, on barrier j & 1
+    uint64_t* full_raw = bar_o + 2 * NQ;                    // [NR] raw bytes landed
+    uint64_t* free_raw = full_raw + NR;                     // [NR] every converter warp is done with the raw stage
+    uint32_t* tmem_slot = (uint32_t*)(((uintptr_t)(free_raw + NR) + 15) & ~(uintptr_t)15);
+    volatile int* fail_s = (volatile int*)(tmem_slot + 1);
+    float* xchg = (float*)(tmem_slot + 4);                  // [NQ][2 parities][X_XCHG]
+
+    const DecodeParams& dp = p.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kvh = blockIdx.y;
+    const PrefixGroup grp = prefix_group_of(pb, blockIdx.x);
+    const int split = (blockIdx.x - grp.cta0) / grp.tiles, tile = (blockIdx.x - grp.cta0) % grp.tiles;
+    int page0, n_tiles;
+    prefix_run(grp, split, &page0, &n_tiles);
+    const int n_rows = grp.n_seqs * dp.G;
+
+    if (tid == 0) {
+        for (int s = 0; s < NK; s++) mbar_init(&full_k[s], FILL_ARRIVALS), mbar_init(&free_k[s], NQ);
+        for (int s = 0; s < NV; s++) mbar_init(&full_v[s], FILL_ARRIVALS), mbar_init(&free_v[s], NQ);
+        for (int i = 0; i < 2 * NQ; i++) mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], X_SM_THREADS / 32);
+        for (int i = 0; i < 2 * NQ; i++) mbar_init(&bar_o[i], 1);
+        for (int s = 0; s < NR; s++) mbar_init(&full_raw[s], 1), mbar_init(&free_raw[s], FT / 32);
+        *fail_s = (smem_u32(smem) & 1023u) ? 1 : 0;  // the swizzled operand tiles need a 1024-byte aligned base
+        mbar_fence_init();
+    }
+    if (warp == 0) tmem_alloc(tmem_slot, COLS_PER_TILE * NQ);
+    grid_dependency_wait();    // the append before this launch has written its pages, and whoever made q is done
+    grid_launch_dependents();  // the next kernel may be scheduled; it waits for this grid before it reads the partials
+
+    const int qt = min(tid / X_SM_THREADS, NQ - 1), w4 = (tid % X_SM_THREADS) >> 5;
+    const int row = w4 * 32 + lane;
+    const int my_row = (tile * NQ + qt) * XM + row;  // row of the group: sequence my_row / G, head my_row % G
+    const bool live = my_row < n_rows;
+    const bool is_softmax = tid < NQ * X_SM_THREADS;
+    const int is_bf16 = dp.dtype == B200KV_BF16;
+    const int mma_bf16 = RAW ? 0 : is_bf16;  // type of the tensor-core operands (Q, K, V, P)
+
+    // ---- Q tile -> shared memory, K-major with the 128-byte swizzle; this thread moves its row ----
+    if (is_softmax) {
+        const int b = grp.b0 + (live ? my_row / dp.G : 0), head = kvh * dp.G + (live ? my_row % dp.G : 0);
+        const uint4* src = (const uint4*)((const uint16_t*)dp.q + (int64_t)b * dp.qb + (int64_t)head * dp.qh);
+#pragma unroll
+        for (int uu = 0; uu < D / 8; uu++) {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            if (live) {
+                if (dp.q_cos || (RAW && is_bf16)) {
+                    // the rotated value is rounded to the query's type, as a separate rope kernel would store it; over
+                    // converted pages a bf16 query becomes f16 (every bf16 value is an f16 value, short of its range)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float a = load_query(dp, D, b, head, uu * 8 + 2 * e), c = load_query(dp, D, b, head, uu * 8 + 2 * e + 1);
+                        if (mma_bf16) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(a, c);
+                            w[e] = *(const uint32_t*)&h;
+                        } else {
+                            const __half2 h = __floats2half2_rn(a, c);
+                            w[e] = *(const uint32_t*)&h;
+                        }
+                    }
+                } else {
+                    const uint4 v = src[uu];
+                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                }
+            }
+            const int plane = uu / 8, u8 = uu % 8;
+            *(uint4*)(q_s + qt * QBYTES + plane * (XM * 128) + row * 128 + ((u8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_async_proxy();  // generic-proxy writes -> visible to the tensor core
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int32_t* pages = dp.table + (int64_t)grp.trow * dp.max_pages_per_seq + page0;
+    auto page_src = [&](int32_t pg) {  // a page id outside the pool is reported and replaced, so that the barriers go on
+        if (pg < 0 || pg >= dp.n_pages) {
+            if (lane == 0) atomicOr(dp.status, STATUS_PAGE_OOB);
+            pg = 0;
+        }
+        return dp.pool + (int64_t)pg * dp.page_bytes + (int64_t)kvh * (2 * p.chunk_bytes);
+    };
+
+    if (!is_softmax) {
+        // Every lane of these warps walks its loop (the values stay warp-uniform); one elected lane issues.
+        const int role = warp - NQ * (X_SM_THREADS / 32);  // 0 .. NQ - 1: MMAs of tile `role`; above: the copy warp or the converters
+        if (role < NQ) {
+            const int t = role;
+            const uint32_t tm = tmem + t * COLS_PER_TILE;
+            const uint32_t idesc_s = instr_desc(mma_bf16, 0, XM, PAGE_TOKENS);
+            const uint32_t idesc_o = instr_desc(mma_bf16, 1, XM, D);
+            const uint64_t q_desc = smem_desc(smem_u32(q_s) + t * QBYTES, 0, 1024);
+            const uint64_t k_desc = smem_desc(smem_u32(k_ring), 0, 1024);
+            // V tile: planes of 64 channels 8192 bytes apart (leading dimension), 8-key groups 1024 bytes apart
+            const uint64_t v_desc = smem_desc(smem_u32(v_ring), PAGE_TOKENS * 128, 1024);
+            const bool adaptive = !mma_bf16;
+            auto issue_qk = [&](int j) {  // S(j) = Q . K(j)^T into buffer j & 1
+                wait_or_fail(&full_k[j % NK], (uint32_t)((j / NK) & 1), fail_s);
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t kd = k_desc + (uint64_t)(((j % NK) * KSTAGE) >> 4);
+#pragma unroll
+                    for (int pl = 0; pl < PLANES; pl++)
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) {
+                            const uint64_t off = (uint64_t)((pl * (XM * 128) + kk * 32) >> 4);
+                            const uint64_t koff = (uint64_t)((pl * (PAGE_TOKENS * 128) + kk * 32) >> 4);
+                            if constexpr (KPARTS == 2) {
+                                tc_mma_ss_a<A_KEEP>(tm + COL_S + 64 * (j & 1), q_desc + off, kd + koff, idesc_s, (pl | kk) ? 1u : 0u);
+                                tc_mma_ss_a<A_REUSE_LAST>(tm + COL_S + 64 * (j & 1), q_desc + off, kd + (uint64_t)(CHUNK >> 4) + koff, idesc_s, 1u);
+                            } else {
+                                tc_mma_ss(tm + COL_S + 64 * (j & 1), q_desc + off, kd + koff, idesc_s, (pl | kk) ? 1u : 0u);
+                            }
+                        }
+                    tc_commit(&bar_s[2 * t + (j & 1)]);
+                    tc_commit(&free_k[j % NK]);
+                }
+                __syncwarp();
+            };
+            issue_qk(0);
+            if (n_tiles > 1) issue_qk(1);
+            for (int j = 0; j < n_tiles; j++) {
+                wait_or_fail(&full_v[j % NV], (uint32_t)((j / NV) & 1), fail_s);
+                wait_or_fail(&bar_p[2 * t + (j & 1)], (uint32_t)((j >> 1) & 1), fail_s);
+                tc_fence_after();
+                const int* flags = (const int*)(xchg + (2 * t + (j & 1)) * X_XCHG);
+                const bool two = !adaptive || __any_sync(0xffffffffu, flags[lane & 3] != 0);
+                if (elect_one()) {
+                    const uint64_t vd = v_desc + (uint64_t)(((j % NV) * CHUNK) >> 4);
+                    const uint32_t pa = tm + COL_S + 64 * (j & 1);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) {
+                        tc_mma_ts(tm + COL_O, pa + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, (j | kk) ? 1u : 0u);
+                        if (two) tc_mma_ts(tm + COL_O, pa + 32 + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, 1u);
+                    }
+                    tc_commit(&bar_o[2 * t + (j & 1)]);
+                    tc_commit(&free_v[j % NV]);
+                }
+                __syncwarp();
+                // S(j + 2) reuses the buffer P(j) sits in: the tensor core runs one thread's MMAs in issue order
+                if (j + 2 < n_tiles) issue_qk(j + 2);
+            }
+        } else if constexpr (!RAW) {
+            // ================= the chunks of a 16-bit page are the operand tiles =================
+            int32_t pg_next = pages[0];
+            for (int i = 0; i < n_tiles; i++) {
+                const uint8_t* src = page_src(pg_next);
+                if (i + 1 < n_tiles) pg_next = pages[i + 1];  // fetched one page ahead of its use
+                if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
+                if (elect_one()) {
+                    mbar_expect_tx(&full_k[i % NK], CHUNK);
+                    bulk_g2s(k_ring + (i % NK) * CHUNK, src, CHUNK, &full_k[i % NK]);
+                }
+                __syncwarp();
+                if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s);
+                if (elect_one()) {
+                    mbar_expect_tx(&full_v[i % NV], CHUNK);
+                    bulk_g2s(v_ring + (i % NV) * CHUNK, src + CHUNK, CHUNK, &full_v[i % NV]);
+                }
+                __syncwarp();
+            }
+        } else {
+            // ================= converter warps: raw chunk pair -> f16 operand tiles =================
+            constexpr int FMT = SRC == PSRC_Q8 ? B200KV_FMT_Q8_1 : B200KV_FMT_Q4_0;
+            const int ft = tid - (NQ * X_SM_THREADS + 32 * NQ);
+            const bool requester = ft < 32;  // the first converter warp also requests the raw pages
+            auto request = [&](int i, int32_t pg) {
+                const uint8_t* src = page_src(pg);
+                if (elect_one()) {
+                    mbar_expect_tx(&full_raw[i % NR], 2 * p.chunk_bytes);
+                    bulk_g2s(raw_ring + (i % NR) * GEO::RAW_STAGE, src, 2 * p.chunk_bytes, &full_raw[i % NR]);
+                }
+                __syncwarp();
+            };
+            int32_t pg_next = 0;
+            if (requester) {
+                for (int i = 0; i < NR && i < n_tiles; i++) request(i, pages[i]);
+                if (NR < n_tiles) pg_next = pages[NR];
+            }
+            for (int i = 0; i < n_tiles; i++) {
+                const uint8_t* raw = raw_ring + (i % NR) * GEO::RAW_STAGE;
+                wait_or_fail(&full_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
+                if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
+                convert_rows<FMT, D, 0, FT, true>(raw, k_ring + (i % NK) * KSTAGE, k_ring + (i % NK) * KSTAGE + CHUNK, PAGE_TOKENS, ft);
+                fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full_k[i % NK]);
+                if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s);
+                convert_rows<FMT, D, 1, FT, true>(raw + p.chunk_bytes, v_ring + (i % NV) * CHUNK, nullptr, PAGE_TOKENS, ft);
+                fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full_v[i % NV]), mbar_arrive(&free_raw[i % NR]);
+                if (requester && i + NR < n_tiles) {  // the stage is free once the other converter warps have left it too
+                    wait_or_fail(&free_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
+                    request(i + NR, pg_next);
+                    if (i + NR + 1 < n_tiles) pg_next = pages[i + NR + 1];
+                }
+            }
+        }
+    } else {
+        // ================= softmax threads =================
+        const uint32_t lane_base = tmem + qt * COLS_PER_TILE + ((uint32_t)(w4 * 32) << 16);  // this warp's lane quarter
+        const bool adaptive = !mma_bf16;
+        const float sl2 = dp.scale * 1.4426950408889634f;  // scores enter the exponent in log2 units
+        float m_ref = -INFINITY, l_run = 0.f, log_thresh = -INFINITY;
+
+        for (int j = 0; j < n_tiles; j++) {
+            const uint32_t sbuf = lane_base + COL_S + 64 * (j & 1);
+            wait_or_fail(&bar_s[2 * qt + (j & 1)], (uint32_t)((j >> 1) & 1), fail_s);
+            tc_fence_after();
+            uint32_t sr[64];
+            tmem_ld32(sbuf, sr);
+            tmem_ld32(sbuf + 32, sr + 32);
+            tmem_ld_wait();
+            const float tmax = row_max64(sr) * sl2;
+            int* flags = (int*)(xchg + (2 * qt + (j & 1)) * X_XCHG);
+            // Two questions per row, one reduction per warp.  Bit 0: the page needs its remainder product (see X_SKIP_FRACTION;
+            // page 0 always).  Bit 1: the reference maximum is exceeded by more than 2^8 (or was -inf until now): O is rescaled.
+            const bool mine = adaptive && (j == 0 || !(tmax - m_ref + 3.f <= log_thresh));
+            const bool raise = tmax > m_ref + 8.f || (m_ref == -INFINITY && tmax > -INFINITY);
+            const uint32_t votes = __reduce_or_sync(0xffffffffu, (mine ? 1u : 0u) | (raise && j > 0 ? 2u : 0u));
+            const bool two = !adaptive || (votes & 1u);
+            if (adaptive && lane == 0) flags[w4] = two ? 1 : 0;
+            float alpha = 1.f;
+            if (raise) {
+                alpha = fast_exp2(m_ref - tmax);
+                m_ref = tmax;
+                l_run *= alpha;
+            }
+            if (votes & 2u) {
+                // O must hold every page before this one: see prefill_tc.cu for why the wait on barrier (j - 1) & 1 cannot
+                // mistake the completion of P.V(j - 3) or P.V(j + 1) for that of P.V(j - 1)
+                wait_or_fail(&bar_o[2 * qt + ((j - 1) & 1)], (uint32_t)(((j - 1) >> 1) & 1), fail_s);
+                tc_fence_after();
+#pragma unroll
+                for (int cc = 0; cc < D / 16; cc++) {
+                    uint32_t orow[16];
+                    tmem_ld16(lane_base + COL_O + cc * 16, orow);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 16; c++) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
+                    tmem_st16(lane_base + COL_O + cc * 16, orow);
+                }
+            }
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            uint32_t pr[32], pr2[32];
+            float page_sum;
+            if (mma_bf16) page_sum = softmax_exps<2>(sr, sl2, m_use, pr, pr2);
+            else if (two) page_sum = softmax_exps<1>(sr, sl2, m_use, pr, pr2);
+            else page_sum = softmax_exps<0>(sr, sl2, m_use, pr, pr2);
+            tmem_st32(sbuf + 32, pr2);
+            tmem_st32(sbuf, pr);
+            l_run += page_sum;
+            log_thresh = fast_log2(p.skip_fraction * l_run);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_p[2 * qt + (j & 1)]);
+        }
+        // ---- the partial of this run: m in natural-log units, l, O ----
+        wait_or_fail(&bar_o[2 * qt + ((n_tiles - 1) & 1)], (uint32_t)(((n_tiles - 1) >> 1) & 1), fail_s);
+        tc_fence_after();
+        const bool ok = !*fail_s;  // a CTA that gave up publishes an empty partial
+        const int64_t rec = (int64_t)grp.base + ((int64_t)split * dp.Hkv + kvh) * n_rows + my_row;
+        float* dst = dp.part_o + rec * D;
+#pragma unroll
+        for (int cc = 0; cc < D / 32; cc++) {
+            uint32_t orow[32];
+            tmem_ld32(lane_base + COL_O + cc * 32, orow);
+            tmem_ld_wait();
+            if (live)
+#pragma unroll
+                for (int c = 0; c < 32; c += 4)
+                    *(uint4*)(dst + cc * 32 + c) = ok ? make_uint4(orow[c], orow[c + 1], orow[c + 2], orow[c + 3]) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (live) *(float2*)(dp.part_ml + rec * 2) = ok ? make_float2(m_ref * 0.6931471805599453f, l_run) : make_float2(-INFINITY, 0.f);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*fail_s) {
+        if (tid == 0) atomicOr(dp.status, STATUS_WAIT_EXPIRED);
+        __nanosleep(200000);  // give copies that may still be in flight time to land before the CTA's memory is released
+        __syncthreads();
+    }
+    if (warp == 0) tmem_dealloc(tmem, COLS_PER_TILE * NQ);
+}
+
+// ---- the same on the CUDA cores: f32 queries or pages, and 16-bit queries whose rows are not 16-byte aligned -------------
+// A tile is 32 rows.  Per page: K and V as f32 in shared memory (read once for the 32 rows), S = Q K^T with 2 x 4 scores per
+// thread, the online softmax with expf (8 threads per row), O += P V with 2 rows x D / 16 channels per thread.  Bound by the
+// FMA pipe and the shared-memory reads that feed it: 4 D flops per row and key.
+constexpr int CR = 32;         // rows of a tile
+constexpr int C_THREADS = 256;
+
+template <int D>
+struct CGeo {
+    static constexpr int LD = D + 4;  // row pitch in floats: 16-byte aligned rows, successive rows 4 banks apart
+    static constexpr size_t SMEM = ((size_t)CR * LD + 2 * (size_t)PAGE_TOKENS * LD + (size_t)CR * (PAGE_TOKENS + 4) + 3 * CR) * 4;
+};
+
+template <int D>
+__global__ void __launch_bounds__(C_THREADS, 2) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb, int fmt) {
+    constexpr int LD = CGeo<D>::LD, PL = PAGE_TOKENS + 4, CPT = D / 16;
+    extern __shared__ __align__(16) float csm[];
+    float* q_s = csm;                     // [32][LD]
+    float* k_s = q_s + CR * LD;           // [64][LD]
+    float* v_s = k_s + PAGE_TOKENS * LD;  // [64][LD]
+    float* p_s = v_s + PAGE_TOKENS * LD;  // [32][PL] scores, then weights
+    float* m_s = p_s + CR * PL;           // [32] running maximum
+    float* l_s = m_s + CR;                // [32] running sum
+    float* a_s = l_s + CR;                // [32] factor of this page's rescale
+    const DecodeParams& dp = p.d;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int kvh = blockIdx.y;
+    const PrefixGroup grp = prefix_group_of(pb, blockIdx.x);
+    const int split = (blockIdx.x - grp.cta0) / grp.tiles, tile = (blockIdx.x - grp.cta0) % grp.tiles;
+    int page0, n_pages;
+    prefix_run(grp, split, &page0, &n_pages);
+    const int n_rows = grp.n_seqs * dp.G, row0 = tile * CR;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    for (int i = tid; i < CR * D; i += C_THREADS) {
+        const int r = i / D, ch = i % D;
+        float v = 0.f;
+        if (row0 + r < n_rows) v = load_query(dp, D, grp.b0 + (row0 + r) / dp.G, kvh * dp.G + (row0 + r) % dp.G, ch);
+        q_s[r * LD + ch] = v;
+    }
+    if (tid < CR) m_s[tid] = -INFINITY, l_s[tid] = 0.f;
+    float acc[2][CPT];
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int e = 0; e < CPT; e++) acc[r][e] = 0.f;
+    const int32_t* pages = dp.table + (int64_t)grp.trow * dp.max_pages_per_seq + page0;
+
+    for (int i = 0; i < n_pages; i++) {
+        int32_t pg = pages[i];
+        if (pg < 0 || pg >= dp.n_pages) {
+            if (tid == 0) atomicOr(dp.status, STATUS_PAGE_OOB);
+            pg = 0;
+        }
+        const uint8_t* kc = dp.pool + (int64_t)pg * dp.page_bytes + (int64_t)kvh * (2 * p.chunk_bytes);
+        __syncthreads();  // the page before has been used (and q, m, l are there)
+        for (int x = 0; x < 2; x++) {
+            const uint8_t* chunk = kc + x * p.chunk_bytes;
+            float* dst = x ? v_s : k_s;
+            if (fmt == B200KV_FMT_F32) {
+                for (int u = tid; u < PAGE_TOKENS * (D / 4); u += C_THREADS) {
+                    const int t = u / (D / 4), c4 = u % (D / 4);
+                    *(float4*)(dst + t * LD + c4 * 4) = *(const float4*)(chunk + chunk_addr(B200KV_FMT_F32, D, x, t, c4 * 16));
+                }
+            } else {
+                for (int u = tid; u < PAGE_TOKENS * D; u += C_THREADS) dst[(u / D) * LD + u % D] = chunk_elem(chunk, fmt, D, x, u / D, u % D);
+            }
+        }
+        __syncthreads();
+        {  // scores: rows 2 ty + {0, 1}, keys tx + 16 {0 .. 3}
+            float s[2][4] = {};
+#pragma unroll 4
+            for (int c = 0; c < D; c += 4) {
+                float4 qv[2], kv[4];
+#pragma unroll
+                for (int r = 0; r < 2; r++) qv[r] = *(const float4*)(q_s + (2 * ty + r) * LD + c);
+#pragma unroll
+                for (int k = 0; k < 4; k++) kv[k] = *(const float4*)(k_s + (tx + 16 * k) * LD + c);
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        s[r][k] = fmaf(qv[r].x, kv[k].x, s[r][k]), s[r][k] = fmaf(qv[r].y, kv[k].y, s[r][k]);
+                        s[r][k] = fmaf(qv[r].z, kv[k].z, s[r][k]), s[r][k] = fmaf(qv[r].w, kv[k].w, s[r][k]);
+                    }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) p_s[(2 * ty + r) * PL + tx + 16 * k] = s[r][k] * dp.scale;
+        }
+        __syncthreads();
+        {  // softmax of the page: threads 8 r .. 8 r + 7 own row r
+            const int r = tid >> 3, part = tid & 7;
+            float x[8], mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = p_s[r * PL + part + 8 * e], mx = fmaxf(mx, x[e]);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float m_old = m_s[r], m_new = fmaxf(m_old, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float w = expf(x[e] - m_use);
+                p_s[r * PL + part + 8 * e] = w;
+                sum += w;
+            }
+#pragma unroll
+            for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            __syncwarp();  // every lane has read the old maximum of its row
+            if (part == 0) {
+                const float a = expf(m_old - m_use);
+                a_s[r] = a, m_s[r] = m_new, l_s[r] = fmaf(l_s[r], a, sum);
+            }
+        }
+        __syncthreads();
+        {  // values: rows 2 ty + {0, 1}, channels tx * 4 + 64 j .. + 3
+            const float a0 = a_s[2 * ty], a1 = a_s[2 * ty + 1];
+#pragma unroll
+            for (int e = 0; e < CPT; e++) acc[0][e] *= a0, acc[1][e] *= a1;
+#pragma unroll 4
+            for (int t = 0; t < PAGE_TOKENS; t++) {
+                const float p0 = p_s[(2 * ty) * PL + t], p1 = p_s[(2 * ty + 1) * PL + t];
+#pragma unroll
+                for (int j = 0; j < CPT / 4; j++) {
+                    const float4 v = *(const float4*)(v_s + t * LD + tx * 4 + 64 * j);
+                    acc[0][4 * j] = fmaf(p0, v.x, acc[0][4 * j]), acc[0][4 * j + 1] = fmaf(p0, v.y, acc[0][4 * j + 1]);
+                    acc[0][4 * j + 2] = fmaf(p0, v.z, acc[0][4 * j + 2]), acc[0][4 * j + 3] = fmaf(p0, v.w, acc[0][4 * j + 3]);
+                    acc[1][4 * j] = fmaf(p1, v.x, acc[1][4 * j]), acc[1][4 * j + 1] = fmaf(p1, v.y, acc[1][4 * j + 1]);
+                    acc[1][4 * j + 2] = fmaf(p1, v.z, acc[1][4 * j + 2]), acc[1][4 * j + 3] = fmaf(p1, v.w, acc[1][4 * j + 3]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int my_row = row0 + 2 * ty + r;
+        if (my_row >= n_rows) continue;
+        const int64_t rec = (int64_t)grp.base + ((int64_t)split * dp.Hkv + kvh) * n_rows + my_row;
+#pragma unroll
+        for (int j = 0; j < CPT / 4; j++)
+            *(float4*)(dp.part_o + rec * D + tx * 4 + 64 * j) = make_float4(acc[r][4 * j], acc[r][4 * j + 1], acc[r][4 * j + 2], acc[r][4 * j + 3]);
+        if (tx == 0) *(float2*)(dp.part_ml + rec * 2) = make_float2(m_s[2 * ty + r], l_s[2 * ty + r]);
+    }
+}
+
+// ---- join the partials of the shared pages and of the sequence's own ------------------------------------------------------
+struct SharedBatch {
+    int4 pre[INLINE_BATCH];  // per batch entry: {first record of its group, runs of the group, rows of the group, its first row}
+};
+struct SharedCombineParams {
+    const float* part_o;
+    const float* part_ml;
+    void* out;  // may be null when `act` is given
+    int64_t ob, oh;
+    int32_t Hkv, G, dtype, n_rows;
+    uint8_t* act;  // the result as the quantised activation of a W4A8 GEMM, or null (see combine_kernel of decode.cu)
+    int* act_status;
+};
+
+// One CTA per (sequence, query head), one thread per channel; at most MAX_SPLITS partials.
+template <int D>
+__global__ void __launch_bounds__(D) combine_shared_kernel(SharedCombineParams p, const __grid_constant__ InlineBatch ib, const __grid_constant__ SharedBatch sb) {
+    __shared__ float m_s[MAX_SPLITS], l_s[MAX_SPLITS], w_s[MAX_SPLITS];
+    const int b = blockIdx.x, hq = blockIdx.y, ch = threadIdx.x;
+    const int kvh = hq / p.G, g = hq % p.G;
+    grid_dependency_wait();
+    const int64_t act_nb = (int64_t)p.Hkv * p.G * D / QK, act_blk = (int64_t)hq * (D / QK) + (ch >> 5);
+    if (p.act) {  // a warp holds one block of 32 columns of row b
+        if (b == 0 && hq == 0 && ch == 0) q40_status_begin(p.act_status);
+        if (b >= p.n_rows) {
+            q40_quantize_block(0.f, false, p.act, p.n_rows, act_nb, b, act_blk, ch & 31);
+            return;
+        }
+    }
+    const int4 own = ib.ent[b], pre = sb.pre[b];
+    const int n_own = own.w, n = n_own + pre.y;
+    auto record = [&](int k) -> int64_t {
+        return k < n_own ? ((int64_t)(own.z + k) * p.Hkv + kvh) * p.G + g
+                         : (int64_t)pre.x + ((int64_t)(k - n_own) * p.Hkv + kvh) * pre.z + pre.w + g;
+    };
+    float v[8];  // the first partial outputs do not depend on the weights: they travel while the weights are made
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = (k < n) ? p.part_o[record(k) * D + ch] : 0.f;
+    if (ch < n) {
+        const float2 ml = *(const float2*)(p.part_ml + record(ch) * 2);
+        m_s[ch] = ml.x, l_s[ch] = ml.y;
+    }
+    __syncthreads();
+    float M = -INFINITY;
+    for (int k = 0; k < n; k++) M = fmaxf(M, m_s[k]);
+    if (ch < n) w_s[ch] = expf(m_s[ch] - M);
+    __syncthreads();
+    float den = 0.f, num = 0.f;
+    for (int k = 0; k < n; k++) den = fmaf(w_s[k], l_s[k], den);
+#pragma unroll
+    for (int k = 0; k < 8; k++) num = fmaf((k < n) ? w_s[k] : 0.f, v[k], num);
+#pragma unroll 1
+    for (int k0 = 8; k0 < n; k0 += 8) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = (k0 + k < n) ? p.part_o[record(k0 + k) * D + ch] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) num = fmaf((k0 + k < n) ? w_s[k0 + k] : 0.f, v[k], num);
+    }
+    const float res = num / den;
+    if (p.out) st_from_f32(p.out, p.dtype, (int64_t)b * p.ob + (int64_t)hq * p.oh + ch, res);
+    if (p.act) q40_quantize_block(round_to_dtype(res, p.dtype), true, p.act, p.n_rows, act_nb, b, act_blk, ch & 31);
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------
+
+// Pages that two sequences share at their beginning.  Pages are only ever shared at the same place of a sequence and with
+// everything before them (b200kv_fork_shared), so the shared ones come first.  A page that is not full for one of them is its
+// last one and never shared for long (an append moves it); it does not count.
+static int shared_pages(const SeqState& a, const SeqState& b) {
+    if (a.start > 0 || b.start > 0) return 0;  // the front of a trimmed sequence is gone
+    int lo = 0, hi = (int)std::min(a.len / PAGE_TOKENS, b.len / PAGE_TOKENS);
+    while (lo < hi) {  // pages [0, lo) are the same, page hi (if there is one) is not
+        const int mid = (lo + hi) / 2;
+        if (a.pages[mid] == b.pages[mid]) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+struct Run {
+    int b0, n, pages;
+};
+// Cuts the batch into runs of neighbours and gives each the pages that all of its sequences share: from the left, always the
+// run that saves most page reads, (n - 1) * pages.
+static std::vector<Run> shared_runs(const b200kv_cache* c, int32_t n_seqs, const int32_t* seqs) {
+    std::vector<int> with_next((size_t)n_seqs, 0);
+    for (int i = 0; i + 1 < n_seqs; i++) with_next[i] = shared_pages(c->seqs[seqs[i]], c->seqs[seqs[i + 1]]);
+    std::vector<Run> runs;
+    for (int i = 0; i < n_seqs;) {
+        Run best{i, 1, 0};
+        int64_t best_saved = 0;
+        int pages = with_next[i];
+        for (int j = i + 1; j < n_seqs && pages > 0; j++) {
+            if ((int64_t)(j - i) * pages > best_saved) best = {i, j - i + 1, pages}, best_saved = (int64_t)(j - i) * pages;
+            pages = std::min(pages, with_next[j]);
+        }
+        runs.push_back(best);
+        i += best.n;
+    }
+    return runs;
+}
+
+template <int NQ, int D, int SRC>
+static cudaError_t launch_prefix_tc_t(const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    using GEO = XGeo<NQ, D, SRC>;
+    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<NQ, D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GEO::SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_after_predecessor(prefix_tc_kernel<NQ, D, SRC>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(GEO::THREADS), GEO::SMEM, stream, p, pb);
+}
+template <int D, int SRC>
+static cudaError_t launch_prefix_tc_nq(int nq, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    return nq == 2 ? launch_prefix_tc_t<2, D, SRC>(p, pb, ctas, stream) : launch_prefix_tc_t<1, D, SRC>(p, pb, ctas, stream);
+}
+static cudaError_t launch_prefix_tc(int fmt, int D, int nq, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    if (fmt == B200KV_FMT_Q8_1) return D == 128 ? launch_prefix_tc_nq<128, PSRC_Q8>(nq, p, pb, ctas, stream) : launch_prefix_tc_nq<64, PSRC_Q8>(nq, p, pb, ctas, stream);
+    if (fmt == B200KV_FMT_Q4_0) return D == 128 ? launch_prefix_tc_nq<128, PSRC_Q4>(nq, p, pb, ctas, stream) : launch_prefix_tc_nq<64, PSRC_Q4>(nq, p, pb, ctas, stream);
+    return D == 128 ? launch_prefix_tc_nq<128, PSRC_PAGES16>(nq, p, pb, ctas, stream) : launch_prefix_tc_nq<64, PSRC_PAGES16>(nq, p, pb, ctas, stream);
+}
+template <int D>
+static cudaError_t launch_prefix_simt(int fmt, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(prefix_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CGeo<D>::SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_after_predecessor(prefix_simt_kernel<D>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(C_THREADS), CGeo<D>::SMEM, stream, p, pb, fmt);
+}
+
+// At most INLINE_BATCH sequences; `ends` as launch_decode takes it.
+static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q, const int64_t* qs, void* out,
+                         const int64_t* os, int32_t dtype, float scale, cudaStream_t stream, const QueryRope& ends) {
+    const int Hkv = c->L.Hkv, D = c->L.D, G = n_q_heads / Hkv;
+    for (int i = 0; i < n_seqs; i++)
+        if (c->seqs[seqs[i]].len <= 0) return fail("sequence %d is empty: nothing to attend to", seqs[i]);
+    std::vector<Run> runs = shared_runs(c, n_seqs, seqs);
+    bool any = false;
+    for (const Run& r : runs) any |= r.n > 1 && r.pages > 0;
+    if (!any) return launch_decode(c, n_seqs, seqs, n_q_heads, q, qs, out, os, dtype, scale, stream, 0, &ends);
+
+    // ---- the shared pages: which kernel, how many rows to a CTA ----
+    const int fmt = c->L.fmt;
+    const bool quant = fmt_is_block_quant(fmt);
+    const bool q_rows16 = (uintptr_t)q % 16 == 0 && qs[0] % 8 == 0 && qs[1] % 8 == 0;
+    const bool tc = dtype != B200KV_F32 && (quant || fmt == dtype) && q_rows16 && !c->force_simt;
+    int max_rows = 0, max_pages = 1;
+    for (const Run& r : runs)
+        if (r.n > 1 && r.pages > 0) max_rows = std::max(max_rows, r.n * G), max_pages = std::max(max_pages, r.pages);
+    const int nq = max_rows > XM ? 2 : 1;
+    const int rows_cta = tc ? nq * XM : CR;
+    const int64_t slots = 148 * (tc && (nq == 2 || quant) ? 1 : 2);  // resident CTAs
+
+    // ---- the own pages of every sequence: as launch_decode cuts them, starting behind the shared ones ----
+    const bool use_mma = decode_mma_supported(fmt, D, dtype) && !c->force_simt;
+    const int nz = (G + (use_mma ? 8 : (G == 1 ? 1 : 4)) - 1) / (use_mma ? 8 : (G == 1 ? 1 : 4));
+    std::vector<int64_t> first((size_t)n_seqs), own_pages((size_t)n_seqs);
+    std::vector<int> most((size_t)n_seqs, MAX_SPLITS);  // runs of a sequence's own pages: a row joins at most MAX_SPLITS partials
+    for (const Run& r : runs)
+        for (int i = r.b0; i < r.b0 + r.n; i++) {
+            const SeqState& s = c->seqs[seqs[i]];
+            first[i] = r.n > 1 && r.pages > 0 ? (int64_t)r.pages * PAGE_TOKENS : s.start;
+            if (r.n > 1 && r.pages > 0) most[i] = MAX_SPLITS / 2;
+            own_pages[i] = (s.len + PAGE_TOKENS - 1) / PAGE_TOKENS - first[i] / PAGE_TOKENS;
+        }
+    int64_t own_chunk = pages_per_split(c, own_pages.data(), n_seqs, use_mma, nz);
+
+    InlineBatch ib{};
+    SharedBatch sb{};
+    PrefixBatch pb{};
+    int n_items = 0, ctas = 0;
+    int64_t n_rec = 0, run_pages = 1;
+    for (int64_t tiles_pages = 0;;) {  // the smallest run length that fills the GPU once
+        tiles_pages = 0;
+        for (const Run& r : runs)
+            if (r.n > 1 && r.pages > 0) tiles_pages += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * ((r.pages + run_pages - 1) / run_pages);
+        if (tiles_pages * Hkv <= slots || run_pages >= max_pages) break;
+        run_pages++;
+    }
+    for (;;) {
+        ib = InlineBatch{};
+        pb = PrefixBatch{};
+        n_items = 0, ctas = 0;
+        for (int i = 0; i < n_seqs; i++) {
+            const int splits = own_pages[i] ? (int)std::min<int64_t>(most[i], (own_pages[i] + own_chunk - 1) / own_chunk) : 0;
+            ib.ent[i] = make_int4(seqs[i], (int)c->seqs[seqs[i]].len, n_items, splits);
+            ib.first[i] = (int32_t)first[i];
+            n_items += splits;
+        }
+        ib.n = n_seqs;
+        n_rec = (int64_t)n_items * Hkv * G;
+        for (const Run& r : runs) {
+            if (r.n <= 1 || r.pages <= 0) continue;
+            const int rows = r.n * G;
+            PrefixGroup& g = pb.g[pb.n++];
+            g.trow = seqs[r.b0], g.n_pages = r.pages, g.b0 = r.b0, g.n_seqs = r.n;
+            g.tiles = (rows + rows_cta - 1) / rows_cta;
+            g.splits = (int)std::min<int64_t>(MAX_SPLITS / 2, (r.pages + run_pages - 1) / run_pages);
+            g.cta0 = ctas, g.base = (int32_t)n_rec;
+            for (int i = 0; i < r.n; i++) sb.pre[r.b0 + i] = make_int4(g.base, g.splits, rows, i * G);
+            ctas += g.tiles * g.splits;
+            n_rec += (int64_t)g.splits * Hkv * rows;
+        }
+        if ((size_t)n_rec * (D + 2) * sizeof(float) <= c->ws_bytes) break;  // sized once, at create: longer runs where it is small
+        bool longest = run_pages >= max_pages;
+        for (int i = 0; i < n_seqs; i++) longest &= own_pages[i] <= own_chunk;
+        if (longest)
+            return fail("%d sequences x %d query heads need %zu bytes of split partials, the workspace holds %zu: create the cache "
+                        "with max_q_heads >= %d", n_seqs, n_q_heads, (size_t)n_rec * (D + 2) * sizeof(float), c->ws_bytes, n_q_heads);
+        run_pages += std::max<int64_t>(1, run_pages / 4);
+        own_chunk += std::max<int64_t>(1, own_chunk / 4);
+    }
+
+    PrefixParams p{};
+    DecodeParams& dp = p.d;
+    dp.pool = c->pool, dp.table = c->d_table, dp.status = c->d_status;
+    dp.q = q, dp.qb = qs[0], dp.qh = qs[1];
+    if (ends.cos) dp.q_cos = ends.cos, dp.q_sin = ends.sin, dp.rope_b = ends.stride_b;
+    dp.part_o = (float*)c->ws, dp.part_ml = dp.part_o + n_rec * D;
+    dp.page_bytes = c->L.page_bytes, dp.n_pages = (int32_t)c->n_pages, dp.max_pages_per_seq = c->max_pages_per_seq;
+    dp.Hkv = Hkv, dp.G = G, dp.dtype = dtype, dp.scale = scale, dp.wait_ns = c->wait_ns;
+    p.chunk_bytes = c->L.chunk_bytes, p.skip_fraction = X_SKIP_FRACTION;
+    cudaError_t e;
+    {
+        ProfScope ps(c, K_PREFIX, stream);
+        e = tc ? launch_prefix_tc(fmt, D, nq, p, pb, ctas, stream)
+               : (D == 128 ? launch_prefix_simt<128>(fmt, p, pb, ctas, stream) : launch_prefix_simt<64>(fmt, p, pb, ctas, stream));
+    }
+    if (e != cudaSuccess) return fail("shared-prefix launch failed: %s", cudaGetErrorString(e));
+    if (n_items > 0) {
+        ProfScope ps(c, K_DECODE, stream);
+        if ((use_mma ? launch_decode_mma(fmt, dp, n_items, stream, &ib) : launch_decode_simt(fmt, D, dp, n_items, stream, &ib)) != B200KV_OK) return B200KV_KO;
+    }
+    SharedCombineParams cp{};
+    cp.part_o = dp.part_o, cp.part_ml = dp.part_ml, cp.out = out, cp.ob = os[0], cp.oh = os[1];
+    cp.Hkv = Hkv, cp.G = G, cp.dtype = dtype, cp.n_rows = n_seqs;
+    if (ends.act_scratch) cp.act = (uint8_t*)ends.act_scratch + Q_HEADER, cp.act_status = (int*)ends.act_scratch;
+    const unsigned rows = cp.act ? (unsigned)((n_seqs + 7) / 8 * 8) : (unsigned)n_seqs;
+    {
+        ProfScope ps(c, K_COMBINE, stream);
+        e = D == 128 ? launch_after_predecessor(combine_shared_kernel<128>, dim3(rows, n_q_heads), dim3(128), 0, stream, cp, ib, sb)
+                     : launch_after_predecessor(combine_shared_kernel<64>, dim3(rows, n_q_heads), dim3(64), 0, stream, cp, ib, sb);
+    }
+    if (e != cudaSuccess) return fail("combine launch failed: %s", cudaGetErrorString(e));
+    return B200KV_OK;
+}
+
+}  // namespace b200kv
+
+using namespace b200kv;
+
+extern "C" int b200kv_attend_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q,
+                                    const int64_t q_strides[3], const void* cos, const void* sin, int64_t rope_stride, void* out,
+                                    const int64_t out_strides[3], void* scratch, int32_t dtype, float scale, void* stream_) {
+    if (validate_seqs(c, n_seqs, seqs) != B200KV_OK) return B200KV_KO;
+    if (!c->L.has_v) return fail("this cache holds one tensor only: attention needs K and V");
+    if (fmt_is_kivi(c->L.fmt)) return fail("the sequences of a KIVI cache share no pages: use b200kv_attend");
+    if (!q || !q_strides || (!out && !scratch) || (out && !out_strides)) return fail("null tensor or strides");
+    if ((cos == nullptr) != (sin == nullptr)) return fail("cos and sin come together");
+    if ((uintptr_t)scratch % 16) return fail("scratch must be 16-byte aligned");
+    if (n_q_heads <= 0 || n_q_heads % c->L.Hkv != 0)
+        return fail("n_q_heads (%d) must be a positive multiple of n_kv_heads (%d)", n_q_heads, c->L.Hkv);
+    if (dtype < B200KV_F32 || dtype > B200KV_BF16) return fail("unknown dtype %d", dtype);
+    if (scale <= 0.f) scale = 1.0f / sqrtf((float)c->L.D);
+    cudaStream_t stream = (cudaStream_t)stream_;
+    DeviceGuard guard(c->cfg.device);
+    const int64_t no_strides[3] = {0, 0, 0};
+    const int64_t* os = out ? out_strides : no_strides;
+    const QueryRope ends{cos, sin, rope_stride, scratch};
+    if (n_seqs <= INLINE_BATCH) return launch_shared(c, n_seqs, seqs, n_q_heads, q, q_strides, out, os, dtype, scale, stream, ends);
+    // the quantised activation of a larger batch is laid out for all of its rows at once: the regular call writes it
+    if (scratch) return launch_decode(c, n_seqs, seqs, n_q_heads, q, q_strides, out, os, dtype, scale, stream, 0, &ends);
+    const int esz = dtype_size(dtype);
+    for (int at = 0; at < n_seqs; at += INLINE_BATCH) {
+        const QueryRope part{cos ? (const uint8_t*)cos + (int64_t)at * rope_stride * esz : nullptr,
+                             sin ? (const uint8_t*)sin + (int64_t)at * rope_stride * esz : nullptr, rope_stride, nullptr};
+        if (launch_shared(c, std::min(INLINE_BATCH, n_seqs - at), seqs + at, n_q_heads, (const uint8_t*)q + (int64_t)at * q_strides[0] * esz, q_strides,
+                          (uint8_t*)out + (int64_t)at * os[0] * esz, os, dtype, scale, stream, part) != B200KV_OK)
+            return B200KV_KO;
+    }
+    return B200KV_OK;
+}
