@@ -332,6 +332,25 @@ int b200kv_silu_mul(const void* gate, const void* up, void* out, int64_t n, int3
 int b200kv_add(const void* a, const void* b, void* out, int64_t n, int32_t dtype, void* stream);
 /* out[r] = index of the first maximum of row r of the f32 matrix [rows, n] (ArgMax over the logits: greedy decoding). */
 int b200kv_argmax(const float* x, int64_t stride, int64_t rows, int32_t n, int32_t* out, void* stream);
+/* The next token of each row of logits [rows, n] (type `dtype`, rows `stride` elements apart), drawn with a given uniform
+ * number per row.  Settings are device arrays of `rows` values, each of which may be NULL (off for every row):
+ *   temperature  w_i = exp((x_i - max x) / T); not above 0 (or NaN): the first maximum, as b200kv_argmax; NULL: 1
+ *   top_k        keeps the k largest logits, equal ones by rising index; 0 or less, or n and more: off
+ *   top_p        of these, in falling order, the shortest beginning whose mass reaches p x the mass of these; 1 and more
+ *                (or NaN): off; 0 and less: the first one alone
+ *   min_p        of these, the ones with w_i >= min_p (the maximum always); 0 and less (or NaN): off
+ *   uniform      u in [0, 1): the token is the first kept index, in rising order, at which the sum of kept weights exceeds
+ *                u x their whole sum (required; numbers outside are taken to the nearer end)
+ * Weights and their sums are 64-bit (fixed point with 44 fractional bits for single weights), independent of the order of
+ * execution: the same inputs give the same token every time.  A NaN logit counts as -inf; infinite logits share the row;
+ * a row without any number above -inf gives 0.  n is at most 524288.  out: int32 [rows].
+ * `scratch`: b200kv_sample_scratch_bytes(rows, n) bytes of device memory, 16-byte aligned, not shared by two calls in
+ * flight (two captured graphs that may run at once need one each).  Has no counterpart in the reference, whose decode loop
+ * is greedy (examples/causal_llm/src/lib.rs:290-408). */
+int64_t b200kv_sample_scratch_bytes(int64_t rows, int32_t n);
+int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, int64_t rows, int32_t n, const float* temperature,
+                  const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* out, void* scratch,
+                  void* stream);
 /* out[i] = table[ids[i]]: rows of row_bytes bytes (a multiple of 16); the embedding lookup (core Gather on axis 0). */
 int b200kv_gather_rows(const void* table, int64_t n_rows_table, int64_t row_bytes, const int32_t* ids, int64_t n_ids, void* out,
                        void* stream);

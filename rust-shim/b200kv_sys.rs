@@ -182,6 +182,11 @@ extern "C" {
     pub fn b200kv_silu_mul(gate: *const c_void, up: *const c_void, out: *mut c_void, n: i64, dtype: i32, stream: *mut c_void) -> c_int;
     pub fn b200kv_add(a: *const c_void, b: *const c_void, out: *mut c_void, n: i64, dtype: i32, stream: *mut c_void) -> c_int;
     pub fn b200kv_argmax(x: *const c_float, stride: i64, rows: i64, n: i32, out: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn b200kv_sample_scratch_bytes(rows: i64, n: i32) -> i64;
+    pub fn b200kv_sample(
+        logits: *const c_void, stride: i64, dtype: i32, rows: i64, n: i32, temperature: *const f32, top_k: *const i32,
+        top_p: *const f32, min_p: *const f32, uniform: *const f32, out: *mut i32, scratch: *mut c_void, stream: *mut c_void,
+    ) -> c_int;
     pub fn b200kv_gather_rows(
         table: *const c_void, n_rows_table: i64, row_bytes: i64, ids: *const i32, n_ids: i64, out: *mut c_void,
         stream: *mut c_void,

@@ -28,7 +28,7 @@ EXPORTS = [
     "b200kv_rms_norm", "b200kv_silu_mul", "b200kv_add", "b200kv_argmax", "b200kv_gather_rows", "b200kv_cast",
     "b200kv_attend_window", "b200kv_trim", "b200kv_attend_rope", "b200kv_attend_q40", "b200kv_append_attend", "b200kv_q40_quantize", "b200kv_q40_gemm_quantized", "b200kv_q40_gemm_quantized_as",
     "b200kv_q40_silu_mul_quantize", "b200kv_q40_add_rms_norm_quantize", "b200kv_workspace_bytes", "b200kv_truncate_many", "b200kv_sdpa_check",
-    "b200kv_fork_shared", "b200kv_seq_free_many", "b200kv_attend_shared",
+    "b200kv_fork_shared", "b200kv_seq_free_many", "b200kv_attend_shared", "b200kv_sample_scratch_bytes", "b200kv_sample",
 ]
 KERNEL_NAMES = {0: "table_scatter", 1: "append", 2: "decode", 3: "combine", 4: "export", 5: "sdpa_dense", 6: "prefill", 7: "share", 8: "prefix"}
 
@@ -89,6 +89,8 @@ def lib():
         L.b200kv_attend_q40.argtypes = [vp, i32, i32p, i32, vp, i64p, vp, vp, i64, vp, i64p, vp, i32, C.c_float, vp]
         L.b200kv_attend_window.argtypes = [vp, i32, i32p, i32, vp, i64p, vp, i64p, i32, C.c_float, i64, vp]
         L.b200kv_trim.argtypes = [vp, i32, i64]
+        L.b200kv_sample_scratch_bytes.argtypes, L.b200kv_sample_scratch_bytes.restype = [i64, i32], i64
+        L.b200kv_sample.argtypes = [vp, i64, i32, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp]
         L.b200kv_fork_shared.argtypes = [vp, i32, i32p, i32p, vp]
         L.b200kv_seq_free_many.argtypes = [vp, i32, i32p]
         L.b200kv_attend_shared.argtypes = [vp, i32, i32p, i32, vp, i64p, vp, vp, i64, vp, i64p, vp, i32, C.c_float, vp]
@@ -580,6 +582,43 @@ def argmax(x, out=None):
     with torch.cuda.device(x.device):
         _ck(lib().b200kv_argmax(C.c_void_p(x.data_ptr()), C.c_int64(x.stride(0)), C.c_int64(x.shape[0]), int(x.shape[1]),
                                 C.c_void_p(out.data_ptr()), _stream()))
+    return out
+
+
+def sample_scratch(rows, n, device=None):
+    """Workspace of sample() for up to `rows` rows of up to `n` logits (one for each call that may be in flight at once)."""
+    import torch
+
+    size = lib().b200kv_sample_scratch_bytes(int(rows), int(n))
+    if size < 0:
+        raise B200KvError(lib().b200kv_last_error().decode())
+    return torch.empty(size, dtype=torch.uint8, device="cuda" if device is None else device)
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, out=None, scratch=None):
+    """The next token (int32 [rows]) of every row of `logits` ([rows, n], f32 / f16 / bf16, rows contiguous): temperature, top-k,
+    top-p and min-p, drawn with the numbers `uniform` in [0, 1).  uniform, temperature, top_p, min_p: f32 [rows]; top_k: int32
+    [rows]; None leaves a setting off (temperature: 1).  A temperature of 0 takes the first maximum, as argmax()."""
+    import torch
+
+    rows, dev = logits.shape[0], logits.device
+    assert logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1) and dev.type == "cuda"
+    if uniform is None:
+        raise B200KvError("sample() takes one uniform number per row")
+    ptrs = []
+    for t, dt in ((temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32), (uniform, torch.float32)):
+        assert t is None or (t.dtype == dt and t.shape == (rows,) and t.is_contiguous() and t.device == dev)
+        ptrs.append(None if t is None else t.data_ptr())
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=dev)
+    assert out.dtype == torch.int32 and out.shape == (rows,) and out.is_contiguous() and out.device == dev
+    if scratch is None:
+        scratch = sample_scratch(rows, logits.shape[1], dev)
+    assert scratch.device == dev and scratch.numel() >= lib().b200kv_sample_scratch_bytes(rows, logits.shape[1])
+    stride = logits.stride(0) if rows > 1 else logits.shape[1]
+    with torch.cuda.device(dev):
+        _ck(lib().b200kv_sample(logits.data_ptr(), stride, _dtype_code(logits), rows, logits.shape[1], *ptrs, out.data_ptr(), scratch.data_ptr(),
+                                _stream()))
     return out
 
 
