@@ -345,7 +345,8 @@ int b200kv_argmax(const float* x, int64_t stride, int64_t rows, int32_t n, int32
  * execution: the same inputs give the same token every time.  A NaN logit counts as -inf; infinite logits share the row;
  * a row without any number above -inf gives 0.  n is at most 524288.  out: int32 [rows].
  * `scratch`: b200kv_sample_scratch_bytes(rows, n) bytes of device memory, 16-byte aligned, not shared by two calls in
- * flight (two captured graphs that may run at once need one each).  Has no counterpart in the reference, whose decode loop
+ * flight (two captured graphs that may run at once need one each); 0 bytes, and then it may be NULL, for n up to 262144,
+ * where a row fits the shared memory of a thread-block cluster.  Has no counterpart in the reference, whose decode loop
  * is greedy (examples/causal_llm/src/lib.rs:290-408). */
 int64_t b200kv_sample_scratch_bytes(int64_t rows, int32_t n);
 int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, int64_t rows, int32_t n, const float* temperature,

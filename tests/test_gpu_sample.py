@@ -91,7 +91,8 @@ MODES = {"plain": {}, "top_k": dict(k=40), "top_p": dict(p=0.9), "min_p": dict(m
 
 @pytest.mark.parametrize("mode", list(MODES))
 @pytest.mark.parametrize("io,rows,n,pad", [("f32", 1, 1, 0), ("f32", 3, 2, 1), ("bf16", 2, 33, 7), ("f32", 5, 1000, 0), ("f16", 4, 2049, 0),
-                                           ("f32", 2, 8193, 3), ("bf16", 3, 50257, 7), ("f32", 3, 128256, 0), ("f16", 2, 200000, 0)])
+                                           ("f32", 2, 8193, 3), ("bf16", 3, 50257, 7), ("f32", 3, 128256, 0), ("f16", 2, 200000, 0),
+                                           ("f32", 2, 300001, 0), ("bf16", 1, 524288, 0)])
 def test_modes_types_and_sizes(kv, mode, io, rows, n, pad):
     x, g = model_logits(n + rows, rows, n, io, pad)
     t = 0.4 + g.random(rows)
@@ -239,10 +240,11 @@ def test_repeats_strides_streams_and_graphs(kv):
 def test_refusals(kv):
     x, u = torch.zeros((2, 100), device="cuda"), torch.zeros(2, device="cuda")
     L = kv.lib()
-    out, scratch = torch.full((2,), -7, dtype=torch.int32, device="cuda"), kv.sample_scratch(2, 100)
+    out, scratch = torch.full((2,), -7, dtype=torch.int32, device="cuda"), kv.sample_scratch(2, 300000)
+    assert scratch.numel() >= 2 * 300000 * 4 and kv.sample_scratch(2, 262144).numel() == 0
     call = lambda logits=x.data_ptr(), stride=100, dtype=0, rows=2, n=100, uniform=u.data_ptr(), o=out.data_ptr(), s=scratch.data_ptr(): L.b200kv_sample(
         logits, stride, dtype, rows, n, None, None, None, None, uniform, o, s, None)
-    for kw, why in ((dict(logits=None), b"null"), (dict(uniform=None), b"null"), (dict(o=None), b"null"), (dict(s=None), b"null"), (dict(rows=0), b"positive"),
+    for kw, why in ((dict(logits=None), b"null"), (dict(uniform=None), b"null"), (dict(o=None), b"null"), (dict(s=None, n=300000, stride=300000), b"workspace"), (dict(rows=0), b"positive"),
                     (dict(n=0), b"positive"), (dict(dtype=3), b"dtype"), (dict(stride=99), b"apart"), (dict(s=scratch.data_ptr() + 8), b"aligned"),
                     (dict(n=524289, stride=524289), b"at most"), (dict(rows=70000), b"at most")):
         assert call(**kw) == 1 and why in L.b200kv_last_error(), kw

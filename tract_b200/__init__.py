@@ -586,7 +586,8 @@ def argmax(x, out=None):
 
 
 def sample_scratch(rows, n, device=None):
-    """Workspace of sample() for up to `rows` rows of up to `n` logits (one for each call that may be in flight at once)."""
+    """Workspace of sample() for `rows` rows of `n` logits (one for each call that may be in flight at once): empty for rows that
+    fit on the chip, of up to 262144 logits."""
     import torch
 
     size = lib().b200kv_sample_scratch_bytes(int(rows), int(n))

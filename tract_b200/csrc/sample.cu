@@ -7,58 +7,56 @@
 //   token = the first kept index i, in rising order, with  sum_{kept j <= i} w_j > u x sum_kept w_j
 //
 // A token changes when u falls between a border of the distribution and its rounded value; 128k borders with the error of
-// 32-bit sums would move one row in a hundred.  Weights are therefore 64-bit: doubles over whole slices of a row, and fixed
-// point with 44 bits behind the point where single tokens are added up -- integer sums, so that the order in which threads
-// add has no influence.
+// 32-bit sums would move one row in a hundred.  Weights are therefore computed in double and added up in fixed point with 44
+// bits behind the point: integer sums, so that neither the order of the threads nor that of the atomics has any influence.
 //
-// Two launches.  sample_stats_kernel reads the logits once, a slice of a row per CTA: maximum and its place, mass (only where
-// a filter or the draw needs the mass of the whole row), and a histogram of every eighth logit over octaves of w.
-// sample_pick_kernel has one CTA per row: the histogram tells how deep the filters can reach, the tokens above that threshold
-// are gathered into shared memory, the cut is found by radix refinement of their bit patterns (1024 bins of counts and masses
-// per round), the token by the same refinement over the indices.  The threshold is an estimate and only that: whether the
-// gathered tokens hold the cut is checked exactly, and if they do not, or do not fit, the rounds read the row itself.
-// Without filters the draw picks the slice from the slices' masses and the token inside it.
-// Bound: the logits once (4 bytes each in f32) plus 11 double operations per logit where the mass is needed.
+// One launch, one thread-block cluster per row, the row split over the shared memories of its CTAs: the logits are read from
+// HBM once, and everything else happens on chip.
+//   1. load, maximum (one exchange over the cluster).  A greedy row ends here.
+//   2. the cut of top-k / top-p: a histogram over 1024 bins of log2 w (counts, and for top-p masses); every CTA adds up an
+//      equal share of the bins over the cluster, and the bin in which the count or mass is reached is found from the shares' totals.
+//   3. where at most 1024 tokens lie above the lower border of that bin -- nearly always -- the first CTA gathers and sorts
+//      them, applies all filters and draws.  Otherwise the bin is refined, by the same histogram over the bit patterns in it,
+//      until the last kept token is known.
+//   4. the draw over whole slices: the kept mass of every CTA, one exchange, and the CTA into whose share the draw falls
+//      finds the token (also the way of rows without top-k and top-p, which start here).
+// Bound: the logits once (4 bytes each in f32), and, for rows that need every weight, 9 double operations per logit and pass.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 
 #include "internal.h"
 
+namespace cg = cooperative_groups;
+
 namespace b200kv {
 
-constexpr int ST_THREADS = 256;   // stats kernel
-constexpr int PK_THREADS = 1024;  // pick kernel
-constexpr int ST_BINS = 32;       // octaves of w below the slice's maximum; the last one takes everything deeper
-constexpr int ST_SAMPLE = 8;      // one logit in this many enters the histogram
-constexpr int PK_CHUNK = 8192;    // logits of a gathering step
-constexpr int PK_BINS = 1024;     // bins of a refinement round
-constexpr int PK_CAP = 5888;      // gathered tokens: 16 bytes each, two CTAs per SM
-constexpr int W_BITS = 44;        // fractional bits of a fixed-point weight
+constexpr int SP_THREADS = 512;
+constexpr int SP_WARPS = SP_THREADS / 32;
+constexpr int SP_CLUSTER = 8;       // most CTAs of a row (the portable cluster size)
+constexpr int SP_SLICE = 16384;     // logits a CTA takes before another one is added: 64 KB, two CTAs per SM
+constexpr int SP_BINS = 1024;
+constexpr int SP_LIST = 1024;       // tokens that are sorted
+constexpr int W_BITS = 44;          // fractional bits of a weight
+constexpr int SP_LIMB = 15;         // a weight enters a histogram as three 15-bit limbs: 2^17 of them fit a 32-bit counter
 constexpr int MAX_VOCAB = 1 << 19;  // so many weights of 1 add up to 2^63
+constexpr int MAX_ON_CHIP = SP_CLUSTER * 32768;  // 128 KB per CTA; the slices of longer rows go to the workspace
+static_assert(MAX_VOCAB / SP_CLUSTER < (1 << 17), "the limbs of a bin of one CTA");
 
-struct SliceStats {
-    double mass;    // sum of exp((x - max of the slice) / T)
-    float max;      // -inf: no number above -inf
-    int32_t at;     // first index of the maximum
-};
-struct SliceBins {
-    uint32_t count[ST_BINS];
-    float mass[ST_BINS];  // relative to 2^floor(max * log2 e / T)
-};
+typedef unsigned long long u64;
 
 struct SampleParams {
     const void* logits;
     int64_t stride;
-    int32_t dtype, n, n_slices, slice;  // slice: elements per slice
+    int32_t dtype, n, slice, vec;  // slice: logits per CTA; vec: rows start on 16-byte boundaries
     const float* temperature;
     const int32_t* top_k;
     const float* top_p;
     const float* min_p;
     const float* uniform;
     int32_t* out;
-    SliceStats* stats;  // [rows][n_slices]
-    SliceBins* bins;    // [rows][n_slices]
-    int32_t vec;        // rows start on 16-byte boundaries
+    float* scratch;  // null, or [rows][SP_CLUSTER][slice]: slices that do not fit on the chip
 };
 
 // The settings of a row, with what means "off" made explicit.
@@ -66,7 +64,6 @@ struct RowSettings {
     float t, p, min_p, u;
     int32_t k;
     bool greedy, use_p, use_k, use_m;
-    __device__ bool need_mass() const { return !greedy && !use_k && (use_p || !use_m); }
 };
 __device__ inline RowSettings row_settings(const SampleParams& p, int row) {
     RowSettings s;
@@ -74,18 +71,17 @@ __device__ inline RowSettings row_settings(const SampleParams& p, int row) {
     s.k = p.top_k ? p.top_k[row] : 0;
     s.p = p.top_p ? p.top_p[row] : 1.f;
     s.min_p = p.min_p ? p.min_p[row] : 0.f;
-    s.u = p.uniform[row];
+    const float u = p.uniform[row];
+    s.u = u > 0.f ? fminf(u, 1.f) : 0.f;
     s.greedy = !(s.t > 0.f);
     s.use_k = s.k > 0 && s.k < p.n;
     s.use_p = s.p < 1.f;
     s.use_m = s.min_p > 0.f;
-    s.min_p = fminf(s.min_p, 1.f);  // the likeliest token always stays
-    if (s.use_p && !(s.p > 0.f)) s.use_k = true, s.k = 1, s.use_p = false;  // an empty beginning: the first token alone
-    if (s.use_k && s.k == 1) s.greedy = true;
+    s.min_p = fminf(s.min_p, 1.f);                                  // the likeliest token always stays
+    s.greedy |= (s.use_k && s.k == 1) || (s.use_p && !(s.p > 0.f));  // an empty beginning: the first token alone
     return s;
 }
 __device__ inline float clean(float x) { return x != x ? -INFINITY : x + 0.f; }  // NaN is never chosen; -0 and +0 are the same logit
-__device__ inline float load_logit(const SampleParams& p, const uint8_t* row, int64_t i) { return clean(ld_as_f32(row, p.dtype, i)); }
 // monotone bit pattern of a logit
 __device__ inline uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -94,89 +90,127 @@ __device__ inline uint32_t key_of(float x) {
 __device__ inline float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t KEY_NEG_INF = 0x007fffffu;
 
-// w of a logit against the row's maximum, in 64 bits; a maximum of +inf shares the row among the infinite logits
-__device__ inline double weight_of(float x, float max, double t) {
-    if (x == max) return 1.0;
-    if (x == -INFINITY || max == INFINITY) return 0.0;
-    return exp(((double)x - (double)max) / t);
-}
-__device__ inline unsigned long long fixed_weight(float x, float max, double t) {
-    return (unsigned long long)__double2ll_rn(weight_of(x, max, t) * (double)(1ull << W_BITS));
+// The place where the running count or mass passes its goal.
+struct Hit {
+    uint32_t bin;               // 0xffffffff: nowhere
+    uint32_t n_before, n_here;  // tokens before the bin and in it
+    u64 w_before, w_here;       // their weights
+};
+
+struct RowShared {
+    uint32_t hist[4][SP_BINS];  // counts; limbs of the masses
+    u64 list[SP_LIST];          // gathered tokens
+    double exp2_table[64];      // 2^(j / 64)
+    u64 sums64[SP_WARPS + 1];
+    uint32_t sums32[SP_WARPS + 1];
+    u64 warp_w[SP_WARPS];
+    // written by the other CTAs of the cluster
+    float x_max[SP_CLUSTER];
+    int32_t x_at[SP_CLUSTER];
+    u64 x_w[SP_CLUSTER];
+    uint32_t x_n[SP_CLUSTER];
+    Hit hit;
+    uint32_t n_list;
+    // of this CTA
+    float red_max[SP_WARPS];
+    int32_t red_at[SP_WARPS];
+    uint32_t key_lo, key_hi, found;
+};
+
+// Inclusive sums over the CTA in thread order.
+template <typename T>
+__device__ inline T block_scan(T v, T* warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+    }
+    __syncthreads();  // the sums of the scan before are no longer read
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    T mine = lane < warp ? warp_sums[lane] : T(0);  // SP_WARPS <= 32
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    return mine + v;
 }
 
-// ---- first launch ---------------------------------------------------------------------------------------------------------
-// EPT logits per thread, all of them in registers: read once, used for the maximum, then for mass and histogram.
-template <int EPT>
-__global__ void __launch_bounds__(ST_THREADS) sample_stats_kernel(SampleParams p) {
-    __shared__ float red_max[ST_THREADS / 32];
-    __shared__ int red_at[ST_THREADS / 32];
-    __shared__ double red_mass[ST_THREADS / 32];
-    __shared__ double exp2_table[64];  // 2^(j / 64)
-    __shared__ uint32_t bin_count[ST_BINS];
-    __shared__ float bin_mass[ST_BINS];
+// Smallest key in [lo, hi] for which the predicate holds (it holds from some key on, for hi at the latest); one warp.
+template <typename F>
+__device__ inline uint32_t first_key(uint32_t lo, uint32_t hi, F holds) {
+    const int lane = threadIdx.x & 31;
+    while (lo < hi) {
+        const uint32_t step = (hi - lo) / 32 + 1;
+        const uint32_t k = lo + step * lane;
+        const bool ok = k >= lo && k <= hi ? holds(k) : true;
+        const uint32_t votes = __ballot_sync(0xffffffffu, ok);
+        if (!votes) {  // none of the 32 samples: it lies behind the last
+            lo = lo + step * 31 + 1;
+            continue;
+        }
+        const int f = __ffs(votes) - 1;
+        const uint32_t at = lo + step * f;
+        if (at <= hi && at >= lo) hi = at;
+        if (f > 0) lo = lo + step * (f - 1) + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
+    extern __shared__ __align__(16) uint8_t row_smem[];
+    RowShared& sh = *(RowShared*)row_smem;
+    cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int slice = blockIdx.x, row = blockIdx.y;
-    const int first = slice * p.slice, count = min(p.slice, p.n - first);
-    if (tid < ST_BINS) bin_count[tid] = 0, bin_mass[tid] = 0.f;
-    if (tid < 64) exp2_table[tid] = exp2((double)tid / 64.0);
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.y;
+    // the slice, cleaned
+    float* x_s = p.scratch ? p.scratch + ((int64_t)row * C + rank) * p.slice : (float*)(row_smem + ((sizeof(RowShared) + 15) & ~(size_t)15));
+    const int first = rank * p.slice, count = max(0, min(p.slice, p.n - first));
+
+    for (int i = tid; i < 4 * SP_BINS; i += SP_THREADS) (&sh.hist[0][0])[i] = 0;
+    if (tid < 64) sh.exp2_table[tid] = exp2((double)tid / 64.0);
+    if (tid == 0) sh.hit.bin = 0xffffffffu, sh.n_list = 0;
     grid_launch_dependents();
     grid_dependency_wait();  // the kernel before has written the logits and the settings
     const RowSettings s = row_settings(p, row);
-    const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
 
-    float x[EPT];
-    int at0, per;  // element e of this thread is at0 + (e / per) * per * ST_THREADS + e % per
-    if (p.vec && p.dtype == B200KV_F32) {
-        per = 4, at0 = tid * 4;
-#pragma unroll
-        for (int e = 0; e < EPT; e += 4) {
-            const int i = at0 + e * ST_THREADS;
-            if (i + 4 <= count) {
+    // ---- 1. the slice into shared memory, its maximum ----
+    float best = -INFINITY;
+    int at = 0x7fffffff;
+    {
+        const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
+        auto take = [&](float v, int i) {  // a thread's indices rise: the first maximum stays
+            v = clean(v);
+            x_s[i] = v;
+            if (v > best) best = v, at = first + i;
+        };
+        int done = 0;
+        if (p.vec && p.dtype == B200KV_F32) {
+            done = count / 4 * 4;
+#pragma unroll 8
+            for (int i = tid * 4; i < done; i += SP_THREADS * 4) {
                 const float4 v = *(const float4*)(base + (int64_t)i * 4);
-                x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) x[e + j] = i + j < count ? ((const float*)base)[i + j] : -INFINITY;
+                take(v.x, i), take(v.y, i + 1), take(v.z, i + 2), take(v.w, i + 3);
             }
-        }
-    } else if (p.vec) {
-        per = 8, at0 = tid * 8;
-#pragma unroll
-        for (int e = 0; e < EPT; e += 8) {
-            const int i = at0 + e * ST_THREADS;
-            if (i + 8 <= count) {
+        } else if (p.vec) {
+            done = count / 8 * 8;
+#pragma unroll 4
+            for (int i = tid * 8; i < done; i += SP_THREADS * 8) {
                 const uint4 v = *(const uint4*)(base + (int64_t)i * 2);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if (p.dtype == B200KV_F16) {
                         const float2 f = __half22float2(*(const __half2*)&w[j]);
-                        x[e + 2 * j] = f.x, x[e + 2 * j + 1] = f.y;
+                        take(f.x, i + 2 * j), take(f.y, i + 2 * j + 1);
                     } else {
-                        x[e + 2 * j] = __uint_as_float(w[j] << 16), x[e + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                        take(__uint_as_float(w[j] << 16), i + 2 * j), take(__uint_as_float(w[j] & 0xffff0000u), i + 2 * j + 1);
                     }
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[e + j] = i + j < count ? ld_as_f32(base, p.dtype, i + j) : -INFINITY;
             }
         }
-    } else {
-        per = 1, at0 = tid;
-#pragma unroll
-        for (int e = 0; e < EPT; e++) {
-            const int i = at0 + e * ST_THREADS;
-            x[e] = i < count ? ld_as_f32(base, p.dtype, i) : -INFINITY;
-        }
+#pragma unroll 8
+        for (int i = done + tid; i < count; i += SP_THREADS) take(ld_as_f32(base, p.dtype, i), i);
     }
-    float best = -INFINITY;
-    int best_e = 0;
-#pragma unroll
-    for (int e = 0; e < EPT; e++) {  // a thread's elements come in rising order of their index
-        x[e] = clean(x[e]);
-        if (x[e] > best) best = x[e], best_e = e;
-    }
-    int at = best > -INFINITY ? first + at0 + (best_e / per) * per * ST_THREADS + best_e % per : 0x7fffffff;
     auto merge = [&](float ov, int oi) {
         if (ov > best || (ov == best && oi < at)) best = ov, at = oi;
     };
@@ -186,503 +220,384 @@ __global__ void __launch_bounds__(ST_THREADS) sample_stats_kernel(SampleParams p
         const int oi = __shfl_xor_sync(0xffffffffu, at, o);
         merge(ov, oi);
     }
-    if (lane == 0) red_max[warp] = best, red_at[warp] = at;
+    if (lane == 0) sh.red_max[warp] = best, sh.red_at[warp] = at;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < ST_THREADS / 32; w++) merge(red_max[w], red_at[w]);
-
-    double mass = 0.0;
-    if (!s.greedy && best > -INFINITY) {
-        if (s.need_mass()) {
-            // exp((x - max) / T) = 2^(t / 64), t = (x - max) * 64 log2 e / T = n + r:  2^(n / 64) from the table and the exponent,
-            // 2^(r / 64) by its Taylor polynomial of degree 4 in r ln 2 / 64 (|r| <= 1/2: the next term is below 4e-14)
-            const double c = 64.0 * 1.4426950408889634074 / (double)s.t, m = (double)best;
-            constexpr double L = 0.69314718055994530942 / 64.0, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
-            double part[2] = {0.0, 0.0};
-#pragma unroll
-            for (int e = 0; e < EPT; e++) {
-                const double t = fmax(((double)x[e] - m) * c, -64.0 * 1000.0);  // below: 2^-1000, nothing beside the maximum's 1
-                const double biased = t + MAGIC, r = t - (biased - MAGIC);
-                const int n = __double2loint(biased);
-                double q = fma(r, L * L * L * L / 24.0, L * L * L / 6.0);
-                q = fma(q, r, L * L / 2.0);
-                q = fma(q, r, L);
-                q = fma(q, r, 1.0);
-                const double tab = exp2_table[n & 63];
-                const double scaled = __hiloint2double(__double2hiint(tab) + ((n >> 6) << 20), __double2loint(tab));
-                part[e & 1] = fma(q, scaled, part[e & 1]);
-            }
-            mass = best == INFINITY ? 0.0 : part[0] + part[1];
-            if (best == INFINITY) {
-#pragma unroll
-                for (int e = 0; e < EPT; e++) mass += x[e] == INFINITY ? 1.0 : 0.0;
-            }
-        }
-        if (s.use_k || s.use_p) {
-            const float c = 1.4426950408889634f / s.t, top = floorf(best * c);
-#pragma unroll
-            for (int e = 0; e < EPT; e += ST_SAMPLE) {
-                if (x[e] > -INFINITY) {
-                    const float z = x[e] * c;
-                    const int j = (int)fmaxf(fminf(top - floorf(z), (float)(ST_BINS - 1)), 0.f);
-                    atomicAdd(&bin_count[j], 1u);
-                    atomicAdd(&bin_mass[j], exp2f(z - top));
-                }
-            }
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-        if (lane == 0) red_mass[warp] = mass;
+    for (int w = 0; w < SP_WARPS; w++) merge(sh.red_max[w], sh.red_at[w]);
+    if (tid < C) {
+        RowShared* other = cluster.map_shared_rank(&sh, tid);
+        other->x_max[rank] = best, other->x_at[rank] = at;
     }
-    __syncthreads();
-    const int64_t slot = (int64_t)row * p.n_slices + slice;
-    if (tid == 0) {
-        double sum = 0.0;
-        if (!s.greedy && best > -INFINITY)
-            for (int w = 0; w < ST_THREADS / 32; w++) sum += red_mass[w];
-        SliceStats st;
-        st.mass = sum, st.max = best, st.at = at;
-        p.stats[slot] = st;
-    }
-    if (tid < ST_BINS && !s.greedy && (s.use_k || s.use_p)) p.bins[slot].count[tid] = bin_count[tid], p.bins[slot].mass[tid] = bin_mass[tid];
-}
-
-// ---- second launch --------------------------------------------------------------------------------------------------------
-// Inclusive sums over the CTA in thread order.
-template <typename T>
-__device__ inline T warp_scan(T v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const T up = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += up;
-    }
-    return v;
-}
-template <typename T>
-__device__ inline T block_scan(T v, T* warp_sums /* [33] */) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    v = warp_scan(v, lane);
-    __syncthreads();  // the sums of the scan before are no longer read
-    if (lane == 31) warp_sums[warp] = v;
-    __syncthreads();
-    T before = T(0);
-    if (warp > 0) {  // every warp adds up the sums before it
-        T mine = lane < warp ? warp_sums[lane] : T(0);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        before = mine;
-    }
-    return before + v;
-}
-
-struct Token {
-    unsigned long long w;
-    uint32_t key;
-    int32_t at;
-};
-struct PickShared {
-    unsigned long long mass[PK_BINS];
-    uint32_t count[PK_BINS];
-    unsigned long long sums64[33];
-    double sums_d[33];
-    uint32_t sums32[33];
-    float max;
-    int32_t at;
-    double total;
-    uint32_t n_list;
-    float bin_count[ST_BINS], bin_mass[ST_BINS];
-    uint32_t hit;                      // bin of a refinement round
-    uint32_t above_n;                  // what lies before that bin
-    unsigned long long above_w;
-    unsigned long long list_mass;
-    int32_t token;
-    float theta;
-};
-
-__global__ void __launch_bounds__(PK_THREADS, 2) sample_pick_kernel(SampleParams p) {
-    extern __shared__ __align__(16) uint8_t pick_smem[];
-    Token* list = (Token*)pick_smem;
-    PickShared& sh = *(PickShared*)(pick_smem + PK_CAP * sizeof(Token));
-    const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x;
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const RowSettings s = row_settings(p, row);
-    const SliceStats* stats = p.stats + (int64_t)row * p.n_slices;
-    const SliceBins* bins = p.bins + (int64_t)row * p.n_slices;
-    const uint8_t* base = (const uint8_t*)p.logits + (int64_t)row * p.stride * dtype_size(p.dtype);
-
-    // ---- the row's maximum and its first index ----
-    if (tid < 32) {
-        float best = -INFINITY;
-        int at = 0x7fffffff;
-        for (int i = lane; i < p.n_slices; i += 32) {
-            const float m = stats[i].max;
-            if (m > best) best = m, at = stats[i].at;  // slices in rising order: the first maximum of this lane
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-            if (ov > best || (ov == best && oi < at)) best = ov, at = oi;
-        }
-        if (lane == 0) sh.max = best, sh.at = best > -INFINITY ? at : 0;  // a row of -inf / NaN only: index 0
-    }
-    if (tid == 0) sh.token = -1, sh.n_list = 0, sh.list_mass = 0;
-    if (tid < ST_BINS) sh.bin_count[tid] = 0.f, sh.bin_mass[tid] = 0.f;
-    __syncthreads();
-    const float max = sh.max;
-    if (s.greedy || max == -INFINITY) {
-        if (tid == 0) p.out[row] = sh.at;
+    cluster.sync();
+    for (int r = 0; r < C; r++) merge(sh.x_max[r], sh.x_at[r]);
+    const float x_top = best;
+    if (s.greedy || x_top == -INFINITY) {  // the same in every CTA; nothing of another CTA is touched any more
+        if (rank == 0 && tid == 0) p.out[row] = x_top == -INFINITY ? 0 : at;
         return;
     }
-    const double t = (double)s.t;
-    const float u = s.u > 0.f ? fminf(s.u, 1.f) : 0.f;
 
-    // ---- the mass of the row, relative to its maximum; without filters also the slice in which the draw falls ----
-    double total = 0.0;
-    if (s.need_mass()) {
-        auto slice_mass = [&](int i) -> double {
-            if (i >= p.n_slices) return 0.0;
-            return stats[i].mass * weight_of(stats[i].max, max, t);
-        };
-        for (int i0 = 0; i0 < p.n_slices; i0 += PK_THREADS) {
-            const double incl = block_scan(slice_mass(i0 + tid), sh.sums_d);
-            if (tid == PK_THREADS - 1) sh.total = incl;
-            __syncthreads();
-            total += sh.total;
+    // ---- weights ----
+    // exp((x - max) / T) = 2^(t / 64), t = (x - max) 64 log2 e / T = n + r, n whole: 2^(n / 64) from the table and the exponent,
+    // 2^(r / 64) by its Taylor polynomial of degree 4 in r ln 2 / 64 (|r| <= 1/2: what is left out is below 4e-14), rounded to 44
+    // fractional bits by adding 1.5 * 2^8.  Below 2^-46: 0.  An infinite maximum shares the row among the infinite logits.
+    const double t64 = 64.0 * 1.4426950408889634074 / (double)s.t;
+    auto weight = [&](float x) -> u64 {
+        if (x == x_top) return 1ull << W_BITS;
+        const double t = ((double)x - (double)x_top) * t64;
+        if (!(t > -64.0 * 46.0)) return 0ull;
+        constexpr double L = 0.69314718055994530942 / 64.0, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
+        const double biased = t + MAGIC, r = t - (biased - MAGIC);
+        const int n = __double2loint(biased);
+        double q = fma(r, L * L * L * L / 24.0, L * L * L / 6.0);
+        q = fma(q, r, L * L / 2.0);
+        q = fma(q, r, L);
+        q = fma(q, r, 1.0);
+        const double tab = sh.exp2_table[n & 63];
+        const double scaled = __hiloint2double(__double2hiint(tab) + ((n >> 6) << 20), __double2loint(tab));
+        return (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
+    };
+    // bins of log2 w, 46 octaves deep; monotone in x, the deepest takes everything below
+    const float zscale = 1.4426950408889634f / s.t * ((float)(SP_BINS - 1) / 46.f);
+    auto z_bin = [&](float x) -> uint32_t { return x == x_top ? 0u : (uint32_t)fminf((x_top - x) * zscale, (float)(SP_BINS - 1)); };
+    // min-p: the smallest bit pattern that passes
+    const uint32_t key_max = key_of(x_top);
+    uint32_t key_m = KEY_NEG_INF + 1;
+    if (s.use_m) {
+        if (warp == 0) {
+            const uint32_t k = first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t key) {
+                return key == key_max || (x_top != INFINITY && exp(((double)of_key(key) - (double)x_top) / (double)s.t) >= (double)s.min_p);
+            });
+            if (lane == 0) sh.found = k;
         }
-        if (!s.use_p && !s.use_m) {
-            double target = (double)u * total, before = 0.0;
-            for (int i0 = 0; i0 < p.n_slices; i0 += PK_THREADS) {
-                const double mine = slice_mass(i0 + tid), incl = block_scan(mine, sh.sums_d) + before;
-                // several may pass where rounding makes the sums meet: the first one is taken
-                if (mine > 0.0 && incl > target) atomicMin((unsigned int*)&sh.token, (unsigned)(i0 + tid));  // -1 is the largest
-                if (tid == PK_THREADS - 1) sh.total = incl;
-                __syncthreads();
-                before = sh.total;
-                if (sh.token >= 0) break;
-            }
-            int slice = sh.token;
-            __syncthreads();
-            if (slice < 0) {  // the draw is past the last sum by a rounding: the last slice that has mass
-                for (int i = tid; i < p.n_slices; i += PK_THREADS)
-                    if (stats[i].mass > 0.0 && weight_of(stats[i].max, max, t) > 0.0) atomicMax(&sh.token, i);
-                __syncthreads();
-                slice = sh.token;
-            }
-            // what lies before the slice, added up in the same order as above
-            double prior = 0.0;
-            for (int i0 = 0; i0 <= slice; i0 += PK_THREADS) {
-                const double incl = block_scan(i0 + tid < slice ? slice_mass(i0 + tid) : 0.0, sh.sums_d);
-                if (tid == PK_THREADS - 1) sh.total = incl;
-                __syncthreads();
-                prior += sh.total;
-            }
-            target -= prior;
-            if (tid == 0) sh.token = -1;
-            // the token: every thread adds up a run of the slice
-            const int first = slice * p.slice, count = min(p.slice, p.n - first), per = (count + PK_THREADS - 1) / PK_THREADS;
-            double mine = 0.0;
-            for (int e = 0; e < per; e++) {
-                const int i = tid * per + e;
-                if (i < count) mine += weight_of(load_logit(p, base, first + i), max, t);
-            }
-            const double incl = block_scan(mine, sh.sums_d);
-            double run = incl - mine;
-            if (mine > 0.0 && incl > target) {
-                int pick = 0x7fffffff, last = 0x7fffffff;
-                for (int e = 0; e < per; e++) {
-                    const int i = tid * per + e;
-                    if (i >= count) break;
-                    const double w = weight_of(load_logit(p, base, first + i), max, t);
-                    run += w;
-                    if (w > 0.0) last = first + i;
-                    if (w > 0.0 && run > target) {
-                        pick = first + i;
-                        break;
-                    }
+        __syncthreads();
+        key_m = sh.found;
+    }
+
+    // ---- a histogram over the cluster, and the bin in which the running count or mass first exceeds its goal ----
+    // bin_of(x, index): 0 .. SP_BINS - 1, or -1 for what does not take part.  goal(all): from the whole count or mass.
+    // *_base: what lies before the first bin.
+    auto round_of = [&](bool by_weight, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
+        for (int i = tid; i < count; i += SP_THREADS) {
+            const float x = x_s[i];
+            const int b = bin_of(x, first + i);
+            if (b < 0) continue;
+            atomicAdd(&sh.hist[0][b], 1u);
+            if (by_weight) {
+                const u64 w = weight(x);
+                if (w) {
+                    atomicAdd(&sh.hist[1][b], (uint32_t)w & 0x7fffu);
+                    atomicAdd(&sh.hist[2][b], (uint32_t)(w >> SP_LIMB) & 0x7fffu);
+                    atomicAdd(&sh.hist[3][b], (uint32_t)(w >> (2 * SP_LIMB)));
                 }
-                atomicMin((unsigned int*)&sh.token, (unsigned)(pick != 0x7fffffff ? pick : last));
             }
-            __syncthreads();
-            int token = sh.token;
-            if (token < 0) {  // past the slice's last sum by a rounding: its last token that has weight
-                for (int i = tid; i < count; i += PK_THREADS)
-                    if (weight_of(load_logit(p, base, first + i), max, t) > 0.0) atomicMax(&sh.token, first + i);
+        }
+        cluster.sync();
+        // this CTA's share of the bins, added up over the cluster; a thread has one bin, or two neighbours (a cluster of one)
+        const int share = SP_BINS / C, per = share > SP_THREADS ? share / SP_THREADS : 1, b0 = rank * share + tid * per;
+        uint32_t n[2] = {0, 0};
+        u64 w[2] = {0, 0};
+        if (tid * per < share) {
+            for (int r = 0; r < C; r++) {
+                const RowShared* other = cluster.map_shared_rank(&sh, r);
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    if (j < per) {
+                        n[j] += other->hist[0][b0 + j];
+                        if (by_weight)
+                            w[j] += (u64)other->hist[1][b0 + j] + ((u64)other->hist[2][b0 + j] << SP_LIMB) + ((u64)other->hist[3][b0 + j] << (2 * SP_LIMB));
+                    }
+            }
+        }
+        uint32_t n_incl = block_scan(n[0] + n[1], sh.sums32);
+        u64 w_incl = by_weight ? block_scan(w[0] + w[1], sh.sums64) : 0ull;
+        if (tid == SP_THREADS - 1) {
+            for (int r = 0; r < C; r++) {
+                RowShared* other = cluster.map_shared_rank(&sh, r);
+                other->x_n[rank] = n_incl, other->x_w[rank] = w_incl;
+            }
+        }
+        cluster.sync();  // every share is known, and nobody reads the histogram any more
+        for (int i = tid; i < (by_weight ? 4 : 1) * SP_BINS; i += SP_THREADS) (&sh.hist[0][0])[i] = 0;
+        u64 all = 0;
+        uint32_t n_low = n_base;
+        u64 w_low = w_base;
+        for (int r = 0; r < C; r++) {
+            all += by_weight ? sh.x_w[r] : (u64)sh.x_n[r];
+            if (r < rank) n_low += sh.x_n[r], w_low += sh.x_w[r];
+        }
+        const u64 target = goal(all);
+        uint32_t n_at = n_low + n_incl - (n[0] + n[1]);
+        u64 w_at = w_low + w_incl - (w[0] + w[1]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const u64 from = by_weight ? w_at : (u64)n_at, to = by_weight ? w_at + w[j] : (u64)(n_at + n[j]);
+            if (from <= target && to > target)
+                for (int r = 0; r < C; r++) cluster.map_shared_rank(&sh, r)->hit = Hit{(uint32_t)(b0 + j), n_at, n[j], w_at, w[j]};
+            n_at += n[j], w_at += w[j];
+        }
+        cluster.sync();
+        const Hit h = sh.hit;
+        __syncthreads();
+        if (tid == 0) sh.hit.bin = 0xffffffffu;  // before the next round's first cluster barrier, behind which others may write it
+        return h;
+    };
+    // The same over positions lo .. hi, 1024 at a time, down to a single one; bin holds the position.
+    auto refine = [&](bool by_weight, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
+        for (;;) {
+            const int bits = 32 - __clz((hi - lo) | 1u), shift = bits > 10 ? bits - 10 : 0;
+            Hit h = round_of(by_weight, n_base, w_base, [&](float x, int i) -> int {
+                uint32_t at;
+                return place(x, i, &at) && at >= lo && at <= hi ? (int)((at - lo) >> shift) : -1;
+            }, [&](u64) { return target; });
+            if (h.bin == 0xffffffffu) return h;
+            h.bin = lo + (h.bin << shift);
+            if (shift == 0) return h;
+            lo = h.bin, hi = min(hi, lo + ((1u << shift) - 1u));
+            n_base = h.n_before, w_base = h.w_before;
+        }
+    };
+
+    // ---- 2. the cut: everything above key_cut, and the first ones (up to index last_same) of those that equal it ----
+    uint32_t key_cut = KEY_NEG_INF + 1, last_same = 0xffffffffu;
+    if (s.use_k || s.use_p) {
+        u64 whole = 0;  // of the row (top-p without top-k)
+        auto p_goal = [&](u64 mass) -> u64 {  // the mass before a kept token is below p x mass: the cut is where the sum reaches it
+            const u64 least = (u64)ceil((double)s.p * (double)mass);
+            return least ? least - 1 : 0;
+        };
+        const Hit top = round_of(!s.use_k, 0, 0, [&](float x, int) -> int { return x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
+            whole = all;
+            return s.use_k ? (u64)(s.k - 1) : p_goal(all);
+        });
+        // ---- 3. few enough tokens above the lower border of that bin: sort them ----
+        const uint32_t n_list = top.bin == 0xffffffffu ? (s.use_k ? (uint32_t)whole : 0xffffffffu) : top.n_before + top.n_here;
+        if (n_list <= SP_LIST) {
+            RowShared* head = cluster.map_shared_rank(&sh, 0);
+            for (int i0 = 0; i0 < count; i0 += SP_THREADS) {
+                const int i = i0 + tid;
+                const float x = i < count ? x_s[i] : -INFINITY;
+                const bool take = x > -INFINITY && z_bin(x) <= top.bin;
+                const uint32_t vote = __ballot_sync(0xffffffffu, take);
+                if (!vote) continue;
+                uint32_t slot = 0;
+                if (lane == 0) slot = atomicAdd(&head->n_list, (uint32_t)__popc(vote));
+                slot = __shfl_sync(0xffffffffu, slot, 0) + (uint32_t)__popc(vote & ((1u << lane) - 1u));
+                if (take) head->list[slot] = ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i);
+            }
+            cluster.sync();
+            if (rank != 0) return;
+            int size = 2;
+            while (size < (int)n_list) size <<= 1;
+            // bitonic sort of list[0 .. size): every step, a thread per pair
+            auto sort = [&](int size) {
+                for (int k = 2; k <= size; k <<= 1)
+                    for (int j = k >> 1; j; j >>= 1) {
+                        __syncthreads();
+                        if (tid < size / 2) {
+                            const int a = 2 * tid - (tid & (j - 1)), b = a + j;
+                            const u64 va = sh.list[a], vb = sh.list[b];
+                            if ((va > vb) == ((a & k) == 0)) sh.list[a] = vb, sh.list[b] = va;
+                        }
+                    }
                 __syncthreads();
-                token = sh.token;
+            };
+            for (int i = (int)n_list + tid; i < size; i += SP_THREADS) sh.list[i] = ~0ull;
+            sort(size);  // falling logits, equal ones by rising index
+            // thread tid has places 2 tid and 2 tid + 1
+            const int e0 = 2 * tid;
+            u64 tok[2];
+            u64 w[2];
+            bool passes[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                tok[j] = e0 + j < (int)n_list ? sh.list[e0 + j] : ~0ull;
+                const uint32_t key = ~(uint32_t)(tok[j] >> 32);
+                w[j] = e0 + j < (int)n_list ? weight(of_key(key)) : 0ull;
+                passes[j] = e0 + j < (int)n_list && (!s.use_k || e0 + j < s.k);
+                if (!passes[j]) w[j] = 0;
             }
-            if (tid == 0) p.out[row] = token;
+            u64 incl = block_scan(w[0] + w[1], sh.sums64);
+            if (tid == SP_THREADS - 1) sh.x_w[0] = incl;
+            __syncthreads();
+            const u64 goal = s.use_p ? p_goal(s.use_k ? sh.x_w[0] : whole) : ~0ull;
+            u64 before = incl - (w[0] + w[1]);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                passes[j] = passes[j] && (before <= goal) && (~(uint32_t)(tok[j] >> 32) >= key_m || e0 + j == 0);
+                before += w[j];
+            }
+            // the kept ones by rising index, each with its place in the order of weights (their weights stay where they can be found)
+            const uint32_t n_kept = (uint32_t)__syncthreads_count(passes[0]) + (uint32_t)__syncthreads_count(passes[1]);
+            u64* weights = (u64*)&sh.hist[0][0];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (passes[j]) {
+                    weights[e0 + j] = w[j];
+                    sh.list[e0 + j] = (tok[j] << 32) | (u64)(uint32_t)(e0 + j);
+                }
+            int kept_size = 2;
+            while (kept_size < (int)n_kept) kept_size <<= 1;
+            __syncthreads();
+            for (int i = (int)n_kept + tid; i < kept_size; i += SP_THREADS) sh.list[i] = ~0ull;
+            sort(kept_size);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                tok[j] = e0 + j < (int)n_kept ? sh.list[e0 + j] : ~0ull;
+                w[j] = e0 + j < (int)n_kept ? weights[(uint32_t)tok[j]] : 0ull;
+            }
+            incl = block_scan(w[0] + w[1], sh.sums64);
+            if (tid == SP_THREADS - 1) sh.x_w[0] = incl;
+            __syncthreads();
+            const u64 mass = sh.x_w[0], target = min((u64)((double)s.u * (double)mass), mass - 1);
+            before = incl - (w[0] + w[1]);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (before <= target && before + w[j] > target) p.out[row] = (int32_t)(tok[j] >> 32);
+                before += w[j];
+            }
             return;
         }
-    }
-
-    // ---- how deep the filters reach ----
-    const float c = 1.4426950408889634f / s.t, top = floorf(max * c);
-    uint32_t key_m = KEY_NEG_INF + 1;  // min-p: the smallest bit pattern that passes
-    if (s.use_m) {
-        if (tid == 0) {
-            // x = max + T ln(min_p) up to rounding, then the neighbours: w is monotone in x
-            const float guess = max == INFINITY ? max : (float)((double)max + t * log((double)s.min_p));
-            uint32_t k = std::max(KEY_NEG_INF + 1, std::min(key_of(clean(guess)), key_of(max)));
-            for (int i = 0; i < 4096 && k > KEY_NEG_INF + 1 && weight_of(of_key(k - 1), max, t) >= (double)s.min_p; i++) k--;
-            for (int i = 0; i < 4096 && k < key_of(max) && !(weight_of(of_key(k), max, t) >= (double)s.min_p); i++) k++;
-            sh.hit = k;
-        }
-        __syncthreads();
-        key_m = sh.hit;
-    }
-    if (s.use_k || s.use_p) {
-        for (int i = tid; i < p.n_slices * ST_BINS; i += PK_THREADS) {
-            const int sl = i / ST_BINS;
-            const uint32_t n = bins[sl].count[i % ST_BINS];
-            if (!n) continue;
-            const float lower = top - floorf(stats[sl].max * c);
-            const int j = (int)fmaxf(fminf((float)(i % ST_BINS) + lower, (float)(ST_BINS - 1)), 0.f);
-            atomicAdd(&sh.bin_count[j], (float)n);
-            atomicAdd(&sh.bin_mass[j], bins[sl].mass[i % ST_BINS] * exp2f(-lower));
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int j = ST_BINS - 1;  // the last octave to gather; the last bin of all: everything
-            if (s.use_k) {
-                float n = 0.f;
-                for (int b = 0; b < ST_BINS - 1; b++) {
-                    n += sh.bin_count[b] * ST_SAMPLE;
-                    if (n >= 1.5f * (float)s.k + 100.f) {
-                        j = b;
-                        break;
-                    }
-                }
-            } else {
-                const float allowed = 0.7f * (1.f - s.p) * (float)total * exp2f(max * c - top);
-                float tail = 0.f;
-                for (int b = ST_BINS - 1; b > 0; b--) {
-                    tail += sh.bin_mass[b] * ST_SAMPLE;
-                    if (!(tail <= allowed)) break;
-                    j = b - 1;
-                }
-            }
-            const float theta = (top - (float)j) / c;
-            sh.theta = j == ST_BINS - 1 || !(theta < max) ? -INFINITY : theta;
-        }
-        __syncthreads();
-    }
-    uint32_t theta = s.use_k || s.use_p ? std::max(key_of(clean(sh.theta)), KEY_NEG_INF + 1) : KEY_NEG_INF + 1;
-    if (s.use_m && !s.use_k) theta = std::max(theta, key_m);  // nothing below passes min-p, and no mass below is asked for one by one
-
-    // ---- gather ----
-    const double unit = (double)(1ull << W_BITS);
-    const unsigned long long reach = s.use_p && !s.use_k ? (unsigned long long)ceil((double)s.p * total * unit) : 0ull;
-    bool in_list;
-    uint32_t n_list;
-    for (;;) {
-        const float theta_x = of_key(theta);
-        const int per_chunk = PK_CHUNK / p.slice;  // slices, of 2048 or 8192 logits, in a chunk
-        for (int chunk = 0; chunk * PK_CHUNK < p.n; chunk++) {
-            bool any = false;
-            for (int sl = chunk * per_chunk; sl < min((chunk + 1) * per_chunk, p.n_slices); sl++) any |= stats[sl].max >= theta_x;
-            if (!any) continue;
-            float x[PK_CHUNK / PK_THREADS];  // all of them in flight
-#pragma unroll
-            for (int e = 0; e < PK_CHUNK / PK_THREADS; e++) {
-                const int i = chunk * PK_CHUNK + e * PK_THREADS + tid;
-                x[e] = i < p.n ? load_logit(p, base, i) : -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < PK_CHUNK / PK_THREADS; e++) {
-                const bool take = x[e] >= theta_x;
-                const uint32_t vote = __ballot_sync(0xffffffffu, take);
-                if (vote) {
-                    uint32_t at = 0;
-                    if (lane == 0) at = atomicAdd(&sh.n_list, (uint32_t)__popc(vote));
-                    at = __shfl_sync(0xffffffffu, at, 0) + (uint32_t)__popc(vote & ((1u << lane) - 1u));
-                    if (take && at < PK_CAP) list[at] = {0ull, key_of(x[e]), chunk * PK_CHUNK + e * PK_THREADS + tid};
-                }
-            }
-        }
-        __syncthreads();
-        n_list = sh.n_list;
-        in_list = n_list <= PK_CAP;
-        if (in_list) {
-            unsigned long long mine = 0;
-            for (uint32_t i = tid; i < n_list; i += PK_THREADS) {
-                const unsigned long long w = fixed_weight(of_key(list[i].key), max, t);
-                list[i].w = w;
-                mine += w;
-            }
-            atomicAdd(&sh.list_mass, mine);
-        }
-        __syncthreads();
-        const unsigned long long list_mass = sh.list_mass;
-        // does the cut lie among the gathered ones?
-        const bool covered = theta <= KEY_NEG_INF + 1 || !in_list || (s.use_k ? n_list >= (uint32_t)s.k : !s.use_p || list_mass >= reach || (s.use_m && theta == key_m));
-        __syncthreads();
-        if (covered) break;
-        theta = s.use_m && !s.use_k ? key_m : KEY_NEG_INF + 1;
-        if (tid == 0) sh.n_list = 0, sh.list_mass = 0;
-        __syncthreads();
-    }
-    // f(key, index, weight) for every gathered token: from the list, or from the row
-    auto for_each = [&](auto f) {
-        if (in_list) {
-            for (uint32_t i = tid; i < n_list; i += PK_THREADS) f(list[i].key, list[i].at, list[i].w);
-        } else {
-            for (int i = tid; i < p.n; i += PK_THREADS) {
-                const float x = load_logit(p, base, i);
-                const uint32_t key = key_of(x);
-                if (key >= theta) f(key, i, fixed_weight(x, max, t));
-            }
-        }
-    };
-    // One refinement: of the tokens that `part` admits, `place` gives the position on an axis, [lo, hi].  Finds the position at
-    // which the sum (of weights, or of ones) first exceeds `target`, and what lies before it; hi + 1 if it never does.
-    struct Found {
-        uint32_t at, n;
-        unsigned long long w;
-        uint32_t n_here;
-        unsigned long long w_here;
-    };
-    auto refine = [&](uint32_t lo, uint32_t hi, unsigned long long target, bool by_weight, auto place, auto part) -> Found {
-        Found r{hi, 0, 0, 0, 0};
-        const uint32_t end = hi;
-        uint32_t n_before = 0;
-        unsigned long long w_before = 0;
-        for (;;) {
-            const uint32_t range = hi - lo;
-            const int bits = 32 - __clz(range | 1u), shift = bits > 10 ? bits - 10 : 0;
-            sh.count[tid] = 0, sh.mass[tid] = 0;
-            if (tid == 0) sh.hit = 0xffffffffu;
+        // many tokens: down to the last kept one
+        auto by_rank = [&](float x, int, uint32_t* at) {  // positions rise as logits fall
+            *at = key_max - key_of(x);
+            return x > -INFINITY;
+        };
+        // the bit patterns of a bin of log2 w
+        auto keys_of_bin = [&](uint32_t bin) {
             __syncthreads();
-            for_each([&](uint32_t key, int32_t at, unsigned long long w) {
-                const uint32_t x = place(key, at);
-                if (x < lo || x > hi || !part(key, at)) return;
-                const uint32_t b = (x - lo) >> shift;
-                atomicAdd(&sh.count[b], 1u);
-                if (w) atomicAdd(&sh.mass[b], w);
-            });
-            __syncthreads();
-            const uint32_t n = sh.count[tid];
-            const unsigned long long w = sh.mass[tid];
-            const unsigned long long w_incl = block_scan(w, sh.sums64) + w_before;
-            const uint32_t n_incl = block_scan(n, sh.sums32) + n_before;
-            const unsigned long long incl = by_weight ? w_incl : (unsigned long long)n_incl;
-            const unsigned long long excl = by_weight ? w_incl - w : (unsigned long long)(n_incl - n);
-            if (excl <= target && incl > target) sh.hit = (uint32_t)tid, sh.above_n = n_incl - n, sh.above_w = w_incl - w;
-            __syncthreads();
-            const uint32_t hit = sh.hit;
-            if (hit == 0xffffffffu) {
-                __syncthreads();
-                return Found{end + 1, 0, 0, 0, 0};
+            if (warp == 0) {
+                const uint32_t lo = first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t k) { return z_bin(of_key(k)) <= bin; });
+                if (lane == 0) sh.key_lo = lo;
+            } else if (warp == 1) {
+                const uint32_t hi = bin == 0 ? key_max + 1 : first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t k) { return z_bin(of_key(k)) < bin; });
+                if (lane == 0) sh.key_hi = hi - 1;
             }
-            n_before = sh.above_n, w_before = sh.above_w;
-            r.at = lo + (hit << shift), r.n = n_before, r.w = w_before, r.n_here = sh.count[hit], r.w_here = sh.mass[hit];
             __syncthreads();
-            if (shift == 0) return r;
-            hi = std::min(hi, r.at + ((1u << shift) - 1u));
-            lo = r.at;
+        };
+        uint32_t n_cut = 0xffffffffu, n_same = 0xffffffffu;
+        Hit hit = top;
+        if (s.use_k && hit.bin != 0xffffffffu) {
+            keys_of_bin(hit.bin);
+            const Hit f = refine(false, key_max - sh.key_hi, key_max - sh.key_lo, hit.n_before, 0, by_rank, (u64)(s.k - 1));
+            key_cut = key_max - f.bin, n_cut = (uint32_t)s.k - f.n_before, n_same = f.n_here;
         }
-    };
-    // ---- the cut: everything above key_cut, and the first n_cut tokens (by index) of those that equal it ----
-    const uint32_t key_max = key_of(max);
-    auto by_rank = [&](uint32_t key, int32_t) { return key_max - key; };  // positions rise as logits fall
-    auto all = [](uint32_t, int32_t) { return true; };
-    uint32_t key_cut = theta, n_cut = 0xffffffffu, n_same = 0xffffffffu;
-    unsigned long long mass_k = 0;
-    if (s.use_k) {
-        const Found f = refine(0, key_max - theta, (unsigned long long)(s.k - 1), false, by_rank, all);
-        if (f.at <= key_max - theta) {
-            key_cut = key_max - f.at, n_cut = (uint32_t)s.k - f.n, n_same = f.n_here;
-            mass_k = f.w + (unsigned long long)n_cut * (f.w_here / f.n_here);
-        } else {
-            // fewer tokens than k: all of them
-            for_each([&](uint32_t, int32_t, unsigned long long w) { mass_k += w; });
-            mass_k = block_scan(mass_k, sh.sums64);
-            if (tid == PK_THREADS - 1) sh.above_w = mass_k;
-            __syncthreads();
-            mass_k = sh.above_w;
-            __syncthreads();
-        }
-    }
-    if (s.use_p) {
-        const double whole = s.use_k ? (double)mass_k : total * unit;
-        const double goal = (double)s.p * whole;  // kept while the mass before is below it: cut at the first sum >= goal
-        const unsigned long long least = (unsigned long long)ceil(goal);
-        const Found f = refine(0, key_max - key_cut, least ? least - 1 : 0, true, by_rank, all);
-        if (f.at <= key_max - key_cut) {
-            const unsigned long long w = f.w_here / f.n_here, missing = least > f.w ? least - f.w : 1;
-            const unsigned long long need = w ? (missing + w - 1) / w : 1;
-            const uint32_t n = (uint32_t)std::min<unsigned long long>(std::max<unsigned long long>(need, 1), f.n_here);
-            const uint32_t key = key_max - f.at;
+        if (s.use_p) {
+            if (s.use_k) {  // the mass of the first k: of everything down to key_cut, without the equal ones that are left out
+                const u64 over = n_same == 0xffffffffu ? 0ull : (u64)(n_same - n_cut) * weight(of_key(key_cut));
+                hit = round_of(true, 0, 0, [&](float x, int) -> int { return key_of(x) >= key_cut ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
+                    whole = all - over;
+                    return p_goal(whole);
+                });
+            }
+            keys_of_bin(hit.bin);
+            const u64 goal = p_goal(whole);
+            const Hit f = refine(true, key_max - sh.key_hi, key_max - max(sh.key_lo, key_cut), hit.n_before, hit.w_before, by_rank, goal);
+            const u64 w = f.w_here / f.n_here;  // all of them have the same weight, which is not 0
+            const uint32_t n = (uint32_t)min((goal + 1 - f.w_before + w - 1) / w, (u64)f.n_here), key = key_max - f.bin;
             if (key > key_cut || n < n_cut) key_cut = key, n_cut = n, n_same = f.n_here;
         }
+        if (s.use_m && key_m > key_cut) key_cut = key_m, n_cut = n_same = 0xffffffffu;
+        if (n_cut < n_same)  // equal logits: the first n_cut by index
+            last_same = refine(false, 0, (uint32_t)p.n - 1, 0, 0, [&](float x, int i, uint32_t* at) {
+                *at = (uint32_t)i;
+                return key_of(x) == key_cut;
+            }, (u64)(n_cut - 1)).bin;
+    } else {
+        key_cut = key_m;
     }
-    if (s.use_m && key_m > key_cut) key_cut = key_m, n_cut = n_same = 0xffffffffu;
-    // ---- the last index among the equal ones that is kept ----
-    uint32_t last_same = 0xffffffffu;
-    if (n_cut < n_same) {
-        const Found f = refine(0, (uint32_t)p.n - 1, (unsigned long long)(n_cut - 1), false, [](uint32_t, int32_t at) { return (uint32_t)at; },
-                               [&](uint32_t key, int32_t) { return key == key_cut; });
-        last_same = f.at;
+
+    // ---- 4. the draw: a run of the slice per warp, the slices over the cluster ----
+    auto kept_weight = [&](int i) -> u64 {
+        const float x = x_s[i];
+        const uint32_t key = key_of(x);
+        return key > key_cut || (key == key_cut && (uint32_t)(first + i) <= last_same) ? weight(x) : 0ull;
+    };
+    const int run = ((count + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;
+    u64 mine = 0;
+    for (int i = warp * run + lane; i < min(count, (warp + 1) * run); i += 32) mine += kept_weight(i);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sh.warp_w[warp] = mine;
+    __syncthreads();
+    u64 of_slice = 0;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) of_slice += sh.warp_w[w];
+    if (tid < C) cluster.map_shared_rank(&sh, tid)->x_w[rank] = of_slice;
+    cluster.sync();
+    u64 mass = 0, before = 0;
+    for (int r = 0; r < C; r++) {
+        if (r == rank) before = mass;
+        mass += sh.x_w[r];
     }
-    auto kept = [&](uint32_t key, int32_t at) { return key > key_cut || (key == key_cut && (uint32_t)at <= last_same); };
-    // ---- the draw ----
-    unsigned long long mass = 0;
-    for_each([&](uint32_t key, int32_t at, unsigned long long w) {
-        if (kept(key, at)) mass += w;
-    });
-    mass = block_scan(mass, sh.sums64);
-    if (tid == PK_THREADS - 1) sh.above_w = mass;
-    __syncthreads();
-    mass = sh.above_w;
-    __syncthreads();
-    const unsigned long long target = std::min((unsigned long long)((double)u * (double)mass), mass - 1);
-    const Found f = refine(0, (uint32_t)p.n - 1, target, true, [](uint32_t, int32_t at) { return (uint32_t)at; }, kept);
-    if (tid == 0) p.out[row] = (int32_t)f.at;
+    const u64 target = min((u64)((double)s.u * (double)mass), mass - 1);
+    if (target < before || target >= before + of_slice) return;
+    int w = 0;
+    for (; w < SP_WARPS - 1 && target >= before + sh.warp_w[w]; w++) before += sh.warp_w[w];
+    const int lo = w * run, hi = min(count, lo + run), per = (hi - lo + SP_THREADS - 1) / SP_THREADS;
+    mine = 0;
+    for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(i);
+    before += block_scan(mine, sh.sums64) - mine;
+    if (before <= target && target < before + mine)
+        for (int i = lo + tid * per;; i++) {
+            before += kept_weight(i);
+            if (target < before) {
+                p.out[row] = first + i;
+                break;
+            }
+        }
 }
 
-// Slices of 8 logits per thread where a launch would otherwise leave SMs without work (a row of 128256 logits is then 63
-// CTAs instead of 16), of 32 otherwise: fewer slices to merge and more loads in flight per thread.
-static int slice_elements(int64_t rows, int32_t n) {
-    const int64_t wide = ST_THREADS * 32;
-    return rows * ((n + wide - 1) / wide) >= 4 * 148 ? (int)wide : ST_THREADS * 8;
+// CTAs per row: as many as the slices need, and while a launch would leave SMs empty, up to eight (of at least 1024 logits each)
+static int sample_slice(int c, int32_t n);
+static int sample_cluster(int64_t rows, int32_t n) {
+    int c = 1;
+    while (c < SP_CLUSTER && n > c * SP_SLICE) c *= 2;
+    while (c < SP_CLUSTER && rows * c <= 148 && n >= 2 * c * 1024) c *= 2;
+    return c;
 }
+// logits per CTA: the next slice starts on a 16-byte boundary when the row does
+static int sample_slice(int c, int32_t n) { return ((n + c - 1) / c + 7) / 8 * 8; }
 
 }  // namespace b200kv
 
 using namespace b200kv;
 
 extern "C" int64_t b200kv_sample_scratch_bytes(int64_t rows, int32_t n) {
-    if (rows <= 0 || n <= 0) {
-        fail("rows and n must be positive");
+    if (rows <= 0 || n <= 0 || n > MAX_VOCAB) {
+        fail("rows and n must be positive, n at most %d", MAX_VOCAB);
         return -1;
     }
-    const int64_t slice = ST_THREADS * 8;  // the finer cut needs more
-    return rows * ((n + slice - 1) / slice) * (int64_t)(sizeof(SliceStats) + sizeof(SliceBins));
+    return n <= MAX_ON_CHIP ? 0 : rows * SP_CLUSTER * (int64_t)sample_slice(SP_CLUSTER, n) * (int64_t)sizeof(float);
 }
 
 extern "C" int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, int64_t rows, int32_t n, const float* temperature,
                              const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* out, void* scratch,
                              void* stream_) {
-    if (!logits || !uniform || !out || !scratch) return fail("null tensor");
+    if (!logits || !uniform || !out) return fail("null tensor");
     if (rows <= 0 || n <= 0) return fail("rows and n must be positive");
     if (rows > 65535) return fail("%lld rows in one call: at most 65535", (long long)rows);
     if (n > MAX_VOCAB) return fail("a vocabulary of %d tokens: at most %d", n, MAX_VOCAB);
     if (dtype < B200KV_F32 || dtype > B200KV_BF16) return fail("unknown dtype %d", dtype);
     if (stride < n && rows > 1) return fail("rows of %d logits cannot be %lld elements apart", n, (long long)stride);
+    if (n > MAX_ON_CHIP && !scratch) return fail("rows of %d logits need a workspace: b200kv_sample_scratch_bytes", n);
     if ((uintptr_t)scratch % 16) return fail("scratch must be 16-byte aligned");
-    cudaStream_t stream = (cudaStream_t)stream_;
     SampleParams p{};
     p.logits = logits, p.stride = stride, p.dtype = dtype, p.n = n;
-    p.slice = slice_elements(rows, n), p.n_slices = (n + p.slice - 1) / p.slice;
     p.temperature = temperature, p.top_k = top_k, p.top_p = top_p, p.min_p = min_p, p.uniform = uniform, p.out = out;
-    p.stats = (SliceStats*)scratch, p.bins = (SliceBins*)(p.stats + rows * p.n_slices);
-    p.vec = (uintptr_t)logits % 16 == 0 && (stride * dtype_size(dtype)) % 16 == 0;
-    const dim3 grid((unsigned)p.n_slices, (unsigned)rows);
-    if (p.slice == ST_THREADS * 32) B200KV_CUDA(launch_after_predecessor(sample_stats_kernel<32>, grid, dim3(ST_THREADS), 0, stream, p));
-    else B200KV_CUDA(launch_after_predecessor(sample_stats_kernel<8>, grid, dim3(ST_THREADS), 0, stream, p));
-    constexpr size_t smem = PK_CAP * sizeof(Token) + sizeof(PickShared);
-    B200KV_CUDA(cudaFuncSetAttribute(sample_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    B200KV_CUDA(launch_after_predecessor(sample_pick_kernel, dim3((unsigned)rows), dim3(PK_THREADS), smem, stream, p));
+    p.vec = (uintptr_t)logits % 16 == 0 && (rows == 1 || (stride * dtype_size(dtype)) % 16 == 0);
+    const int c = sample_cluster(rows, n);
+    p.slice = sample_slice(c, n);
+    p.scratch = n > MAX_ON_CHIP ? (float*)scratch : nullptr;
+    const size_t smem = ((sizeof(RowShared) + 15) & ~(size_t)15) + (p.scratch ? 0 : (size_t)p.slice * sizeof(float));
+    B200KV_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)c, (unsigned)rows), cfg.blockDim = dim3(SP_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream_;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 2;
+    B200KV_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel, p));
     return B200KV_OK;
 }
