@@ -13,11 +13,13 @@
 // One launch, one thread-block cluster per row, the row split over the shared memories of its CTAs: the logits are read from
 // HBM once, and everything else happens on chip.
 //   1. load, maximum (one exchange over the cluster).  A greedy row ends here.
-//   2. the cut of top-k / top-p: a histogram over 1024 bins of log2 w (counts, and for top-p masses); every CTA adds up an
-//      equal share of the bins over the cluster, and the bin in which the count or mass is reached is found from the shares' totals.
-//   3. where at most 1024 tokens lie above the lower border of that bin -- nearly always -- the first CTA gathers and sorts
-//      them, applies all filters and draws.  Otherwise the bin is refined, by the same histogram over the bit patterns in it,
-//      until the last kept token is known.
+//   2. the cut of top-k / top-p: a histogram over 1024 bins of log2 w (counts, and for top-p masses).  The CTAs exchange the
+//      sums of 32 runs of 32 bins; then each finds the run in which the count or mass is reached and reads that run's bins
+//      from the others: one cluster barrier for the whole search.
+//   3. at most 1024 tokens down to the lower border of the bin: the first CTA gathers and sorts them, applies all filters
+//      and draws.  At most 1024 in the bin (top-p): every CTA gathers and sorts those; the masses above the bin are known from
+//      the histograms, so the CTA into whose share the draw falls finds the token alone.  Otherwise the bin is refined, by the
+//      same histogram over the bit patterns in it, until the last kept token is known.
 //   4. the draw over whole slices: the kept mass of every CTA, one exchange, and the CTA into whose share the draw falls
 //      finds the token (also the way of rows without top-k and top-p, which start here).
 // Bound: the logits once (4 bytes each in f32), and, for rows that need every weight, 9 double operations per logit and pass.
@@ -100,6 +102,7 @@ struct Hit {
 struct RowShared {
     uint32_t hist[4][SP_BINS];  // counts; limbs of the masses
     u64 list[SP_LIST];          // gathered tokens
+    u64 weights[SP_LIST];
     double exp2_table[64];      // 2^(j / 64)
     u64 sums64[SP_WARPS + 1];
     uint32_t sums32[SP_WARPS + 1];
@@ -108,13 +111,19 @@ struct RowShared {
     float x_max[SP_CLUSTER];
     int32_t x_at[SP_CLUSTER];
     u64 x_w[SP_CLUSTER];
-    uint32_t x_n[SP_CLUSTER];
-    Hit hit;
+    uint32_t run_n[SP_CLUSTER][32];  // sums of 32 runs of 32 bins of every CTA
+    u64 run_w[SP_CLUSTER][32];
     uint32_t n_list;
     // of this CTA
     float red_max[SP_WARPS];
     int32_t red_at[SP_WARPS];
     uint32_t key_lo, key_hi, found;
+    uint32_t bin_n[SP_CLUSTER][32];  // the bins of one run of every CTA
+    u64 bin_w[SP_CLUSTER][32];
+    u64 before_w[SP_CLUSTER];        // mass of every CTA before the hit
+    uint32_t here_n[SP_CLUSTER];     // tokens of every CTA in the hit
+    u64 pick_w;
+    uint32_t pick;
 };
 
 // Inclusive sums over the CTA in thread order.
@@ -166,51 +175,64 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     float* x_s = p.scratch ? p.scratch + ((int64_t)row * C + rank) * p.slice : (float*)(row_smem + ((sizeof(RowShared) + 15) & ~(size_t)15));
     const int first = rank * p.slice, count = max(0, min(p.slice, p.n - first));
 
-    for (int i = tid; i < 4 * SP_BINS; i += SP_THREADS) (&sh.hist[0][0])[i] = 0;
-    if (tid < 64) sh.exp2_table[tid] = exp2((double)tid / 64.0);
-    if (tid == 0) sh.hit.bin = 0xffffffffu, sh.n_list = 0;
+    cluster.barrier_arrive();  // every CTA of the cluster runs before one writes into another's shared memory
     grid_launch_dependents();
     grid_dependency_wait();  // the kernel before has written the logits and the settings
-    const RowSettings s = row_settings(p, row);
 
     // ---- 1. the slice into shared memory, its maximum ----
     float best = -INFINITY;
     int at = 0x7fffffff;
+    const RowSettings s = row_settings(p, row);
     {
         const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
-        auto take = [&](float v, int i) {  // a thread's indices rise: the first maximum stays
+        auto take = [&](float v, int i) -> float {  // a thread's indices rise: the first maximum stays
             v = clean(v);
-            x_s[i] = v;
             if (v > best) best = v, at = first + i;
+            return v;
         };
-        int done = 0;
-        if (p.vec && p.dtype == B200KV_F32) {
-            done = count / 4 * 4;
-#pragma unroll 8
-            for (int i = tid * 4; i < done; i += SP_THREADS * 4) {
-                const float4 v = *(const float4*)(base + (int64_t)i * 4);
-                take(v.x, i), take(v.y, i + 1), take(v.z, i + 2), take(v.w, i + 3);
-            }
-        } else if (p.vec) {
-            done = count / 8 * 8;
-#pragma unroll 4
-            for (int i = tid * 8; i < done; i += SP_THREADS * 8) {
-                const uint4 v = *(const uint4*)(base + (int64_t)i * 2);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        // every thread has 128 bytes on their way before it uses the first
+        constexpr int STEP = 8 * SP_THREADS;  // 16-byte units per round
+        const int per = p.vec ? 16 / dtype_size(p.dtype) : 0, units = p.vec ? count / per : 0;
+        for (int u0 = tid; u0 < units; u0 += STEP) {
+            uint4 v[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (p.dtype == B200KV_F16) {
-                        const float2 f = __half22float2(*(const __half2*)&w[j]);
-                        take(f.x, i + 2 * j), take(f.y, i + 2 * j + 1);
-                    } else {
-                        take(__uint_as_float(w[j] << 16), i + 2 * j), take(__uint_as_float(w[j] & 0xffff0000u), i + 2 * j + 1);
+            for (int j = 0; j < 8; j++)
+                if (u0 + j * SP_THREADS < units) v[j] = ((const uint4*)base)[u0 + j * SP_THREADS];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int u = u0 + j * SP_THREADS;
+                if (u >= units) continue;
+                const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                float f[8];
+                if (p.dtype == B200KV_F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f[e] = take(__uint_as_float(w[e]), 4 * u + e);
+                    ((float4*)x_s)[u] = make_float4(f[0], f[1], f[2], f[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float2 g = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+                        if (p.dtype == B200KV_F16) g = __half22float2(*(const __half2*)&w[e]);
+                        f[2 * e] = take(g.x, 8 * u + 2 * e), f[2 * e + 1] = take(g.y, 8 * u + 2 * e + 1);
                     }
+                    ((float4*)x_s)[2 * u] = make_float4(f[0], f[1], f[2], f[3]);
+                    ((float4*)x_s)[2 * u + 1] = make_float4(f[4], f[5], f[6], f[7]);
                 }
             }
         }
-#pragma unroll 8
-        for (int i = done + tid; i < count; i += SP_THREADS) take(ld_as_f32(base, p.dtype, i), i);
+        for (int i0 = units * per + tid; i0 < count; i0 += 16 * SP_THREADS) {  // rows off the 16-byte grid, and the last few logits
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (i0 + j * SP_THREADS < count) v[j] = ld_as_f32(base, p.dtype, i0 + j * SP_THREADS);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (i0 + j * SP_THREADS < count) x_s[i0 + j * SP_THREADS] = take(v[j], i0 + j * SP_THREADS);
+        }
     }
+    for (int i = tid; i < SP_BINS; i += SP_THREADS) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid < 64) sh.exp2_table[tid] = exp2((double)tid / 64.0);
+    if (tid == 0) sh.n_list = 0;
     auto merge = [&](float ov, int oi) {
         if (ov > best || (ov == best && oi < at)) best = ov, at = oi;
     };
@@ -224,6 +246,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < SP_WARPS; w++) merge(sh.red_max[w], sh.red_at[w]);
+    cluster.barrier_wait();
     if (tid < C) {
         RowShared* other = cluster.map_shared_rank(&sh, tid);
         other->x_max[rank] = best, other->x_at[rank] = at;
@@ -275,7 +298,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
 
     // ---- a histogram over the cluster, and the bin in which the running count or mass first exceeds its goal ----
     // bin_of(x, index): 0 .. SP_BINS - 1, or -1 for what does not take part.  goal(all): from the whole count or mass.
-    // *_base: what lies before the first bin.
+    // *_base: what lies before the first bin.  The caller sees to it that the histogram is clear and that the CTAs have left it.
     auto round_of = [&](bool by_weight, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
         for (int i = tid; i < count; i += SP_THREADS) {
             const float x = x_s[i];
@@ -284,67 +307,83 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             atomicAdd(&sh.hist[0][b], 1u);
             if (by_weight) {
                 const u64 w = weight(x);
-                if (w) {
-                    atomicAdd(&sh.hist[1][b], (uint32_t)w & 0x7fffu);
-                    atomicAdd(&sh.hist[2][b], (uint32_t)(w >> SP_LIMB) & 0x7fffu);
-                    atomicAdd(&sh.hist[3][b], (uint32_t)(w >> (2 * SP_LIMB)));
-                }
+                const uint32_t l0 = (uint32_t)w & 0x7fffu, l1 = (uint32_t)(w >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w >> (2 * SP_LIMB));
+                if (l0) atomicAdd(&sh.hist[1][b], l0);
+                if (l1) atomicAdd(&sh.hist[2][b], l1);
+                if (l2) atomicAdd(&sh.hist[3][b], l2);
             }
         }
-        cluster.sync();
-        // this CTA's share of the bins, added up over the cluster; a thread has one bin, or two neighbours (a cluster of one)
-        const int share = SP_BINS / C, per = share > SP_THREADS ? share / SP_THREADS : 1, b0 = rank * share + tid * per;
-        uint32_t n[2] = {0, 0};
-        u64 w[2] = {0, 0};
-        if (tid * per < share) {
-            for (int r = 0; r < C; r++) {
-                const RowShared* other = cluster.map_shared_rank(&sh, r);
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    if (j < per) {
-                        n[j] += other->hist[0][b0 + j];
-                        if (by_weight)
-                            w[j] += (u64)other->hist[1][b0 + j] + ((u64)other->hist[2][b0 + j] << SP_LIMB) + ((u64)other->hist[3][b0 + j] << (2 * SP_LIMB));
-                    }
-            }
-        }
-        uint32_t n_incl = block_scan(n[0] + n[1], sh.sums32);
-        u64 w_incl = by_weight ? block_scan(w[0] + w[1], sh.sums64) : 0ull;
-        if (tid == SP_THREADS - 1) {
-            for (int r = 0; r < C; r++) {
-                RowShared* other = cluster.map_shared_rank(&sh, r);
-                other->x_n[rank] = n_incl, other->x_w[rank] = w_incl;
-            }
-        }
-        cluster.sync();  // every share is known, and nobody reads the histogram any more
-        for (int i = tid; i < (by_weight ? 4 : 1) * SP_BINS; i += SP_THREADS) (&sh.hist[0][0])[i] = 0;
-        u64 all = 0;
-        uint32_t n_low = n_base;
-        u64 w_low = w_base;
-        for (int r = 0; r < C; r++) {
-            all += by_weight ? sh.x_w[r] : (u64)sh.x_n[r];
-            if (r < rank) n_low += sh.x_n[r], w_low += sh.x_w[r];
-        }
-        const u64 target = goal(all);
-        uint32_t n_at = n_low + n_incl - (n[0] + n[1]);
-        u64 w_at = w_low + w_incl - (w[0] + w[1]);
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const u64 from = by_weight ? w_at : (u64)n_at, to = by_weight ? w_at + w[j] : (u64)(n_at + n[j]);
-            if (from <= target && to > target)
-                for (int r = 0; r < C; r++) cluster.map_shared_rank(&sh, r)->hit = Hit{(uint32_t)(b0 + j), n_at, n[j], w_at, w[j]};
-            n_at += n[j], w_at += w[j];
-        }
-        cluster.sync();
-        const Hit h = sh.hit;
         __syncthreads();
-        if (tid == 0) sh.hit.bin = 0xffffffffu;  // before the next round's first cluster barrier, behind which others may write it
+        auto limbs = [](const uint32_t (*h)[SP_BINS], int b) -> u64 { return (u64)h[1][b] + ((u64)h[2][b] << SP_LIMB) + ((u64)h[3][b] << (2 * SP_LIMB)); };
+        {  // 16 threads per run of 32 bins; the sums go to every CTA
+            uint32_t n = sh.hist[0][2 * tid] + sh.hist[0][2 * tid + 1];
+            u64 w = by_weight ? limbs(sh.hist, 2 * tid) + limbs(sh.hist, 2 * tid + 1) : 0ull;
+#pragma unroll
+            for (int o = 8; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o), w += __shfl_xor_sync(0xffffffffu, w, o);
+            const int to = tid & 15;
+            if (to < C) {
+                RowShared* other = cluster.map_shared_rank(&sh, to);
+                other->run_n[rank][tid >> 4] = n, other->run_w[rank][tid >> 4] = w;
+            }
+        }
+        cluster.sync();
+        // lane = run: the run in which the goal is passed, then lane = bin of that run.  Inclusive sums over the lanes.
+        auto scan = [&](uint32_t& n, u64& w) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t un = __shfl_up_sync(0xffffffffu, n, o);
+                const u64 uw = __shfl_up_sync(0xffffffffu, w, o);
+                if (lane >= o) n += un, w += uw;
+            }
+        };
+        uint32_t n = 0;
+        u64 w = 0;
+        for (int r = 0; r < C; r++) n += sh.run_n[r][lane], w += sh.run_w[r][lane];
+        uint32_t n_incl = n;
+        u64 w_incl = w;
+        scan(n_incl, w_incl);
+        const u64 target = goal(__shfl_sync(0xffffffffu, by_weight ? w_incl : (u64)n_incl, 31));
+        const uint32_t runs = __ballot_sync(0xffffffffu, (by_weight ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
+        if (!runs) return Hit{0xffffffffu, 0, 0, 0, 0};  // in every CTA alike
+        const int run = __ffs(runs) - 1;
+        const uint32_t n_run = n_base + __shfl_sync(0xffffffffu, n_incl - n, run);
+        const u64 w_run = w_base + __shfl_sync(0xffffffffu, w_incl - w, run);
+        if (warp < C) {
+            const RowShared* other = cluster.map_shared_rank(&sh, warp);
+            sh.bin_n[warp][lane] = other->hist[0][run * 32 + lane];
+            sh.bin_w[warp][lane] = by_weight ? limbs(other->hist, run * 32 + lane) : 0ull;
+        }
+        __syncthreads();
+        n = 0, w = 0;
+        for (int r = 0; r < C; r++) n += sh.bin_n[r][lane], w += sh.bin_w[r][lane];
+        n_incl = n, w_incl = w;
+        scan(n_incl, w_incl);
+        const uint32_t bins = __ballot_sync(0xffffffffu, (by_weight ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
+        const int bin = __ffs(bins) - 1;
+        Hit h;
+        h.bin = (uint32_t)(run * 32 + bin);
+        h.n_here = __shfl_sync(0xffffffffu, n, bin), h.w_here = __shfl_sync(0xffffffffu, w, bin);
+        h.n_before = n_run + __shfl_sync(0xffffffffu, n_incl - n, bin), h.w_before = w_run + __shfl_sync(0xffffffffu, w_incl - w, bin);
+        if (warp < C) {  // what every CTA has before the bin, and in it
+            u64 v = (lane < run ? sh.run_w[warp][lane] : 0ull) + (lane < bin ? sh.bin_w[warp][lane] : 0ull);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) sh.before_w[warp] = v, sh.here_n[warp] = sh.bin_n[warp][bin];
+        }
+        __syncthreads();
         return h;
+    };
+    // clears the histogram for another round, once every CTA has read what it needs of the last one
+    auto next_round = [&]() {
+        cluster.sync();
+        for (int i = tid; i < SP_BINS; i += SP_THREADS) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
     };
     // The same over positions lo .. hi, 1024 at a time, down to a single one; bin holds the position.
     auto refine = [&](bool by_weight, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
         for (;;) {
             const int bits = 32 - __clz((hi - lo) | 1u), shift = bits > 10 ? bits - 10 : 0;
+            next_round();
             Hit h = round_of(by_weight, n_base, w_base, [&](float x, int i) -> int {
                 uint32_t at;
                 return place(x, i, &at) && at >= lo && at <= hi ? (int)((at - lo) >> shift) : -1;
@@ -357,8 +396,54 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         }
     };
 
-    // ---- 2. the cut: everything above key_cut, and the first ones (up to index last_same) of those that equal it ----
+    // ---- 4. the draw over whole slices ----
+    // kept: everything above key_cut, and of those that equal it the ones up to index last_same
     uint32_t key_cut = KEY_NEG_INF + 1, last_same = 0xffffffffu;
+    u64 of_slice = 0;
+    bool runs_known = false;
+    auto kept_weight = [&](int i) -> u64 {
+        const float x = x_s[i];
+        const uint32_t key = key_of(x);
+        return key > key_cut || (key == key_cut && (uint32_t)(first + i) <= last_same) ? weight(x) : 0ull;
+    };
+    const int run = ((count + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;
+    // the kept mass of the slice; of a run per warp in warp_w
+    auto run_masses = [&]() -> u64 {
+        u64 mine = 0;
+        for (int i = warp * run + lane; i < min(count, (warp + 1) * run); i += 32) mine += kept_weight(i);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        __syncthreads();
+        if (lane == 0) sh.warp_w[warp] = mine;
+        __syncthreads();
+        u64 sum = 0;
+#pragma unroll
+        for (int w = 0; w < SP_WARPS; w++) sum += sh.warp_w[w];
+        runs_known = true;
+        return sum;
+    };
+    // mass: kept mass of the row; before, here: of the slices before this one, and of this one
+    auto draw = [&](u64 mass, u64 before, u64 here) {
+        const u64 target = min((u64)((double)s.u * (double)mass), mass - 1);
+        if (target < before || target >= before + here) return;
+        if (!runs_known) run_masses();
+        int w = 0;
+        for (; w < SP_WARPS - 1 && target >= before + sh.warp_w[w]; w++) before += sh.warp_w[w];
+        const int lo = w * run, hi = min(count, lo + run), per = (hi - lo + SP_THREADS - 1) / SP_THREADS;
+        u64 mine = 0;
+        for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(i);
+        before += block_scan(mine, sh.sums64) - mine;
+        if (before <= target && target < before + mine)
+            for (int i = lo + tid * per;; i++) {
+                before += kept_weight(i);
+                if (target < before) {
+                    p.out[row] = first + i;
+                    break;
+                }
+            }
+    };
+
+    // ---- 2. the cut ----
     if (s.use_k || s.use_p) {
         u64 whole = 0;  // of the row (top-p without top-k)
         auto p_goal = [&](u64 mass) -> u64 {  // the mass before a kept token is below p x mass: the cut is where the sum reaches it
@@ -369,7 +454,25 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             whole = all;
             return s.use_k ? (u64)(s.k - 1) : p_goal(all);
         });
-        // ---- 3. few enough tokens above the lower border of that bin: sort them ----
+        // bitonic sort of list[0 .. n): every step, a thread per pair; steps of up to 32 stay inside the 64 entries of a warp
+        auto sort = [&](int n) {
+            int size = 64;
+            while (size < n) size <<= 1;
+            __syncthreads();
+            for (int i = n + tid; i < size; i += SP_THREADS) sh.list[i] = ~0ull;
+            __syncthreads();
+            for (int k = 2; k <= size; k <<= 1)
+                for (int j = k >> 1; j; j >>= 1) {
+                    if (tid < size / 2) {
+                        const int a = 2 * tid - (tid & (j - 1)), b = a + j;
+                        const u64 va = sh.list[a], vb = sh.list[b];
+                        if ((va > vb) == ((a & k) == 0)) sh.list[a] = vb, sh.list[b] = va;
+                    }
+                    if (j > 32 || (j == 1 && k >= 64)) __syncthreads();
+                    else __syncwarp();
+                }
+        };
+        // ---- 3. few enough tokens down to the lower border of that bin: sort them ----
         const uint32_t n_list = top.bin == 0xffffffffu ? (s.use_k ? (uint32_t)whole : 0xffffffffu) : top.n_before + top.n_here;
         if (n_list <= SP_LIST) {
             RowShared* head = cluster.map_shared_rank(&sh, 0);
@@ -386,23 +489,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             }
             cluster.sync();
             if (rank != 0) return;
-            int size = 2;
-            while (size < (int)n_list) size <<= 1;
-            // bitonic sort of list[0 .. size): every step, a thread per pair
-            auto sort = [&](int size) {
-                for (int k = 2; k <= size; k <<= 1)
-                    for (int j = k >> 1; j; j >>= 1) {
-                        __syncthreads();
-                        if (tid < size / 2) {
-                            const int a = 2 * tid - (tid & (j - 1)), b = a + j;
-                            const u64 va = sh.list[a], vb = sh.list[b];
-                            if ((va > vb) == ((a & k) == 0)) sh.list[a] = vb, sh.list[b] = va;
-                        }
-                    }
-                __syncthreads();
-            };
-            for (int i = (int)n_list + tid; i < size; i += SP_THREADS) sh.list[i] = ~0ull;
-            sort(size);  // falling logits, equal ones by rising index
+            sort((int)n_list);  // falling logits, equal ones by rising index
             // thread tid has places 2 tid and 2 tid + 1
             const int e0 = 2 * tid;
             u64 tok[2];
@@ -428,22 +515,17 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             }
             // the kept ones by rising index, each with its place in the order of weights (their weights stay where they can be found)
             const uint32_t n_kept = (uint32_t)__syncthreads_count(passes[0]) + (uint32_t)__syncthreads_count(passes[1]);
-            u64* weights = (u64*)&sh.hist[0][0];
 #pragma unroll
             for (int j = 0; j < 2; j++)
                 if (passes[j]) {
-                    weights[e0 + j] = w[j];
+                    sh.weights[e0 + j] = w[j];
                     sh.list[e0 + j] = (tok[j] << 32) | (u64)(uint32_t)(e0 + j);
                 }
-            int kept_size = 2;
-            while (kept_size < (int)n_kept) kept_size <<= 1;
-            __syncthreads();
-            for (int i = (int)n_kept + tid; i < kept_size; i += SP_THREADS) sh.list[i] = ~0ull;
-            sort(kept_size);
+            sort((int)n_kept);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 tok[j] = e0 + j < (int)n_kept ? sh.list[e0 + j] : ~0ull;
-                w[j] = e0 + j < (int)n_kept ? weights[(uint32_t)tok[j]] : 0ull;
+                w[j] = e0 + j < (int)n_kept ? sh.weights[(uint32_t)tok[j]] : 0ull;
             }
             incl = block_scan(w[0] + w[1], sh.sums64);
             if (tid == SP_THREADS - 1) sh.x_w[0] = incl;
@@ -455,6 +537,53 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
                 if (before <= target && before + w[j] > target) p.out[row] = (int32_t)(tok[j] >> 32);
                 before += w[j];
             }
+            return;
+        }
+        if (!s.use_k && !s.use_m && top.n_here <= SP_LIST) {
+            // top-p alone: the tokens of the bin, in every CTA
+            uint32_t offset = 0;
+            for (int r = 0; r < rank; r++) offset += sh.here_n[r];
+            for (int i0 = 0; i0 < count; i0 += SP_THREADS) {
+                const int i = i0 + tid;
+                const float x = i < count ? x_s[i] : -INFINITY;
+                if (x > -INFINITY && z_bin(x) == top.bin) {
+                    const uint32_t slot = offset + atomicAdd(&sh.n_list, 1u);
+                    const u64 tok = ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i);
+                    for (int r = 0; r < C; r++) cluster.map_shared_rank(&sh, r)->list[slot] = tok;
+                }
+            }
+            cluster.sync();
+            sort((int)top.n_here);
+            const int e0 = 2 * tid;
+            u64 tok[2], w[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                tok[j] = e0 + j < (int)top.n_here ? sh.list[e0 + j] : ~0ull;
+                w[j] = e0 + j < (int)top.n_here ? weight(of_key(~(uint32_t)(tok[j] >> 32))) : 0ull;
+            }
+            const u64 incl = block_scan(w[0] + w[1], sh.sums64), goal = p_goal(whole);
+            u64 sum = top.w_before + incl - (w[0] + w[1]);
+            u64 own = 0, low = 0;  // kept mass of the bin in this CTA's slice, and in the slices before it
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (w[j] && sum <= goal) {
+                    const int at = (int)(uint32_t)tok[j];
+                    if (at < first) low += w[j];
+                    else if (at < first + count) own += w[j];
+                    if (sum + w[j] > goal) sh.pick = (uint32_t)(e0 + j), sh.pick_w = sum + w[j];  // the last kept token, and the kept mass
+                }
+                sum += w[j];
+            }
+            low = block_scan(low, sh.sums64);
+            if (tid == SP_THREADS - 1) sh.x_w[0] = low;
+            own = block_scan(own, sh.sums64);
+            if (tid == SP_THREADS - 1) sh.x_w[1] = own;
+            __syncthreads();
+            const u64 last = sh.list[sh.pick];
+            key_cut = ~(uint32_t)(last >> 32), last_same = (uint32_t)last;
+            u64 before = sh.x_w[0];
+            for (int r = 0; r < rank; r++) before += sh.before_w[r];
+            draw(sh.pick_w, before, sh.before_w[rank] + sh.x_w[1]);
             return;
         }
         // many tokens: down to the last kept one
@@ -484,6 +613,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         if (s.use_p) {
             if (s.use_k) {  // the mass of the first k: of everything down to key_cut, without the equal ones that are left out
                 const u64 over = n_same == 0xffffffffu ? 0ull : (u64)(n_same - n_cut) * weight(of_key(key_cut));
+                next_round();
                 hit = round_of(true, 0, 0, [&](float x, int) -> int { return key_of(x) >= key_cut ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
                     whole = all - over;
                     return p_goal(whole);
@@ -506,22 +636,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         key_cut = key_m;
     }
 
-    // ---- 4. the draw: a run of the slice per warp, the slices over the cluster ----
-    auto kept_weight = [&](int i) -> u64 {
-        const float x = x_s[i];
-        const uint32_t key = key_of(x);
-        return key > key_cut || (key == key_cut && (uint32_t)(first + i) <= last_same) ? weight(x) : 0ull;
-    };
-    const int run = ((count + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;
-    u64 mine = 0;
-    for (int i = warp * run + lane; i < min(count, (warp + 1) * run); i += 32) mine += kept_weight(i);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sh.warp_w[warp] = mine;
-    __syncthreads();
-    u64 of_slice = 0;
-#pragma unroll
-    for (int w = 0; w < SP_WARPS; w++) of_slice += sh.warp_w[w];
+    of_slice = run_masses();
     if (tid < C) cluster.map_shared_rank(&sh, tid)->x_w[rank] = of_slice;
     cluster.sync();
     u64 mass = 0, before = 0;
@@ -529,22 +644,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         if (r == rank) before = mass;
         mass += sh.x_w[r];
     }
-    const u64 target = min((u64)((double)s.u * (double)mass), mass - 1);
-    if (target < before || target >= before + of_slice) return;
-    int w = 0;
-    for (; w < SP_WARPS - 1 && target >= before + sh.warp_w[w]; w++) before += sh.warp_w[w];
-    const int lo = w * run, hi = min(count, lo + run), per = (hi - lo + SP_THREADS - 1) / SP_THREADS;
-    mine = 0;
-    for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(i);
-    before += block_scan(mine, sh.sums64) - mine;
-    if (before <= target && target < before + mine)
-        for (int i = lo + tid * per;; i++) {
-            before += kept_weight(i);
-            if (target < before) {
-                p.out[row] = first + i;
-                break;
-            }
-        }
+    draw(mass, before, of_slice);
 }
 
 // CTAs per row: as many as the slices need, and while a launch would leave SMs empty, up to eight (of at least 1024 logits each)
