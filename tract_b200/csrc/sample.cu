@@ -40,6 +40,8 @@ constexpr int SP_CLUSTER = 8;       // most CTAs of a row (the portable cluster 
 constexpr int SP_SLICE = 16384;     // logits a CTA takes before another one is added: 64 KB, two CTAs per SM
 constexpr int SP_BINS = 1024;
 constexpr int SP_LIST = 1024;       // tokens that are sorted
+constexpr int SP_PART = SP_LIST / SP_CLUSTER;  // top-p: a CTA's part of them
+constexpr int SP_TABLE = 256;       // steps of 2^(1 / 256)
 constexpr int W_BITS = 44;          // fractional bits of a weight
 constexpr int SP_LIMB = 15;         // a weight enters a histogram as three 15-bit limbs: 2^17 of them fit a 32-bit counter
 constexpr int MAX_VOCAB = 1 << 19;  // so many weights of 1 add up to 2^63
@@ -76,6 +78,7 @@ __device__ inline RowSettings row_settings(const SampleParams& p, int row) {
     const float u = p.uniform[row];
     s.u = u > 0.f ? fminf(u, 1.f) : 0.f;
     s.greedy = !(s.t > 0.f);
+    s.t = fminf(fmaxf(s.t, 1e-30f), 1e30f);  // beyond: the maxima alone, or a draw among all finite logits, as it is there
     s.use_k = s.k > 0 && s.k < p.n;
     s.use_p = s.p < 1.f;
     s.use_m = s.min_p > 0.f;
@@ -83,7 +86,7 @@ __device__ inline RowSettings row_settings(const SampleParams& p, int row) {
     s.greedy |= (s.use_k && s.k == 1) || (s.use_p && !(s.p > 0.f));  // an empty beginning: the first token alone
     return s;
 }
-__device__ inline float clean(float x) { return x != x ? -INFINITY : x + 0.f; }  // NaN is never chosen; -0 and +0 are the same logit
+__device__ inline float clean(float x) { return fmaxf(x + 0.f, -INFINITY); }  // NaN is never chosen; -0 and +0 are the same logit
 // monotone bit pattern of a logit
 __device__ inline uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -100,45 +103,40 @@ struct Hit {
 };
 
 struct RowShared {
-    uint32_t hist[4][SP_BINS];  // counts; limbs of the masses
-    u64 list[SP_LIST];          // gathered tokens
-    u64 weights[SP_LIST];
-    double exp2_table[64];      // 2^(j / 64)
-    u64 sums64[SP_WARPS + 1];
-    uint32_t sums32[SP_WARPS + 1];
-    u64 warp_w[SP_WARPS];
+    uint32_t hist[4][SP_BINS];     // limbs of the masses; counts
+    u64 list[SP_LIST];             // gathered tokens
+    double exp2_table[SP_TABLE];   // 2^(j / SP_TABLE)
     // written by the other CTAs of the cluster
     float x_max[SP_CLUSTER];
-    int32_t x_at[SP_CLUSTER];
     u64 x_w[SP_CLUSTER];
     uint32_t run_n[SP_CLUSTER][32];  // sums of 32 runs of 32 bins of every CTA
     u64 run_w[SP_CLUSTER][32];
-    uint32_t n_list;
+    uint32_t n_list;                 // entries of the list (top-k), or a CTA's own part of it (top-p)
+    uint32_t part[SP_CLUSTER];       // tokens of every CTA in the list (top-p)
     // of this CTA
-    float red_max[SP_WARPS];
-    int32_t red_at[SP_WARPS];
-    uint32_t key_lo, key_hi, found;
     uint32_t bin_n[SP_CLUSTER][32];  // the bins of one run of every CTA
     u64 bin_w[SP_CLUSTER][32];
     u64 before_w[SP_CLUSTER];        // mass of every CTA before the hit
-    uint32_t here_n[SP_CLUSTER];     // tokens of every CTA in the hit
+    u64 sums64[SP_WARPS + 1];
+    u64 warp_w[SP_WARPS];
+    float red_max[SP_WARPS];
+    uint32_t key_lo, key_hi, found;
     u64 pick_w;
     uint32_t pick;
 };
 
 // Inclusive sums over the CTA in thread order.
-template <typename T>
-__device__ inline T block_scan(T v, T* warp_sums) {
+__device__ inline u64 block_scan(u64 v, u64* warp_sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const T up = __shfl_up_sync(0xffffffffu, v, o);
+        const u64 up = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += up;
     }
     __syncthreads();  // the sums of the scan before are no longer read
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
-    T mine = lane < warp ? warp_sums[lane] : T(0);  // SP_WARPS <= 32
+    u64 mine = lane < warp ? warp_sums[lane] : 0ull;  // SP_WARPS <= 32
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     return mine + v;
@@ -171,49 +169,46 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.y;
-    // the slice, cleaned
+    // the slice, cleaned, and filled up with -inf to a multiple of 4
     float* x_s = p.scratch ? p.scratch + ((int64_t)row * C + rank) * p.slice : (float*)(row_smem + ((sizeof(RowShared) + 15) & ~(size_t)15));
-    const int first = rank * p.slice, count = max(0, min(p.slice, p.n - first));
+    const int first = rank * p.slice, count = max(0, min(p.slice, p.n - first)), quads = (count + 3) / 4;
+    auto other = [&](int r) -> RowShared* { return cluster.map_shared_rank(&sh, r); };
 
     cluster.barrier_arrive();  // every CTA of the cluster runs before one writes into another's shared memory
     grid_launch_dependents();
     grid_dependency_wait();  // the kernel before has written the logits and the settings
 
     // ---- 1. the slice into shared memory, its maximum ----
-    float best = -INFINITY;
-    int at = 0x7fffffff;
     const RowSettings s = row_settings(p, row);
+    float best = -INFINITY;
     {
         const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
-        auto take = [&](float v, int i) -> float {  // a thread's indices rise: the first maximum stays
+        auto take = [&](float v) -> float {
             v = clean(v);
-            if (v > best) best = v, at = first + i;
+            best = fmaxf(best, v);
             return v;
         };
         // every thread has 128 bytes on their way before it uses the first
-        constexpr int STEP = 8 * SP_THREADS;  // 16-byte units per round
         const int per = p.vec ? 16 / dtype_size(p.dtype) : 0, units = p.vec ? count / per : 0;
-        for (int u0 = tid; u0 < units; u0 += STEP) {
+        for (int u0 = tid; u0 < units; u0 += 8 * SP_THREADS) {
             uint4 v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (u0 + j * SP_THREADS < units) v[j] = ((const uint4*)base)[u0 + j * SP_THREADS];
+                if (u0 + j * SP_THREADS < units) v[j] = __ldcs((const uint4*)base + u0 + j * SP_THREADS);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int u = u0 + j * SP_THREADS;
                 if (u >= units) continue;
                 const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-                float f[8];
                 if (p.dtype == B200KV_F32) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) f[e] = take(__uint_as_float(w[e]), 4 * u + e);
-                    ((float4*)x_s)[u] = make_float4(f[0], f[1], f[2], f[3]);
+                    ((float4*)x_s)[u] = make_float4(take(__uint_as_float(w[0])), take(__uint_as_float(w[1])), take(__uint_as_float(w[2])), take(__uint_as_float(w[3])));
                 } else {
+                    float f[8];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         float2 g = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
                         if (p.dtype == B200KV_F16) g = __half22float2(*(const __half2*)&w[e]);
-                        f[2 * e] = take(g.x, 8 * u + 2 * e), f[2 * e + 1] = take(g.y, 8 * u + 2 * e + 1);
+                        f[2 * e] = take(g.x), f[2 * e + 1] = take(g.y);
                     }
                     ((float4*)x_s)[2 * u] = make_float4(f[0], f[1], f[2], f[3]);
                     ((float4*)x_s)[2 * u + 1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -227,104 +222,123 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
                 if (i0 + j * SP_THREADS < count) v[j] = ld_as_f32(base, p.dtype, i0 + j * SP_THREADS);
 #pragma unroll
             for (int j = 0; j < 16; j++)
-                if (i0 + j * SP_THREADS < count) x_s[i0 + j * SP_THREADS] = take(v[j], i0 + j * SP_THREADS);
+                if (i0 + j * SP_THREADS < count) x_s[i0 + j * SP_THREADS] = take(v[j]);
         }
+        if (tid < quads * 4 - count) x_s[count + tid] = -INFINITY;
     }
-    for (int i = tid; i < SP_BINS; i += SP_THREADS) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (tid < 64) sh.exp2_table[tid] = exp2((double)tid / 64.0);
-    if (tid == 0) sh.n_list = 0;
-    auto merge = [&](float ov, int oi) {
-        if (ov > best || (ov == best && oi < at)) best = ov, at = oi;
-    };
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-        const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-        merge(ov, oi);
+    for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) sh.red_max[warp] = best;
+    if (!s.greedy) {
+        if (s.use_k || s.use_p)
+            for (int i = tid; i < SP_BINS; i += SP_THREADS) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = tid; i < SP_TABLE; i += SP_THREADS) sh.exp2_table[i] = exp2((double)i / SP_TABLE);
+        if (tid == 0) sh.n_list = 0;
     }
-    if (lane == 0) sh.red_max[warp] = best, sh.red_at[warp] = at;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SP_WARPS; w++) merge(sh.red_max[w], sh.red_at[w]);
+    for (int w = 0; w < SP_WARPS; w++) best = fmaxf(best, sh.red_max[w]);
     cluster.barrier_wait();
-    if (tid < C) {
-        RowShared* other = cluster.map_shared_rank(&sh, tid);
-        other->x_max[rank] = best, other->x_at[rank] = at;
-    }
+    if (tid < C) other(tid)->x_max[rank] = best;
     cluster.sync();
-    for (int r = 0; r < C; r++) merge(sh.x_max[r], sh.x_at[r]);
-    const float x_top = best;
-    if (s.greedy || x_top == -INFINITY) {  // the same in every CTA; nothing of another CTA is touched any more
-        if (rank == 0 && tid == 0) p.out[row] = x_top == -INFINITY ? 0 : at;
+    float x_top = -INFINITY;
+    int top_rank = 0;
+    for (int r = C - 1; r >= 0; r--)
+        if (sh.x_max[r] >= x_top) x_top = sh.x_max[r], top_rank = r;
+    if (s.greedy || x_top == -INFINITY) {  // the first maximum; nothing of another CTA is touched any more
+        if (rank != top_rank) return;
+        int at = x_top == -INFINITY ? 0 : 0x7fffffff;
+        if (at)
+            for (int u = tid; u < quads; u += SP_THREADS) {
+                const float4 v = ((const float4*)x_s)[u];
+                const int i = v.x == x_top ? 0 : v.y == x_top ? 1 : v.z == x_top ? 2 : v.w == x_top ? 3 : 4;
+                if (i < 4) at = min(at, 4 * u + i);
+            }
+        at = __reduce_min_sync(0xffffffffu, at);
+        __syncthreads();
+        if (lane == 0) sh.red_max[warp] = __int_as_float(at);
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < SP_WARPS; w++) at = min(at, __float_as_int(sh.red_max[w]));
+            p.out[row] = x_top == -INFINITY ? 0 : first + at;
+        }
         return;
+    }
+    if (x_top == INFINITY) {  // infinite logits share the row
+        for (int i = tid; i < quads * 4; i += SP_THREADS) x_s[i] = x_s[i] == INFINITY ? 0.f : -INFINITY;
+        x_top = 0.f;
+        __syncthreads();
     }
 
     // ---- weights ----
-    // exp((x - max) / T) = 2^(t / 64), t = (x - max) 64 log2 e / T = n + r, n whole: 2^(n / 64) from the table and the exponent,
-    // 2^(r / 64) by its Taylor polynomial of degree 4 in r ln 2 / 64 (|r| <= 1/2: what is left out is below 4e-14), rounded to 44
-    // fractional bits by adding 1.5 * 2^8.  Below 2^-46: 0.  An infinite maximum shares the row among the infinite logits.
-    const double t64 = 64.0 * 1.4426950408889634074 / (double)s.t;
+    // depth of a logit: 1023 / 46 x log2(1 / w), cut off at 1023; monotone in x
+    const float zscale = 1.4426950408889634f / s.t * ((float)(SP_BINS - 1) / 46.f);
+    auto depth = [&](float x) -> float { return fminf((x_top - x) * zscale, (float)(SP_BINS - 1)); };
+    auto z_bin = [&](float x) -> uint32_t { return __float_as_uint(depth(x) + 8388608.f) & (SP_BINS - 1); };  // rounded to the nearest whole number
+    // exp((x - max) / T) = 2^(t / 256), t = (x - max) 256 log2 e / T = n + r, n whole: 2^(n / 256) from the table and the exponent,
+    // 2^(r / 256) by its Taylor polynomial of degree 3 in r ln 2 / 256 (|r| <= 1/2: what is left out is below 1.5e-13), rounded
+    // to 44 fractional bits by adding 1.5 * 2^8.  From depth 1023 on (2^-46): 0.
+    const double t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)s.t, top64 = (double)x_top;
     auto weight = [&](float x) -> u64 {
-        if (x == x_top) return 1ull << W_BITS;
-        const double t = ((double)x - (double)x_top) * t64;
-        if (!(t > -64.0 * 46.0)) return 0ull;
-        constexpr double L = 0.69314718055994530942 / 64.0, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
+        constexpr double L = 0.69314718055994530942 / SP_TABLE, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
+        const double t = ((double)x - top64) * t_unit;
         const double biased = t + MAGIC, r = t - (biased - MAGIC);
         const int n = __double2loint(biased);
-        double q = fma(r, L * L * L * L / 24.0, L * L * L / 6.0);
-        q = fma(q, r, L * L / 2.0);
+        double q = fma(r, L * L * L / 6.0, L * L / 2.0);
         q = fma(q, r, L);
         q = fma(q, r, 1.0);
-        const double tab = sh.exp2_table[n & 63];
-        const double scaled = __hiloint2double(__double2hiint(tab) + ((n >> 6) << 20), __double2loint(tab));
-        return (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
+        const double tab = sh.exp2_table[n & (SP_TABLE - 1)];
+        const double scaled = __hiloint2double(__double2hiint(tab) + ((n >> 8) << 20), __double2loint(tab));
+        const u64 w = (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
+        return depth(x) < (float)(SP_BINS - 1) ? w : 0ull;
     };
-    // bins of log2 w, 46 octaves deep; monotone in x, the deepest takes everything below
-    const float zscale = 1.4426950408889634f / s.t * ((float)(SP_BINS - 1) / 46.f);
-    auto z_bin = [&](float x) -> uint32_t { return x == x_top ? 0u : (uint32_t)fminf((x_top - x) * zscale, (float)(SP_BINS - 1)); };
-    // min-p: the smallest bit pattern that passes
+    // f(x, place in the slice) for every logit of the slice; the fill is -inf
+    auto each = [&](auto f) {
+        for (int u = tid; u < quads; u += SP_THREADS) {
+            const float4 v = ((const float4*)x_s)[u];
+            f(v.x, 4 * u), f(v.y, 4 * u + 1), f(v.z, 4 * u + 2), f(v.w, 4 * u + 3);
+        }
+    };
+    // min-p: the smallest logit that passes
     const uint32_t key_max = key_of(x_top);
-    uint32_t key_m = KEY_NEG_INF + 1;
+    float x_m = -INFINITY;
     if (s.use_m) {
         if (warp == 0) {
             const uint32_t k = first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t key) {
-                return key == key_max || (x_top != INFINITY && exp(((double)of_key(key) - (double)x_top) / (double)s.t) >= (double)s.min_p);
+                return key == key_max || exp(((double)of_key(key) - top64) / (double)s.t) >= (double)s.min_p;
             });
             if (lane == 0) sh.found = k;
         }
         __syncthreads();
-        key_m = sh.found;
+        x_m = of_key(sh.found);
     }
 
     // ---- a histogram over the cluster, and the bin in which the running count or mass first exceeds its goal ----
     // bin_of(x, index): 0 .. SP_BINS - 1, or -1 for what does not take part.  goal(all): from the whole count or mass.
     // *_base: what lies before the first bin.  The caller sees to it that the histogram is clear and that the CTAs have left it.
-    auto round_of = [&](bool by_weight, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
-        for (int i = tid; i < count; i += SP_THREADS) {
-            const float x = x_s[i];
+    // COUNT / WEIGHT: what is added up (the goal is a mass where there are weights).
+    auto limbs = [](const RowShared* o, int b) -> u64 { return (u64)o->hist[0][b] + ((u64)o->hist[1][b] << SP_LIMB) + ((u64)o->hist[2][b] << (2 * SP_LIMB)); };
+    auto round_of = [&](bool counts, bool weights, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
+        each([&](float x, int i) {
             const int b = bin_of(x, first + i);
-            if (b < 0) continue;
-            atomicAdd(&sh.hist[0][b], 1u);
-            if (by_weight) {
+            if (b < 0) return;
+            if (counts) atomicAdd(&sh.hist[3][b], 1u);
+            if (weights) {
                 const u64 w = weight(x);
                 const uint32_t l0 = (uint32_t)w & 0x7fffu, l1 = (uint32_t)(w >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w >> (2 * SP_LIMB));
-                if (l0) atomicAdd(&sh.hist[1][b], l0);
-                if (l1) atomicAdd(&sh.hist[2][b], l1);
-                if (l2) atomicAdd(&sh.hist[3][b], l2);
+                if (l0) atomicAdd(&sh.hist[0][b], l0);
+                if (l1) atomicAdd(&sh.hist[1][b], l1);
+                if (l2) atomicAdd(&sh.hist[2][b], l2);
             }
-        }
+        });
         __syncthreads();
-        auto limbs = [](const uint32_t (*h)[SP_BINS], int b) -> u64 { return (u64)h[1][b] + ((u64)h[2][b] << SP_LIMB) + ((u64)h[3][b] << (2 * SP_LIMB)); };
         {  // 16 threads per run of 32 bins; the sums go to every CTA
-            uint32_t n = sh.hist[0][2 * tid] + sh.hist[0][2 * tid + 1];
-            u64 w = by_weight ? limbs(sh.hist, 2 * tid) + limbs(sh.hist, 2 * tid + 1) : 0ull;
+            uint32_t n = counts ? sh.hist[3][2 * tid] + sh.hist[3][2 * tid + 1] : 0u;
+            u64 w = weights ? limbs(&sh, 2 * tid) + limbs(&sh, 2 * tid + 1) : 0ull;
 #pragma unroll
             for (int o = 8; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o), w += __shfl_xor_sync(0xffffffffu, w, o);
             const int to = tid & 15;
-            if (to < C) {
-                RowShared* other = cluster.map_shared_rank(&sh, to);
-                other->run_n[rank][tid >> 4] = n, other->run_w[rank][tid >> 4] = w;
-            }
+            if (to < C) other(to)->run_n[rank][tid >> 4] = n, other(to)->run_w[rank][tid >> 4] = w;
         }
         cluster.sync();
         // lane = run: the run in which the goal is passed, then lane = bin of that run.  Inclusive sums over the lanes.
@@ -342,33 +356,33 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         uint32_t n_incl = n;
         u64 w_incl = w;
         scan(n_incl, w_incl);
-        const u64 target = goal(__shfl_sync(0xffffffffu, by_weight ? w_incl : (u64)n_incl, 31));
-        const uint32_t runs = __ballot_sync(0xffffffffu, (by_weight ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
+        const u64 target = goal(__shfl_sync(0xffffffffu, weights ? w_incl : (u64)n_incl, 31));
+        const uint32_t runs = __ballot_sync(0xffffffffu, (weights ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
         if (!runs) return Hit{0xffffffffu, 0, 0, 0, 0};  // in every CTA alike
         const int run = __ffs(runs) - 1;
         const uint32_t n_run = n_base + __shfl_sync(0xffffffffu, n_incl - n, run);
         const u64 w_run = w_base + __shfl_sync(0xffffffffu, w_incl - w, run);
         if (warp < C) {
-            const RowShared* other = cluster.map_shared_rank(&sh, warp);
-            sh.bin_n[warp][lane] = other->hist[0][run * 32 + lane];
-            sh.bin_w[warp][lane] = by_weight ? limbs(other->hist, run * 32 + lane) : 0ull;
+            const RowShared* o = other(warp);
+            sh.bin_n[warp][lane] = counts ? o->hist[3][run * 32 + lane] : 0u;
+            sh.bin_w[warp][lane] = weights ? limbs(o, run * 32 + lane) : 0ull;
         }
         __syncthreads();
         n = 0, w = 0;
         for (int r = 0; r < C; r++) n += sh.bin_n[r][lane], w += sh.bin_w[r][lane];
         n_incl = n, w_incl = w;
         scan(n_incl, w_incl);
-        const uint32_t bins = __ballot_sync(0xffffffffu, (by_weight ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
+        const uint32_t bins = __ballot_sync(0xffffffffu, (weights ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
         const int bin = __ffs(bins) - 1;
         Hit h;
         h.bin = (uint32_t)(run * 32 + bin);
         h.n_here = __shfl_sync(0xffffffffu, n, bin), h.w_here = __shfl_sync(0xffffffffu, w, bin);
         h.n_before = n_run + __shfl_sync(0xffffffffu, n_incl - n, bin), h.w_before = w_run + __shfl_sync(0xffffffffu, w_incl - w, bin);
-        if (warp < C) {  // what every CTA has before the bin, and in it
+        if (warp < C && weights) {  // what every CTA has before the bin
             u64 v = (lane < run ? sh.run_w[warp][lane] : 0ull) + (lane < bin ? sh.bin_w[warp][lane] : 0ull);
 #pragma unroll
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) sh.before_w[warp] = v, sh.here_n[warp] = sh.bin_n[warp][bin];
+            if (lane == 0) sh.before_w[warp] = v;
         }
         __syncthreads();
         return h;
@@ -380,11 +394,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         __syncthreads();
     };
     // The same over positions lo .. hi, 1024 at a time, down to a single one; bin holds the position.
-    auto refine = [&](bool by_weight, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
+    auto refine = [&](bool weights, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
         for (;;) {
             const int bits = 32 - __clz((hi - lo) | 1u), shift = bits > 10 ? bits - 10 : 0;
             next_round();
-            Hit h = round_of(by_weight, n_base, w_base, [&](float x, int i) -> int {
+            Hit h = round_of(true, weights, n_base, w_base, [&](float x, int i) -> int {
                 uint32_t at;
                 return place(x, i, &at) && at >= lo && at <= hi ? (int)((at - lo) >> shift) : -1;
             }, [&](u64) { return target; });
@@ -397,20 +411,29 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     };
 
     // ---- 4. the draw over whole slices ----
-    // kept: everything above key_cut, and of those that equal it the ones up to index last_same
-    uint32_t key_cut = KEY_NEG_INF + 1, last_same = 0xffffffffu;
+    // kept: everything above x_cut, and of those that equal it the ones up to index last_same
+    float x_cut = -INFINITY;
+    uint32_t last_same = 0xffffffffu;
     u64 of_slice = 0;
     bool runs_known = false;
-    auto kept_weight = [&](int i) -> u64 {
-        const float x = x_s[i];
-        const uint32_t key = key_of(x);
-        return key > key_cut || (key == key_cut && (uint32_t)(first + i) <= last_same) ? weight(x) : 0ull;
-    };
-    const int run = ((count + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;
+    auto kept_weight = [&](float x, int i) -> u64 { return x > x_cut || (x == x_cut && (uint32_t)(first + i) <= last_same) ? weight(x) : 0ull; };
+    const int run = ((quads + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;  // quads of a warp
     // the kept mass of the slice; of a run per warp in warp_w
     auto run_masses = [&]() -> u64 {
         u64 mine = 0;
-        for (int i = warp * run + lane; i < min(count, (warp + 1) * run); i += 32) mine += kept_weight(i);
+        const int end = min(quads, (warp + 1) * run);
+        if (x_cut == -INFINITY) {
+            for (int u = warp * run + lane; u < end; u += 32) {
+                const float4 v = ((const float4*)x_s)[u];
+                mine += weight(v.x) + weight(v.y) + weight(v.z) + weight(v.w);
+            }
+        } else {
+            for (int u = warp * run + lane; u < end; u += 32) {
+                const float4 v = ((const float4*)x_s)[u];
+                if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x_cut)
+                    mine += kept_weight(v.x, 4 * u) + kept_weight(v.y, 4 * u + 1) + kept_weight(v.z, 4 * u + 2) + kept_weight(v.w, 4 * u + 3);
+            }
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         __syncthreads();
@@ -429,13 +452,13 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         if (!runs_known) run_masses();
         int w = 0;
         for (; w < SP_WARPS - 1 && target >= before + sh.warp_w[w]; w++) before += sh.warp_w[w];
-        const int lo = w * run, hi = min(count, lo + run), per = (hi - lo + SP_THREADS - 1) / SP_THREADS;
+        const int lo = 4 * w * run, hi = 4 * min(quads, (w + 1) * run), per = (hi - lo + SP_THREADS - 1) / SP_THREADS;
         u64 mine = 0;
-        for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(i);
+        for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(x_s[i], i);
         before += block_scan(mine, sh.sums64) - mine;
         if (before <= target && target < before + mine)
             for (int i = lo + tid * per;; i++) {
-                before += kept_weight(i);
+                before += kept_weight(x_s[i], i);
                 if (target < before) {
                     p.out[row] = first + i;
                     break;
@@ -445,12 +468,12 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
 
     // ---- 2. the cut ----
     if (s.use_k || s.use_p) {
-        u64 whole = 0;  // of the row (top-p without top-k)
+        u64 whole = 0;  // count of the row's numbers (top-k), or its mass
         auto p_goal = [&](u64 mass) -> u64 {  // the mass before a kept token is below p x mass: the cut is where the sum reaches it
             const u64 least = (u64)ceil((double)s.p * (double)mass);
             return least ? least - 1 : 0;
         };
-        const Hit top = round_of(!s.use_k, 0, 0, [&](float x, int) -> int { return x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
+        const Hit top = round_of(s.use_k, !s.use_k, 0, 0, [&](float x, int) -> int { return x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
             whole = all;
             return s.use_k ? (u64)(s.k - 1) : p_goal(all);
         });
@@ -472,65 +495,53 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
                     else __syncwarp();
                 }
         };
+        auto token_of = [&](float x, int i) -> u64 { return ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i); };  // sorts by falling logits, then by index
+        auto logit_of = [](u64 token) -> float { return of_key(~(uint32_t)(token >> 32)); };
+        const int e0 = 2 * tid;  // of a sorted list, thread tid has places 2 tid and 2 tid + 1
         // ---- 3. few enough tokens down to the lower border of that bin: sort them ----
-        const uint32_t n_list = top.bin == 0xffffffffu ? (s.use_k ? (uint32_t)whole : 0xffffffffu) : top.n_before + top.n_here;
+        const uint32_t n_list = !s.use_k ? 0xffffffffu : top.bin == 0xffffffffu ? (uint32_t)min(whole, (u64)SP_LIST + 1) : top.n_before + top.n_here;
         if (n_list <= SP_LIST) {
-            RowShared* head = cluster.map_shared_rank(&sh, 0);
-            for (int i0 = 0; i0 < count; i0 += SP_THREADS) {
-                const int i = i0 + tid;
-                const float x = i < count ? x_s[i] : -INFINITY;
-                const bool take = x > -INFINITY && z_bin(x) <= top.bin;
-                const uint32_t vote = __ballot_sync(0xffffffffu, take);
-                if (!vote) continue;
-                uint32_t slot = 0;
-                if (lane == 0) slot = atomicAdd(&head->n_list, (uint32_t)__popc(vote));
-                slot = __shfl_sync(0xffffffffu, slot, 0) + (uint32_t)__popc(vote & ((1u << lane) - 1u));
-                if (take) head->list[slot] = ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i);
-            }
+            RowShared* head = other(0);
+            each([&](float x, int i) {
+                if (x > -INFINITY && z_bin(x) <= top.bin) head->list[atomicAdd(&head->n_list, 1u)] = token_of(x, i);
+            });
             cluster.sync();
             if (rank != 0) return;
-            sort((int)n_list);  // falling logits, equal ones by rising index
-            // thread tid has places 2 tid and 2 tid + 1
-            const int e0 = 2 * tid;
-            u64 tok[2];
-            u64 w[2];
+            sort((int)n_list);
+            u64* weights = (u64*)&sh.hist[0][0];  // nobody reads the histogram any more
+            u64 tok[2], w[2];
             bool passes[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                tok[j] = e0 + j < (int)n_list ? sh.list[e0 + j] : ~0ull;
-                const uint32_t key = ~(uint32_t)(tok[j] >> 32);
-                w[j] = e0 + j < (int)n_list ? weight(of_key(key)) : 0ull;
-                passes[j] = e0 + j < (int)n_list && (!s.use_k || e0 + j < s.k);
-                if (!passes[j]) w[j] = 0;
+                passes[j] = e0 + j < (int)n_list && e0 + j < s.k;
+                tok[j] = passes[j] ? sh.list[e0 + j] : ~0ull;
+                w[j] = passes[j] ? weight(logit_of(tok[j])) : 0ull;
             }
             u64 incl = block_scan(w[0] + w[1], sh.sums64);
-            if (tid == SP_THREADS - 1) sh.x_w[0] = incl;
+            if (tid == SP_THREADS - 1) sh.pick_w = incl;
             __syncthreads();
-            const u64 goal = s.use_p ? p_goal(s.use_k ? sh.x_w[0] : whole) : ~0ull;
+            const u64 goal = s.use_p ? p_goal(sh.pick_w) : ~0ull;
             u64 before = incl - (w[0] + w[1]);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                passes[j] = passes[j] && (before <= goal) && (~(uint32_t)(tok[j] >> 32) >= key_m || e0 + j == 0);
+                passes[j] = passes[j] && before <= goal && (logit_of(tok[j]) >= x_m || e0 + j == 0);
                 before += w[j];
             }
-            // the kept ones by rising index, each with its place in the order of weights (their weights stay where they can be found)
-            const uint32_t n_kept = (uint32_t)__syncthreads_count(passes[0]) + (uint32_t)__syncthreads_count(passes[1]);
+            // the kept ones by rising index, each with its place in the order of weights, where its weight stays
+            const int n_kept = __syncthreads_count(passes[0]) + __syncthreads_count(passes[1]);
 #pragma unroll
             for (int j = 0; j < 2; j++)
-                if (passes[j]) {
-                    sh.weights[e0 + j] = w[j];
-                    sh.list[e0 + j] = (tok[j] << 32) | (u64)(uint32_t)(e0 + j);
-                }
-            sort((int)n_kept);
+                if (passes[j]) weights[e0 + j] = w[j], sh.list[e0 + j] = (tok[j] << 32) | (u64)(uint32_t)(e0 + j);
+            sort(n_kept);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                tok[j] = e0 + j < (int)n_kept ? sh.list[e0 + j] : ~0ull;
-                w[j] = e0 + j < (int)n_kept ? sh.weights[(uint32_t)tok[j]] : 0ull;
+                tok[j] = e0 + j < n_kept ? sh.list[e0 + j] : ~0ull;
+                w[j] = e0 + j < n_kept ? weights[(uint32_t)tok[j]] : 0ull;
             }
             incl = block_scan(w[0] + w[1], sh.sums64);
-            if (tid == SP_THREADS - 1) sh.x_w[0] = incl;
+            if (tid == SP_THREADS - 1) sh.pick_w = incl;
             __syncthreads();
-            const u64 mass = sh.x_w[0], target = min((u64)((double)s.u * (double)mass), mass - 1);
+            const u64 mass = sh.pick_w, target = min((u64)((double)s.u * (double)mass), mass - 1);
             before = incl - (w[0] + w[1]);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -539,52 +550,55 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             }
             return;
         }
-        if (!s.use_k && !s.use_m && top.n_here <= SP_LIST) {
-            // top-p alone: the tokens of the bin, in every CTA
-            uint32_t offset = 0;
-            for (int r = 0; r < rank; r++) offset += sh.here_n[r];
-            for (int i0 = 0; i0 < count; i0 += SP_THREADS) {
-                const int i = i0 + tid;
-                const float x = i < count ? x_s[i] : -INFINITY;
+        if (!s.use_k && !s.use_m) {
+            // top-p alone: the tokens of the bin, in every CTA; each CTA has a part of the list
+            each([&](float x, int i) {
                 if (x > -INFINITY && z_bin(x) == top.bin) {
-                    const uint32_t slot = offset + atomicAdd(&sh.n_list, 1u);
-                    const u64 tok = ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i);
-                    for (int r = 0; r < C; r++) cluster.map_shared_rank(&sh, r)->list[slot] = tok;
+                    const uint32_t slot = atomicAdd(&sh.n_list, 1u);
+                    if (slot < SP_PART)
+                        for (int r = 0; r < C; r++) other(r)->list[rank * SP_PART + slot] = token_of(x, i);
                 }
-            }
-            cluster.sync();
-            sort((int)top.n_here);
-            const int e0 = 2 * tid;
-            u64 tok[2], w[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                tok[j] = e0 + j < (int)top.n_here ? sh.list[e0 + j] : ~0ull;
-                w[j] = e0 + j < (int)top.n_here ? weight(of_key(~(uint32_t)(tok[j] >> 32))) : 0ull;
-            }
-            const u64 incl = block_scan(w[0] + w[1], sh.sums64), goal = p_goal(whole);
-            u64 sum = top.w_before + incl - (w[0] + w[1]);
-            u64 own = 0, low = 0;  // kept mass of the bin in this CTA's slice, and in the slices before it
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                if (w[j] && sum <= goal) {
-                    const int at = (int)(uint32_t)tok[j];
-                    if (at < first) low += w[j];
-                    else if (at < first + count) own += w[j];
-                    if (sum + w[j] > goal) sh.pick = (uint32_t)(e0 + j), sh.pick_w = sum + w[j];  // the last kept token, and the kept mass
-                }
-                sum += w[j];
-            }
-            low = block_scan(low, sh.sums64);
-            if (tid == SP_THREADS - 1) sh.x_w[0] = low;
-            own = block_scan(own, sh.sums64);
-            if (tid == SP_THREADS - 1) sh.x_w[1] = own;
+            });
             __syncthreads();
-            const u64 last = sh.list[sh.pick];
-            key_cut = ~(uint32_t)(last >> 32), last_same = (uint32_t)last;
-            u64 before = sh.x_w[0];
-            for (int r = 0; r < rank; r++) before += sh.before_w[r];
-            draw(sh.pick_w, before, sh.before_w[rank] + sh.x_w[1]);
-            return;
+            if (tid < C) other(tid)->part[rank] = sh.n_list;
+            cluster.sync();
+            uint32_t most = 0;
+            for (int r = 0; r < C; r++) most = max(most, sh.part[r]);
+            if (most <= SP_PART) {  // the same in every CTA
+                for (int i = tid; i < C * SP_PART; i += SP_THREADS)
+                    if (i % SP_PART >= (int)sh.part[i / SP_PART]) sh.list[i] = ~0ull;
+                sort(C * SP_PART);
+                u64 tok[2], w[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    tok[j] = e0 + j < C * SP_PART ? sh.list[e0 + j] : ~0ull;
+                    w[j] = tok[j] != ~0ull ? weight(logit_of(tok[j])) : 0ull;
+                }
+                u64 sum = top.w_before + block_scan(w[0] + w[1], sh.sums64) - (w[0] + w[1]);
+                const u64 goal = p_goal(whole);
+                u64 own = 0, low = 0;  // kept mass of the bin in this CTA's slice, and in the slices before it
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if (w[j] && sum <= goal) {
+                        const int at = (int)(uint32_t)tok[j];
+                        if (at < first) low += w[j];
+                        else if (at < first + count) own += w[j];
+                        if (sum + w[j] > goal) sh.pick = (uint32_t)(e0 + j), sh.pick_w = sum + w[j];  // the last kept token, and the kept mass
+                    }
+                    sum += w[j];
+                }
+                low = block_scan(low, sh.sums64);
+                if (tid == SP_THREADS - 1) sh.x_w[0] = low;
+                own = block_scan(own, sh.sums64);
+                if (tid == SP_THREADS - 1) sh.x_w[1] = own;
+                __syncthreads();
+                const u64 last = sh.list[sh.pick];
+                x_cut = logit_of(last), last_same = (uint32_t)last;
+                u64 before = sh.x_w[0];
+                for (int r = 0; r < rank; r++) before += sh.before_w[r];
+                draw(sh.pick_w, before, sh.before_w[rank] + sh.x_w[1]);
+                return;
+            }
         }
         // many tokens: down to the last kept one
         auto by_rank = [&](float x, int, uint32_t* at) {  // positions rise as logits fall
@@ -608,36 +622,36 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         if (s.use_k && hit.bin != 0xffffffffu) {
             keys_of_bin(hit.bin);
             const Hit f = refine(false, key_max - sh.key_hi, key_max - sh.key_lo, hit.n_before, 0, by_rank, (u64)(s.k - 1));
-            key_cut = key_max - f.bin, n_cut = (uint32_t)s.k - f.n_before, n_same = f.n_here;
+            x_cut = of_key(key_max - f.bin), n_cut = (uint32_t)s.k - f.n_before, n_same = f.n_here;
         }
         if (s.use_p) {
-            if (s.use_k) {  // the mass of the first k: of everything down to key_cut, without the equal ones that are left out
-                const u64 over = n_same == 0xffffffffu ? 0ull : (u64)(n_same - n_cut) * weight(of_key(key_cut));
+            if (s.use_k) {  // the mass of the first k: of everything down to x_cut, without the equal ones that are left out
+                const u64 over = n_same == 0xffffffffu ? 0ull : (u64)(n_same - n_cut) * weight(x_cut);
                 next_round();
-                hit = round_of(true, 0, 0, [&](float x, int) -> int { return key_of(x) >= key_cut ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
+                hit = round_of(true, true, 0, 0, [&](float x, int) -> int { return x >= x_cut && x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
                     whole = all - over;
                     return p_goal(whole);
                 });
             }
             keys_of_bin(hit.bin);
             const u64 goal = p_goal(whole);
-            const Hit f = refine(true, key_max - sh.key_hi, key_max - max(sh.key_lo, key_cut), hit.n_before, hit.w_before, by_rank, goal);
+            const Hit f = refine(true, key_max - sh.key_hi, key_max - max(sh.key_lo, key_of(x_cut)), hit.n_before, hit.w_before, by_rank, goal);
             const u64 w = f.w_here / f.n_here;  // all of them have the same weight, which is not 0
-            const uint32_t n = (uint32_t)min((goal + 1 - f.w_before + w - 1) / w, (u64)f.n_here), key = key_max - f.bin;
-            if (key > key_cut || n < n_cut) key_cut = key, n_cut = n, n_same = f.n_here;
+            const uint32_t n = (uint32_t)min((goal + 1 - f.w_before + w - 1) / w, (u64)f.n_here);
+            const float x = of_key(key_max - f.bin);
+            if (x > x_cut || n < n_cut) x_cut = x, n_cut = n, n_same = f.n_here;
         }
-        if (s.use_m && key_m > key_cut) key_cut = key_m, n_cut = n_same = 0xffffffffu;
+        if (x_m > x_cut) x_cut = x_m, n_cut = n_same = 0xffffffffu;
         if (n_cut < n_same)  // equal logits: the first n_cut by index
             last_same = refine(false, 0, (uint32_t)p.n - 1, 0, 0, [&](float x, int i, uint32_t* at) {
                 *at = (uint32_t)i;
-                return key_of(x) == key_cut;
+                return x == x_cut;
             }, (u64)(n_cut - 1)).bin;
     } else {
-        key_cut = key_m;
+        x_cut = x_m;
     }
-
     of_slice = run_masses();
-    if (tid < C) cluster.map_shared_rank(&sh, tid)->x_w[rank] = of_slice;
+    if (tid < C) other(tid)->x_w[rank] = of_slice;
     cluster.sync();
     u64 mass = 0, before = 0;
     for (int r = 0; r < C; r++) {
