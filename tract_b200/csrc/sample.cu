@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -34,12 +35,12 @@ namespace cg = cooperative_groups;
 
 namespace b200kv {
 
-constexpr int SP_THREADS = 512;
-constexpr int SP_WARPS = SP_THREADS / 32;
+constexpr int SP_MAX_WARPS = 32;
 constexpr int SP_CLUSTER = 8;       // most CTAs of a row (the portable cluster size)
 constexpr int SP_SLICE = 16384;     // logits a CTA takes before another one is added: 64 KB, two CTAs per SM
 constexpr int SP_BINS = 1024;
-constexpr int SP_LIST = 1024;       // tokens that are sorted
+constexpr int SP_LIST = 1024;       // tokens that are gathered
+constexpr int SP_COUNT = 256;       // up to so many are put in order by counting, more by sorting
 constexpr int SP_PART = SP_LIST / SP_CLUSTER;  // top-p: a CTA's part of them
 constexpr int SP_TABLE = 256;       // steps of 2^(1 / 256)
 constexpr int W_BITS = 44;          // fractional bits of a weight
@@ -100,6 +101,7 @@ struct Hit {
     uint32_t bin;               // 0xffffffff: nowhere
     uint32_t n_before, n_here;  // tokens before the bin and in it
     u64 w_before, w_here;       // their weights
+    u64 all;                    // the whole count or mass
 };
 
 struct RowShared {
@@ -111,18 +113,19 @@ struct RowShared {
     u64 x_w[SP_CLUSTER];
     uint32_t run_n[SP_CLUSTER][32];  // sums of 32 runs of 32 bins of every CTA
     u64 run_w[SP_CLUSTER][32];
-    uint32_t n_list;                 // entries of the list (top-k), or a CTA's own part of it (top-p)
-    uint32_t part[SP_CLUSTER];       // tokens of every CTA in the list (top-p)
+    uint32_t part[SP_CLUSTER];       // entries of every CTA in the list
     // of this CTA
+    uint16_t part_n[1024];
     uint32_t bin_n[SP_CLUSTER][32];  // the bins of one run of every CTA
     u64 bin_w[SP_CLUSTER][32];
     u64 before_w[SP_CLUSTER];        // mass of every CTA before the hit
-    u64 sums64[SP_WARPS + 1];
-    u64 warp_w[SP_WARPS];
-    float red_max[SP_WARPS];
+    u64 sums64[SP_MAX_WARPS + 1];
+    u64 warp_w[SP_MAX_WARPS];
+    float red_max[SP_MAX_WARPS];
+    uint32_t n_list;                 // this CTA's entries of the list so far
     uint32_t key_lo, key_hi, found;
     u64 pick_w;
-    uint32_t pick;
+    Hit hit;
 };
 
 // Inclusive sums over the CTA in thread order.
@@ -136,7 +139,7 @@ __device__ inline u64 block_scan(u64 v, u64* warp_sums) {
     __syncthreads();  // the sums of the scan before are no longer read
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
-    u64 mine = lane < warp ? warp_sums[lane] : 0ull;  // SP_WARPS <= 32
+    u64 mine = lane < warp ? warp_sums[lane] : 0ull;
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     return mine + v;
@@ -163,7 +166,10 @@ __device__ inline uint32_t first_key(uint32_t lo, uint32_t hi, F holds) {
     return lo;
 }
 
-__global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
+// T threads: 512, two CTAs per SM, or 1024 where a launch has no second CTA for an SM anyway.
+template <int T>
+__global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
+    constexpr int SP_THREADS = T, SP_WARPS = T / 32;
     extern __shared__ __align__(16) uint8_t row_smem[];
     RowShared& sh = *(RowShared*)row_smem;
     cg::cluster_group cluster = cg::this_cluster();
@@ -180,6 +186,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
 
     // ---- 1. the slice into shared memory, its maximum ----
     const RowSettings s = row_settings(p, row);
+    constexpr float PER_OCTAVE = (float)(SP_BINS - 1) / 28.f;
+    const float zscale = 1.4426950408889634f / s.t * PER_OCTAVE;
+    const double t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;
     float best = -INFINITY;
     {
         const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
@@ -271,14 +280,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     }
 
     // ---- weights ----
-    // depth of a logit: 1023 / 46 x log2(1 / w), cut off at 1023; monotone in x
-    const float zscale = 1.4426950408889634f / s.t * ((float)(SP_BINS - 1) / 46.f);
-    auto depth = [&](float x) -> float { return fminf((x_top - x) * zscale, (float)(SP_BINS - 1)); };
-    auto z_bin = [&](float x) -> uint32_t { return __float_as_uint(depth(x) + 8388608.f) & (SP_BINS - 1); };  // rounded to the nearest whole number
+    // bins of log2(1 / w), 1 / 36 wide; the last one takes everything from 28 on; monotone in x
+    auto z_bin = [&](float x) -> uint32_t {  // rounded to the nearest whole number
+        return __float_as_uint(fminf((x_top - x) * zscale, (float)(SP_BINS - 1)) + 8388608.f) & (SP_BINS - 1);
+    };
     // exp((x - max) / T) = 2^(t / 256), t = (x - max) 256 log2 e / T = n + r, n whole: 2^(n / 256) from the table and the exponent,
     // 2^(r / 256) by its Taylor polynomial of degree 3 in r ln 2 / 256 (|r| <= 1/2: what is left out is below 1.5e-13), rounded
-    // to 44 fractional bits by adding 1.5 * 2^8.  From depth 1023 on (2^-46): 0.
-    const double t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)s.t, top64 = (double)x_top;
+    // to 44 fractional bits by adding 1.5 * 2^8.  Below 2^-46: 0.
+    const double top64 = (double)x_top;
     auto weight = [&](float x) -> u64 {
         constexpr double L = 0.69314718055994530942 / SP_TABLE, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
         const double t = ((double)x - top64) * t_unit;
@@ -290,7 +299,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         const double tab = sh.exp2_table[n & (SP_TABLE - 1)];
         const double scaled = __hiloint2double(__double2hiint(tab) + ((n >> 8) << 20), __double2loint(tab));
         const u64 w = (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
-        return depth(x) < (float)(SP_BINS - 1) ? w : 0ull;
+        return (x_top - x) * zscale < 46.f * PER_OCTAVE ? w : 0ull;
     };
     // f(x, place in the slice) for every logit of the slice; the fill is -inf
     auto each = [&](auto f) {
@@ -316,29 +325,54 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     // ---- a histogram over the cluster, and the bin in which the running count or mass first exceeds its goal ----
     // bin_of(x, index): 0 .. SP_BINS - 1, or -1 for what does not take part.  goal(all): from the whole count or mass.
     // *_base: what lies before the first bin.  The caller sees to it that the histogram is clear and that the CTAs have left it.
-    // COUNT / WEIGHT: what is added up (the goal is a mass where there are weights).
+    // counts / weights: what is added up (std::true_type or false_type; the goal is a mass where there are weights).
     auto limbs = [](const RowShared* o, int b) -> u64 { return (u64)o->hist[0][b] + ((u64)o->hist[1][b] << SP_LIMB) + ((u64)o->hist[2][b] << (2 * SP_LIMB)); };
-    auto round_of = [&](bool counts, bool weights, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
+    auto round_of = [&](auto counts_, auto weights_, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
+        // The last bin, which takes all that is deep, is added up in registers: atomics on one address follow one another.
+        constexpr bool counts = decltype(counts_)::value, weights = decltype(weights_)::value;
+        uint32_t deep_n = 0;
+        u64 deep_w = 0;
         each([&](float x, int i) {
             const int b = bin_of(x, first + i);
-            if (b < 0) return;
+            const u64 w = weights ? weight(x) : 0ull;
+            const bool deep = b == SP_BINS - 1;
+            if (counts) deep_n += deep;
+            if (weights) deep_w += deep ? w : 0ull;
+            if (b < 0 || deep) return;
             if (counts) atomicAdd(&sh.hist[3][b], 1u);
-            if (weights) {
-                const u64 w = weight(x);
-                const uint32_t l0 = (uint32_t)w & 0x7fffu, l1 = (uint32_t)(w >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w >> (2 * SP_LIMB));
-                if (l0) atomicAdd(&sh.hist[0][b], l0);
-                if (l1) atomicAdd(&sh.hist[1][b], l1);
-                if (l2) atomicAdd(&sh.hist[2][b], l2);
-            }
+            if (!weights) return;
+            const uint32_t l0 = (uint32_t)w & 0x7fffu, l1 = (uint32_t)(w >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w >> (2 * SP_LIMB));
+            if (l0) atomicAdd(&sh.hist[0][b], l0);
+            if (l1) atomicAdd(&sh.hist[1][b], l1);
+            if (l2) atomicAdd(&sh.hist[2][b], l2);
         });
-        __syncthreads();
-        {  // 16 threads per run of 32 bins; the sums go to every CTA
-            uint32_t n = counts ? sh.hist[3][2 * tid] + sh.hist[3][2 * tid + 1] : 0u;
-            u64 w = weights ? limbs(&sh, 2 * tid) + limbs(&sh, 2 * tid + 1) : 0ull;
+        if (counts) {
+            deep_n = __reduce_add_sync(0xffffffffu, deep_n);
+            if (lane == 0 && deep_n) atomicAdd(&sh.hist[3][SP_BINS - 1], deep_n);
+        }
+        if (weights) {
 #pragma unroll
-            for (int o = 8; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o), w += __shfl_xor_sync(0xffffffffu, w, o);
-            const int to = tid & 15;
-            if (to < C) other(to)->run_n[rank][tid >> 4] = n, other(to)->run_w[rank][tid >> 4] = w;
+            for (int o = 16; o; o >>= 1) deep_w += __shfl_xor_sync(0xffffffffu, deep_w, o);
+            if (lane == 0 && deep_w) {
+                atomicAdd(&sh.hist[0][SP_BINS - 1], (uint32_t)deep_w & 0x7fffu);
+                atomicAdd(&sh.hist[1][SP_BINS - 1], (uint32_t)(deep_w >> SP_LIMB) & 0x7fffu);
+                atomicAdd(&sh.hist[2][SP_BINS - 1], (uint32_t)(deep_w >> (2 * SP_LIMB)));
+            }
+        }
+        __syncthreads();
+        {  // the sums of every run of 32 bins go to every CTA
+            constexpr int PER = SP_BINS / T, LANES = 32 / PER;  // bins per thread, threads per run
+            uint32_t n = 0;
+            u64 w = 0;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                if (counts) n += sh.hist[3][PER * tid + j];
+                if (weights) w += limbs(&sh, PER * tid + j);
+            }
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o), w += __shfl_xor_sync(0xffffffffu, w, o);
+            const int to = tid % LANES;
+            if (to < C) other(to)->run_n[rank][tid / LANES] = n, other(to)->run_w[rank][tid / LANES] = w;
         }
         cluster.sync();
         // lane = run: the run in which the goal is passed, then lane = bin of that run.  Inclusive sums over the lanes.
@@ -350,43 +384,55 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
                 if (lane >= o) n += un, w += uw;
             }
         };
-        uint32_t n = 0;
-        u64 w = 0;
-        for (int r = 0; r < C; r++) n += sh.run_n[r][lane], w += sh.run_w[r][lane];
-        uint32_t n_incl = n;
-        u64 w_incl = w;
-        scan(n_incl, w_incl);
-        const u64 target = goal(__shfl_sync(0xffffffffu, weights ? w_incl : (u64)n_incl, 31));
-        const uint32_t runs = __ballot_sync(0xffffffffu, (weights ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
-        if (!runs) return Hit{0xffffffffu, 0, 0, 0, 0};  // in every CTA alike
-        const int run = __ffs(runs) - 1;
-        const uint32_t n_run = n_base + __shfl_sync(0xffffffffu, n_incl - n, run);
-        const u64 w_run = w_base + __shfl_sync(0xffffffffu, w_incl - w, run);
+        // (a warp per CTA of the cluster: the search itself is the same in all of them)
+        uint32_t n = 0, n_incl = 0, n_run = 0, runs = 0;
+        u64 w = 0, w_incl = 0, w_run = 0, all = 0, target = 0;
+        int run = 0;
         if (warp < C) {
-            const RowShared* o = other(warp);
-            sh.bin_n[warp][lane] = counts ? o->hist[3][run * 32 + lane] : 0u;
-            sh.bin_w[warp][lane] = weights ? limbs(o, run * 32 + lane) : 0ull;
+            for (int r = 0; r < C; r++) n += sh.run_n[r][lane], w += sh.run_w[r][lane];
+            n_incl = n, w_incl = w;
+            scan(n_incl, w_incl);
+            all = __shfl_sync(0xffffffffu, weights ? w_incl : (u64)n_incl, 31);
+            target = goal(all);
+            runs = __ballot_sync(0xffffffffu, (weights ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
+            if (runs) {
+                run = __ffs(runs) - 1;
+                const RowShared* o = other(warp);
+                sh.bin_n[warp][lane] = counts ? o->hist[3][run * 32 + lane] : 0u;
+                sh.bin_w[warp][lane] = weights ? limbs(o, run * 32 + lane) : 0ull;
+                n_run = n_base + __shfl_sync(0xffffffffu, n_incl - n, run);
+                w_run = w_base + __shfl_sync(0xffffffffu, w_incl - w, run);
+            }
         }
         __syncthreads();
-        n = 0, w = 0;
-        for (int r = 0; r < C; r++) n += sh.bin_n[r][lane], w += sh.bin_w[r][lane];
-        n_incl = n, w_incl = w;
-        scan(n_incl, w_incl);
-        const uint32_t bins = __ballot_sync(0xffffffffu, (weights ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
-        const int bin = __ffs(bins) - 1;
-        Hit h;
-        h.bin = (uint32_t)(run * 32 + bin);
-        h.n_here = __shfl_sync(0xffffffffu, n, bin), h.w_here = __shfl_sync(0xffffffffu, w, bin);
-        h.n_before = n_run + __shfl_sync(0xffffffffu, n_incl - n, bin), h.w_before = w_run + __shfl_sync(0xffffffffu, w_incl - w, bin);
-        if (warp < C && weights) {  // what every CTA has before the bin
-            u64 v = (lane < run ? sh.run_w[warp][lane] : 0ull) + (lane < bin ? sh.bin_w[warp][lane] : 0ull);
+        if (warp < C) {
+            if (runs) {
+                n = 0, w = 0;
+                for (int r = 0; r < C; r++) n += sh.bin_n[r][lane], w += sh.bin_w[r][lane];
+                n_incl = n, w_incl = w;
+                scan(n_incl, w_incl);
+                const uint32_t bins = __ballot_sync(0xffffffffu, (weights ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
+                const int bin = __ffs(bins) - 1;
+                if (warp == 0 && lane == bin) sh.hit = Hit{(uint32_t)(run * 32 + bin), n_run + n_incl - n, n, w_run + w_incl - w, w, all};
+                if (weights) {  // what every CTA has before the bin
+                    u64 v = (lane < run ? sh.run_w[warp][lane] : 0ull) + (lane < bin ? sh.bin_w[warp][lane] : 0ull);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) sh.before_w[warp] = v;
+                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (lane == 0) sh.before_w[warp] = v;
+                }
+                if (counts) {  // its tokens up to the end of the bin
+                    const uint32_t v = __reduce_add_sync(0xffffffffu, (lane < run ? sh.run_n[warp][lane] : 0u) + (lane <= bin ? sh.bin_n[warp][lane] : 0u));
+                    if (lane == 0) sh.part[warp] = v;
+                }
+            } else if (warp == 0 && lane == 0) {
+                sh.hit = Hit{0xffffffffu, 0, 0, 0, 0, all};  // in every CTA alike
+            }
         }
         __syncthreads();
-        return h;
+        return sh.hit;
     };
+    const std::true_type yes;
+    const std::false_type no;
     // clears the histogram for another round, once every CTA has read what it needs of the last one
     auto next_round = [&]() {
         cluster.sync();
@@ -394,11 +440,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         __syncthreads();
     };
     // The same over positions lo .. hi, 1024 at a time, down to a single one; bin holds the position.
-    auto refine = [&](bool weights, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
+    auto refine = [&](auto weights, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
         for (;;) {
             const int bits = 32 - __clz((hi - lo) | 1u), shift = bits > 10 ? bits - 10 : 0;
             next_round();
-            Hit h = round_of(true, weights, n_base, w_base, [&](float x, int i) -> int {
+            Hit h = round_of(yes, weights, n_base, w_base, [&](float x, int i) -> int {
                 uint32_t at;
                 return place(x, i, &at) && at >= lo && at <= hi ? (int)((at - lo) >> shift) : -1;
             }, [&](u64) { return target; });
@@ -416,7 +462,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
     uint32_t last_same = 0xffffffffu;
     u64 of_slice = 0;
     bool runs_known = false;
-    auto kept_weight = [&](float x, int i) -> u64 { return x > x_cut || (x == x_cut && (uint32_t)(first + i) <= last_same) ? weight(x) : 0ull; };
+    auto kept = [&](float x, int i) -> bool { return x > x_cut || (x == x_cut && (uint32_t)(first + i) <= last_same); };
+    auto kept_weight = [&](float x, int i) -> u64 { return kept(x, i) ? weight(x) : 0ull; };
     const int run = ((quads + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;  // quads of a warp
     // the kept mass of the slice; of a run per warp in warp_w
     auto run_masses = [&]() -> u64 {
@@ -428,10 +475,13 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
                 mine += weight(v.x) + weight(v.y) + weight(v.z) + weight(v.w);
             }
         } else {
-            for (int u = warp * run + lane; u < end; u += 32) {
-                const float4 v = ((const float4*)x_s)[u];
-                if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x_cut)
-                    mine += kept_weight(v.x, 4 * u) + kept_weight(v.y, 4 * u + 1) + kept_weight(v.z, 4 * u + 2) + kept_weight(v.w, 4 * u + 3);
+            for (int u0 = warp * run; u0 < end; u0 += 32) {
+                const int u = u0 + lane;
+                const float4 v = u < end ? ((const float4*)x_s)[u] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x_cut)) continue;
+                // all four without branches: they run side by side
+                const u64 w[4] = {weight(v.x), weight(v.y), weight(v.z), weight(v.w)};
+                mine += (kept(v.x, 4 * u) ? w[0] : 0ull) + (kept(v.y, 4 * u + 1) ? w[1] : 0ull) + (kept(v.z, 4 * u + 2) ? w[2] : 0ull) + (kept(v.w, 4 * u + 3) ? w[3] : 0ull);
             }
         }
 #pragma unroll
@@ -473,10 +523,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             const u64 least = (u64)ceil((double)s.p * (double)mass);
             return least ? least - 1 : 0;
         };
-        const Hit top = round_of(s.use_k, !s.use_k, 0, 0, [&](float x, int) -> int { return x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
-            whole = all;
-            return s.use_k ? (u64)(s.k - 1) : p_goal(all);
-        });
+        auto by_depth = [&](float x, int) -> int { return x > -INFINITY ? (int)z_bin(x) : -1; };
+        const Hit top = s.use_k ? round_of(yes, no, 0, 0, by_depth, [&](u64) -> u64 { return (u64)(s.k - 1); }) : round_of(no, yes, 0, 0, by_depth, p_goal);
+        whole = top.all;
         // bitonic sort of list[0 .. n): every step, a thread per pair; steps of up to 32 stay inside the 64 entries of a warp
         auto sort = [&](int n) {
             int size = 64;
@@ -498,22 +547,83 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         auto token_of = [&](float x, int i) -> u64 { return ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i); };  // sorts by falling logits, then by index
         auto logit_of = [](u64 token) -> float { return of_key(~(uint32_t)(token >> 32)); };
         const int e0 = 2 * tid;  // of a sorted list, thread tid has places 2 tid and 2 tid + 1
-        // ---- 3. few enough tokens down to the lower border of that bin: sort them ----
+        // For every entry of list[0 .. n), n <= SP_COUNT, what lies before it in the order of the entries: their number and the
+        // sum of weights[].  Thread i < n gets entry i.  All threads count: every warp walks a share of the list, each lane for
+        // an entry of its own.
+        u64* weights = (u64*)&sh.hist[0][0];          // the histogram is not used any more by then
+        u64* part_w = weights + SP_LIST;              // [T]
+        static_assert((SP_LIST + 1024) * 8 <= sizeof(sh.hist), "weights, and a sum for each thread");
+        auto count_before = [&](int n, uint32_t* n_before, u64* w_before) {
+            int wide = 32;
+            while (wide < n) wide <<= 1;
+            const int shares = T / wide, i = tid & (wide - 1), share = tid / wide;
+            const u64 mine = i < n ? sh.list[i] : 0ull;
+            uint32_t cn = 0;
+            u64 cw = 0;
+            for (int j = share * n / shares; j < (share + 1) * n / shares; j++)
+                if (sh.list[j] < mine) cn++, cw += weights[j];
+            __syncthreads();
+            part_w[tid] = cw, sh.part_n[tid] = (uint16_t)cn;
+            __syncthreads();
+            cn = 0, cw = 0;
+            if (tid < n)
+                for (int j = 0; j < shares; j++) cn += sh.part_n[j * wide + tid], cw += part_w[j * wide + tid];
+            *n_before = cn, *w_before = cw;
+        };
+        // sums of a over the CTA, one after the other; everybody gets them
+        auto block_sums = [&](u64 a, u64 b, u64* sa, u64* sb) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o), b += __shfl_xor_sync(0xffffffffu, b, o);
+            __syncthreads();
+            if (lane == 0) sh.sums64[warp] = a, sh.warp_w[warp] = b;
+            __syncthreads();
+            *sa = *sb = 0;
+#pragma unroll
+            for (int w = 0; w < SP_WARPS; w++) *sa += sh.sums64[w], *sb += sh.warp_w[w];
+        };
+        // ---- 3. few enough tokens down to the lower border of that bin: put them in order ----
         const uint32_t n_list = !s.use_k ? 0xffffffffu : top.bin == 0xffffffffu ? (uint32_t)min(whole, (u64)SP_LIST + 1) : top.n_before + top.n_here;
         if (n_list <= SP_LIST) {
+            uint32_t offset = 0;
+            if (top.bin != 0xffffffffu) {
+                for (int r = 0; r < rank; r++) offset += sh.part[r];
+            } else {  // all numbers of the row
+                for (int r = 0; r < rank; r++)
+                    for (int j = 0; j < 32; j++) offset += sh.run_n[r][j];
+            }
             RowShared* head = other(0);
             each([&](float x, int i) {
-                if (x > -INFINITY && z_bin(x) <= top.bin) head->list[atomicAdd(&head->n_list, 1u)] = token_of(x, i);
+                if (x > -INFINITY && z_bin(x) <= top.bin) head->list[offset + atomicAdd(&sh.n_list, 1u)] = token_of(x, i);
             });
             cluster.sync();
             if (rank != 0) return;
-            sort((int)n_list);
-            u64* weights = (u64*)&sh.hist[0][0];  // nobody reads the histogram any more
+            const int n = (int)n_list;
+            if (n <= SP_COUNT) {
+                const u64 tok = tid < n ? sh.list[tid] : ~0ull, w = tid < n ? weight(logit_of(tok)) : 0ull;
+                if (tid < n) weights[tid] = w;
+                __syncthreads();
+                uint32_t at;
+                u64 before;
+                count_before(n, &at, &before);
+                if (tid < n && (int)at == min(n, s.k) - 1) sh.pick_w = before + w;  // the mass of the first k
+                __syncthreads();
+                const u64 goal = s.use_p ? p_goal(sh.pick_w) : ~0ull;
+                const bool keeps = tid < n && (int)at < s.k && before <= goal && (logit_of(tok) >= x_m || at == 0);
+                const int n_kept = __syncthreads_count(keeps);
+                if (keeps && (int)at == n_kept - 1) sh.pick_w = before + w;  // the kept mass
+                if (tid < n) sh.list[tid] = (tok << 32) | (u64)tid, weights[tid] = keeps ? w : 0ull;  // by rising index now
+                __syncthreads();
+                const u64 mass = sh.pick_w, target = min((u64)((double)s.u * (double)mass), mass - 1);
+                count_before(n, &at, &before);
+                if (keeps && before <= target && before + w > target) p.out[row] = (int32_t)(uint32_t)tok;
+                return;
+            }
+            sort(n);
             u64 tok[2], w[2];
             bool passes[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                passes[j] = e0 + j < (int)n_list && e0 + j < s.k;
+                passes[j] = e0 + j < n && e0 + j < s.k;
                 tok[j] = passes[j] ? sh.list[e0 + j] : ~0ull;
                 w[j] = passes[j] ? weight(logit_of(tok[j])) : 0ull;
             }
@@ -565,38 +675,56 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
             uint32_t most = 0;
             for (int r = 0; r < C; r++) most = max(most, sh.part[r]);
             if (most <= SP_PART) {  // the same in every CTA
-                for (int i = tid; i < C * SP_PART; i += SP_THREADS)
-                    if (i % SP_PART >= (int)sh.part[i / SP_PART]) sh.list[i] = ~0ull;
-                sort(C * SP_PART);
+                // close the gaps between the parts
+                int n = 0, to[2] = {-1, -1};
                 u64 tok[2], w[2];
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    tok[j] = e0 + j < C * SP_PART ? sh.list[e0 + j] : ~0ull;
-                    w[j] = tok[j] != ~0ull ? weight(logit_of(tok[j])) : 0ull;
+                for (int j = 0; j < 2; j++) tok[j] = e0 + j < C * SP_PART ? sh.list[e0 + j] : 0ull;
+                for (int r = 0; r < C; r++) {
+                    const int d = e0 - r * SP_PART, m = (int)sh.part[r];
+                    if (d >= 0 && d < m) to[0] = n + d;
+                    if (d + 1 >= 0 && d + 1 < m) to[1] = n + d + 1;
+                    n += m;
                 }
-                u64 sum = top.w_before + block_scan(w[0] + w[1], sh.sums64) - (w[0] + w[1]);
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    if (to[j] >= 0) sh.list[to[j]] = tok[j];
+                __syncthreads();
                 const u64 goal = p_goal(whole);
                 u64 own = 0, low = 0;  // kept mass of the bin in this CTA's slice, and in the slices before it
+                auto keep = [&](u64 token, u64 w, u64 sum) {
+                    if (!w || sum > goal) return;
+                    const int at = (int)(uint32_t)token;
+                    if (at < first) low += w;
+                    else if (at < first + count) own += w;
+                    if (sum + w > goal) sh.list[SP_LIST - 1] = token, sh.pick_w = sum + w;  // the last kept token, and the kept mass
+                };
+                if (n <= SP_COUNT) {
+                    const u64 token = tid < n ? sh.list[tid] : 0ull, mine = tid < n ? weight(logit_of(token)) : 0ull;
+                    if (tid < n) weights[tid] = mine;
+                    __syncthreads();
+                    uint32_t at;
+                    u64 before;
+                    count_before(n, &at, &before);
+                    keep(token, mine, top.w_before + before);
+                } else {
+                    sort(n);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if (w[j] && sum <= goal) {
-                        const int at = (int)(uint32_t)tok[j];
-                        if (at < first) low += w[j];
-                        else if (at < first + count) own += w[j];
-                        if (sum + w[j] > goal) sh.pick = (uint32_t)(e0 + j), sh.pick_w = sum + w[j];  // the last kept token, and the kept mass
+                    for (int j = 0; j < 2; j++) {
+                        tok[j] = e0 + j < n ? sh.list[e0 + j] : ~0ull;
+                        w[j] = e0 + j < n ? weight(logit_of(tok[j])) : 0ull;
                     }
-                    sum += w[j];
+                    const u64 sum = top.w_before + block_scan(w[0] + w[1], sh.sums64) - (w[0] + w[1]);
+                    keep(tok[0], w[0], sum);
+                    keep(tok[1], w[1], sum + w[0]);
                 }
-                low = block_scan(low, sh.sums64);
-                if (tid == SP_THREADS - 1) sh.x_w[0] = low;
-                own = block_scan(own, sh.sums64);
-                if (tid == SP_THREADS - 1) sh.x_w[1] = own;
-                __syncthreads();
-                const u64 last = sh.list[sh.pick];
+                u64 below, here;
+                block_sums(low, own, &below, &here);
+                const u64 last = sh.list[SP_LIST - 1];
                 x_cut = logit_of(last), last_same = (uint32_t)last;
-                u64 before = sh.x_w[0];
-                for (int r = 0; r < rank; r++) before += sh.before_w[r];
-                draw(sh.pick_w, before, sh.before_w[rank] + sh.x_w[1]);
+                for (int r = 0; r < rank; r++) below += sh.before_w[r];
+                draw(sh.pick_w, below, here + sh.before_w[rank]);
                 return;
             }
         }
@@ -621,21 +749,19 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         Hit hit = top;
         if (s.use_k && hit.bin != 0xffffffffu) {
             keys_of_bin(hit.bin);
-            const Hit f = refine(false, key_max - sh.key_hi, key_max - sh.key_lo, hit.n_before, 0, by_rank, (u64)(s.k - 1));
+            const Hit f = refine(no, key_max - sh.key_hi, key_max - sh.key_lo, hit.n_before, 0, by_rank, (u64)(s.k - 1));
             x_cut = of_key(key_max - f.bin), n_cut = (uint32_t)s.k - f.n_before, n_same = f.n_here;
         }
         if (s.use_p) {
             if (s.use_k) {  // the mass of the first k: of everything down to x_cut, without the equal ones that are left out
                 const u64 over = n_same == 0xffffffffu ? 0ull : (u64)(n_same - n_cut) * weight(x_cut);
                 next_round();
-                hit = round_of(true, true, 0, 0, [&](float x, int) -> int { return x >= x_cut && x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 {
-                    whole = all - over;
-                    return p_goal(whole);
-                });
+                hit = round_of(yes, yes, 0, 0, [&](float x, int) -> int { return x >= x_cut && x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 { return p_goal(all - over); });
+                whole = hit.all - over;
             }
             keys_of_bin(hit.bin);
             const u64 goal = p_goal(whole);
-            const Hit f = refine(true, key_max - sh.key_hi, key_max - max(sh.key_lo, key_of(x_cut)), hit.n_before, hit.w_before, by_rank, goal);
+            const Hit f = refine(yes, key_max - sh.key_hi, key_max - max(sh.key_lo, key_of(x_cut)), hit.n_before, hit.w_before, by_rank, goal);
             const u64 w = f.w_here / f.n_here;  // all of them have the same weight, which is not 0
             const uint32_t n = (uint32_t)min((goal + 1 - f.w_before + w - 1) / w, (u64)f.n_here);
             const float x = of_key(key_max - f.bin);
@@ -643,7 +769,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleParams p) {
         }
         if (x_m > x_cut) x_cut = x_m, n_cut = n_same = 0xffffffffu;
         if (n_cut < n_same)  // equal logits: the first n_cut by index
-            last_same = refine(false, 0, (uint32_t)p.n - 1, 0, 0, [&](float x, int i, uint32_t* at) {
+            last_same = refine(no, 0, (uint32_t)p.n - 1, 0, 0, [&](float x, int i, uint32_t* at) {
                 *at = (uint32_t)i;
                 return x == x_cut;
             }, (u64)(n_cut - 1)).bin;
@@ -702,16 +828,19 @@ extern "C" int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, 
     const int c = sample_cluster(rows, n);
     p.slice = sample_slice(c, n);
     p.scratch = n > MAX_ON_CHIP ? (float*)scratch : nullptr;
+    // 1024 threads where a launch has at most one CTA for an SM
+    const bool wide = rows * c <= 148;
     const size_t smem = ((sizeof(RowShared) + 15) & ~(size_t)15) + (p.scratch ? 0 : (size_t)p.slice * sizeof(float));
-    B200KV_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    auto kernel = wide ? sample_kernel<1024> : sample_kernel<512>;
+    B200KV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)c, (unsigned)rows), cfg.blockDim = dim3(SP_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream_;
+    cfg.gridDim = dim3((unsigned)c, (unsigned)rows), cfg.blockDim = dim3(wide ? 1024 : 512), cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream_;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = 2;
-    B200KV_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel, p));
+    B200KV_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return B200KV_OK;
 }
