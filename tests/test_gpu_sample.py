@@ -187,6 +187,12 @@ def test_settings_at_their_ends(kv):
         first, last = kv.sample(x, dev(one(0.0)), **kw), kv.sample(x, dev(one(np.nextafter(np.float32(1), np.float32(0)))), **kw)
         assert torch.equal(kv.sample(x, dev(one(-3.0)), **kw), first) and torch.equal(kv.sample(x, dev(one(float("nan"))), **kw), first)
         assert bool((kv.sample(x, dev(one(7.0)), **kw) >= last).all())
+    for t in (1e-3, 1e-5, 1e-7, 1e-9, 1e-12, 1e-30):  # down to where neighbouring floats are far apart
+        near = torch.full((2, 5000), 9.0, device="cuda")
+        near[:, 7::3] = float(np.nextafter(np.float32(10), np.float32(0)))
+        near[:, 9::11] = 10.0
+        for kw in (dict(), dict(p=np.full(2, 0.7, np.float32)), dict(k=np.full(2, 900, np.int32))):
+            check(kv, near, [0.31, 0.87], np.full(2, t), **kw)
     inf_t = kv.sample(x, dev(one(0.5)), temperature=dev(one(float("inf"))))  # a uniform draw
     assert (inf_t.cpu().numpy() == 1500).all()
 

@@ -111,6 +111,7 @@ struct RowShared {
     // written by the other CTAs of the cluster
     float x_max[SP_CLUSTER];
     u64 x_w[SP_CLUSTER];
+    u64 last, pick_w;                // the last kept token, and the kept mass
     uint32_t run_n[SP_CLUSTER][32];  // sums of 32 runs of 32 bins of every CTA
     u64 run_w[SP_CLUSTER][32];
     uint32_t part[SP_CLUSTER];       // entries of every CTA in the list
@@ -124,7 +125,6 @@ struct RowShared {
     float red_max[SP_MAX_WARPS];
     uint32_t n_list;                 // this CTA's entries of the list so far
     uint32_t key_lo, key_hi, found;
-    u64 pick_w;
     Hit hit;
 };
 
@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     // ---- 1. the slice into shared memory, its maximum ----
     const RowSettings s = row_settings(p, row);
     constexpr float PER_OCTAVE = (float)(SP_BINS - 1) / 28.f;
-    const float zscale = 1.4426950408889634f / s.t * PER_OCTAVE;
-    const double t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;
+    float zscale = 1.4426950408889634f / s.t * PER_OCTAVE;
+    double t_unit = s.greedy ? 0.0 : (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;
     float best = -INFINITY;
     {
         const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
@@ -279,6 +279,13 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         __syncthreads();
     }
 
+    if (s.t < fabsf(x_top) * 0x1p-34f) {
+        // Other logits lie at least 2^-24 |max| below the maximum: they have no weight at this temperature, nor at the one that is
+        // taken in its place, at which products with 1 / T keep their accuracy.
+        const float t = fabsf(x_top) * 0x1p-34f;
+        t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)t, zscale = 1.4426950408889634f / t * PER_OCTAVE;
+    }
+
     // ---- weights ----
     // bins of log2(1 / w), 1 / 36 wide; the last one takes everything from 28 on; monotone in x
     auto z_bin = [&](float x) -> uint32_t {  // rounded to the nearest whole number
@@ -287,19 +294,19 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     // exp((x - max) / T) = 2^(t / 256), t = (x - max) 256 log2 e / T = n + r, n whole: 2^(n / 256) from the table and the exponent,
     // 2^(r / 256) by its Taylor polynomial of degree 3 in r ln 2 / 256 (|r| <= 1/2: what is left out is below 1.5e-13), rounded
     // to 44 fractional bits by adding 1.5 * 2^8.  Below 2^-46: 0.
-    const double top64 = (double)x_top;
+    const double t_top = -(double)x_top * t_unit;
+    const float x_floor = __double2float_rd((double)x_top - 46.5 * (double)SP_TABLE / t_unit);  // 2^-46.5 rounds to 0
     auto weight = [&](float x) -> u64 {
         constexpr double L = 0.69314718055994530942 / SP_TABLE, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
-        const double t = ((double)x - top64) * t_unit;
+        const double t = fma((double)fmaxf(x, x_floor), t_unit, t_top);
         const double biased = t + MAGIC, r = t - (biased - MAGIC);
-        const int n = __double2loint(biased);
+        const int n = max(__double2loint(biased), -64 * SP_TABLE);  // the next float below the maximum may be deeper than that
         double q = fma(r, L * L * L / 6.0, L * L / 2.0);
         q = fma(q, r, L);
         q = fma(q, r, 1.0);
         const double tab = sh.exp2_table[n & (SP_TABLE - 1)];
-        const double scaled = __hiloint2double(__double2hiint(tab) + ((n >> 8) << 20), __double2loint(tab));
-        const u64 w = (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
-        return (x_top - x) * zscale < 46.f * PER_OCTAVE ? w : 0ull;
+        const double scaled = __hiloint2double(__double2hiint(tab) + ((n << 12) & 0xfff00000), __double2loint(tab));
+        return (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
     };
     // f(x, place in the slice) for every logit of the slice; the fill is -inf
     auto each = [&](auto f) {
@@ -314,7 +321,7 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     if (s.use_m) {
         if (warp == 0) {
             const uint32_t k = first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t key) {
-                return key == key_max || exp(((double)of_key(key) - top64) / (double)s.t) >= (double)s.min_p;
+                return key == key_max || exp(((double)of_key(key) - (double)x_top) / (double)s.t) >= (double)s.min_p;
             });
             if (lane == 0) sh.found = k;
         }
@@ -332,20 +339,31 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         constexpr bool counts = decltype(counts_)::value, weights = decltype(weights_)::value;
         uint32_t deep_n = 0;
         u64 deep_w = 0;
-        each([&](float x, int i) {
-            const int b = bin_of(x, first + i);
-            const u64 w = weights ? weight(x) : 0ull;
-            const bool deep = b == SP_BINS - 1;
-            if (counts) deep_n += deep;
-            if (weights) deep_w += deep ? w : 0ull;
-            if (b < 0 || deep) return;
-            if (counts) atomicAdd(&sh.hist[3][b], 1u);
-            if (!weights) return;
-            const uint32_t l0 = (uint32_t)w & 0x7fffu, l1 = (uint32_t)(w >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w >> (2 * SP_LIMB));
-            if (l0) atomicAdd(&sh.hist[0][b], l0);
-            if (l1) atomicAdd(&sh.hist[1][b], l1);
-            if (l2) atomicAdd(&sh.hist[2][b], l2);
-        });
+        for (int u = tid; u < quads; u += SP_THREADS) {
+            const float4 v = ((const float4*)x_s)[u];
+            const float x[4] = {v.x, v.y, v.z, v.w};
+            u64 w[4];
+            int b[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {  // the four side by side, then their atomics
+                b[e] = bin_of(x[e], first + 4 * u + e);
+                w[e] = weights ? weight(x[e]) : 0ull;
+                const bool deep = b[e] == SP_BINS - 1;
+                if (counts) deep_n += deep && x[e] > -INFINITY;
+                if (weights) deep_w += deep ? w[e] : 0ull;
+                if (deep) b[e] = -1;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (b[e] < 0) continue;
+                if (counts) atomicAdd(&sh.hist[3][b[e]], 1u);
+                if (!weights) continue;
+                const uint32_t l0 = (uint32_t)w[e] & 0x7fffu, l1 = (uint32_t)(w[e] >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w[e] >> (2 * SP_LIMB));
+                if (l0) atomicAdd(&sh.hist[0][b[e]], l0);
+                if (l1) atomicAdd(&sh.hist[1][b[e]], l1);
+                if (l2) atomicAdd(&sh.hist[2][b[e]], l2);
+            }
+        }
         if (counts) {
             deep_n = __reduce_add_sync(0xffffffffu, deep_n);
             if (lane == 0 && deep_n) atomicAdd(&sh.hist[3][SP_BINS - 1], deep_n);
@@ -523,7 +541,7 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             const u64 least = (u64)ceil((double)s.p * (double)mass);
             return least ? least - 1 : 0;
         };
-        auto by_depth = [&](float x, int) -> int { return x > -INFINITY ? (int)z_bin(x) : -1; };
+        auto by_depth = [&](float x, int) -> int { return (int)z_bin(x); };
         const Hit top = s.use_k ? round_of(yes, no, 0, 0, by_depth, [&](u64) -> u64 { return (u64)(s.k - 1); }) : round_of(no, yes, 0, 0, by_depth, p_goal);
         whole = top.all;
         // bitonic sort of list[0 .. n): every step, a thread per pair; steps of up to 32 stay inside the 64 entries of a warp
@@ -569,17 +587,6 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             if (tid < n)
                 for (int j = 0; j < shares; j++) cn += sh.part_n[j * wide + tid], cw += part_w[j * wide + tid];
             *n_before = cn, *w_before = cw;
-        };
-        // sums of a over the CTA, one after the other; everybody gets them
-        auto block_sums = [&](u64 a, u64 b, u64* sa, u64* sb) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o), b += __shfl_xor_sync(0xffffffffu, b, o);
-            __syncthreads();
-            if (lane == 0) sh.sums64[warp] = a, sh.warp_w[warp] = b;
-            __syncthreads();
-            *sa = *sb = 0;
-#pragma unroll
-            for (int w = 0; w < SP_WARPS; w++) *sa += sh.sums64[w], *sb += sh.warp_w[w];
         };
         // ---- 3. few enough tokens down to the lower border of that bin: put them in order ----
         const uint32_t n_list = !s.use_k ? 0xffffffffu : top.bin == 0xffffffffu ? (uint32_t)min(whole, (u64)SP_LIST + 1) : top.n_before + top.n_here;
@@ -660,10 +667,11 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             }
             return;
         }
-        if (!s.use_k && !s.use_m) {
+        if (!s.use_k && !s.use_m && top.bin < SP_BINS - 1) {
             // top-p alone: the tokens of the bin, in every CTA; each CTA has a part of the list
+            const float in_bin = 8388608.f + (float)top.bin;  // what z_bin rounds them to
             each([&](float x, int i) {
-                if (x > -INFINITY && z_bin(x) == top.bin) {
+                if ((x_top - x) * zscale + 8388608.f == in_bin) {
                     const uint32_t slot = atomicAdd(&sh.n_list, 1u);
                     if (slot < SP_PART)
                         for (int r = 0; r < C; r++) other(r)->list[rank * SP_PART + slot] = token_of(x, i);
@@ -675,56 +683,40 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             uint32_t most = 0;
             for (int r = 0; r < C; r++) most = max(most, sh.part[r]);
             if (most <= SP_PART) {  // the same in every CTA
-                // close the gaps between the parts
-                int n = 0, to[2] = {-1, -1};
-                u64 tok[2], w[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) tok[j] = e0 + j < C * SP_PART ? sh.list[e0 + j] : 0ull;
-                for (int r = 0; r < C; r++) {
-                    const int d = e0 - r * SP_PART, m = (int)sh.part[r];
-                    if (d >= 0 && d < m) to[0] = n + d;
-                    if (d + 1 >= 0 && d + 1 < m) to[1] = n + d + 1;
-                    n += m;
-                }
+                for (int i = tid; i < C * SP_PART; i += SP_THREADS) weights[i] = i % SP_PART < (int)sh.part[i / SP_PART] ? weight(logit_of(sh.list[i])) : 0ull;
                 __syncthreads();
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    if (to[j] >= 0) sh.list[to[j]] = tok[j];
-                __syncthreads();
+                // the mass before each of this CTA's own tokens, in the order of the whole bin: 4 threads per token
                 const u64 goal = p_goal(whole);
-                u64 own = 0, low = 0;  // kept mass of the bin in this CTA's slice, and in the slices before it
-                auto keep = [&](u64 token, u64 w, u64 sum) {
-                    if (!w || sum > goal) return;
-                    const int at = (int)(uint32_t)token;
-                    if (at < first) low += w;
-                    else if (at < first + count) own += w;
-                    if (sum + w > goal) sh.list[SP_LIST - 1] = token, sh.pick_w = sum + w;  // the last kept token, and the kept mass
-                };
-                if (n <= SP_COUNT) {
-                    const u64 token = tid < n ? sh.list[tid] : 0ull, mine = tid < n ? weight(logit_of(token)) : 0ull;
-                    if (tid < n) weights[tid] = mine;
-                    __syncthreads();
-                    uint32_t at;
-                    u64 before;
-                    count_before(n, &at, &before);
-                    keep(token, mine, top.w_before + before);
-                } else {
-                    sort(n);
+                const int mine = tid / 4;  // SP_PART tokens, 4 * SP_PART = 512 threads
+                const bool is_token = mine < (int)sh.part[rank];
+                const u64 token = is_token ? sh.list[rank * SP_PART + mine] : 0ull;
+                u64 sum = 0;
+                for (int r = 0; r < C; r++)
+                    for (int j = tid & 3; j < (int)sh.part[r]; j += 4)
+                        if (sh.list[r * SP_PART + j] < token) sum += weights[r * SP_PART + j];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum += top.w_before;
+                const u64 w = is_token ? weights[rank * SP_PART + mine] : 0ull;
+                const bool keeps = w && sum <= goal;
+                if (keeps && sum + w > goal && (tid & 3) == 0)  // the last kept token: everybody learns of it
+                    for (int r = 0; r < C; r++) other(r)->last = token, other(r)->pick_w = sum + w;
+                u64 kept_here = keeps && (tid & 3) == 0 ? w : 0ull;
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        tok[j] = e0 + j < n ? sh.list[e0 + j] : ~0ull;
-                        w[j] = e0 + j < n ? weight(logit_of(tok[j])) : 0ull;
-                    }
-                    const u64 sum = top.w_before + block_scan(w[0] + w[1], sh.sums64) - (w[0] + w[1]);
-                    keep(tok[0], w[0], sum);
-                    keep(tok[1], w[1], sum + w[0]);
+                for (int o = 16; o; o >>= 1) kept_here += __shfl_xor_sync(0xffffffffu, kept_here, o);
+                __syncthreads();
+                if (lane == 0) sh.warp_w[warp] = kept_here;
+                __syncthreads();
+                if (tid < C) {
+                    kept_here = sh.before_w[rank];
+                    for (int w = 0; w < SP_WARPS; w++) kept_here += sh.warp_w[w];
+                    other(tid)->x_w[rank] = kept_here;
                 }
-                u64 below, here;
-                block_sums(low, own, &below, &here);
-                const u64 last = sh.list[SP_LIST - 1];
-                x_cut = logit_of(last), last_same = (uint32_t)last;
-                for (int r = 0; r < rank; r++) below += sh.before_w[r];
-                draw(sh.pick_w, below, here + sh.before_w[rank]);
+                cluster.sync();
+                x_cut = logit_of(sh.last), last_same = (uint32_t)sh.last;
+                u64 below = 0;
+                for (int r = 0; r < rank; r++) below += sh.x_w[r];
+                draw(sh.pick_w, below, sh.x_w[rank]);
                 return;
             }
         }
