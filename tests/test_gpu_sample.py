@@ -59,7 +59,7 @@ def plain_row(x, t, k, p, m, u):
     return token, float(np.abs(borders - goal).min() / cdf[-1]) if u > 0 else 1.0
 
 
-def check(kv, logits, u, t=None, k=None, p=None, m=None, near=2.0 ** -36):
+def checked(kv, logits, u, t=None, k=None, p=None, m=None, near=2.0 ** -36):
     """All rows against plain_row.  Fixed-point weights are off by at most 2^-45, n of them by n 2^-45 (n <= 2^18: 2^-27 in the
     worst case, 2^-36 for errors of either sign): a row whose draw is nearer to a border than that would say nothing, and none
     may be."""
@@ -75,6 +75,9 @@ def check(kv, logits, u, t=None, k=None, p=None, m=None, near=2.0 ** -36):
         assert gap > near, ("borders too near", i, gap)
         assert got[i] == want, (i, int(got[i]), want)
     return got
+
+
+check = checked
 
 
 def model_logits(seed, rows, n, io="f32", pad=0, spread=2.2):
@@ -116,17 +119,21 @@ def test_many_rows_with_settings_of_their_own(kv, rows, n):
 
 @pytest.mark.parametrize("mode", ["plain", "top_p", "top_k", "k_p"])
 @pytest.mark.parametrize("spread,temperature", [(0.02, 1.0), (2.0, 30.0), (1.0, 1.0), (6.0, 0.05)])
-def test_flat_and_peaked_rows(kv, mode, spread, temperature):
+@pytest.mark.parametrize("rows", [3, 200])
+def test_flat_and_peaked_rows(kv, mode, spread, temperature, rows):
     # flat rows keep more tokens than are gathered, peaked ones a single one
-    rows, n = 3, 30000
+    n = 30000
     g = np.random.Generator(np.random.Philox(key=7))
     x = torch.from_numpy((g.standard_normal((rows, n)) * spread).astype(np.float32)).cuda()
     kw = dict(plain={}, top_p=dict(p=np.full(rows, 0.97)), top_k=dict(k=np.full(rows, 12345)), k_p=dict(k=np.full(rows, 20000), p=np.full(rows, 0.6)))[mode]
     check(kv, x, g.random(rows), np.full(rows, temperature), **kw)
 
 
-def test_equal_logits_are_taken_by_rising_index(kv):
+@pytest.mark.parametrize("copies", [1, 50])
+def test_equal_logits_are_taken_by_rising_index(kv, copies):
     n = 9000
+    six = lambda a: np.tile(np.asarray(a), copies)
+    check = lambda kv, x, u, **kw: checked(kv, x.repeat(copies, 1), six(u), **{k: six(v) for k, v in kw.items()})[:len(u)]
     x = torch.full((6, n), -1.0, device="cuda")
     x[:, 5::7] = 2.0  # 1285 equal maxima
     x[:, 3::7] = 1.5
@@ -147,7 +154,8 @@ def test_equal_logits_are_taken_by_rising_index(kv):
     assert check(kv, zero, [0.6], k=[5])[0] == 3
 
 
-def test_infinities_nan_and_empty_rows(kv):
+@pytest.mark.parametrize("copies", [1, 40])  # few rows, many rows
+def test_infinities_nan_and_empty_rows(kv, copies):
     inf, nan = float("inf"), float("nan")
     n = 5000
     x = torch.randn((8, n), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
@@ -161,9 +169,11 @@ def test_infinities_nan_and_empty_rows(kv):
     x[6, :] = torch.finfo(torch.float32).min  # masks of the type's lowest value: a row of them is flat
     x[7, :] = torch.finfo(torch.float32).min
     x[7, 17] = 1.0
-    u = np.full(8, 0.71)
-    for kw in ({}, dict(k=np.full(8, 20)), dict(p=np.full(8, 0.9, np.float32)), dict(m=np.full(8, 0.1, np.float32)),
-               dict(k=np.full(8, 2500), p=np.full(8, 0.8, np.float32)), dict(k=np.full(8, 4990))):
+    x = x.repeat(copies, 1)
+    rows = 8 * copies
+    u = np.full(rows, 0.71)
+    for kw in ({}, dict(k=np.full(rows, 20)), dict(p=np.full(rows, 0.9, np.float32)), dict(m=np.full(rows, 0.1, np.float32)),
+               dict(k=np.full(rows, 2500), p=np.full(rows, 0.8, np.float32)), dict(k=np.full(rows, 4990))):
         got = check(kv, x, u, **kw)
         assert got[0] == 0 and got[1] == 0 and got[2] < 100 and got[3] == 4000 and got[4] % 2 == 0 and got[5] == 4321 and got[7] == 17
 

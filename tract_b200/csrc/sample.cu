@@ -41,13 +41,13 @@ constexpr int SP_SLICE = 16384;     // logits a CTA takes before another one is 
 constexpr int SP_BINS = 1024;
 constexpr int SP_LIST = 1024;       // tokens that are gathered
 constexpr int SP_COUNT = 256;       // up to so many are put in order by counting, more by sorting
-constexpr int SP_PART = SP_LIST / SP_CLUSTER;  // top-p: a CTA's part of them
 constexpr int SP_TABLE = 256;       // steps of 2^(1 / 256)
 constexpr int W_BITS = 44;          // fractional bits of a weight
 constexpr int SP_LIMB = 15;         // a weight enters a histogram as three 15-bit limbs: 2^17 of them fit a 32-bit counter
 constexpr int MAX_VOCAB = 1 << 19;  // so many weights of 1 add up to 2^63
 constexpr int MAX_ON_CHIP = SP_CLUSTER * 32768;  // 128 KB per CTA; the slices of longer rows go to the workspace
-static_assert(MAX_VOCAB / SP_CLUSTER < (1 << 17), "the limbs of a bin of one CTA");
+constexpr int MAX_SLICE = 1 << 17;  // logits whose limbs a 32-bit counter holds
+static_assert(MAX_VOCAB <= SP_CLUSTER * MAX_SLICE, "slices of the longest rows");
 
 typedef unsigned long long u64;
 
@@ -106,6 +106,7 @@ struct Hit {
 
 struct RowShared {
     uint32_t hist[4][SP_BINS];     // limbs of the masses; counts
+    uint32_t aside[32];            // one for each lane: where what does not take part is counted
     u64 list[SP_LIST];             // gathered tokens
     double exp2_table[SP_TABLE];   // 2^(j / SP_TABLE)
     // written by the other CTAs of the cluster
@@ -166,82 +167,129 @@ __device__ inline uint32_t first_key(uint32_t lo, uint32_t hi, F holds) {
     return lo;
 }
 
-// T threads: 512, two CTAs per SM, or 1024 where a launch has no second CTA for an SM anyway.
-template <int T>
+__device__ inline void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory");
+}
+__device__ inline void cp_async8(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory");
+}
+__device__ inline void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ inline void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+constexpr int RING = 4;  // quads of a thread on their way
+
+// T threads, 1024 per SM.  ON_CHIP: the slice stays in shared memory; otherwise every pass reads it again, from L2 for the
+// most part, and many rows are in flight at once.
+template <int T, bool ON_CHIP>
 __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
-    constexpr int SP_THREADS = T, SP_WARPS = T / 32;
+    constexpr int SP_WARPS = T / 32;
     extern __shared__ __align__(16) uint8_t row_smem[];
     RowShared& sh = *(RowShared*)row_smem;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.y;
-    // the slice, cleaned, and filled up with -inf to a multiple of 4
+    // the slice on the chip, cleaned, and filled up with -inf to a multiple of 4
     float* x_s = p.scratch ? p.scratch + ((int64_t)row * C + rank) * p.slice : (float*)(row_smem + ((sizeof(RowShared) + 15) & ~(size_t)15));
     const int first = rank * p.slice, count = max(0, min(p.slice, p.n - first)), quads = (count + 3) / 4;
+    const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
     auto other = [&](int r) -> RowShared* { return cluster.map_shared_rank(&sh, r); };
+    auto widen = [&](uint32_t lo, uint32_t hi) -> float4 {  // four 16-bit logits
+        if (p.dtype == B200KV_F16) {
+            const float2 a = __half22float2(*(const __half2*)&lo), b = __half22float2(*(const __half2*)&hi);
+            return make_float4(a.x, a.y, b.x, b.y);
+        }
+        return make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
+    };
+    // logits 4 u .. 4 u + 3 of the slice as they are (a NaN stays one off the chip: it passes no comparison and has no weight)
+    auto from_memory = [&](int u) -> float4 {
+        if (p.vec && 4 * u + 4 <= count) {
+            if (p.dtype == B200KV_F32) return __ldg((const float4*)base + u);
+            const uint2 w = __ldg((const uint2*)base + u);
+            return widen(w.x, w.y);
+        }
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = 4 * u + e < count ? ld_as_f32(base, p.dtype, 4 * u + e) : -INFINITY;
+        return make_float4(v[0], v[1], v[2], v[3]);
+    };
+    auto quad = [&](int u) -> float4 { return ON_CHIP ? ((const float4*)x_s)[u] : from_memory(u); };
+    auto logit = [&](int i) -> float { return ON_CHIP ? x_s[i] : i < count ? ld_as_f32(base, p.dtype, i) : -INFINITY; };
+    // f(quad, its number) for quads u, u + step, .. < end.  Off the chip a thread has RING quads on their way to slots of its own
+    // in shared memory (registers for them would cost occupancy, unrolled code for them the instruction cache).
+    uint4* ring = (uint4*)(row_smem + ((sizeof(RowShared) + 15) & ~(size_t)15)) + tid;
+    auto sweep = [&](int u, int step, int end, auto f) {
+        if (ON_CHIP || !p.vec) {
+#pragma unroll 1
+            for (; u < end; u += step) f(quad(u), u);
+            return;
+        }
+        const bool f32 = p.dtype == B200KV_F32;
+        auto request = [&](int at, int slot) {
+            if (at < end && 4 * at + 4 <= count) {
+                if (f32) cp_async16(ring + slot * T, (const float4*)base + at);
+                else cp_async8(ring + slot * T, (const uint2*)base + at);
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int j = 0; j < RING; j++) request(u + j * step, j);
+        int slot = 0;
+#pragma unroll 1
+        for (; u < end; u += step) {
+            cp_async_wait<RING - 1>();
+            float4 v;
+            if (4 * u + 4 > count) {
+                v = from_memory(u);  // the last, partial one
+            } else {
+                const uint4 w = ring[slot * T];
+                if (f32) v = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+                else v = widen(w.x, w.y);
+            }
+            f(v, u);
+            request(u + RING * step, slot);  // the slot has been read: f used it
+            slot = (slot + 1) % RING;
+        }
+        cp_async_wait<0>();
+    };
 
     cluster.barrier_arrive();  // every CTA of the cluster runs before one writes into another's shared memory
     grid_launch_dependents();
     grid_dependency_wait();  // the kernel before has written the logits and the settings
 
-    // ---- 1. the slice into shared memory, its maximum ----
+    // ---- 1. the maximum, the slice onto the chip ----
     const RowSettings s = row_settings(p, row);
-    constexpr float PER_OCTAVE = (float)(SP_BINS - 1) / 28.f;
-    float zscale = 1.4426950408889634f / s.t * PER_OCTAVE;
+    // Bins of log2(1 / w), 28 octaves deep, or for top-p as deep as its cut can lie: what is deeper than log2(n / (1 - p)) has, all
+    // of it together, less than 1 - p of the maximum's weight.
+    const float octaves = s.use_p && !s.use_k ? fminf(28.f, log2f((float)p.n / (1.f - s.p)) + 1.f) : 28.f;
+    const float per_octave = (float)(SP_BINS - 1) / octaves;
+    float zscale = 1.4426950408889634f / s.t * per_octave;
     double t_unit = s.greedy ? 0.0 : (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;
     float best = -INFINITY;
-    {
-        const uint8_t* base = (const uint8_t*)p.logits + ((int64_t)row * p.stride + first) * dtype_size(p.dtype);
-        auto take = [&](float v) -> float {
-            v = clean(v);
-            best = fmaxf(best, v);
-            return v;
-        };
-        // every thread has 128 bytes on their way before it uses the first
-        const int per = p.vec ? 16 / dtype_size(p.dtype) : 0, units = p.vec ? count / per : 0;
-        for (int u0 = tid; u0 < units; u0 += 8 * SP_THREADS) {
-            uint4 v[8];
+    for (int u0 = tid; u0 < quads; u0 += 8 * T) {  // every thread has eight quads on their way before it uses the first
+        float4 v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (u0 + j * SP_THREADS < units) v[j] = __ldcs((const uint4*)base + u0 + j * SP_THREADS);
+        for (int j = 0; j < 8; j++)
+            if (u0 + j * T < quads) v[j] = from_memory(u0 + j * T);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int u = u0 + j * SP_THREADS;
-                if (u >= units) continue;
-                const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-                if (p.dtype == B200KV_F32) {
-                    ((float4*)x_s)[u] = make_float4(take(__uint_as_float(w[0])), take(__uint_as_float(w[1])), take(__uint_as_float(w[2])), take(__uint_as_float(w[3])));
-                } else {
-                    float f[8];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float2 g = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
-                        if (p.dtype == B200KV_F16) g = __half22float2(*(const __half2*)&w[e]);
-                        f[2 * e] = take(g.x), f[2 * e + 1] = take(g.y);
-                    }
-                    ((float4*)x_s)[2 * u] = make_float4(f[0], f[1], f[2], f[3]);
-                    ((float4*)x_s)[2 * u + 1] = make_float4(f[4], f[5], f[6], f[7]);
+        for (int j = 0; j < 8; j++)
+            if (u0 + j * T < quads) {
+                if (ON_CHIP) {
+                    v[j] = make_float4(clean(v[j].x), clean(v[j].y), clean(v[j].z), clean(v[j].w));
+                    ((float4*)x_s)[u0 + j * T] = v[j];
                 }
+                best = fmaxf(best, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
             }
-        }
-        for (int i0 = units * per + tid; i0 < count; i0 += 16 * SP_THREADS) {  // rows off the 16-byte grid, and the last few logits
-            float v[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (i0 + j * SP_THREADS < count) v[j] = ld_as_f32(base, p.dtype, i0 + j * SP_THREADS);
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (i0 + j * SP_THREADS < count) x_s[i0 + j * SP_THREADS] = take(v[j]);
-        }
-        if (tid < quads * 4 - count) x_s[count + tid] = -INFINITY;
     }
+    const float own_max = best;  // of this thread's logits
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) sh.red_max[warp] = best;
     if (!s.greedy) {
         if (s.use_k || s.use_p)
-            for (int i = tid; i < SP_BINS; i += SP_THREADS) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
-        for (int i = tid; i < SP_TABLE; i += SP_THREADS) sh.exp2_table[i] = exp2((double)i / SP_TABLE);
+            for (int i = tid; i < SP_BINS; i += T) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = tid; i < SP_TABLE; i += T) sh.exp2_table[i] = exp2((double)i / SP_TABLE);
         if (tid == 0) sh.n_list = 0;
     }
     __syncthreads();
@@ -258,11 +306,10 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         if (rank != top_rank) return;
         int at = x_top == -INFINITY ? 0 : 0x7fffffff;
         if (at)
-            for (int u = tid; u < quads; u += SP_THREADS) {
-                const float4 v = ((const float4*)x_s)[u];
+            sweep(tid, T, quads, [&](const float4& v, int u) {
                 const int i = v.x == x_top ? 0 : v.y == x_top ? 1 : v.z == x_top ? 2 : v.w == x_top ? 3 : 4;
                 if (i < 4) at = min(at, 4 * u + i);
-            }
+            });
         at = __reduce_min_sync(0xffffffffu, at);
         __syncthreads();
         if (lane == 0) sh.red_max[warp] = __int_as_float(at);
@@ -273,21 +320,37 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         }
         return;
     }
-    if (x_top == INFINITY) {  // infinite logits share the row
-        for (int i = tid; i < quads * 4; i += SP_THREADS) x_s[i] = x_s[i] == INFINITY ? 0.f : -INFINITY;
-        x_top = 0.f;
-        __syncthreads();
+    if (x_top == INFINITY) {  // infinite logits share the row: all of the same weight, taken by rising index
+        uint32_t mine = 0;
+        sweep(tid, T, quads, [&](const float4& v, int) { mine += (v.x == INFINITY) + (v.y == INFINITY) + (v.z == INFINITY) + (v.w == INFINITY); });
+        mine = (uint32_t)block_scan(mine, sh.sums64);
+        if (tid == T - 1)
+            for (int r = 0; r < C; r++) other(r)->x_w[rank] = mine;
+        cluster.sync();
+        u64 n = 0, before = 0;
+        for (int r = 0; r < C; r++) {
+            if (r == rank) before = n;
+            n += sh.x_w[r];
+        }
+        if (s.use_k) n = min(n, (u64)s.k);
+        if (s.use_p) n = max((u64)ceil((double)s.p * (double)n), 1ull);
+        const u64 place = min((u64)((double)s.u * (double)n), n - 1);
+        if (place < before || place >= before + sh.x_w[rank] || tid) return;
+        for (int i = 0;; i++)
+            if (logit(i) == INFINITY && before++ == place) {
+                p.out[row] = first + i;
+                return;
+            }
     }
-
     if (s.t < fabsf(x_top) * 0x1p-34f) {
         // Other logits lie at least 2^-24 |max| below the maximum: they have no weight at this temperature, nor at the one that is
         // taken in its place, at which products with 1 / T keep their accuracy.
         const float t = fabsf(x_top) * 0x1p-34f;
-        t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)t, zscale = 1.4426950408889634f / t * PER_OCTAVE;
+        t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)t, zscale = 1.4426950408889634f / t * per_octave;
     }
 
     // ---- weights ----
-    // bins of log2(1 / w), 1 / 36 wide; the last one takes everything from 28 on; monotone in x
+    // the last bin takes everything that is deeper; monotone in x
     auto z_bin = [&](float x) -> uint32_t {  // rounded to the nearest whole number
         return __float_as_uint(fminf((x_top - x) * zscale, (float)(SP_BINS - 1)) + 8388608.f) & (SP_BINS - 1);
     };
@@ -310,13 +373,10 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     };
     // f(x, place in the slice) for every logit of the slice; the fill is -inf
     auto each = [&](auto f) {
-        for (int u = tid; u < quads; u += SP_THREADS) {
-            const float4 v = ((const float4*)x_s)[u];
-            f(v.x, 4 * u), f(v.y, 4 * u + 1), f(v.z, 4 * u + 2), f(v.w, 4 * u + 3);
-        }
+        sweep(tid, T, quads, [&](const float4& v, int u) { f(v.x, 4 * u), f(v.y, 4 * u + 1), f(v.z, 4 * u + 2), f(v.w, 4 * u + 3); });
     };
     // min-p: the smallest logit that passes
-    const uint32_t key_max = key_of(x_top);
+    const uint32_t key_max = key_of(clean(x_top));
     float x_m = -INFINITY;
     if (s.use_m) {
         if (warp == 0) {
@@ -330,20 +390,20 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     }
 
     // ---- a histogram over the cluster, and the bin in which the running count or mass first exceeds its goal ----
-    // bin_of(x, index): 0 .. SP_BINS - 1, or -1 for what does not take part.  goal(all): from the whole count or mass.
+    // feed(f) calls f(quad, its number) for what is looked at.  bin_of(x, index): 0 .. SP_BINS - 1, or -1 for what does not take part.  goal(all): from the whole count or mass.
     // *_base: what lies before the first bin.  The caller sees to it that the histogram is clear and that the CTAs have left it.
-    // counts / weights: what is added up (std::true_type or false_type; the goal is a mass where there are weights).
+    // counts / weights: what is added up (std::true_type or false_type); by_weight: the goal is a mass.
     auto limbs = [](const RowShared* o, int b) -> u64 { return (u64)o->hist[0][b] + ((u64)o->hist[1][b] << SP_LIMB) + ((u64)o->hist[2][b] << (2 * SP_LIMB)); };
-    auto round_of = [&](auto counts_, auto weights_, uint32_t n_base, u64 w_base, auto bin_of, auto goal) -> Hit {
+    auto round_of = [&](auto counts_, auto weights_, auto feed, uint32_t n_base, u64 w_base, auto bin_of, auto goal, bool by_weight) -> Hit {
         // The last bin, which takes all that is deep, is added up in registers: atomics on one address follow one another.
         constexpr bool counts = decltype(counts_)::value, weights = decltype(weights_)::value;
         uint32_t deep_n = 0;
         u64 deep_w = 0;
-        for (int u = tid; u < quads; u += SP_THREADS) {
-            const float4 v = ((const float4*)x_s)[u];
+        feed([&](const float4& v, int u) {
             const float x[4] = {v.x, v.y, v.z, v.w};
             u64 w[4];
             int b[4];
+            bool any = false;
 #pragma unroll
             for (int e = 0; e < 4; e++) {  // the four side by side, then their atomics
                 b[e] = bin_of(x[e], first + 4 * u + e);
@@ -352,18 +412,21 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                 if (counts) deep_n += deep && x[e] > -INFINITY;
                 if (weights) deep_w += deep ? w[e] : 0ull;
                 if (deep) b[e] = -1;
+                any |= b[e] >= 0;
             }
+            if (!any) return;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (b[e] < 0) continue;
-                if (counts) atomicAdd(&sh.hist[3][b[e]], 1u);
-                if (!weights) continue;
-                const uint32_t l0 = (uint32_t)w[e] & 0x7fffu, l1 = (uint32_t)(w[e] >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w[e] >> (2 * SP_LIMB));
-                if (l0) atomicAdd(&sh.hist[0][b[e]], l0);
-                if (l1) atomicAdd(&sh.hist[1][b[e]], l1);
-                if (l2) atomicAdd(&sh.hist[2][b[e]], l2);
+                if (counts) atomicAdd(b[e] < 0 ? &sh.aside[lane] : &sh.hist[3][b[e]], 1u);
+                if (weights) {
+                    if (b[e] < 0) w[e] = 0;
+                    const uint32_t l0 = (uint32_t)w[e] & 0x7fffu, l1 = (uint32_t)(w[e] >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w[e] >> (2 * SP_LIMB));
+                    if (l0) atomicAdd(&sh.hist[0][b[e]], l0);
+                    if (l1) atomicAdd(&sh.hist[1][b[e]], l1);
+                    if (l2) atomicAdd(&sh.hist[2][b[e]], l2);
+                }
             }
-        }
+        });
         if (counts) {
             deep_n = __reduce_add_sync(0xffffffffu, deep_n);
             if (lane == 0 && deep_n) atomicAdd(&sh.hist[3][SP_BINS - 1], deep_n);
@@ -410,9 +473,9 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             for (int r = 0; r < C; r++) n += sh.run_n[r][lane], w += sh.run_w[r][lane];
             n_incl = n, w_incl = w;
             scan(n_incl, w_incl);
-            all = __shfl_sync(0xffffffffu, weights ? w_incl : (u64)n_incl, 31);
+            all = __shfl_sync(0xffffffffu, by_weight ? w_incl : (u64)n_incl, 31);
             target = goal(all);
-            runs = __ballot_sync(0xffffffffu, (weights ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
+            runs = __ballot_sync(0xffffffffu, (by_weight ? w_base + w_incl : (u64)(n_base + n_incl)) > target);
             if (runs) {
                 run = __ffs(runs) - 1;
                 const RowShared* o = other(warp);
@@ -429,7 +492,7 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                 for (int r = 0; r < C; r++) n += sh.bin_n[r][lane], w += sh.bin_w[r][lane];
                 n_incl = n, w_incl = w;
                 scan(n_incl, w_incl);
-                const uint32_t bins = __ballot_sync(0xffffffffu, (weights ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
+                const uint32_t bins = __ballot_sync(0xffffffffu, (by_weight ? w_run + w_incl : (u64)(n_run + n_incl)) > target);
                 const int bin = __ffs(bins) - 1;
                 if (warp == 0 && lane == bin) sh.hit = Hit{(uint32_t)(run * 32 + bin), n_run + n_incl - n, n, w_run + w_incl - w, w, all};
                 if (weights) {  // what every CTA has before the bin
@@ -451,27 +514,12 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     };
     const std::true_type yes;
     const std::false_type no;
+    auto whole_slice = [&](auto f) { sweep(tid, T, quads, f); };
     // clears the histogram for another round, once every CTA has read what it needs of the last one
     auto next_round = [&]() {
         cluster.sync();
-        for (int i = tid; i < SP_BINS; i += SP_THREADS) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = tid; i < SP_BINS; i += T) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
-    };
-    // The same over positions lo .. hi, 1024 at a time, down to a single one; bin holds the position.
-    auto refine = [&](auto weights, uint32_t lo, uint32_t hi, uint32_t n_base, u64 w_base, auto place, u64 target) -> Hit {
-        for (;;) {
-            const int bits = 32 - __clz((hi - lo) | 1u), shift = bits > 10 ? bits - 10 : 0;
-            next_round();
-            Hit h = round_of(yes, weights, n_base, w_base, [&](float x, int i) -> int {
-                uint32_t at;
-                return place(x, i, &at) && at >= lo && at <= hi ? (int)((at - lo) >> shift) : -1;
-            }, [&](u64) { return target; });
-            if (h.bin == 0xffffffffu) return h;
-            h.bin = lo + (h.bin << shift);
-            if (shift == 0) return h;
-            lo = h.bin, hi = min(hi, lo + ((1u << shift) - 1u));
-            n_base = h.n_before, w_base = h.w_before;
-        }
     };
 
     // ---- 4. the draw over whole slices ----
@@ -487,21 +535,13 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     auto run_masses = [&]() -> u64 {
         u64 mine = 0;
         const int end = min(quads, (warp + 1) * run);
-        if (x_cut == -INFINITY) {
-            for (int u = warp * run + lane; u < end; u += 32) {
-                const float4 v = ((const float4*)x_s)[u];
-                mine += weight(v.x) + weight(v.y) + weight(v.z) + weight(v.w);
-            }
-        } else {
-            for (int u0 = warp * run; u0 < end; u0 += 32) {
-                const int u = u0 + lane;
-                const float4 v = u < end ? ((const float4*)x_s)[u] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x_cut)) continue;
-                // all four without branches: they run side by side
-                const u64 w[4] = {weight(v.x), weight(v.y), weight(v.z), weight(v.w)};
-                mine += (kept(v.x, 4 * u) ? w[0] : 0ull) + (kept(v.y, 4 * u + 1) ? w[1] : 0ull) + (kept(v.z, 4 * u + 2) ? w[2] : 0ull) + (kept(v.w, 4 * u + 3) ? w[3] : 0ull);
-            }
-        }
+        sweep(warp * run + lane, 32, end, [&](const float4& v, int u) {
+            // (the votes of the lanes that are still in the loop) nothing kept in any of them: on
+            if (!__any_sync(__activemask(), fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x_cut)) return;
+            // all four without branches: they run side by side
+            const u64 w[4] = {weight(v.x), weight(v.y), weight(v.z), weight(v.w)};
+            mine += (kept(v.x, 4 * u) ? w[0] : 0ull) + (kept(v.y, 4 * u + 1) ? w[1] : 0ull) + (kept(v.z, 4 * u + 2) ? w[2] : 0ull) + (kept(v.w, 4 * u + 3) ? w[3] : 0ull);
+        });
 #pragma unroll
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         __syncthreads();
@@ -520,13 +560,13 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         if (!runs_known) run_masses();
         int w = 0;
         for (; w < SP_WARPS - 1 && target >= before + sh.warp_w[w]; w++) before += sh.warp_w[w];
-        const int lo = 4 * w * run, hi = 4 * min(quads, (w + 1) * run), per = (hi - lo + SP_THREADS - 1) / SP_THREADS;
+        const int lo = 4 * w * run, hi = 4 * min(quads, (w + 1) * run), per = (hi - lo + T - 1) / T;
         u64 mine = 0;
-        for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(x_s[i], i);
+        for (int i = lo + tid * per; i < min(hi, lo + (tid + 1) * per); i++) mine += kept_weight(logit(i), i);
         before += block_scan(mine, sh.sums64) - mine;
         if (before <= target && target < before + mine)
             for (int i = lo + tid * per;; i++) {
-                before += kept_weight(x_s[i], i);
+                before += kept_weight(logit(i), i);
                 if (target < before) {
                     p.out[row] = first + i;
                     break;
@@ -542,19 +582,23 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             return least ? least - 1 : 0;
         };
         auto by_depth = [&](float x, int) -> int { return (int)z_bin(x); };
-        const Hit top = s.use_k ? round_of(yes, no, 0, 0, by_depth, [&](u64) -> u64 { return (u64)(s.k - 1); }) : round_of(no, yes, 0, 0, by_depth, p_goal);
+        auto of_k = [&](u64) -> u64 { return (u64)(s.k - 1); };
+        // Top-k looks at the maxima of the threads first: the k-th largest of them bounds the k-th largest logit from below, and
+        // little more than k logits lie above it.
+        Hit top = s.use_k ? round_of(yes, no, [&](auto f) { f(make_float4(own_max, -INFINITY, -INFINITY, -INFINITY), 0); }, 0, 0, by_depth, of_k, false)
+                          : round_of(no, yes, whole_slice, 0, 0, by_depth, p_goal, true);
         whole = top.all;
         // bitonic sort of list[0 .. n): every step, a thread per pair; steps of up to 32 stay inside the 64 entries of a warp
         auto sort = [&](int n) {
             int size = 64;
             while (size < n) size <<= 1;
             __syncthreads();
-            for (int i = n + tid; i < size; i += SP_THREADS) sh.list[i] = ~0ull;
+            for (int i = n + tid; i < size; i += T) sh.list[i] = ~0ull;
             __syncthreads();
             for (int k = 2; k <= size; k <<= 1)
                 for (int j = k >> 1; j; j >>= 1) {
-                    if (tid < size / 2) {
-                        const int a = 2 * tid - (tid & (j - 1)), b = a + j;
+                    for (int pair = tid; pair < size / 2; pair += T) {
+                        const int a = 2 * pair - (pair & (j - 1)), b = a + j;
                         const u64 va = sh.list[a], vb = sh.list[b];
                         if ((va > vb) == ((a & k) == 0)) sh.list[a] = vb, sh.list[b] = va;
                     }
@@ -562,9 +606,10 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                     else __syncwarp();
                 }
         };
-        auto token_of = [&](float x, int i) -> u64 { return ((u64)~key_of(x) << 32) | (u64)(uint32_t)(first + i); };  // sorts by falling logits, then by index
+        auto token_of = [&](float x, int i) -> u64 { return ((u64)~key_of(clean(x)) << 32) | (u64)(uint32_t)(first + i); };  // sorts by falling logits, then by index
         auto logit_of = [](u64 token) -> float { return of_key(~(uint32_t)(token >> 32)); };
-        const int e0 = 2 * tid;  // of a sorted list, thread tid has places 2 tid and 2 tid + 1
+        constexpr int PLACES = SP_LIST / T;  // of a sorted list, a thread has places e0 .. e0 + PLACES - 1
+        const int e0 = PLACES * tid;
         // For every entry of list[0 .. n), n <= SP_COUNT, what lies before it in the order of the entries: their number and the
         // sum of weights[].  Thread i < n gets entry i.  All threads count: every warp walks a share of the list, each lane for
         // an entry of its own.
@@ -588,23 +633,46 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                 for (int j = 0; j < shares; j++) cn += sh.part_n[j * wide + tid], cw += part_w[j * wide + tid];
             *n_before = cn, *w_before = cw;
         };
-        // ---- 3. few enough tokens down to the lower border of that bin: put them in order ----
-        const uint32_t n_list = !s.use_k ? 0xffffffffu : top.bin == 0xffffffffu ? (uint32_t)min(whole, (u64)SP_LIST + 1) : top.n_before + top.n_here;
-        if (n_list <= SP_LIST) {
-            uint32_t offset = 0;
-            if (top.bin != 0xffffffffu) {
-                for (int r = 0; r < rank; r++) offset += sh.part[r];
-            } else {  // all numbers of the row
-                for (int r = 0; r < rank; r++)
-                    for (int j = 0; j < 32; j++) offset += sh.run_n[r][j];
-            }
-            RowShared* head = other(0);
+        // ---- 3. few enough tokens: put them in order ----
+        // Each CTA has a part of the list, `cap` entries; false: more than that in some CTA (the same answer in every CTA).
+        const int cap = SP_LIST / C;
+        auto gather = [&](bool to_all, auto takes) -> bool {
             each([&](float x, int i) {
-                if (x > -INFINITY && z_bin(x) <= top.bin) head->list[offset + atomicAdd(&sh.n_list, 1u)] = token_of(x, i);
+                if (!takes(x)) return;
+                const uint32_t slot = atomicAdd(&sh.n_list, 1u);
+                if (slot >= (uint32_t)cap) return;
+                const u64 token = token_of(x, i);
+                if (!to_all) other(0)->list[rank * cap + slot] = token;
+                else
+                    for (int r = 0; r < C; r++) other(r)->list[rank * cap + slot] = token;
             });
+            __syncthreads();
+            if (tid < C) other(tid)->part[rank] = sh.n_list;
             cluster.sync();
+            uint32_t most = 0;
+            for (int r = 0; r < C; r++) most = max(most, sh.part[r]);
+            return most <= (uint32_t)cap;
+        };
+        if (s.use_k && top.bin < SP_BINS - 1 && gather(false, [&](float x) { return z_bin(x) <= top.bin; })) {
             if (rank != 0) return;
-            const int n = (int)n_list;
+            // close the gaps between the parts
+            int n = 0, to[PLACES];
+            u64 tok[PLACES], w[PLACES];
+#pragma unroll
+            for (int j = 0; j < PLACES; j++) tok[j] = sh.list[e0 + j], to[j] = -1;
+            for (int r = 0; r < C; r++) {
+#pragma unroll
+                for (int j = 0; j < PLACES; j++) {
+                    const int d = e0 + j - r * cap;
+                    if (d >= 0 && d < (int)sh.part[r]) to[j] = n + d;
+                }
+                n += (int)sh.part[r];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PLACES; j++)
+                if (to[j] >= 0) sh.list[to[j]] = tok[j];
+            __syncthreads();
             if (n <= SP_COUNT) {
                 const u64 tok = tid < n ? sh.list[tid] : ~0ull, w = tid < n ? weight(logit_of(tok)) : 0ull;
                 if (tid < n) weights[tid] = w;
@@ -626,82 +694,79 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                 return;
             }
             sort(n);
-            u64 tok[2], w[2];
-            bool passes[2];
+            u64 sum = 0;
+            bool passes[PLACES];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < PLACES; j++) {
                 passes[j] = e0 + j < n && e0 + j < s.k;
                 tok[j] = passes[j] ? sh.list[e0 + j] : ~0ull;
                 w[j] = passes[j] ? weight(logit_of(tok[j])) : 0ull;
+                sum += w[j];
             }
-            u64 incl = block_scan(w[0] + w[1], sh.sums64);
-            if (tid == SP_THREADS - 1) sh.pick_w = incl;
+            u64 incl = block_scan(sum, sh.sums64);
+            if (tid == T - 1) sh.pick_w = incl;
             __syncthreads();
             const u64 goal = s.use_p ? p_goal(sh.pick_w) : ~0ull;
-            u64 before = incl - (w[0] + w[1]);
+            u64 before = incl - sum;
+            int n_kept = 0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < PLACES; j++) {
                 passes[j] = passes[j] && before <= goal && (logit_of(tok[j]) >= x_m || e0 + j == 0);
                 before += w[j];
+                n_kept += __syncthreads_count(passes[j]);
             }
             // the kept ones by rising index, each with its place in the order of weights, where its weight stays
-            const int n_kept = __syncthreads_count(passes[0]) + __syncthreads_count(passes[1]);
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < PLACES; j++)
                 if (passes[j]) weights[e0 + j] = w[j], sh.list[e0 + j] = (tok[j] << 32) | (u64)(uint32_t)(e0 + j);
             sort(n_kept);
+            sum = 0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < PLACES; j++) {
                 tok[j] = e0 + j < n_kept ? sh.list[e0 + j] : ~0ull;
                 w[j] = e0 + j < n_kept ? weights[(uint32_t)tok[j]] : 0ull;
+                sum += w[j];
             }
-            incl = block_scan(w[0] + w[1], sh.sums64);
-            if (tid == SP_THREADS - 1) sh.pick_w = incl;
+            incl = block_scan(sum, sh.sums64);
+            if (tid == T - 1) sh.pick_w = incl;
             __syncthreads();
             const u64 mass = sh.pick_w, target = min((u64)((double)s.u * (double)mass), mass - 1);
-            before = incl - (w[0] + w[1]);
+            before = incl - sum;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < PLACES; j++) {
                 if (before <= target && before + w[j] > target) p.out[row] = (int32_t)(tok[j] >> 32);
                 before += w[j];
             }
             return;
         }
         if (!s.use_k && !s.use_m && top.bin < SP_BINS - 1) {
-            // top-p alone: the tokens of the bin, in every CTA; each CTA has a part of the list
+            // top-p alone: the tokens of the bin, in every CTA
             const float in_bin = 8388608.f + (float)top.bin;  // what z_bin rounds them to
-            each([&](float x, int i) {
-                if ((x_top - x) * zscale + 8388608.f == in_bin) {
-                    const uint32_t slot = atomicAdd(&sh.n_list, 1u);
-                    if (slot < SP_PART)
-                        for (int r = 0; r < C; r++) other(r)->list[rank * SP_PART + slot] = token_of(x, i);
-                }
-            });
-            __syncthreads();
-            if (tid < C) other(tid)->part[rank] = sh.n_list;
-            cluster.sync();
-            uint32_t most = 0;
-            for (int r = 0; r < C; r++) most = max(most, sh.part[r]);
-            if (most <= SP_PART) {  // the same in every CTA
-                for (int i = tid; i < C * SP_PART; i += SP_THREADS) weights[i] = i % SP_PART < (int)sh.part[i / SP_PART] ? weight(logit_of(sh.list[i])) : 0ull;
+            if (gather(true, [&](float x) { return (x_top - x) * zscale + 8388608.f == in_bin; })) {
+                for (int i = tid; i < C * cap; i += T)
+                    if (i % cap < (int)sh.part[i / cap]) weights[i] = weight(logit_of(sh.list[i]));
                 __syncthreads();
-                // the mass before each of this CTA's own tokens, in the order of the whole bin: 4 threads per token
+                // the mass before each of this CTA's own tokens, in the order of the whole bin; a few threads per token
+                constexpr int LANES = T >= 1024 ? 8 : 4;
                 const u64 goal = p_goal(whole);
-                const int mine = tid / 4;  // SP_PART tokens, 4 * SP_PART = 512 threads
-                const bool is_token = mine < (int)sh.part[rank];
-                const u64 token = is_token ? sh.list[rank * SP_PART + mine] : 0ull;
-                u64 sum = 0;
-                for (int r = 0; r < C; r++)
-                    for (int j = tid & 3; j < (int)sh.part[r]; j += 4)
-                        if (sh.list[r * SP_PART + j] < token) sum += weights[r * SP_PART + j];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                sum += top.w_before;
-                const u64 w = is_token ? weights[rank * SP_PART + mine] : 0ull;
-                const bool keeps = w && sum <= goal;
-                if (keeps && sum + w > goal && (tid & 3) == 0)  // the last kept token: everybody learns of it
-                    for (int r = 0; r < C; r++) other(r)->last = token, other(r)->pick_w = sum + w;
-                u64 kept_here = keeps && (tid & 3) == 0 ? w : 0ull;
+                const int n_own = (int)sh.part[rank];
+                u64 kept_here = 0;
+                for (int m0 = 0; m0 < n_own; m0 += T / LANES) {
+                    const int m = m0 + tid / LANES;
+                    const u64 token = m < n_own ? sh.list[rank * cap + m] : 0ull;
+                    u64 sum = 0;
+                    for (int r = 0; r < C; r++)
+                        for (int j = tid % LANES; j < (int)sh.part[r]; j += LANES)
+                            if (sh.list[r * cap + j] < token) sum += weights[r * cap + j];
+#pragma unroll
+                    for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    sum += top.w_before;
+                    const u64 w = m < n_own ? weights[rank * cap + m] : 0ull;
+                    if (!w || sum > goal || tid % LANES) continue;
+                    kept_here += w;
+                    if (sum + w > goal)  // the last kept token: everybody learns of it
+                        for (int r = 0; r < C; r++) other(r)->last = token, other(r)->pick_w = sum + w;
+                }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) kept_here += __shfl_xor_sync(0xffffffffu, kept_here, o);
                 __syncthreads();
@@ -720,51 +785,78 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                 return;
             }
         }
-        // many tokens: down to the last kept one
-        auto by_rank = [&](float x, int, uint32_t* at) {  // positions rise as logits fall
-            *at = key_max - key_of(x);
-            return x > -INFINITY;
-        };
-        // the bit patterns of a bin of log2 w
-        auto keys_of_bin = [&](uint32_t bin) {
-            __syncthreads();
-            if (warp == 0) {
-                const uint32_t lo = first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t k) { return z_bin(of_key(k)) <= bin; });
-                if (lane == 0) sh.key_lo = lo;
-            } else if (warp == 1) {
-                const uint32_t hi = bin == 0 ? key_max + 1 : first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t k) { return z_bin(of_key(k)) < bin; });
-                if (lane == 0) sh.key_hi = hi - 1;
-            }
-            __syncthreads();
-        };
+        // Many tokens: down to the last kept one, by the same histogram over bit patterns (falling logits) or indices, 1024
+        // positions at a time.  Four questions, one after the other, through one piece of code:
+        //   K     the k-th logit, among the bit patterns of its bin
+        //   MASS  top-p of the first k: their mass, and the bin of log2 w in which p of it is reached
+        //   P     the logit at which it is reached, among the bit patterns of that bin
+        //   SAME  of the logits equal to the last kept one, the index of the last that is kept
+        if (s.use_k) {
+            next_round();
+            top = round_of(yes, no, whole_slice, 0, 0, by_depth, of_k, false);
+        }
+        enum { K, MASS, P, SAME };
         uint32_t n_cut = 0xffffffffu, n_same = 0xffffffffu;
         Hit hit = top;
-        if (s.use_k && hit.bin != 0xffffffffu) {
-            keys_of_bin(hit.bin);
-            const Hit f = refine(no, key_max - sh.key_hi, key_max - sh.key_lo, hit.n_before, 0, by_rank, (u64)(s.k - 1));
-            x_cut = of_key(key_max - f.bin), n_cut = (uint32_t)s.k - f.n_before, n_same = f.n_here;
-        }
-        if (s.use_p) {
-            if (s.use_k) {  // the mass of the first k: of everything down to x_cut, without the equal ones that are left out
-                const u64 over = n_same == 0xffffffffu ? 0ull : (u64)(n_same - n_cut) * weight(x_cut);
-                next_round();
-                hit = round_of(yes, yes, 0, 0, [&](float x, int) -> int { return x >= x_cut && x > -INFINITY ? (int)z_bin(x) : -1; }, [&](u64 all) -> u64 { return p_goal(all - over); });
-                whole = hit.all - over;
+#pragma unroll 1
+        for (int step = K; step <= SAME; step++) {
+            uint32_t lo = 0, hi = SP_BINS - 1, n_base = 0;
+            u64 w_base = 0, goal = 0;
+            u64 over = 0;  // mass of logits equal to the k-th that are not among the first k
+            if (step == K) {
+                if (!s.use_k || hit.bin == 0xffffffffu) continue;
+                goal = (u64)(s.k - 1);
+            } else if (step == MASS) {
+                if (!s.use_k || !s.use_p) continue;
+                if (n_same != 0xffffffffu) over = (u64)(n_same - n_cut) * weight(x_cut);
+            } else if (step == P) {
+                if (!s.use_p) continue;
+                goal = p_goal(whole);
+            } else {
+                if (x_m > x_cut) x_cut = x_m, n_cut = n_same = 0xffffffffu;
+                if (n_cut >= n_same) continue;
+                hi = (uint32_t)p.n - 1, goal = (u64)(n_cut - 1);
             }
-            keys_of_bin(hit.bin);
-            const u64 goal = p_goal(whole);
-            const Hit f = refine(yes, key_max - sh.key_hi, key_max - max(sh.key_lo, key_of(x_cut)), hit.n_before, hit.w_before, by_rank, goal);
-            const u64 w = f.w_here / f.n_here;  // all of them have the same weight, which is not 0
-            const uint32_t n = (uint32_t)min((goal + 1 - f.w_before + w - 1) / w, (u64)f.n_here);
-            const float x = of_key(key_max - f.bin);
-            if (x > x_cut || n < n_cut) x_cut = x, n_cut = n, n_same = f.n_here;
+            if (step == K || step == P) {  // the bit patterns of the bin
+                const uint32_t bin = hit.bin;
+                __syncthreads();
+                if (warp < 2) {
+                    const uint32_t border = bin + 1 - (uint32_t)warp;  // the first pattern less deep than that
+                    const uint32_t k = border == 0 ? key_max + 1 : first_key(KEY_NEG_INF + 1, key_max, [&](uint32_t k) { return z_bin(of_key(k)) < border; });
+                    if (lane == 0) (warp ? sh.key_hi : sh.key_lo) = k;
+                }
+                __syncthreads();
+                lo = key_max - (sh.key_hi - 1), hi = key_max - max(sh.key_lo, key_of(x_cut));
+                n_base = hit.n_before, w_base = step == P ? hit.w_before : 0ull;
+            }
+            Hit f;
+#pragma unroll 1
+            for (;;) {
+                const int bits = 32 - __clz((hi - lo) | 1u), shift = bits > 10 ? bits - 10 : 0;
+                next_round();
+                f = round_of(yes, yes, whole_slice, n_base, w_base, [&](float x, int i) -> int {
+                    const uint32_t at = step == MASS ? z_bin(x) : step == SAME ? (uint32_t)i : key_max - key_of(clean(x));
+                    const bool part = step == SAME ? x == x_cut : x > -INFINITY && x >= x_cut;
+                    return part && at >= lo && at <= hi ? (int)((at - lo) >> shift) : -1;
+                }, [&](u64 all) -> u64 { return step == MASS ? p_goal(all - over) : goal; }, step == MASS || step == P);
+                f.bin = lo + (f.bin << shift);
+                if (shift == 0) break;
+                lo = f.bin, hi = min(hi, lo + ((1u << shift) - 1u));
+                n_base = f.n_before, w_base = f.w_before;
+            }
+            if (step == K) {
+                x_cut = of_key(key_max - f.bin), n_cut = (uint32_t)s.k - f.n_before, n_same = f.n_here;
+            } else if (step == MASS) {
+                hit = f, whole = f.all - over;
+            } else if (step == P) {
+                const u64 w = f.w_here / f.n_here;  // all of them have the same weight, which is not 0
+                const uint32_t n = (uint32_t)min((goal + 1 - f.w_before + w - 1) / w, (u64)f.n_here);
+                const float x = of_key(key_max - f.bin);
+                if (x > x_cut || n < n_cut) x_cut = x, n_cut = n, n_same = f.n_here;
+            } else {
+                last_same = f.bin;
+            }
         }
-        if (x_m > x_cut) x_cut = x_m, n_cut = n_same = 0xffffffffu;
-        if (n_cut < n_same)  // equal logits: the first n_cut by index
-            last_same = refine(no, 0, (uint32_t)p.n - 1, 0, 0, [&](float x, int i, uint32_t* at) {
-                *at = (uint32_t)i;
-                return x == x_cut;
-            }, (u64)(n_cut - 1)).bin;
     } else {
         x_cut = x_m;
     }
@@ -779,16 +871,24 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     draw(mass, before, of_slice);
 }
 
-// CTAs per row: as many as the slices need, and while a launch would leave SMs empty, up to eight (of at least 1024 logits each)
-static int sample_slice(int c, int32_t n);
-static int sample_cluster(int64_t rows, int32_t n) {
-    int c = 1;
-    while (c < SP_CLUSTER && n > c * SP_SLICE) c *= 2;
-    while (c < SP_CLUSTER && rows * c <= 148 && n >= 2 * c * 1024) c *= 2;
-    return c;
+// How a launch is cut: up to eight CTAs per row (of at least 1024 logits each).
+//   every CTA has an SM of its own           1024 threads, the slices on the chip
+//   two fit an SM                            512 threads, the slices on the chip
+//   more                                     256 threads, four per SM, that read their slice again from L2 where they need it: twice
+//                                            as many rows are in flight, and the exchanges of one hide behind the work of the others
+// Measured on rows of 128256 f32 logits with mixed settings: @@MEASURED@@
+struct SampleCut {
+    int c, slice, threads;  // CTAs per row, logits per CTA (the next slice starts on a 16-byte boundary when the row does)
+};
+static SampleCut sample_cut(int64_t rows, int32_t n) {
+    SampleCut k{1, 0, 1024};
+    while (k.c < SP_CLUSTER && n >= 2 * k.c * 1024 && (n > k.c * SP_SLICE || rows * k.c * 2 <= 148)) k.c *= 2;
+    if (n > MAX_ON_CHIP) k.c = SP_CLUSTER;
+    k.slice = ((n + k.c - 1) / k.c + 7) / 8 * 8;
+    const bool two_fit = k.slice <= SP_SLICE;
+    if (n <= MAX_ON_CHIP && rows * k.c > 148) k.threads = two_fit && rows * k.c <= 2 * 148 ? 512 : 256;
+    return k;
 }
-// logits per CTA: the next slice starts on a 16-byte boundary when the row does
-static int sample_slice(int c, int32_t n) { return ((n + c - 1) / c + 7) / 8 * 8; }
 
 }  // namespace b200kv
 
@@ -799,7 +899,7 @@ extern "C" int64_t b200kv_sample_scratch_bytes(int64_t rows, int32_t n) {
         fail("rows and n must be positive, n at most %d", MAX_VOCAB);
         return -1;
     }
-    return n <= MAX_ON_CHIP ? 0 : rows * SP_CLUSTER * (int64_t)sample_slice(SP_CLUSTER, n) * (int64_t)sizeof(float);
+    return n <= MAX_ON_CHIP ? 0 : rows * SP_CLUSTER * (int64_t)sample_cut(rows, n).slice * (int64_t)sizeof(float);
 }
 
 extern "C" int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, int64_t rows, int32_t n, const float* temperature,
@@ -817,19 +917,17 @@ extern "C" int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, 
     p.logits = logits, p.stride = stride, p.dtype = dtype, p.n = n;
     p.temperature = temperature, p.top_k = top_k, p.top_p = top_p, p.min_p = min_p, p.uniform = uniform, p.out = out;
     p.vec = (uintptr_t)logits % 16 == 0 && (rows == 1 || (stride * dtype_size(dtype)) % 16 == 0);
-    const int c = sample_cluster(rows, n);
-    p.slice = sample_slice(c, n);
+    const SampleCut cut = sample_cut(rows, n);
+    p.slice = cut.slice;
     p.scratch = n > MAX_ON_CHIP ? (float*)scratch : nullptr;
-    // 1024 threads where a launch has at most one CTA for an SM
-    const bool wide = rows * c <= 148;
-    const size_t smem = ((sizeof(RowShared) + 15) & ~(size_t)15) + (p.scratch ? 0 : (size_t)p.slice * sizeof(float));
-    auto kernel = wide ? sample_kernel<1024> : sample_kernel<512>;
+    const size_t smem = ((sizeof(RowShared) + 15) & ~(size_t)15) + (p.scratch ? 0 : cut.threads > 256 ? (size_t)p.slice * sizeof(float) : (size_t)RING * 256 * 16);
+    auto kernel = cut.threads == 1024 ? sample_kernel<1024, true> : cut.threads == 512 ? sample_kernel<512, true> : sample_kernel<256, false>;
     B200KV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)c, (unsigned)rows), cfg.blockDim = dim3(wide ? 1024 : 512), cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream_;
+    cfg.gridDim = dim3((unsigned)cut.c, (unsigned)rows), cfg.blockDim = dim3((unsigned)cut.threads), cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream_;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = (unsigned)cut.c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = 2;
