@@ -96,6 +96,22 @@ __device__ inline uint32_t key_of(float x) {
 __device__ inline float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t KEY_NEG_INF = 0x007fffffu;
 
+// 2^(j / 256), j < 256: e^x by its series, x = j ln 2 / 256 < 0.7 (the 20th term is below 1e-21)
+struct Exp2Table {
+    double v[SP_TABLE];
+};
+constexpr Exp2Table make_exp2_table() {
+    Exp2Table t{};
+    for (int j = 0; j < SP_TABLE; j++) {
+        const double x = j * 0.69314718055994530942 / SP_TABLE;
+        double sum = 0.0;
+        for (int k = 20; k > 0; k--) sum = (sum + 1.0) * x / k;  // from the smallest terms on
+        t.v[j] = 1.0 + sum;
+    }
+    return t;
+}
+__device__ const Exp2Table g_exp2_table = make_exp2_table();
+
 // The place where the running count or mass passes its goal.
 struct Hit {
     uint32_t bin;               // 0xffffffff: nowhere
@@ -106,7 +122,6 @@ struct Hit {
 
 struct RowShared {
     uint32_t hist[4][SP_BINS];     // limbs of the masses; counts
-    uint32_t aside[32];            // one for each lane: where what does not take part is counted
     u64 list[SP_LIST];             // gathered tokens
     double exp2_table[SP_TABLE];   // 2^(j / SP_TABLE)
     // written by the other CTAs of the cluster
@@ -127,6 +142,7 @@ struct RowShared {
     uint32_t n_list;                 // this CTA's entries of the list so far
     uint32_t key_lo, key_hi, found;
     Hit hit;
+    double t_unit;                   // 256 log2 e / T
 };
 
 // Inclusive sums over the CTA in thread order.
@@ -167,6 +183,10 @@ __device__ inline uint32_t first_key(uint32_t lo, uint32_t hi, F holds) {
     return lo;
 }
 
+// atomicAdd to shared memory under a predicate: as an `if` each one costs a branch and its reconvergence
+__device__ inline void add_if(uint32_t* p, uint32_t v, bool yes) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q red.shared.add.u32 [%0], %1;\n}\n" ::"r"(smem_u32(p)), "r"(v), "r"((uint32_t)yes) : "memory");
+}
 __device__ inline void cp_async16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory");
 }
@@ -226,32 +246,27 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             return;
         }
         const bool f32 = p.dtype == B200KV_F32;
-        auto request = [&](int at, int slot) {
-            if (at < end && 4 * at + 4 <= count) {
-                if (f32) cp_async16(ring + slot * T, (const float4*)base + at);
-                else cp_async8(ring + slot * T, (const uint2*)base + at);
-            }
+        const int full = min(end, count / 4), last = max(full - 1, 0);  // quads that are whole
+        auto request = [&](int at, int slot) {  // past the end: the last one again
+            if (f32) cp_async16(ring + slot * T, (const float4*)base + min(at, last));
+            else cp_async8(ring + slot * T, (const uint2*)base + min(at, last));
             cp_async_commit();
         };
+        if (full > 0) {
 #pragma unroll
-        for (int j = 0; j < RING; j++) request(u + j * step, j);
-        int slot = 0;
+            for (int j = 0; j < RING; j++) request(u + j * step, j);
+            int slot = 0;
 #pragma unroll 1
-        for (; u < end; u += step) {
-            cp_async_wait<RING - 1>();
-            float4 v;
-            if (4 * u + 4 > count) {
-                v = from_memory(u);  // the last, partial one
-            } else {
+            for (; u < full; u += step) {
+                cp_async_wait<RING - 1>();
                 const uint4 w = ring[slot * T];
-                if (f32) v = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
-                else v = widen(w.x, w.y);
+                f(f32 ? make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)) : widen(w.x, w.y), u);
+                request(u + RING * step, slot);  // the slot has been read: f used it
+                slot = (slot + 1) % RING;
             }
-            f(v, u);
-            request(u + RING * step, slot);  // the slot has been read: f used it
-            slot = (slot + 1) % RING;
+            cp_async_wait<0>();
         }
-        cp_async_wait<0>();
+        if (u == full && u < end) f(from_memory(u), u);  // the partial one
     };
 
     cluster.barrier_arrive();  // every CTA of the cluster runs before one writes into another's shared memory
@@ -265,7 +280,7 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     const float octaves = s.use_p && !s.use_k ? fminf(28.f, log2f((float)p.n / (1.f - s.p)) + 1.f) : 28.f;
     const float per_octave = (float)(SP_BINS - 1) / octaves;
     float zscale = 1.4426950408889634f / s.t * per_octave;
-    double t_unit = s.greedy ? 0.0 : (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;
+    if (tid == 0 && !s.greedy) sh.t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;  // one division for all
     float best = -INFINITY;
     for (int u0 = tid; u0 < quads; u0 += 8 * T) {  // every thread has eight quads on their way before it uses the first
         float4 v[8];
@@ -289,7 +304,7 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     if (!s.greedy) {
         if (s.use_k || s.use_p)
             for (int i = tid; i < SP_BINS; i += T) ((uint4*)&sh.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
-        for (int i = tid; i < SP_TABLE; i += T) sh.exp2_table[i] = exp2((double)i / SP_TABLE);
+        for (int i = tid; i < SP_TABLE; i += T) sh.exp2_table[i] = g_exp2_table.v[i];
         if (tid == 0) sh.n_list = 0;
     }
     __syncthreads();
@@ -342,11 +357,13 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                 return;
             }
     }
+    double t_unit = sh.t_unit;
+    float t_used = s.t;
     if (s.t < fabsf(x_top) * 0x1p-34f) {
         // Other logits lie at least 2^-24 |max| below the maximum: they have no weight at this temperature, nor at the one that is
         // taken in its place, at which products with 1 / T keep their accuracy.
-        const float t = fabsf(x_top) * 0x1p-34f;
-        t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)t, zscale = 1.4426950408889634f / t * per_octave;
+        t_used = fabsf(x_top) * 0x1p-34f;
+        t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)t_used, zscale = 1.4426950408889634f / t_used * per_octave;
     }
 
     // ---- weights ----
@@ -358,14 +375,17 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     // 2^(r / 256) by its Taylor polynomial of degree 3 in r ln 2 / 256 (|r| <= 1/2: what is left out is below 1.5e-13), rounded
     // to 44 fractional bits by adding 1.5 * 2^8.  Below 2^-46: 0.
     const double t_top = -(double)x_top * t_unit;
-    const float x_floor = __double2float_rd((double)x_top - 46.5 * (double)SP_TABLE / t_unit);  // 2^-46.5 rounds to 0
+    const float x_floor = __double2float_rd((double)x_top - 46.5 * 0.69314718055994530942 * (double)t_used);  // 2^-46.5 rounds to 0
+    constexpr double L = 0.69314718055994530942 / SP_TABLE;
+    double taylor1 = L, taylor2 = L * L / 2.0, taylor3 = L * L * L / 6.0;
+    asm volatile("" : "+d"(taylor1), "+d"(taylor2), "+d"(taylor3));  // in registers: two moves per use otherwise
     auto weight = [&](float x) -> u64 {
-        constexpr double L = 0.69314718055994530942 / SP_TABLE, MAGIC = 6755399441055744.0;  // 1.5 * 2^52
+        constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52
         const double t = fma((double)fmaxf(x, x_floor), t_unit, t_top);
         const double biased = t + MAGIC, r = t - (biased - MAGIC);
         const int n = max(__double2loint(biased), -64 * SP_TABLE);  // the next float below the maximum may be deeper than that
-        double q = fma(r, L * L * L / 6.0, L * L / 2.0);
-        q = fma(q, r, L);
+        double q = fma(r, taylor3, taylor2);
+        q = fma(q, r, taylor1);
         q = fma(q, r, 1.0);
         const double tab = sh.exp2_table[n & (SP_TABLE - 1)];
         const double scaled = __hiloint2double(__double2hiint(tab) + ((n << 12) & 0xfff00000), __double2loint(tab));
@@ -401,29 +421,22 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         u64 deep_w = 0;
         feed([&](const float4& v, int u) {
             const float x[4] = {v.x, v.y, v.z, v.w};
-            u64 w[4];
-            int b[4];
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {  // the four side by side, then their atomics
-                b[e] = bin_of(x[e], first + 4 * u + e);
-                w[e] = weights ? weight(x[e]) : 0ull;
-                const bool deep = b[e] == SP_BINS - 1;
-                if (counts) deep_n += deep && x[e] > -INFINITY;
-                if (weights) deep_w += deep ? w[e] : 0ull;
-                if (deep) b[e] = -1;
-                any |= b[e] >= 0;
-            }
-            if (!any) return;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (counts) atomicAdd(b[e] < 0 ? &sh.aside[lane] : &sh.hist[3][b[e]], 1u);
+                const int b = bin_of(x[e], first + 4 * u + e);
+                const bool deep = b == SP_BINS - 1, binned = (b >= 0) & !deep;
+                uint32_t* at = &sh.hist[0][b];
+                if (counts) {
+                    deep_n += deep & (x[e] > -INFINITY);
+                    add_if(at + 3 * SP_BINS, 1u, binned);
+                }
                 if (weights) {
-                    if (b[e] < 0) w[e] = 0;
-                    const uint32_t l0 = (uint32_t)w[e] & 0x7fffu, l1 = (uint32_t)(w[e] >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w[e] >> (2 * SP_LIMB));
-                    if (l0) atomicAdd(&sh.hist[0][b[e]], l0);
-                    if (l1) atomicAdd(&sh.hist[1][b[e]], l1);
-                    if (l2) atomicAdd(&sh.hist[2][b[e]], l2);
+                    const u64 w = weight(x[e]);
+                    deep_w += deep ? w : 0ull;
+                    const uint32_t l0 = (uint32_t)w & 0x7fffu, l1 = (uint32_t)(w >> SP_LIMB) & 0x7fffu, l2 = (uint32_t)(w >> (2 * SP_LIMB));
+                    add_if(at, l0, binned);
+                    add_if(at + SP_BINS, l1, binned & (w >> SP_LIMB != 0));
+                    add_if(at + 2 * SP_BINS, l2, binned & (l2 != 0));
                 }
             }
         });
@@ -528,13 +541,16 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     uint32_t last_same = 0xffffffffu;
     u64 of_slice = 0;
     bool runs_known = false;
-    auto kept = [&](float x, int i) -> bool { return x > x_cut || (x == x_cut && (uint32_t)(first + i) <= last_same); };
+    auto kept = [&](float x, int i) -> bool { return (x > x_cut) | ((x == x_cut) & ((uint32_t)(first + i) <= last_same)); };
     auto kept_weight = [&](float x, int i) -> u64 { return kept(x, i) ? weight(x) : 0ull; };
     const int run = ((quads + SP_WARPS - 1) / SP_WARPS + 31) / 32 * 32;  // quads of a warp
     // the kept mass of the slice; of a run per warp in warp_w
     auto run_masses = [&]() -> u64 {
         u64 mine = 0;
         const int end = min(quads, (warp + 1) * run);
+        if (x_cut == -INFINITY)
+            sweep(warp * run + lane, 32, end, [&](const float4& v, int) { mine += weight(v.x) + weight(v.y) + weight(v.z) + weight(v.w); });
+        else
         sweep(warp * run + lane, 32, end, [&](const float4& v, int u) {
             // (the votes of the lanes that are still in the loop) nothing kept in any of them: on
             if (!__any_sync(__activemask(), fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x_cut)) return;
@@ -635,7 +651,8 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         };
         // ---- 3. few enough tokens: put them in order ----
         // Each CTA has a part of the list, `cap` entries; false: more than that in some CTA (the same answer in every CTA).
-        const int cap = SP_LIST / C;
+        const int cap_bits = 10 - (31 - __clz(C)), cap = 1 << cap_bits;
+        static_assert(SP_LIST == 1 << 10, "the parts of the list");
         auto gather = [&](bool to_all, auto takes) -> bool {
             each([&](float x, int i) {
                 if (!takes(x)) return;
@@ -744,7 +761,7 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
             const float in_bin = 8388608.f + (float)top.bin;  // what z_bin rounds them to
             if (gather(true, [&](float x) { return (x_top - x) * zscale + 8388608.f == in_bin; })) {
                 for (int i = tid; i < C * cap; i += T)
-                    if (i % cap < (int)sh.part[i / cap]) weights[i] = weight(logit_of(sh.list[i]));
+                    if ((i & (cap - 1)) < (int)sh.part[i >> cap_bits]) weights[i] = weight(logit_of(sh.list[i]));
                 __syncthreads();
                 // the mass before each of this CTA's own tokens, in the order of the whole bin; a few threads per token
                 constexpr int LANES = T >= 1024 ? 8 : 4;
@@ -755,9 +772,11 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
                     const int m = m0 + tid / LANES;
                     const u64 token = m < n_own ? sh.list[rank * cap + m] : 0ull;
                     u64 sum = 0;
-                    for (int r = 0; r < C; r++)
-                        for (int j = tid % LANES; j < (int)sh.part[r]; j += LANES)
-                            if (sh.list[r * cap + j] < token) sum += weights[r * cap + j];
+                    for (int r = 0; r < C; r++) {
+                        const int end = r * cap + (int)sh.part[r];
+#pragma unroll 4
+                        for (int j = r * cap + tid % LANES; j < end; j += LANES) sum += sh.list[j] < token ? weights[j] : 0ull;
+                    }
 #pragma unroll
                     for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     sum += top.w_before;
