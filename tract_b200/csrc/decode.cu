@@ -62,8 +62,8 @@ __device__ inline float warp_sum(float v) {
     return v;
 }
 
-template <int FMT, int D, int GT>
-__global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __grid_constant__ InlineBatch ib) {
+template <int FMT, int D, int GT, typename SHARED>
+__global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __grid_constant__ InlineBatch ib, const __grid_constant__ SHARED sb) {
     using Gm = Geo<FMT, D>;
     const bool PRECISE = p.dtype == B200KV_F32;  // f32 callers get expf, 16-bit callers the fast exponential
     constexpr int NS = Gm::NS;
@@ -78,9 +78,10 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int sub = lane & 7, tl = lane >> 3;
     const int tg = tid >> 4, cu = tid & 15;
-    const WorkItem w = ib.n ? resolve_work_item(ib, blockIdx.x) : p.items[blockIdx.x];
     const int kvh = blockIdx.y;
-    const int g0 = blockIdx.z * GT;
+    const DecodeWork work = decode_work(p, ib, sb, kvh, GT * gridDim.z);
+    const WorkItem& w = work.w;
+    const int g0 = work.row0 + blockIdx.z * GT;
     const int n_tiles = w.n_pages;
 
     auto issue = [&](int i) {  // thread 0 only
@@ -110,13 +111,13 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
     float qr[GT][Gm::EPL];
 #pragma unroll
     for (int g = 0; g < GT; g++) {
-        int head = kvh * p.G + min(g0 + g, p.G - 1);
+        const int row = min(g0 + g, work.rows - 1);
 #pragma unroll
         for (int pc = 0; pc < Gm::NPC; pc++) {
             int rb = pc * (8 * Gm::PB) + sub * Gm::PB;
 #pragma unroll
             for (int e = 0; e < Gm::EPP; e++)
-                qr[g][pc * Gm::EPP + e] = load_query(p, D, w.batch, head, row_channel<FMT>(rb, e, Gm::PB));
+                qr[g][pc * Gm::EPP + e] = load_query_row<SHARED>(p, work, D, kvh, row, row_channel<FMT>(rb, e, Gm::PB));
         }
     }
 
@@ -267,15 +268,15 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
     }
 
     // ---- write the partial of this split ----
-    const int64_t pbase = ((int64_t)blockIdx.x * p.Hkv + kvh) * p.G;
+    const int64_t pbase = work.base;
     if (failed) {
         // outstanding copies (if any) are left to land in this CTA's shared memory, which nothing
         // reads any more; publish an empty partial so the combine pass ignores this split
         for (int idx = tid; idx < GT * D; idx += 128) {
             int g = idx / D;
-            if (g0 + g < p.G) p.part_o[(pbase + g0 + g) * D + idx % D] = 0.f;
+            if (g0 + g < work.rows) p.part_o[(pbase + g0 + g) * D + idx % D] = 0.f;
         }
-        if (tid < GT && g0 + tid < p.G) {
+        if (tid < GT && g0 + tid < work.rows) {
             p.part_ml[(pbase + g0 + tid) * 2] = -INFINITY;
             p.part_ml[(pbase + g0 + tid) * 2 + 1] = 0.f;
         }
@@ -302,9 +303,9 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; k++) sum += red[(k * GT + g) * D + ch];
-        if (g0 + g < p.G) p.part_o[(pbase + g0 + g) * D + ch] = sum;
+        if (g0 + g < work.rows) p.part_o[(pbase + g0 + g) * D + ch] = sum;
     }
-    if (tid < GT && g0 + tid < p.G) {
+    if (tid < GT && g0 + tid < work.rows) {
         p.part_ml[(pbase + g0 + tid) * 2] = ml_s[tid * 2];
         p.part_ml[(pbase + g0 + tid) * 2 + 1] = ml_s[tid * 2 + 1];
     }
@@ -380,20 +381,32 @@ __global__ void combine_kernel(CombineParams p, const __grid_constant__ InlineBa
     if (p.act) q40_quantize_block(round_to_dtype(res, p.dtype), true, p.act, p.n_rows, act_nb, b, act_blk, ch & 31);  // what a quantiser would read back from `out`
 }
 
-template <int FMT, int D, int GT>
-static int launch_decode_t(const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib) {
+template <int FMT, int D, int GT, typename SHARED>
+static int launch_decode_t(const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib, const SHARED& sb) {
     using Gm = Geo<FMT, D>;
     const size_t smem = (size_t)Gm::NS * Gm::STAGE + decode_tail_bytes<GT>();
-    B200KV_CUDA(cudaFuncSetAttribute(decode_kernel<FMT, D, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    B200KV_CUDA(cudaFuncSetAttribute(decode_kernel<FMT, D, GT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     dim3 grid(n_items, p.Hkv, (p.G + GT - 1) / GT);
-    B200KV_CUDA(launch_after_predecessor(decode_kernel<FMT, D, GT>, grid, dim3(128), smem, stream, p, ib));
+    B200KV_CUDA(launch_after_predecessor(decode_kernel<FMT, D, GT, SHARED>, grid, dim3(128), smem, stream, p, ib, sb));
     return B200KV_OK;
 }
 
-template <int FMT>
-static int launch_decode_f(const DecodeParams& p, int D, int n_items, cudaStream_t stream, const InlineBatch& ib) {
-    if (p.G == 1) return D == 128 ? launch_decode_t<FMT, 128, 1>(p, n_items, stream, ib) : launch_decode_t<FMT, 64, 1>(p, n_items, stream, ib);
-    return D == 128 ? launch_decode_t<FMT, 128, 4>(p, n_items, stream, ib) : launch_decode_t<FMT, 64, 4>(p, n_items, stream, ib);
+template <int FMT, typename SHARED>
+static int launch_decode_f(const DecodeParams& p, int D, int n_items, cudaStream_t stream, const InlineBatch& ib, const SHARED& sb) {
+    if constexpr (sizeof(SHARED) == sizeof(NoPrefix))
+        if (p.G == 1) return D == 128 ? launch_decode_t<FMT, 128, 1>(p, n_items, stream, ib, sb) : launch_decode_t<FMT, 64, 1>(p, n_items, stream, ib, sb);
+    return D == 128 ? launch_decode_t<FMT, 128, 4>(p, n_items, stream, ib, sb) : launch_decode_t<FMT, 64, 4>(p, n_items, stream, ib, sb);
+}
+template <typename SHARED>
+static int launch_decode_fmt(int fmt, int D, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib, const SHARED& sb) {
+    switch (fmt) {
+        case B200KV_FMT_F32: return launch_decode_f<B200KV_FMT_F32>(p, D, n_items, stream, ib, sb);
+        case B200KV_FMT_F16: return launch_decode_f<B200KV_FMT_F16>(p, D, n_items, stream, ib, sb);
+        case B200KV_FMT_BF16: return launch_decode_f<B200KV_FMT_BF16>(p, D, n_items, stream, ib, sb);
+        case B200KV_FMT_Q8_1: return launch_decode_f<B200KV_FMT_Q8_1>(p, D, n_items, stream, ib, sb);
+        case B200KV_FMT_Q4_0: return launch_decode_f<B200KV_FMT_Q4_0>(p, D, n_items, stream, ib, sb);
+    }
+    return fail("format %d has no decode kernel", fmt);
 }
 
 // The two launch steps of a decode call, for callers in other translation units.
@@ -402,16 +415,9 @@ const InlineBatch& empty_inline_batch() {
     return e;
 }
 
-int launch_decode_simt(int fmt, int D, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ibp) {
+int launch_decode_simt(int fmt, int D, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ibp, const PrefixBatch* sb, int shared_ctas) {
     const InlineBatch& ib = ibp ? *ibp : empty_inline_batch();
-    switch (fmt) {
-        case B200KV_FMT_F32: return launch_decode_f<B200KV_FMT_F32>(p, D, n_items, stream, ib);
-        case B200KV_FMT_F16: return launch_decode_f<B200KV_FMT_F16>(p, D, n_items, stream, ib);
-        case B200KV_FMT_BF16: return launch_decode_f<B200KV_FMT_BF16>(p, D, n_items, stream, ib);
-        case B200KV_FMT_Q8_1: return launch_decode_f<B200KV_FMT_Q8_1>(p, D, n_items, stream, ib);
-        case B200KV_FMT_Q4_0: return launch_decode_f<B200KV_FMT_Q4_0>(p, D, n_items, stream, ib);
-    }
-    return fail("format %d has no decode kernel", fmt);
+    return sb ? launch_decode_fmt(fmt, D, p, n_items + shared_ctas, stream, ib, *sb) : launch_decode_fmt(fmt, D, p, n_items, stream, ib, NoPrefix{});
 }
 int launch_combine(const DecodeParams& p, const int32_t* batch_info, void* out, int64_t ob, int64_t oh, int n_seqs,
                    int n_q_heads, int D, cudaStream_t stream, const InlineBatch* ibp) {
@@ -551,14 +557,8 @@ int launch_decode(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t 
     ProfScope ps(c, K_DECODE, stream);
     if (decode_mma_supported(c->L.fmt, D, dtype) && !c->force_simt) {
         rc = launch_decode_mma(c->L.fmt, p, n_items, stream, &ib);
-    } else
-    switch (c->L.fmt) {
-        case B200KV_FMT_F32: rc = launch_decode_f<B200KV_FMT_F32>(p, D, n_items, stream, ib); break;
-        case B200KV_FMT_F16: rc = launch_decode_f<B200KV_FMT_F16>(p, D, n_items, stream, ib); break;
-        case B200KV_FMT_BF16: rc = launch_decode_f<B200KV_FMT_BF16>(p, D, n_items, stream, ib); break;
-        case B200KV_FMT_Q8_1: rc = launch_decode_f<B200KV_FMT_Q8_1>(p, D, n_items, stream, ib); break;
-        case B200KV_FMT_Q4_0: rc = launch_decode_f<B200KV_FMT_Q4_0>(p, D, n_items, stream, ib); break;
-        default: rc = fail("format %d has no decode kernel", c->L.fmt);
+    } else {
+        rc = launch_decode_simt(c->L.fmt, D, p, n_items, stream, &ib);
     }
     }
     if (rc == B200KV_OK) {

@@ -83,13 +83,82 @@ __device__ inline WorkItem resolve_work_item(const InlineBatch& ib, int item) {
     return make_work_item(ib.ent[lo], lo, item - ib.ent[lo].z, ib.first[lo]);
 }
 
+// One run of batch entries that share their first n_pages pages.
+struct PrefixGroup {
+    int32_t trow;       // page-table row of one of them
+    int32_t n_pages;    // shared pages, all of them full
+    int32_t b0, n_seqs; // batch entries b0 .. b0 + n_seqs - 1
+    int32_t tiles;      // CTAs (x) that cover the n_seqs * G rows between them
+    int32_t splits;     // runs of pages
+    int32_t cta0;       // first CTA (x) of the group, after the work items of the sequences' own pages: cta0 + split * tiles + tile
+    int32_t base;       // first partial record: base + (split * Hkv + kvh) * n_seqs * G + row
+};
+constexpr int PREFIX_GROUPS = INLINE_BATCH / 2;
+struct PrefixBatch {
+    int32_t n;
+    int32_t n_own;  // work items of the sequences' own pages in the same launch: CTAs (x) 0 .. n_own - 1
+    int32_t pad[2];
+    PrefixGroup g[PREFIX_GROUPS];
+};
+struct NoPrefix {};  // a decode launch without shared pages
+__device__ inline PrefixGroup prefix_group_of(const PrefixBatch& pb, int cta) {
+    int lo = 0, hi = pb.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pb.g[mid].cta0 <= cta) lo = mid;
+        else hi = mid - 1;
+    }
+    return pb.g[lo];
+}
+// pages [first, first + count) of split k
+__device__ inline void prefix_run(const PrefixGroup& g, int k, int* first, int* count) {
+    const int base = g.n_pages / g.splits, rem = g.n_pages % g.splits;
+    *first = k * base + min(k, rem);
+    *count = base + (k < rem ? 1 : 0);
+}
+
+// What a CTA of a decode kernel works on: a run of pages of one sequence against the query heads of a kv head's group, or of
+// pages shared by a run of sequences against the rows (sequence, head of the group) of all of them.
+struct DecodeWork {
+    WorkItem w;
+    int32_t row0, rows;  // first row of this CTA, rows in all: row r is query head kvh * G + r % G of batch entry w.batch + r / G
+    int64_t base;        // partial record of row 0
+};
+template <typename SHARED>
+__device__ inline DecodeWork decode_work(const DecodeParams& p, const InlineBatch& ib, const SHARED& sb, int kvh, int rows_per_cta) {
+    DecodeWork d;
+    if constexpr (sizeof(SHARED) > sizeof(NoPrefix)) {
+        if ((int)blockIdx.x >= sb.n_own) {
+            const PrefixGroup g = prefix_group_of(sb, blockIdx.x);
+            const int local = (int)blockIdx.x - g.cta0, split = local / g.tiles;
+            d.rows = g.n_seqs * p.G, d.row0 = (local % g.tiles) * rows_per_cta;
+            prefix_run(g, split, &d.w.page_begin, &d.w.n_pages);
+            d.w.trow = g.trow, d.w.len = g.n_pages * PAGE_TOKENS, d.w.batch = g.b0, d.w.split = split, d.w.first = 0, d.w.pad1 = 0;
+            d.base = (int64_t)g.base + ((int64_t)split * p.Hkv + kvh) * d.rows;
+            return d;
+        }
+    }
+    d.w = ib.n ? resolve_work_item(ib, blockIdx.x) : p.items[blockIdx.x];
+    d.row0 = 0, d.rows = p.G;
+    d.base = ((int64_t)blockIdx.x * p.Hkv + kvh) * p.G;
+    return d;
+}
+// load_query for row `row` of the work
+template <typename SHARED>
+__device__ inline float load_query_row(const DecodeParams& p, const DecodeWork& d, int D, int kvh, int row, int ch) {
+    if constexpr (sizeof(SHARED) > sizeof(NoPrefix)) return load_query(p, D, d.w.batch + row / p.G, kvh * p.G + row % p.G, ch);
+    else return load_query(p, D, d.w.batch, kvh * p.G + row, ch);
+}
+
 // decode.cu
-int launch_decode_simt(int fmt, int D, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ib = nullptr);
+int launch_decode_simt(int fmt, int D, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ib = nullptr,
+                       const PrefixBatch* sb = nullptr, int shared_ctas = 0);
 int launch_combine(const DecodeParams& p, const int32_t* batch_info, void* out, int64_t ob, int64_t oh, int n_seqs,
                    int n_q_heads, int D, cudaStream_t stream, const InlineBatch* ib = nullptr);
 // decode_mma.cu
 bool decode_mma_supported(int fmt, int D, int dtype);
-int launch_decode_mma(int fmt, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ib = nullptr);
+int launch_decode_mma(int fmt, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ib = nullptr, const PrefixBatch* sb = nullptr,
+                      int shared_ctas = 0);
 // An InlineBatch with n = 0, for launches that read their batch from device memory.
 const InlineBatch& empty_inline_batch();
 

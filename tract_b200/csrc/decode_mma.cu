@@ -49,8 +49,9 @@ struct MGeo {
 // Shared memory after the stage ring: q as f32 [8][128], then the barriers.
 constexpr size_t MMA_TAIL = 8 * MD * 4 + 32 * 4 + 128;
 
-template <int FMT>
-__global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS) decode_mma_kernel(DecodeParams p, const __grid_constant__ InlineBatch ib) {
+template <int FMT, typename SHARED>
+__global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS)
+    decode_mma_kernel(DecodeParams p, const __grid_constant__ InlineBatch ib, const __grid_constant__ SHARED sb) {
     using Gm = MGeo<FMT>;
     constexpr int NS = Gm::NS;
     constexpr bool QUANT = Gm::QUANT;
@@ -71,10 +72,11 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS) decode_mma_kernel(De
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r = lane >> 2, c = lane & 3;
-    const WorkItem w = ib.n ? resolve_work_item(ib, blockIdx.x) : p.items[blockIdx.x];
     const int kvh = blockIdx.y;
-    const int g0 = blockIdx.z * 8;
-    const int ng = min(8, p.G - g0);  // q heads of this CTA
+    const DecodeWork work = decode_work(p, ib, sb, kvh, 8 * gridDim.z);
+    const WorkItem& w = work.w;
+    const int g0 = work.row0 + blockIdx.z * 8;
+    const int ng = min(8, work.rows - g0);  // q heads of this CTA
     const int n_tiles = w.n_pages;
 
     const int32_t* trow_p = p.table + (int64_t)w.trow * p.max_pages_per_seq + w.page_begin;
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS) decode_mma_kernel(De
     for (int idx = tid; idx < 8 * MD; idx += 128) {
         int g = idx / MD, ch = idx % MD;
         float v = 0.f;
-        if (g < ng) v = load_query(p, MD, w.batch, kvh * p.G + g0 + g, ch);
+        if (g < ng) v = load_query_row<SHARED>(p, work, MD, kvh, g0 + g, ch);
         if (QUANT) v = __half2float(__float2half_rn(v));  // the operand the tensor cores will see
         q_s[idx] = v;
     }
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS) decode_mma_kernel(De
     }
 
     // ---- merge the four warps and publish the partial of this split ----
-    const int64_t pbase = ((int64_t)blockIdx.x * p.Hkv + kvh) * p.G + g0;
+    const int64_t pbase = work.base + g0;
     if (failed) {
         if (tid == 0) atomicOr(p.status, STATUS_WAIT_EXPIRED);
         for (int idx = tid; idx < ng * MD; idx += 128) p.part_o[(pbase + idx / MD) * MD + idx % MD] = 0.f;
@@ -440,15 +442,15 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS) decode_mma_kernel(De
     }
 }
 
-template <int FMT>
-static int launch_mma_t(const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib) {
+template <int FMT, typename SHARED>
+static int launch_mma_t(const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib, const SHARED& sb) {
     using Gm = MGeo<FMT>;
     const size_t ring = (size_t)Gm::NS * Gm::STAGE;
     const size_t merge = (size_t)(4 * 8 * MD + 4 * 8 * 2) * 4;  // the warp merge reuses the ring
     const size_t smem = std::max(ring, merge) + MMA_TAIL;
-    B200KV_CUDA(cudaFuncSetAttribute(decode_mma_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    B200KV_CUDA(cudaFuncSetAttribute(decode_mma_kernel<FMT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     dim3 grid(n_items, p.Hkv, (p.G + 7) / 8);
-    B200KV_CUDA(launch_after_predecessor(decode_mma_kernel<FMT>, grid, dim3(128), smem, stream, p, ib));
+    B200KV_CUDA(launch_after_predecessor(decode_mma_kernel<FMT, SHARED>, grid, dim3(128), smem, stream, p, ib, sb));
     return B200KV_OK;
 }
 
@@ -460,15 +462,19 @@ bool decode_mma_supported(int fmt, int D, int dtype) {
     return false;
 }
 
-int launch_decode_mma(int fmt, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ibp) {
-    const InlineBatch& ib = ibp ? *ibp : empty_inline_batch();
+template <typename SHARED>
+static int launch_mma_fmt(int fmt, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib, const SHARED& sb) {
     switch (fmt) {
-        case B200KV_FMT_F16: return launch_mma_t<B200KV_FMT_F16>(p, n_items, stream, ib);
-        case B200KV_FMT_BF16: return launch_mma_t<B200KV_FMT_BF16>(p, n_items, stream, ib);
-        case B200KV_FMT_Q8_1: return launch_mma_t<B200KV_FMT_Q8_1>(p, n_items, stream, ib);
-        case B200KV_FMT_Q4_0: return launch_mma_t<B200KV_FMT_Q4_0>(p, n_items, stream, ib);
+        case B200KV_FMT_F16: return launch_mma_t<B200KV_FMT_F16>(p, n_items, stream, ib, sb);
+        case B200KV_FMT_BF16: return launch_mma_t<B200KV_FMT_BF16>(p, n_items, stream, ib, sb);
+        case B200KV_FMT_Q8_1: return launch_mma_t<B200KV_FMT_Q8_1>(p, n_items, stream, ib, sb);
+        case B200KV_FMT_Q4_0: return launch_mma_t<B200KV_FMT_Q4_0>(p, n_items, stream, ib, sb);
     }
     return fail("format %d has no tensor-core decode kernel", fmt);
+}
+int launch_decode_mma(int fmt, const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch* ibp, const PrefixBatch* sb, int shared_ctas) {
+    const InlineBatch& ib = ibp ? *ibp : empty_inline_batch();
+    return sb ? launch_mma_fmt(fmt, p, n_items + shared_ctas, stream, ib, *sb) : launch_mma_fmt(fmt, p, n_items, stream, ib, NoPrefix{});
 }
 
 }  // namespace b200kv

@@ -18,43 +18,11 @@
 
 namespace b200kv {
 
-// One run of batch entries that share their first n_pages pages.
-struct PrefixGroup {
-    int32_t trow;       // page-table row of one of them
-    int32_t n_pages;    // shared pages, all of them full
-    int32_t b0, n_seqs; // batch entries b0 .. b0 + n_seqs - 1
-    int32_t tiles;      // row tiles (of one CTA) that cover n_seqs * G rows
-    int32_t splits;     // runs of pages
-    int32_t cta0;       // first CTA (x) of the group: cta0 + split * tiles + tile
-    int32_t base;       // first partial record: base + (split * Hkv + kvh) * n_seqs * G + row
-};
-constexpr int PREFIX_GROUPS = INLINE_BATCH / 2;
-struct PrefixBatch {
-    int32_t n;
-    int32_t pad[3];
-    PrefixGroup g[PREFIX_GROUPS];
-};
 struct PrefixParams {
     DecodeParams d;  // q, rotary embedding, pool, table, workspace: as the decode kernels get them
     int32_t chunk_bytes;
     float skip_fraction;
 };
-
-__device__ inline PrefixGroup prefix_group_of(const PrefixBatch& pb, int cta) {
-    int lo = 0, hi = pb.n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pb.g[mid].cta0 <= cta) lo = mid;
-        else hi = mid - 1;
-    }
-    return pb.g[lo];
-}
-// pages [first, first + count) of split k
-__device__ inline void prefix_run(const PrefixGroup& g, int k, int* first, int* count) {
-    const int base = g.n_pages / g.splits, rem = g.n_pages % g.splits;
-    *first = k * base + min(k, rem);
-    *count = base + (k < rem ? 1 : 0);
-}
 
 constexpr int XM = 128;            // rows of a tile
 constexpr int X_SM_THREADS = 128;  // softmax threads per tile: one per row
@@ -676,6 +644,8 @@ static cudaError_t launch_prefix_simt(int fmt, const PrefixParams& p, const Pref
     return launch_after_predecessor(prefix_simt_kernel<D>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(C_THREADS), CGeo<D>::SMEM, stream, p, pb, fmt);
 }
 
+constexpr int TOGETHER_ROWS = 32;
+
 // At most INLINE_BATCH sequences; `ends` as launch_decode takes it.
 static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q, const int64_t* qs, void* out,
                          const int64_t* os, int32_t dtype, float scale, cudaStream_t stream, const QueryRope& ends) {
@@ -696,12 +666,12 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     for (const Run& r : runs)
         if (r.n > 1 && r.pages > 0) max_rows = std::max(max_rows, r.n * G), max_pages = std::max(max_pages, r.pages);
     const int nq = max_rows > XM ? 2 : 1;
-    const int rows_cta = tc ? nq * XM : CR;
+    int rows_cta = tc ? nq * XM : CR;
     const int64_t slots = 148 * (tc && (nq == 2 || quant) ? 1 : 2);  // resident CTAs
 
     // ---- the own pages of every sequence: as launch_decode cuts them, starting behind the shared ones ----
     const bool use_mma = decode_mma_supported(fmt, D, dtype) && !c->force_simt;
-    const int nz = (G + (use_mma ? 8 : (G == 1 ? 1 : 4)) - 1) / (use_mma ? 8 : (G == 1 ? 1 : 4));
+    const int nz = (G + (use_mma ? 7 : 3)) / (use_mma ? 8 : 4);
     std::vector<int64_t> first((size_t)n_seqs), own_pages((size_t)n_seqs);
     std::vector<int> most((size_t)n_seqs, MAX_SPLITS);  // runs of a sequence's own pages: a row joins at most MAX_SPLITS partials
     for (const Run& r : runs)
@@ -711,14 +681,23 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
             if (r.n > 1 && r.pages > 0) most[i] = MAX_SPLITS / 2;
             own_pages[i] = (s.len + PAGE_TOKENS - 1) / PAGE_TOKENS - first[i] / PAGE_TOKENS;
         }
-    int64_t own_chunk = pages_per_split(c, own_pages.data(), n_seqs, use_mma, nz);
+    // Few rows: the shared pages go through the decode kernel as further work items, eight (four) rows at a time, in one launch
+    // with the own pages.  Each CTA of rows reads the pages again, from L2.
+    const bool together = max_rows <= TOGETHER_ROWS;
+    if (together) rows_cta = nz * (use_mma ? 8 : 4);
+    std::vector<int64_t> all_pages = own_pages;
+    if (together)
+        for (const Run& r : runs)
+            if (r.n > 1 && r.pages > 0) all_pages.insert(all_pages.end(), (size_t)((r.n * G + rows_cta - 1) / rows_cta), r.pages);
+    int64_t own_chunk = pages_per_split(c, all_pages.data(), (int)all_pages.size(), use_mma, nz);
 
     InlineBatch ib{};
     SharedBatch sb{};
     PrefixBatch pb{};
     int n_items = 0, ctas = 0;
     int64_t n_rec = 0, run_pages = 1;
-    for (int64_t tiles_pages = 0;;) {  // the smallest run length that fills the GPU once
+    if (together) run_pages = std::min<int64_t>(own_chunk, max_pages);
+    else for (int64_t tiles_pages = 0;;) {  // the smallest run length that fills the GPU once
         tiles_pages = 0;
         for (const Run& r : runs)
             if (r.n > 1 && r.pages > 0) tiles_pages += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * ((r.pages + run_pages - 1) / run_pages);
@@ -737,6 +716,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
         }
         ib.n = n_seqs;
         n_rec = (int64_t)n_items * Hkv * G;
+        if (together) pb.n_own = ctas = n_items;
         for (const Run& r : runs) {
             if (r.n <= 1 || r.pages <= 0) continue;
             const int rows = r.n * G;
@@ -768,16 +748,19 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     dp.page_bytes = c->L.page_bytes, dp.n_pages = (int32_t)c->n_pages, dp.max_pages_per_seq = c->max_pages_per_seq;
     dp.Hkv = Hkv, dp.G = G, dp.dtype = dtype, dp.scale = scale, dp.wait_ns = c->wait_ns;
     p.chunk_bytes = c->L.chunk_bytes, p.skip_fraction = X_SKIP_FRACTION;
-    cudaError_t e;
-    {
+    cudaError_t e = cudaSuccess;
+    if (!together) {
         ProfScope ps(c, K_PREFIX, stream);
         e = tc ? launch_prefix_tc(fmt, D, nq, p, pb, ctas, stream)
                : (D == 128 ? launch_prefix_simt<128>(fmt, p, pb, ctas, stream) : launch_prefix_simt<64>(fmt, p, pb, ctas, stream));
     }
     if (e != cudaSuccess) return fail("shared-prefix launch failed: %s", cudaGetErrorString(e));
-    if (n_items > 0) {
+    if (together || n_items > 0) {
         ProfScope ps(c, K_DECODE, stream);
-        if ((use_mma ? launch_decode_mma(fmt, dp, n_items, stream, &ib) : launch_decode_simt(fmt, D, dp, n_items, stream, &ib)) != B200KV_OK) return B200KV_KO;
+        const PrefixBatch* with = together ? &pb : nullptr;
+        const int more = together ? ctas - n_items : 0;
+        if ((use_mma ? launch_decode_mma(fmt, dp, n_items, stream, &ib, with, more) : launch_decode_simt(fmt, D, dp, n_items, stream, &ib, with, more)) != B200KV_OK)
+            return B200KV_KO;
     }
     SharedCombineParams cp{};
     cp.part_o = dp.part_o, cp.part_ml = dp.part_ml, cp.out = out, cp.ob = os[0], cp.oh = os[1];
