@@ -89,7 +89,7 @@ struct PrefixGroup {
     int32_t n_pages;    // shared pages, all of them full
     int32_t b0, n_seqs; // batch entries b0 .. b0 + n_seqs - 1
     int32_t tiles;      // CTAs (x) that cover the n_seqs * G rows between them
-    int32_t splits;     // runs of pages
+    int32_t splits;     // runs of pages, one partial each
     int32_t cta0;       // first CTA (x) of the group, after the work items of the sequences' own pages: cta0 + split * tiles + tile
     int32_t base;       // first partial record: base + (split * Hkv + kvh) * n_seqs * G + row
 };
@@ -110,9 +110,9 @@ __device__ inline PrefixGroup prefix_group_of(const PrefixBatch& pb, int cta) {
     }
     return pb.g[lo];
 }
-// pages [first, first + count) of split k
-__device__ inline void prefix_run(const PrefixGroup& g, int k, int* first, int* count) {
-    const int base = g.n_pages / g.splits, rem = g.n_pages % g.splits;
+// pages [first, first + count) of run k of n
+__device__ inline void prefix_run(const PrefixGroup& g, int n, int k, int* first, int* count) {
+    const int base = g.n_pages / n, rem = g.n_pages % n;
     *first = k * base + min(k, rem);
     *count = base + (k < rem ? 1 : 0);
 }
@@ -132,7 +132,7 @@ __device__ inline DecodeWork decode_work(const DecodeParams& p, const InlineBatc
             const PrefixGroup g = prefix_group_of(sb, blockIdx.x);
             const int local = (int)blockIdx.x - g.cta0, split = local / g.tiles;
             d.rows = g.n_seqs * p.G, d.row0 = (local % g.tiles) * rows_per_cta;
-            prefix_run(g, split, &d.w.page_begin, &d.w.n_pages);
+            prefix_run(g, g.splits, split, &d.w.page_begin, &d.w.n_pages);
             d.w.trow = g.trow, d.w.len = g.n_pages * PAGE_TOKENS, d.w.batch = g.b0, d.w.split = split, d.w.first = 0, d.w.pad1 = 0;
             d.base = (int64_t)g.base + ((int64_t)split * p.Hkv + kvh) * d.rows;
             return d;

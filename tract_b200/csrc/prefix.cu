@@ -7,14 +7,17 @@
 //   out = sum_k e^(m_k - m) O_k / sum_k e^(m_k - m) l_k,   m = max m_k      combine_shared_kernel
 // Semantics of each row: transformers/src/ops/flash_sdpa.rs:239-341 with one query.  The reference has no counterpart of the
 // sharing itself: its states are cloned whole (gpu/src/ops/dyn_kv_cache.rs:136-168).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 #include <vector>
 
 #include "attn_convert.cuh"
 #include "decode_common.h"
 #include "q40_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace b200kv {
 
@@ -32,27 +35,34 @@ constexpr int X_XCHG = 8;          // per tile and page parity: one flag per sof
 constexpr float X_SKIP_FRACTION = 0.125f;
 enum { PSRC_PAGES16 = 0, PSRC_Q8 = 1, PSRC_Q4 = 2 };
 
-template <int NQ, int D, int SRC>
+constexpr int X_CLUSTER = 2;  // CTAs that join their runs before a partial leaves the chip
+
+// ALT: one tile of 128 rows, whose pages two pipelines take in turn; otherwise two tiles, which read every staged page twice.
+template <bool ALT, int D, int SRC>
 struct XGeo {
     static constexpr bool RAW = SRC != PSRC_PAGES16;   // block-quantised pages: converter warps rebuild the operand tiles
     static constexpr int FT = RAW ? 128 : 32;          // converter threads, or the copy warp
+    static constexpr int ROWS = ALT ? XM : 2 * XM;     // rows of a CTA
+    static constexpr int USERS = ALT ? 1 : 2;          // pipelines that read a staged page
     static constexpr int PLANES = D / 64;
     static constexpr int CHUNK = PAGE_TOKENS * D * 2;  // one operand tile: 64 keys
     static constexpr int QBYTES = XM * D * 2;
     static constexpr int KPARTS = RAW ? 2 : 1;         // K as value + remainder where it was rounded
     static constexpr int KSTAGE = KPARTS * CHUNK;
-    static constexpr int RESIDENT = (NQ == 1 && !RAW) ? 2 : 1;  // CTAs per SM
-    static constexpr int NK = RAW ? 2 : (NQ == 2 ? 4 : (D == 64 ? 4 : 2));
-    static constexpr int NV = RAW ? 3 : (NQ == 2 ? 5 : (D == 64 ? 4 : 2));
+    static constexpr int NK = RAW ? (ALT ? 3 : 2) : 4;
+    static constexpr int NV = RAW ? 3 : 5;
     static constexpr int NR = RAW ? 2 : 1;
     static constexpr int RAW_STAGE = RAW ? 2 * (PAGE_TOKENS * D + PAGE_TOKENS * (D / 32) * 2) : 0;
-    static constexpr int THREADS = NQ * X_SM_THREADS + 32 * NQ + FT;
-    static constexpr int N_BARS = 2 * NK + 2 * NV + 6 * NQ + 2 * NR;
+    static constexpr int THREADS = 2 * X_SM_THREADS + 64 + FT;
+    static constexpr int N_BARS = 2 * NK + 2 * NV + 12 + 2 * NR;
     static constexpr uint32_t COL_S = D, COLS_PER_TILE = 256;  // TMEM: O in columns 0 .. D-1, the two S buffers behind it
-    static constexpr size_t SMEM = (size_t)NQ * QBYTES + (size_t)NK * KSTAGE + (size_t)NV * CHUNK + (size_t)NR * RAW_STAGE + N_BARS * 8 + 32 +
-                                   NQ * 2 * X_XCHG * 4;
-    static_assert(COL_S + 128 <= COLS_PER_TILE && NQ * COLS_PER_TILE * RESIDENT <= 512, "TMEM columns of an SM");
-    static_assert(RESIDENT * (SMEM + 1024) <= 228 * 1024 && SMEM <= 227 * 1024, "shared memory of an SM");
+    static constexpr int PARTS = (ALT ? 2 : 1) * X_CLUSTER;    // partials of a row in a cluster
+    static constexpr int ML_BYTES = PARTS * ROWS * 8;
+    // what the other parts send of the columns that a CTA joins: over the operand rings, which are done with by then
+    static constexpr size_t JOIN = (size_t)(PARTS - 1) * ROWS * (D / X_CLUSTER) * 4;
+    static constexpr size_t RINGS = (size_t)NK * KSTAGE + (size_t)NV * CHUNK + (size_t)NR * RAW_STAGE;
+    static constexpr size_t SMEM = (size_t)ROWS * D * 2 + RINGS + N_BARS * 8 + 32 + 4 * X_XCHG * 4 + ML_BYTES;
+    static_assert(COL_S + 128 <= COLS_PER_TILE && JOIN <= RINGS && SMEM <= 227 * 1024, "TMEM columns and shared memory of an SM");
 };
 
 // The shared pages against every row that sees them, on the 5th-generation tensor cores.
@@ -60,88 +70,101 @@ struct XGeo {
 //   P = 2^(scale log2e S - m)   one thread per row, m raised only when exceeded by 2^8, l = sum P
 //   O += P V    A = P from TMEM, B = V as it lies in the page
 // The pipeline -- S double-buffered in TMEM, P over the S it came from, rings of K and V tiles, bounded waits -- is the one
-// of prefill_tc.cu and attn_tc.cu; there are no masks (every row sees every shared page whole), the rows come from different
-// sequences, and the result is the run's partial (m, l, O) in f32 for the combine pass.
-// Bound: a page and kv head is 32 KB of f16 (1340 cycles of an SM's share of HBM at the copy rate); its products for 128 rows
-// take 640 to 900 cycles of the tensor pipe.  Up to 128 rows one tile per CTA and two CTAs per SM (16-bit pages), so that one
-// CTA's softmax runs under the other's products; more rows go two tiles to a CTA, which read each staged page twice.
-template <int NQ, int D, int SRC>
-__global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::RESIDENT)
+// of prefill_tc.cu and attn_tc.cu; there are no masks (every row sees every shared page whole) and the rows come from different
+// sequences.  The result is a run's partial (m, l, O) in f32 for the combine pass.
+// Bound: a page and kv head is 32 KB of f16, 1340 cycles of an SM's share of HBM at the copy rate; its products for 128 rows
+// take 640 to 900 cycles of the tensor pipe, but one pipeline needs 3400 cycles from a page to the next (product, softmax,
+// product, each waiting for the one before).  Two pipelines per CTA therefore: up to 128 rows they take the pages in turn.
+// A CTA has a run of pages; the two CTAs of a cluster have neighbouring runs and join (m, l, O) through distributed shared
+// memory, each for half of the channels, before a partial is written: half of the partials' traffic and workspace, which
+// otherwise limits the runs to fewer than the GPU has SMs.
+template <bool ALT, int D, int SRC>
+__global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims__(X_CLUSTER, 1, 1)
     prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
-    using GEO = XGeo<NQ, D, SRC>;
+    using GEO = XGeo<ALT, D, SRC>;
     constexpr int NK = GEO::NK, NV = GEO::NV, NR = GEO::NR, CHUNK = GEO::CHUNK, QBYTES = GEO::QBYTES, PLANES = GEO::PLANES;
-    constexpr int KSTAGE = GEO::KSTAGE, KPARTS = GEO::KPARTS, FT = GEO::FT;
+    constexpr int KSTAGE = GEO::KSTAGE, KPARTS = GEO::KPARTS, FT = GEO::FT, ROWS = GEO::ROWS, PARTS = GEO::PARTS;
     constexpr bool RAW = GEO::RAW;  // converted pages: f16 operands whatever the query type
     constexpr uint32_t COL_O = 0, COL_S = GEO::COL_S, COLS_PER_TILE = GEO::COLS_PER_TILE;
     constexpr int FILL_ARRIVALS = RAW ? FT / 32 : 1;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* q_s = smem;                                    // [NQ][PLANES][128 rows][128 B], swizzled
-    uint8_t* k_ring = smem + NQ * QBYTES;                   // NK K stages of KPARTS tiles
+    uint8_t* q_s = smem;                                    // [ROWS / 128][PLANES][128 rows][128 B], swizzled
+    uint8_t* k_ring = smem + ROWS * D * 2;                  // NK K stages of KPARTS tiles
     uint8_t* v_ring = k_ring + NK * KSTAGE;                 // NV V tiles
     uint8_t* raw_ring = v_ring + NV * CHUNK;                // NR raw chunk pairs
     uint64_t* full_k = (uint64_t*)(raw_ring + NR * GEO::RAW_STAGE);  // [NK] the tile is complete
     uint64_t* full_v = full_k + NK;                         // [NV]
-    uint64_t* free_k = full_v + NV;                         // [NK] every tile's Q.K^T on the stage has completed
-    uint64_t* free_v = free_k + NK;                         // [NV] every tile's P.V on the stage has completed
-    uint64_t* bar_s = free_v + NV;                          // [NQ][2] S buffer written
-    uint64_t* bar_p = bar_s + 2 * NQ;                       // [NQ][2] P written by the softmax warps
-    uint64_t* bar_o = bar_p + 2 * NQ;                       // [NQ][2] P.V of page j completed, on barrier j & 1
-    uint64_t* full_raw = bar_o + 2 * NQ;                    // [NR] raw bytes landed
+    uint64_t* free_k = full_v + NV;                         // [NK] every Q.K^T on the stage has completed
+    uint64_t* free_v = free_k + NK;                         // [NV] every P.V on the stage has completed
+    uint64_t* bar_s = free_v + NV;                          // [2 pipelines][2] S buffer written
+    uint64_t* bar_p = bar_s + 4;                            // [2][2] P written by the softmax warps
+    uint64_t* bar_o = bar_p + 4;                            // [2][2] P.V of a pipeline's page i completed, on barrier i & 1
+    uint64_t* full_raw = bar_o + 4;                         // [NR] raw bytes landed
     uint64_t* free_raw = full_raw + NR;                     // [NR] every converter warp is done with the raw stage
     uint32_t* tmem_slot = (uint32_t*)(((uintptr_t)(free_raw + NR) + 15) & ~(uintptr_t)15);
     volatile int* fail_s = (volatile int*)(tmem_slot + 1);
-    float* xchg = (float*)(tmem_slot + 4);                  // [NQ][2 parities][X_XCHG]
+    float* xchg = (float*)(tmem_slot + 4);                  // [2][2 parities][X_XCHG]
+    float2* ml_s = (float2*)(xchg + 4 * X_XCHG);            // [PARTS][ROWS] (m, l) of every part of the cluster
+    float4* join_s = (float4*)k_ring;                       // [PARTS - 1][D / X_CLUSTER / 4][ROWS]
 
     const DecodeParams& dp = p.d;
+    cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kvh = blockIdx.y;
+    const int kvh = blockIdx.y, rank = (int)cluster.block_rank();
     const PrefixGroup grp = prefix_group_of(pb, blockIdx.x);
-    const int split = (blockIdx.x - grp.cta0) / grp.tiles, tile = (blockIdx.x - grp.cta0) % grp.tiles;
-    int page0, n_tiles;
-    prefix_run(grp, split, &page0, &n_tiles);
+    const int at = ((int)blockIdx.x - grp.cta0) / X_CLUSTER, joined = at / grp.tiles, tile = at % grp.tiles;
+    int page0, n_pages;
+    prefix_run(grp, grp.splits * X_CLUSTER, joined * X_CLUSTER + rank, &page0, &n_pages);
     const int n_rows = grp.n_seqs * dp.G;
+    // pages of pipeline t, and the page its i-th one is
+    auto pages_of = [&](int t) { return ALT ? (n_pages - t + 1) / 2 : n_pages; };
+    auto page_at = [&](int t, int i) { return ALT ? 2 * i + t : i; };
 
     if (tid == 0) {
-        for (int s = 0; s < NK; s++) mbar_init(&full_k[s], FILL_ARRIVALS), mbar_init(&free_k[s], NQ);
-        for (int s = 0; s < NV; s++) mbar_init(&full_v[s], FILL_ARRIVALS), mbar_init(&free_v[s], NQ);
-        for (int i = 0; i < 2 * NQ; i++) mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], X_SM_THREADS / 32);
-        for (int i = 0; i < 2 * NQ; i++) mbar_init(&bar_o[i], 1);
+        for (int s = 0; s < NK; s++) mbar_init(&full_k[s], FILL_ARRIVALS), mbar_init(&free_k[s], GEO::USERS);
+        for (int s = 0; s < NV; s++) mbar_init(&full_v[s], FILL_ARRIVALS), mbar_init(&free_v[s], GEO::USERS);
+        for (int i = 0; i < 4; i++) mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], X_SM_THREADS / 32);
+        for (int i = 0; i < 4; i++) mbar_init(&bar_o[i], 1);
         for (int s = 0; s < NR; s++) mbar_init(&full_raw[s], 1), mbar_init(&free_raw[s], FT / 32);
         *fail_s = (smem_u32(smem) & 1023u) ? 1 : 0;  // the swizzled operand tiles need a 1024-byte aligned base
         mbar_fence_init();
     }
-    if (warp == 0) tmem_alloc(tmem_slot, COLS_PER_TILE * NQ);
+    if (warp == 0) tmem_alloc(tmem_slot, COLS_PER_TILE * 2);
+    cluster.barrier_arrive();  // every CTA of the cluster runs before one writes into the other's shared memory
     grid_dependency_wait();    // the append before this launch has written its pages, and whoever made q is done
     grid_launch_dependents();  // the next kernel may be scheduled; it waits for this grid before it reads the partials
 
-    const int qt = min(tid / X_SM_THREADS, NQ - 1), w4 = (tid % X_SM_THREADS) >> 5;
+    const int qt = min(tid / X_SM_THREADS, 1), w4 = (tid % X_SM_THREADS) >> 5;  // pipeline, lane quarter
     const int row = w4 * 32 + lane;
-    const int my_row = (tile * NQ + qt) * XM + row;  // row of the group: sequence my_row / G, head my_row % G
+    const int cta_row = ALT ? row : qt * XM + row;
+    const int my_row = tile * ROWS + cta_row;  // row of the group: sequence my_row / G, head my_row % G
     const bool live = my_row < n_rows;
-    const bool is_softmax = tid < NQ * X_SM_THREADS;
+    const bool is_softmax = tid < 2 * X_SM_THREADS;
     const int is_bf16 = dp.dtype == B200KV_BF16;
     const int mma_bf16 = RAW ? 0 : is_bf16;  // type of the tensor-core operands (Q, K, V, P)
 
-    // ---- Q tile -> shared memory, K-major with the 128-byte swizzle; this thread moves its row ----
+    // ---- Q tile -> shared memory, K-major with the 128-byte swizzle; a thread moves its row, or (ALT) half of it ----
     if (is_softmax) {
         const int b = grp.b0 + (live ? my_row / dp.G : 0), head = kvh * dp.G + (live ? my_row % dp.G : 0);
         const uint4* src = (const uint4*)((const uint16_t*)dp.q + (int64_t)b * dp.qb + (int64_t)head * dp.qh);
+        constexpr int UNITS = ALT ? D / 16 : D / 8;
 #pragma unroll
-        for (int uu = 0; uu < D / 8; uu++) {
+        for (int e = 0; e < UNITS; e++) {
+            const int uu = ALT ? qt * UNITS + e : e;
             uint32_t w[4] = {0u, 0u, 0u, 0u};
             if (live) {
                 if (dp.q_cos || (RAW && is_bf16)) {
                     // the rotated value is rounded to the query's type, as a separate rope kernel would store it; over
                     // converted pages a bf16 query becomes f16 (every bf16 value is an f16 value, short of its range)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float a = load_query(dp, D, b, head, uu * 8 + 2 * e), c = load_query(dp, D, b, head, uu * 8 + 2 * e + 1);
+                    for (int j = 0; j < 4; j++) {
+                        const float a = load_query(dp, D, b, head, uu * 8 + 2 * j), c = load_query(dp, D, b, head, uu * 8 + 2 * j + 1);
                         if (mma_bf16) {
                             const __nv_bfloat162 h = __floats2bfloat162_rn(a, c);
-                            w[e] = *(const uint32_t*)&h;
+                            w[j] = *(const uint32_t*)&h;
                         } else {
                             const __half2 h = __floats2half2_rn(a, c);
-                            w[e] = *(const uint32_t*)&h;
+                            w[j] = *(const uint32_t*)&h;
                         }
                     }
                 } else {
@@ -150,7 +173,7 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
                 }
             }
             const int plane = uu / 8, u8 = uu % 8;
-            *(uint4*)(q_s + qt * QBYTES + plane * (XM * 128) + row * 128 + ((u8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *(uint4*)(q_s + (ALT ? 0 : qt * QBYTES) + plane * (XM * 128) + row * 128 + ((u8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         fence_async_proxy();  // generic-proxy writes -> visible to the tensor core
     }
@@ -167,21 +190,24 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
         }
         return dp.pool + (int64_t)pg * dp.page_bytes + (int64_t)kvh * (2 * p.chunk_bytes);
     };
+    const uint32_t lane_base = tmem + qt * COLS_PER_TILE + ((uint32_t)(w4 * 32) << 16);  // softmax threads: this warp's lane quarter
+    float m_ref = -INFINITY, l_run = 0.f;
 
     if (!is_softmax) {
         // Every lane of these warps walks its loop (the values stay warp-uniform); one elected lane issues.
-        const int role = warp - NQ * (X_SM_THREADS / 32);  // 0 .. NQ - 1: MMAs of tile `role`; above: the copy warp or the converters
-        if (role < NQ) {
-            const int t = role;
+        const int role = warp - 2 * (X_SM_THREADS / 32);  // 0, 1: MMAs of that pipeline; above: the copy warp or the converters
+        if (role < 2) {
+            const int t = role, n = pages_of(t);
             const uint32_t tm = tmem + t * COLS_PER_TILE;
             const uint32_t idesc_s = instr_desc(mma_bf16, 0, XM, PAGE_TOKENS);
             const uint32_t idesc_o = instr_desc(mma_bf16, 1, XM, D);
-            const uint64_t q_desc = smem_desc(smem_u32(q_s) + t * QBYTES, 0, 1024);
+            const uint64_t q_desc = smem_desc(smem_u32(q_s) + (ALT ? 0 : t * QBYTES), 0, 1024);
             const uint64_t k_desc = smem_desc(smem_u32(k_ring), 0, 1024);
             // V tile: planes of 64 channels 8192 bytes apart (leading dimension), 8-key groups 1024 bytes apart
             const uint64_t v_desc = smem_desc(smem_u32(v_ring), PAGE_TOKENS * 128, 1024);
             const bool adaptive = !mma_bf16;
-            auto issue_qk = [&](int j) {  // S(j) = Q . K(j)^T into buffer j & 1
+            auto issue_qk = [&](int i) {  // S(i) = Q . K^T of the pipeline's i-th page into buffer i & 1
+                const int j = page_at(t, i);
                 wait_or_fail(&full_k[j % NK], (uint32_t)((j / NK) & 1), fail_s);
                 tc_fence_after();
                 if (elect_one()) {
@@ -193,46 +219,47 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
                             const uint64_t off = (uint64_t)((pl * (XM * 128) + kk * 32) >> 4);
                             const uint64_t koff = (uint64_t)((pl * (PAGE_TOKENS * 128) + kk * 32) >> 4);
                             if constexpr (KPARTS == 2) {
-                                tc_mma_ss_a<A_KEEP>(tm + COL_S + 64 * (j & 1), q_desc + off, kd + koff, idesc_s, (pl | kk) ? 1u : 0u);
-                                tc_mma_ss_a<A_REUSE_LAST>(tm + COL_S + 64 * (j & 1), q_desc + off, kd + (uint64_t)(CHUNK >> 4) + koff, idesc_s, 1u);
+                                tc_mma_ss_a<A_KEEP>(tm + COL_S + 64 * (i & 1), q_desc + off, kd + koff, idesc_s, (pl | kk) ? 1u : 0u);
+                                tc_mma_ss_a<A_REUSE_LAST>(tm + COL_S + 64 * (i & 1), q_desc + off, kd + (uint64_t)(CHUNK >> 4) + koff, idesc_s, 1u);
                             } else {
-                                tc_mma_ss(tm + COL_S + 64 * (j & 1), q_desc + off, kd + koff, idesc_s, (pl | kk) ? 1u : 0u);
+                                tc_mma_ss(tm + COL_S + 64 * (i & 1), q_desc + off, kd + koff, idesc_s, (pl | kk) ? 1u : 0u);
                             }
                         }
-                    tc_commit(&bar_s[2 * t + (j & 1)]);
+                    tc_commit(&bar_s[2 * t + (i & 1)]);
                     tc_commit(&free_k[j % NK]);
                 }
                 __syncwarp();
             };
-            issue_qk(0);
-            if (n_tiles > 1) issue_qk(1);
-            for (int j = 0; j < n_tiles; j++) {
+            if (n > 0) issue_qk(0);
+            if (n > 1) issue_qk(1);
+            for (int i = 0; i < n; i++) {
+                const int j = page_at(t, i);
                 wait_or_fail(&full_v[j % NV], (uint32_t)((j / NV) & 1), fail_s);
-                wait_or_fail(&bar_p[2 * t + (j & 1)], (uint32_t)((j >> 1) & 1), fail_s);
+                wait_or_fail(&bar_p[2 * t + (i & 1)], (uint32_t)((i >> 1) & 1), fail_s);
                 tc_fence_after();
-                const int* flags = (const int*)(xchg + (2 * t + (j & 1)) * X_XCHG);
+                const int* flags = (const int*)(xchg + (2 * t + (i & 1)) * X_XCHG);
                 const bool two = !adaptive || __any_sync(0xffffffffu, flags[lane & 3] != 0);
                 if (elect_one()) {
                     const uint64_t vd = v_desc + (uint64_t)(((j % NV) * CHUNK) >> 4);
-                    const uint32_t pa = tm + COL_S + 64 * (j & 1);
+                    const uint32_t pa = tm + COL_S + 64 * (i & 1);
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++) {
-                        tc_mma_ts(tm + COL_O, pa + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, (j | kk) ? 1u : 0u);
+                        tc_mma_ts(tm + COL_O, pa + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, (i | kk) ? 1u : 0u);
                         if (two) tc_mma_ts(tm + COL_O, pa + 32 + kk * 8, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, 1u);
                     }
-                    tc_commit(&bar_o[2 * t + (j & 1)]);
+                    tc_commit(&bar_o[2 * t + (i & 1)]);
                     tc_commit(&free_v[j % NV]);
                 }
                 __syncwarp();
-                // S(j + 2) reuses the buffer P(j) sits in: the tensor core runs one thread's MMAs in issue order
-                if (j + 2 < n_tiles) issue_qk(j + 2);
+                // S(i + 2) reuses the buffer P(i) sits in: the tensor core runs one thread's MMAs in issue order
+                if (i + 2 < n) issue_qk(i + 2);
             }
         } else if constexpr (!RAW) {
             // ================= the chunks of a 16-bit page are the operand tiles =================
-            int32_t pg_next = pages[0];
-            for (int i = 0; i < n_tiles; i++) {
+            int32_t pg_next = n_pages > 0 ? pages[0] : 0;
+            for (int i = 0; i < n_pages; i++) {
                 const uint8_t* src = page_src(pg_next);
-                if (i + 1 < n_tiles) pg_next = pages[i + 1];  // fetched one page ahead of its use
+                if (i + 1 < n_pages) pg_next = pages[i + 1];  // fetched one page ahead of its use
                 if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
                 if (elect_one()) {
                     mbar_expect_tx(&full_k[i % NK], CHUNK);
@@ -249,7 +276,7 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
         } else {
             // ================= converter warps: raw chunk pair -> f16 operand tiles =================
             constexpr int FMT = SRC == PSRC_Q8 ? B200KV_FMT_Q8_1 : B200KV_FMT_Q4_0;
-            const int ft = tid - (NQ * X_SM_THREADS + 32 * NQ);
+            const int ft = tid - (2 * X_SM_THREADS + 64);
             const bool requester = ft < 32;  // the first converter warp also requests the raw pages
             auto request = [&](int i, int32_t pg) {
                 const uint8_t* src = page_src(pg);
@@ -261,10 +288,10 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
             };
             int32_t pg_next = 0;
             if (requester) {
-                for (int i = 0; i < NR && i < n_tiles; i++) request(i, pages[i]);
-                if (NR < n_tiles) pg_next = pages[NR];
+                for (int i = 0; i < NR && i < n_pages; i++) request(i, pages[i]);
+                if (NR < n_pages) pg_next = pages[NR];
             }
-            for (int i = 0; i < n_tiles; i++) {
+            for (int i = 0; i < n_pages; i++) {
                 const uint8_t* raw = raw_ring + (i % NR) * GEO::RAW_STAGE;
                 wait_or_fail(&full_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
                 if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
@@ -277,35 +304,34 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
                 fence_async_proxy();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full_v[i % NV]), mbar_arrive(&free_raw[i % NR]);
-                if (requester && i + NR < n_tiles) {  // the stage is free once the other converter warps have left it too
+                if (requester && i + NR < n_pages) {  // the stage is free once the other converter warps have left it too
                     wait_or_fail(&free_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
                     request(i + NR, pg_next);
-                    if (i + NR + 1 < n_tiles) pg_next = pages[i + NR + 1];
+                    if (i + NR + 1 < n_pages) pg_next = pages[i + NR + 1];
                 }
             }
         }
     } else {
         // ================= softmax threads =================
-        const uint32_t lane_base = tmem + qt * COLS_PER_TILE + ((uint32_t)(w4 * 32) << 16);  // this warp's lane quarter
         const bool adaptive = !mma_bf16;
         const float sl2 = dp.scale * 1.4426950408889634f;  // scores enter the exponent in log2 units
-        float m_ref = -INFINITY, l_run = 0.f, log_thresh = -INFINITY;
-
-        for (int j = 0; j < n_tiles; j++) {
-            const uint32_t sbuf = lane_base + COL_S + 64 * (j & 1);
-            wait_or_fail(&bar_s[2 * qt + (j & 1)], (uint32_t)((j >> 1) & 1), fail_s);
+        float log_thresh = -INFINITY;
+        const int n = pages_of(qt);
+        for (int i = 0; i < n; i++) {
+            const uint32_t sbuf = lane_base + COL_S + 64 * (i & 1);
+            wait_or_fail(&bar_s[2 * qt + (i & 1)], (uint32_t)((i >> 1) & 1), fail_s);
             tc_fence_after();
             uint32_t sr[64];
             tmem_ld32(sbuf, sr);
             tmem_ld32(sbuf + 32, sr + 32);
             tmem_ld_wait();
             const float tmax = row_max64(sr) * sl2;
-            int* flags = (int*)(xchg + (2 * qt + (j & 1)) * X_XCHG);
+            int* flags = (int*)(xchg + (2 * qt + (i & 1)) * X_XCHG);
             // Two questions per row, one reduction per warp.  Bit 0: the page needs its remainder product (see X_SKIP_FRACTION;
-            // page 0 always).  Bit 1: the reference maximum is exceeded by more than 2^8 (or was -inf until now): O is rescaled.
-            const bool mine = adaptive && (j == 0 || !(tmax - m_ref + 3.f <= log_thresh));
+            // the first one always).  Bit 1: the reference maximum is exceeded by more than 2^8 (or was -inf until now): O is rescaled.
+            const bool mine = adaptive && (i == 0 || !(tmax - m_ref + 3.f <= log_thresh));
             const bool raise = tmax > m_ref + 8.f || (m_ref == -INFINITY && tmax > -INFINITY);
-            const uint32_t votes = __reduce_or_sync(0xffffffffu, (mine ? 1u : 0u) | (raise && j > 0 ? 2u : 0u));
+            const uint32_t votes = __reduce_or_sync(0xffffffffu, (mine ? 1u : 0u) | (raise && i > 0 ? 2u : 0u));
             const bool two = !adaptive || (votes & 1u);
             if (adaptive && lane == 0) flags[w4] = two ? 1 : 0;
             float alpha = 1.f;
@@ -315,9 +341,9 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
                 l_run *= alpha;
             }
             if (votes & 2u) {
-                // O must hold every page before this one: see prefill_tc.cu for why the wait on barrier (j - 1) & 1 cannot
-                // mistake the completion of P.V(j - 3) or P.V(j + 1) for that of P.V(j - 1)
-                wait_or_fail(&bar_o[2 * qt + ((j - 1) & 1)], (uint32_t)(((j - 1) >> 1) & 1), fail_s);
+                // O must hold every page before this one: see prefill_tc.cu for why the wait on barrier (i - 1) & 1 cannot
+                // mistake the completion of P.V(i - 3) or P.V(i + 1) for that of P.V(i - 1)
+                wait_or_fail(&bar_o[2 * qt + ((i - 1) & 1)], (uint32_t)(((i - 1) >> 1) & 1), fail_s);
                 tc_fence_after();
 #pragma unroll
                 for (int cc = 0; cc < D / 16; cc++) {
@@ -342,25 +368,77 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_p[2 * qt + (j & 1)]);
+            if (lane == 0) mbar_arrive(&bar_p[2 * qt + (i & 1)]);
         }
-        // ---- the partial of this run: m in natural-log units, l, O ----
-        wait_or_fail(&bar_o[2 * qt + ((n_tiles - 1) & 1)], (uint32_t)(((n_tiles - 1) >> 1) & 1), fail_s);
+        if (n > 0) wait_or_fail(&bar_o[2 * qt + ((n - 1) & 1)], (uint32_t)(((n - 1) >> 1) & 1), fail_s);
         tc_fence_after();
-        const bool ok = !*fail_s;  // a CTA that gave up publishes an empty partial
-        const int64_t rec = (int64_t)grp.base + ((int64_t)split * dp.Hkv + kvh) * n_rows + my_row;
-        float* dst = dp.part_o + rec * D;
+        if (n == 0 || *fail_s) m_ref = -INFINITY, l_run = 0.f;  // no pages, or a CTA that gave up: an empty partial
+    }
+
+    // ---- join the parts of the cluster: (m, l) to both CTAs, then each CTA's half of the channels ----
+    const int part = ALT ? 2 * rank + qt : rank;
+    cluster.barrier_wait();
+    if (is_softmax)
 #pragma unroll
-        for (int cc = 0; cc < D / 32; cc++) {
-            uint32_t orow[32];
-            tmem_ld32(lane_base + COL_O + cc * 32, orow);
-            tmem_ld_wait();
-            if (live)
+        for (int r = 0; r < X_CLUSTER; r++) cluster.map_shared_rank(ml_s, r)[part * ROWS + cta_row] = make_float2(m_ref, l_run);
+    cluster.sync();  // every pipeline of both CTAs has ended: the operand rings are free
+    constexpr int COLS = D / X_CLUSTER;  // channels a CTA joins: COLS * rank ..
+    float M = -INFINITY, total = 0.f, mine = 0.f;
+    if (is_softmax) {
 #pragma unroll
-                for (int c = 0; c < 32; c += 4)
-                    *(uint4*)(dst + cc * 32 + c) = ok ? make_uint4(orow[c], orow[c + 1], orow[c + 2], orow[c + 3]) : make_uint4(0u, 0u, 0u, 0u);
+        for (int q = 0; q < PARTS; q++) M = fmaxf(M, ml_s[q * ROWS + cta_row].x);
+#pragma unroll
+        for (int q = 0; q < PARTS; q++) {
+            const float2 ml = ml_s[q * ROWS + cta_row];
+            const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+            total = fmaf(f, ml.y, total);
+            if (q == part) mine = f;
         }
-        if (live) *(float2*)(dp.part_ml + rec * 2) = ok ? make_float2(m_ref * 0.6931471805599453f, l_run) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int r = 0; r < X_CLUSTER; r++) {
+            const int home = ALT ? 2 * r : r;  // the part that stays in TMEM until the sum
+            if (part == home) continue;
+            float4* dst = cluster.map_shared_rank(join_s, r) + (size_t)(part < home ? part : part - 1) * (COLS / 4) * ROWS + cta_row;
+#pragma unroll
+            for (int cc = 0; cc < COLS / 16; cc++) {
+                uint32_t o[16];
+                tmem_ld16(lane_base + COL_O + r * COLS + cc * 16, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);  // (an empty part's TMEM holds anything)
+                    if (mine > 0.f)
+                        v = make_float4(__uint_as_float(o[4 * c]) * mine, __uint_as_float(o[4 * c + 1]) * mine, __uint_as_float(o[4 * c + 2]) * mine,
+                                        __uint_as_float(o[4 * c + 3]) * mine);
+                    dst[(cc * 4 + c) * ROWS] = v;
+                }
+            }
+        }
+    }
+    cluster.sync();
+    if (is_softmax && (!ALT || qt == 0)) {
+        const int64_t rec = (int64_t)grp.base + ((int64_t)joined * dp.Hkv + kvh) * n_rows + my_row;
+        float* dst = dp.part_o + rec * D + rank * COLS;
+#pragma unroll
+        for (int cc = 0; cc < COLS / 16; cc++) {
+            uint32_t o[16];
+            tmem_ld16(lane_base + COL_O + rank * COLS + cc * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (mine > 0.f)
+                    v = make_float4(__uint_as_float(o[4 * c]) * mine, __uint_as_float(o[4 * c + 1]) * mine, __uint_as_float(o[4 * c + 2]) * mine,
+                                    __uint_as_float(o[4 * c + 3]) * mine);
+#pragma unroll
+                for (int q = 0; q < PARTS - 1; q++) {
+                    const float4 x = join_s[((size_t)q * (COLS / 4) + cc * 4 + c) * ROWS + cta_row];
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+                if (live) ((float4*)dst)[cc * 4 + c] = v;
+            }
+        }
+        if (live && rank == 0) *(float2*)(dp.part_ml + rec * 2) = make_float2(M * 0.6931471805599453f, total);  // natural-log units
     }
     tc_fence_before();
     __syncthreads();
@@ -369,7 +447,7 @@ __global__ void __launch_bounds__(XGeo<NQ, D, SRC>::THREADS, XGeo<NQ, D, SRC>::R
         __nanosleep(200000);  // give copies that may still be in flight time to land before the CTA's memory is released
         __syncthreads();
     }
-    if (warp == 0) tmem_dealloc(tmem, COLS_PER_TILE * NQ);
+    if (warp == 0) tmem_dealloc(tmem, COLS_PER_TILE * 2);
 }
 
 // ---- the same on the CUDA cores: f32 queries or pages, and 16-bit queries whose rows are not 16-byte aligned -------------
@@ -402,7 +480,7 @@ __global__ void __launch_bounds__(C_THREADS, 2) prefix_simt_kernel(const __grid_
     const PrefixGroup grp = prefix_group_of(pb, blockIdx.x);
     const int split = (blockIdx.x - grp.cta0) / grp.tiles, tile = (blockIdx.x - grp.cta0) % grp.tiles;
     int page0, n_pages;
-    prefix_run(grp, split, &page0, &n_pages);
+    prefix_run(grp, grp.splits, split, &page0, &n_pages);
     const int n_rows = grp.n_seqs * dp.G, row0 = tile * CR;
     grid_dependency_wait();
     grid_launch_dependents();
@@ -621,21 +699,21 @@ static std::vector<Run> shared_runs(const b200kv_cache* c, int32_t n_seqs, const
     return runs;
 }
 
-template <int NQ, int D, int SRC>
+template <bool ALT, int D, int SRC>
 static cudaError_t launch_prefix_tc_t(const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
-    using GEO = XGeo<NQ, D, SRC>;
-    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<NQ, D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GEO::SMEM);
+    using GEO = XGeo<ALT, D, SRC>;
+    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<ALT, D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GEO::SMEM);
     if (e != cudaSuccess) return e;
-    return launch_after_predecessor(prefix_tc_kernel<NQ, D, SRC>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(GEO::THREADS), GEO::SMEM, stream, p, pb);
+    return launch_after_predecessor(prefix_tc_kernel<ALT, D, SRC>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(GEO::THREADS), GEO::SMEM, stream, p, pb);
 }
 template <int D, int SRC>
-static cudaError_t launch_prefix_tc_nq(int nq, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
-    return nq == 2 ? launch_prefix_tc_t<2, D, SRC>(p, pb, ctas, stream) : launch_prefix_tc_t<1, D, SRC>(p, pb, ctas, stream);
+static cudaError_t launch_prefix_tc_rows(bool one_tile, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    return one_tile ? launch_prefix_tc_t<true, D, SRC>(p, pb, ctas, stream) : launch_prefix_tc_t<false, D, SRC>(p, pb, ctas, stream);
 }
-static cudaError_t launch_prefix_tc(int fmt, int D, int nq, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
-    if (fmt == B200KV_FMT_Q8_1) return D == 128 ? launch_prefix_tc_nq<128, PSRC_Q8>(nq, p, pb, ctas, stream) : launch_prefix_tc_nq<64, PSRC_Q8>(nq, p, pb, ctas, stream);
-    if (fmt == B200KV_FMT_Q4_0) return D == 128 ? launch_prefix_tc_nq<128, PSRC_Q4>(nq, p, pb, ctas, stream) : launch_prefix_tc_nq<64, PSRC_Q4>(nq, p, pb, ctas, stream);
-    return D == 128 ? launch_prefix_tc_nq<128, PSRC_PAGES16>(nq, p, pb, ctas, stream) : launch_prefix_tc_nq<64, PSRC_PAGES16>(nq, p, pb, ctas, stream);
+static cudaError_t launch_prefix_tc(int fmt, int D, bool one, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    if (fmt == B200KV_FMT_Q8_1) return D == 128 ? launch_prefix_tc_rows<128, PSRC_Q8>(one, p, pb, ctas, stream) : launch_prefix_tc_rows<64, PSRC_Q8>(one, p, pb, ctas, stream);
+    if (fmt == B200KV_FMT_Q4_0) return D == 128 ? launch_prefix_tc_rows<128, PSRC_Q4>(one, p, pb, ctas, stream) : launch_prefix_tc_rows<64, PSRC_Q4>(one, p, pb, ctas, stream);
+    return D == 128 ? launch_prefix_tc_rows<128, PSRC_PAGES16>(one, p, pb, ctas, stream) : launch_prefix_tc_rows<64, PSRC_PAGES16>(one, p, pb, ctas, stream);
 }
 template <int D>
 static cudaError_t launch_prefix_simt(int fmt, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
@@ -665,9 +743,10 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     int max_rows = 0, max_pages = 1;
     for (const Run& r : runs)
         if (r.n > 1 && r.pages > 0) max_rows = std::max(max_rows, r.n * G), max_pages = std::max(max_pages, r.pages);
-    const int nq = max_rows > XM ? 2 : 1;
-    int rows_cta = tc ? nq * XM : CR;
-    const int64_t slots = 148 * (tc && (nq == 2 || quant) ? 1 : 2);  // resident CTAs
+    const bool one_tile = max_rows <= XM;
+    const int cluster = tc ? X_CLUSTER : 1;                  // CTAs that write one partial
+    int rows_cta = tc ? (one_tile ? XM : 2 * XM) : CR;
+    const int64_t slots = tc ? 148 / X_CLUSTER : 148 * 2;    // resident CTAs, or clusters
 
     // ---- the own pages of every sequence: as launch_decode cuts them, starting behind the shared ones ----
     const bool use_mma = decode_mma_supported(fmt, D, dtype) && !c->force_simt;
@@ -697,13 +776,13 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     int n_items = 0, ctas = 0;
     int64_t n_rec = 0, run_pages = 1;
     if (together) run_pages = std::min<int64_t>(own_chunk, max_pages);
-    else for (int64_t tiles_pages = 0;;) {  // the smallest run length that fills the GPU once
-        tiles_pages = 0;
-        for (const Run& r : runs)
-            if (r.n > 1 && r.pages > 0) tiles_pages += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * ((r.pages + run_pages - 1) / run_pages);
-        if (tiles_pages * Hkv <= slots || run_pages >= max_pages) break;
-        run_pages++;
-    }
+    else
+        for (;; run_pages++) {  // the shortest runs for which every CTA is resident: a run is `cluster` CTAs' pages
+            int64_t n = 0;
+            for (const Run& r : runs)
+                if (r.n > 1 && r.pages > 0) n += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * ((r.pages + run_pages - 1) / run_pages);
+            if (n * Hkv <= slots || run_pages >= max_pages) break;
+        }
     for (;;) {
         ib = InlineBatch{};
         pb = PrefixBatch{};
@@ -726,7 +805,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
             g.splits = (int)std::min<int64_t>(MAX_SPLITS / 2, (r.pages + run_pages - 1) / run_pages);
             g.cta0 = ctas, g.base = (int32_t)n_rec;
             for (int i = 0; i < r.n; i++) sb.pre[r.b0 + i] = make_int4(g.base, g.splits, rows, i * G);
-            ctas += g.tiles * g.splits;
+            ctas += g.tiles * g.splits * (together ? 1 : cluster);
             n_rec += (int64_t)g.splits * Hkv * rows;
         }
         if ((size_t)n_rec * (D + 2) * sizeof(float) <= c->ws_bytes) break;  // sized once, at create: longer runs where it is small
@@ -751,7 +830,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     cudaError_t e = cudaSuccess;
     if (!together) {
         ProfScope ps(c, K_PREFIX, stream);
-        e = tc ? launch_prefix_tc(fmt, D, nq, p, pb, ctas, stream)
+        e = tc ? launch_prefix_tc(fmt, D, one_tile, p, pb, ctas, stream)
                : (D == 128 ? launch_prefix_simt<128>(fmt, p, pb, ctas, stream) : launch_prefix_simt<64>(fmt, p, pb, ctas, stream));
     }
     if (e != cudaSuccess) return fail("shared-prefix launch failed: %s", cudaGetErrorString(e));
