@@ -41,7 +41,7 @@ constexpr int X_CLUSTER = 2;  // CTAs that join their runs before a partial leav
 template <bool ALT, int D, int SRC>
 struct XGeo {
     static constexpr bool RAW = SRC != PSRC_PAGES16;   // block-quantised pages: converter warps rebuild the operand tiles
-    static constexpr int FT = RAW ? 128 : 32;          // converter threads, or the copy warp
+    static constexpr int FT = RAW ? 256 : 0;           // converter threads, beside the copy warp
     static constexpr int ROWS = ALT ? XM : 2 * XM;     // rows of a CTA
     static constexpr int USERS = ALT ? 1 : 2;          // pipelines that read a staged page
     static constexpr int PLANES = D / 64;
@@ -49,11 +49,11 @@ struct XGeo {
     static constexpr int QBYTES = XM * D * 2;
     static constexpr int KPARTS = RAW ? 2 : 1;         // K as value + remainder where it was rounded
     static constexpr int KSTAGE = KPARTS * CHUNK;
-    static constexpr int NK = RAW ? (ALT ? 3 : 2) : 4;
-    static constexpr int NV = RAW ? 3 : 5;
-    static constexpr int NR = RAW ? 2 : 1;
+    static constexpr int NK = RAW ? 2 : 4;
+    static constexpr int NV = RAW ? (ALT ? 4 : 3) : 5;
+    static constexpr int NR = RAW ? (ALT ? 3 : 2) : 1;
     static constexpr int RAW_STAGE = RAW ? 2 * (PAGE_TOKENS * D + PAGE_TOKENS * (D / 32) * 2) : 0;
-    static constexpr int THREADS = 2 * X_SM_THREADS + 64 + FT;
+    static constexpr int THREADS = 2 * X_SM_THREADS + 64 + 32 + FT;
     static constexpr int N_BARS = 2 * NK + 2 * NV + 12 + 2 * NR;
     static constexpr uint32_t COL_S = D, COLS_PER_TILE = 256;  // TMEM: O in columns 0 .. D-1, the two S buffers behind it
     static constexpr int PARTS = (ALT ? 2 : 1) * X_CLUSTER;    // partials of a row in a cluster
@@ -274,40 +274,37 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                 __syncwarp();
             }
         } else {
-            // ================= converter warps: raw chunk pair -> f16 operand tiles =================
             constexpr int FMT = SRC == PSRC_Q8 ? B200KV_FMT_Q8_1 : B200KV_FMT_Q4_0;
-            const int ft = tid - (2 * X_SM_THREADS + 64);
-            const bool requester = ft < 32;  // the first converter warp also requests the raw pages
-            auto request = [&](int i, int32_t pg) {
-                const uint8_t* src = page_src(pg);
-                if (elect_one()) {
-                    mbar_expect_tx(&full_raw[i % NR], 2 * p.chunk_bytes);
-                    bulk_g2s(raw_ring + (i % NR) * GEO::RAW_STAGE, src, 2 * p.chunk_bytes, &full_raw[i % NR]);
+            const int ft = tid - (2 * X_SM_THREADS + 64 + 32);
+            if (ft < 0) {
+                // ================= raw chunk pairs, for the converter warps =================
+                int32_t pg_next = n_pages > 0 ? pages[0] : 0;
+                for (int i = 0; i < n_pages; i++) {
+                    const uint8_t* src = page_src(pg_next);
+                    if (i + 1 < n_pages) pg_next = pages[i + 1];
+                    if (i >= NR) wait_or_fail(&free_raw[i % NR], (uint32_t)((i / NR - 1) & 1), fail_s);
+                    if (elect_one()) {
+                        mbar_expect_tx(&full_raw[i % NR], 2 * p.chunk_bytes);
+                        bulk_g2s(raw_ring + (i % NR) * GEO::RAW_STAGE, src, 2 * p.chunk_bytes, &full_raw[i % NR]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-            };
-            int32_t pg_next = 0;
-            if (requester) {
-                for (int i = 0; i < NR && i < n_pages; i++) request(i, pages[i]);
-                if (NR < n_pages) pg_next = pages[NR];
-            }
-            for (int i = 0; i < n_pages; i++) {
-                const uint8_t* raw = raw_ring + (i % NR) * GEO::RAW_STAGE;
-                wait_or_fail(&full_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
-                if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
-                convert_rows<FMT, D, 0, FT, true>(raw, k_ring + (i % NK) * KSTAGE, k_ring + (i % NK) * KSTAGE + CHUNK, PAGE_TOKENS, ft);
-                fence_async_proxy();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full_k[i % NK]);
-                if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s);
-                convert_rows<FMT, D, 1, FT, true>(raw + p.chunk_bytes, v_ring + (i % NV) * CHUNK, nullptr, PAGE_TOKENS, ft);
-                fence_async_proxy();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full_v[i % NV]), mbar_arrive(&free_raw[i % NR]);
-                if (requester && i + NR < n_pages) {  // the stage is free once the other converter warps have left it too
-                    wait_or_fail(&free_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
-                    request(i + NR, pg_next);
-                    if (i + NR + 1 < n_pages) pg_next = pages[i + NR + 1];
+            } else {
+                // ================= converter warps: raw chunk pair -> f16 operand tiles =================
+                // No warp waits for another one: each goes on with the next page as soon as its share of this one is written.
+                for (int i = 0; i < n_pages; i++) {
+                    const uint8_t* raw = raw_ring + (i % NR) * GEO::RAW_STAGE;
+                    wait_or_fail(&full_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
+                    if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
+                    convert_rows<FMT, D, 0, FT, true>(raw, k_ring + (i % NK) * KSTAGE, k_ring + (i % NK) * KSTAGE + CHUNK, PAGE_TOKENS, ft);
+                    fence_async_proxy();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full_k[i % NK]);
+                    if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s);
+                    convert_rows<FMT, D, 1, FT, true>(raw + p.chunk_bytes, v_ring + (i % NV) * CHUNK, nullptr, PAGE_TOKENS, ft);
+                    fence_async_proxy();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full_v[i % NV]), mbar_arrive(&free_raw[i % NR]);
                 }
             }
         }
