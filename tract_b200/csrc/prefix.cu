@@ -59,7 +59,7 @@ struct XGeo {
     static constexpr int PARTS = (ALT ? 2 : 1) * X_CLUSTER;    // partials of a row in a cluster
     static constexpr int ML_BYTES = PARTS * ROWS * 8;
     // what the other parts send of the columns that a CTA joins: over the operand rings, which are done with by then
-    static constexpr size_t JOIN = (size_t)(PARTS - 1) * ROWS * (D / X_CLUSTER) * 4;
+    static constexpr size_t JOIN = (size_t)(PARTS - 1) * ROWS * (D / X_CLUSTER) * 4 + (size_t)ROWS * (D / X_CLUSTER / 4 + 1) * 16;
     static constexpr size_t RINGS = (size_t)NK * KSTAGE + (size_t)NV * CHUNK + (size_t)NR * RAW_STAGE;
     static constexpr size_t SMEM = (size_t)ROWS * D * 2 + RINGS + N_BARS * 8 + 32 + 4 * X_XCHG * 4 + ML_BYTES;
     static_assert(COL_S + 128 <= COLS_PER_TILE && JOIN <= RINGS && SMEM <= 227 * 1024, "TMEM columns and shared memory of an SM");
@@ -143,22 +143,26 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     const int is_bf16 = dp.dtype == B200KV_BF16;
     const int mma_bf16 = RAW ? 0 : is_bf16;  // type of the tensor-core operands (Q, K, V, P)
 
-    // ---- Q tile -> shared memory, K-major with the 128-byte swizzle; a thread moves its row, or (ALT) half of it ----
+    __syncthreads();  // the barriers are there: the copy warp starts, the others fetch Q meanwhile
+    const int role = warp - 2 * (X_SM_THREADS / 32);  // 0, 1: MMAs of that pipeline; above: copies and conversion; below 0: softmax
+    // ---- Q tiles -> shared memory, K-major with the 128-byte swizzle; neighbouring threads fetch neighbouring units of a row ----
     if (is_softmax) {
-        const int b = grp.b0 + (live ? my_row / dp.G : 0), head = kvh * dp.G + (live ? my_row % dp.G : 0);
-        const uint4* src = (const uint4*)((const uint16_t*)dp.q + (int64_t)b * dp.qb + (int64_t)head * dp.qh);
-        constexpr int UNITS = ALT ? D / 16 : D / 8;
-#pragma unroll
-        for (int e = 0; e < UNITS; e++) {
-            const int uu = ALT ? qt * UNITS + e : e;
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-            if (live) {
-                if (dp.q_cos || (RAW && is_bf16)) {
-                    // the rotated value is rounded to the query's type, as a separate rope kernel would store it; over
-                    // converted pages a bf16 query becomes f16 (every bf16 value is an f16 value, short of its range)
+        constexpr int UNITS = D / 8;
+        auto place = [&](int x) -> uint4* {  // unit x % UNITS of row x / UNITS
+            const int r = x / UNITS, uu = x % UNITS, in_tile = r % XM;
+            return (uint4*)(q_s + (r / XM) * QBYTES + (uu / 8) * (XM * 128) + in_tile * 128 + (((uu % 8) ^ (in_tile & 7)) << 4));
+        };
+        if (dp.q_cos || (RAW && is_bf16)) {
+            // the rotated value is rounded to the query's type, as a separate rope kernel would store it; over converted
+            // pages a bf16 query becomes f16 (every bf16 value is an f16 value, short of its range)
+#pragma unroll 1
+            for (int x = tid; x < ROWS * UNITS; x += 2 * X_SM_THREADS) {
+                const int g_row = tile * ROWS + x / UNITS, b = grp.b0 + g_row / dp.G, head = kvh * dp.G + g_row % dp.G;
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+                if (g_row < n_rows)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const float a = load_query(dp, D, b, head, uu * 8 + 2 * j), c = load_query(dp, D, b, head, uu * 8 + 2 * j + 1);
+                        const float a = load_query(dp, D, b, head, (x % UNITS) * 8 + 2 * j), c = load_query(dp, D, b, head, (x % UNITS) * 8 + 2 * j + 1);
                         if (mma_bf16) {
                             const __nv_bfloat162 h = __floats2bfloat162_rn(a, c);
                             w[j] = *(const uint32_t*)&h;
@@ -167,20 +171,33 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                             w[j] = *(const uint32_t*)&h;
                         }
                     }
-                } else {
-                    const uint4 v = src[uu];
-                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                }
+                *place(x) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            const int plane = uu / 8, u8 = uu % 8;
-            *(uint4*)(q_s + (ALT ? 0 : qt * QBYTES) + plane * (XM * 128) + row * 128 + ((u8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            constexpr int BATCH = ROWS * UNITS / (2 * X_SM_THREADS) < 8 ? ROWS * UNITS / (2 * X_SM_THREADS) : 8;
+#pragma unroll 1
+            for (int x0 = tid; x0 < ROWS * UNITS; x0 += BATCH * 2 * X_SM_THREADS) {
+                uint4 w[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {  // all of them on their way before the first is stored
+                    const int x = x0 + i * 2 * X_SM_THREADS, g_row = tile * ROWS + x / UNITS;
+                    const int b = grp.b0 + g_row / dp.G, head = kvh * dp.G + g_row % dp.G;
+                    w[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (g_row < n_rows) w[i] = ((const uint4*)((const uint16_t*)dp.q + (int64_t)b * dp.qb + (int64_t)head * dp.qh))[x % UNITS];
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) *place(x0 + i * 2 * X_SM_THREADS) = w[i];
+            }
         }
         fence_async_proxy();  // generic-proxy writes -> visible to the tensor core
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    uint32_t tmem = 0;
+    if (role < 2) {
+        tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(2 * X_SM_THREADS + 64) : "memory");  // softmax and MMA warps
+        tc_fence_after();
+        tmem = *tmem_slot;
+    }
 
     const int32_t* pages = dp.table + (int64_t)grp.trow * dp.max_pages_per_seq + page0;
     auto page_src = [&](int32_t pg) {  // a page id outside the pool is reported and replaced, so that the barriers go on
@@ -195,7 +212,6 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
 
     if (!is_softmax) {
         // Every lane of these warps walks its loop (the values stay warp-uniform); one elected lane issues.
-        const int role = warp - 2 * (X_SM_THREADS / 32);  // 0, 1: MMAs of that pipeline; above: the copy warp or the converters
         if (role < 2) {
             const int t = role, n = pages_of(t);
             const uint32_t tm = tmem + t * COLS_PER_TILE;
@@ -415,7 +431,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     cluster.sync();
     if (is_softmax && (!ALT || qt == 0)) {
         const int64_t rec = (int64_t)grp.base + ((int64_t)joined * dp.Hkv + kvh) * n_rows + my_row;
-        float* dst = dp.part_o + rec * D + rank * COLS;
+        float4* out_s = join_s + (size_t)(PARTS - 1) * (COLS / 4) * ROWS;  // [ROWS][COLS / 4 + 1]
 #pragma unroll
         for (int cc = 0; cc < COLS / 16; cc++) {
             uint32_t o[16];
@@ -432,8 +448,15 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                     const float4 x = join_s[((size_t)q * (COLS / 4) + cc * 4 + c) * ROWS + cta_row];
                     v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
                 }
-                if (live) ((float4*)dst)[cc * 4 + c] = v;
+                out_s[cta_row * (COLS / 4 + 1) + cc * 4 + c] = v;
             }
+        }
+        // from rows per thread to neighbouring threads per row
+        asm volatile("bar.sync 2, %0;" ::"n"(ROWS) : "memory");
+        const int64_t rec0 = (int64_t)grp.base + ((int64_t)joined * dp.Hkv + kvh) * n_rows + tile * ROWS;
+        for (int x = cta_row; x < ROWS * (COLS / 4); x += ROWS) {
+            const int r = x / (COLS / 4), u = x % (COLS / 4);
+            if (tile * ROWS + r < n_rows) ((float4*)(dp.part_o + (rec0 + r) * D + rank * COLS))[u] = out_s[r * (COLS / 4 + 1) + u];
         }
         if (live && rank == 0) *(float2*)(dp.part_ml + rec * 2) = make_float2(M * 0.6931471805599453f, total);  // natural-log units
     }
