@@ -96,8 +96,7 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
         bulk_g2s(stages + (size_t)st * Gm::STAGE, src, Gm::STAGE, &bars[st]);
     };
 
-    grid_dependency_wait();    // the append that precedes this launch has written its pages
-    grid_launch_dependents();  // the combine pass may be scheduled; it waits for this grid before reading partials
+    decode_begin(p);
     if (tid == 0) {
         for (int s = 0; s < NS; s++) mbar_init(&bars[s], 1);
         mbar_fence_init();
@@ -280,6 +279,7 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
             p.part_ml[(pbase + g0 + tid) * 2] = -INFINITY;
             p.part_ml[(pbase + g0 + tid) * 2 + 1] = 0.f;
         }
+        decode_end(p);
         return;
     }
     if (warp < GT && lane == 0) {
@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(128) decode_kernel(DecodeParams p, const __gri
         p.part_ml[(pbase + g0 + tid) * 2] = ml_s[tid * 2];
         p.part_ml[(pbase + g0 + tid) * 2 + 1] = ml_s[tid * 2 + 1];
     }
+    decode_end(p);
 }
 
 struct CombineParams {

@@ -34,7 +34,9 @@ struct DecodeParams {
     uint64_t wait_ns = 1000000000ull;  // limit of each bounded barrier wait
     int32_t stall_item = -1;  // -1, or (a test hook) the work item whose CTA of kv head 0 never issues its copies: its first wait
                          // runs out, it flags STATUS_WAIT_EXPIRED, publishes an empty partial and returns
-    int32_t pad0 = 0;
+    // The launch before this one (the attention over shared pages) runs beside it: nothing of it is read here, it has waited for
+    // everything before itself, and one CTA of this grid ends only after it, so that who waits for this grid waits for both.
+    int32_t beside = 0;
 };
 
 // Per-call batch description small enough to travel as a kernel parameter (no host-to-device copy, no
@@ -142,6 +144,13 @@ __device__ inline DecodeWork decode_work(const DecodeParams& p, const InlineBatc
     d.row0 = 0, d.rows = p.G;
     d.base = ((int64_t)blockIdx.x * p.Hkv + kvh) * p.G;
     return d;
+}
+__device__ inline void decode_begin(const DecodeParams& p) {
+    if (!p.beside) grid_dependency_wait();  // the append that precedes this launch has written its pages
+    grid_launch_dependents();               // the combine pass may be scheduled; it waits for this grid before reading partials
+}
+__device__ inline void decode_end(const DecodeParams& p) {
+    if (p.beside && (blockIdx.x | blockIdx.y | blockIdx.z) == 0) grid_dependency_wait();
 }
 // load_query for row `row` of the work
 template <typename SHARED>

@@ -90,8 +90,7 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS)
         mbar_expect_tx(&bars[st], Gm::STAGE);
         bulk_g2s(stages + (size_t)st * Gm::STAGE, src, Gm::STAGE, &bars[st]);
     };
-    grid_dependency_wait();    // the append that precedes this launch has written its pages
-    grid_launch_dependents();  // the combine pass may be scheduled; it waits for this grid before reading partials
+    decode_begin(p);
     int32_t pg_next = 0;  // thread 0: id of the next page to request
     if (tid == 0) {
         for (int s = 0; s < NS; s++) mbar_init(&bars[s], 1);
@@ -394,6 +393,7 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS)
         if (tid == 0) atomicOr(p.status, STATUS_WAIT_EXPIRED);
         for (int idx = tid; idx < ng * MD; idx += 128) p.part_o[(pbase + idx / MD) * MD + idx % MD] = 0.f;
         if (tid < ng) p.part_ml[(pbase + tid) * 2] = -INFINITY, p.part_ml[(pbase + tid) * 2 + 1] = 0.f;
+        decode_end(p);
         return;
     }
     float* om = (float*)stages;                 // [4 warps][8 heads][128 ch]; every stage is consumed by now
@@ -440,6 +440,7 @@ __global__ void __launch_bounds__(128, MGeo<FMT>::MIN_CTAS)
         p.part_ml[(pbase + tid) * 2] = M * 0.6931471805599453f;  // back to natural-log units for the combine pass
         p.part_ml[(pbase + tid) * 2 + 1] = den;
     }
+    decode_end(p);
 }
 
 template <int FMT, typename SHARED>

@@ -766,7 +766,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     const bool one_tile = max_rows <= XM;
     const int cluster = tc ? X_CLUSTER : 1;                  // CTAs that write one partial
     int rows_cta = tc ? (one_tile ? XM : 2 * XM) : CR;
-    const int64_t slots = tc ? 148 / X_CLUSTER : 148 * 2;    // resident CTAs, or clusters
+    int64_t slots = tc ? 148 / X_CLUSTER : 148 * 2;          // resident CTAs, or clusters
 
     // ---- the own pages of every sequence: as launch_decode cuts them, starting behind the shared ones ----
     const bool use_mma = decode_mma_supported(fmt, D, dtype) && !c->force_simt;
@@ -780,6 +780,16 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
             if (r.n > 1 && r.pages > 0) most[i] = MAX_SPLITS / 2;
             own_pages[i] = (s.len + PAGE_TOKENS - 1) / PAGE_TOKENS - first[i] / PAGE_TOKENS;
         }
+    // The own pages run beside the shared ones, on the SMs that these leave: each gets its share of the work (in microseconds of
+    // an SM per page and head: 1.0 to 1.2 for a tile pair, 0.75 for 32 KB of an own page at the copy rate).
+    if (tc) {
+        int64_t own = 0, shared = 0;
+        for (int i = 0; i < n_seqs; i++) own += own_pages[i];
+        for (const Run& r : runs)
+            if (r.n > 1 && r.pages > 0) shared += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * r.pages;
+        const double own_us = (double)own * (2.0 * c->L.chunk_bytes / 32768.0) * 0.75, shared_us = (double)shared * 1.1;
+        slots = std::max<int64_t>(slots / 4, (int64_t)(slots * shared_us / (shared_us + own_us)));
+    }
     // Few rows: the shared pages go through the decode kernel as further work items, eight (four) rows at a time, in one launch
     // with the own pages.  Each CTA of rows reads the pages again, from L2.
     const bool together = max_rows <= TOGETHER_ROWS;
@@ -856,6 +866,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     if (e != cudaSuccess) return fail("shared-prefix launch failed: %s", cudaGetErrorString(e));
     if (together || n_items > 0) {
         ProfScope ps(c, K_DECODE, stream);
+        dp.beside = !together;
         const PrefixBatch* with = together ? &pb : nullptr;
         const int more = together ? ctas - n_items : 0;
         if ((use_mma ? launch_decode_mma(fmt, dp, n_items, stream, &ib, with, more) : launch_decode_simt(fmt, D, dp, n_items, stream, &ib, with, more)) != B200KV_OK)
