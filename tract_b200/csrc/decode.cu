@@ -386,7 +386,7 @@ template <int FMT, int D, int GT, typename SHARED>
 static int launch_decode_t(const DecodeParams& p, int n_items, cudaStream_t stream, const InlineBatch& ib, const SHARED& sb) {
     using Gm = Geo<FMT, D>;
     const size_t smem = (size_t)Gm::NS * Gm::STAGE + decode_tail_bytes<GT>();
-    B200KV_CUDA(cudaFuncSetAttribute(decode_kernel<FMT, D, GT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    B200KV_CUDA((allow_shared_memory<decode_kernel<FMT, D, GT, SHARED>>(smem)));
     dim3 grid(n_items, p.Hkv, (p.G + GT - 1) / GT);
     B200KV_CUDA(launch_after_predecessor(decode_kernel<FMT, D, GT, SHARED>, grid, dim3(128), smem, stream, p, ib, sb));
     return B200KV_OK;

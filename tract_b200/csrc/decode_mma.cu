@@ -449,7 +449,7 @@ static int launch_mma_t(const DecodeParams& p, int n_items, cudaStream_t stream,
     const size_t ring = (size_t)Gm::NS * Gm::STAGE;
     const size_t merge = (size_t)(4 * 8 * MD + 4 * 8 * 2) * 4;  // the warp merge reuses the ring
     const size_t smem = std::max(ring, merge) + MMA_TAIL;
-    B200KV_CUDA(cudaFuncSetAttribute(decode_mma_kernel<FMT, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    B200KV_CUDA((allow_shared_memory<decode_mma_kernel<FMT, SHARED>>(smem)));
     dim3 grid(n_items, p.Hkv, (p.G + 7) / 8);
     B200KV_CUDA(launch_after_predecessor(decode_mma_kernel<FMT, SHARED>, grid, dim3(128), smem, stream, p, ib, sb));
     return B200KV_OK;

@@ -1,5 +1,6 @@
 // Host-side state of a cache handle and helpers shared by the translation units.
 #pragma once
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -29,6 +30,20 @@ struct DeviceGuard {
         if (switched) cudaSetDevice(prev);
     }
 };
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; the driver is asked once per kernel and device.
+template <auto KERNEL>
+inline cudaError_t allow_shared_memory(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 
 struct SeqState {
     bool live = false;

@@ -722,7 +722,7 @@ static std::vector<Run> shared_runs(const b200kv_cache* c, int32_t n_seqs, const
 template <bool ALT, int D, int SRC>
 static cudaError_t launch_prefix_tc_t(const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
     using GEO = XGeo<ALT, D, SRC>;
-    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<ALT, D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GEO::SMEM);
+    cudaError_t e = allow_shared_memory<prefix_tc_kernel<ALT, D, SRC>>(GEO::SMEM);
     if (e != cudaSuccess) return e;
     return launch_after_predecessor(prefix_tc_kernel<ALT, D, SRC>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(GEO::THREADS), GEO::SMEM, stream, p, pb);
 }
@@ -737,7 +737,7 @@ static cudaError_t launch_prefix_tc(int fmt, int D, bool one, const PrefixParams
 }
 template <int D>
 static cudaError_t launch_prefix_simt(int fmt, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(prefix_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)CGeo<D>::SMEM);
+    cudaError_t e = allow_shared_memory<prefix_simt_kernel<D>>(CGeo<D>::SMEM);
     if (e != cudaSuccess) return e;
     return launch_after_predecessor(prefix_simt_kernel<D>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(C_THREADS), CGeo<D>::SMEM, stream, p, pb, fmt);
 }

@@ -940,8 +940,10 @@ extern "C" int b200kv_sample(const void* logits, int64_t stride, int32_t dtype, 
     p.slice = cut.slice;
     p.scratch = n > MAX_ON_CHIP ? (float*)scratch : nullptr;
     const size_t smem = ((sizeof(RowShared) + 15) & ~(size_t)15) + (p.scratch ? 0 : cut.threads > 256 ? (size_t)p.slice * sizeof(float) : (size_t)RING * 256 * 16);
+    constexpr size_t most = ((sizeof(RowShared) + 15) & ~(size_t)15) + 4 * std::max(MAX_ON_CHIP / SP_CLUSTER, 4 * 256 * RING);
     auto kernel = cut.threads == 1024 ? sample_kernel<1024, true> : cut.threads == 512 ? sample_kernel<512, true> : sample_kernel<256, false>;
-    B200KV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    B200KV_CUDA((cut.threads == 1024 ? allow_shared_memory<sample_kernel<1024, true>>(most)
+                                     : cut.threads == 512 ? allow_shared_memory<sample_kernel<512, true>>(most) : allow_shared_memory<sample_kernel<256, false>>(most)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)cut.c, (unsigned)rows), cfg.blockDim = dim3((unsigned)cut.threads), cfg.dynamicSmemBytes = smem, cfg.stream = (cudaStream_t)stream_;
     cudaLaunchAttribute attr[2];
