@@ -372,7 +372,9 @@ int b200kv_cast(const void* src, int64_t src_stride, int32_t src_dtype, void* ds
  * kernel alone; bit 3 (a test hook, consumed by the next decode launch of a non-KIVI cache) exercises the give-up path of
  * the bounded waits without any fault: one CTA of that launch issues no copies, its first wait runs out after 1 ms, it
  * sets the status word, publishes an empty partial and returns -- b200kv_check then reports the expired wait, the
- * output of that call is not meaningful, and the cache is usable as before. */
+ * output of that call is not meaningful, and the cache is usable as before; bits 4 and 5 (test hooks) take one way of
+ * b200kv_attend_shared whatever the sizes: the shared pages as work items of the decode kernel, or through the kernels that
+ * meet all rows at once (where they take the format). */
 int b200kv_profile(b200kv_cache* cache, int32_t enable);
 int b200kv_profile_read(b200kv_cache* cache, int32_t max_records, int32_t* kernel_ids, float* ms, int32_t* n_out);
 

@@ -263,11 +263,13 @@ def family(kv, fmt, io, Hkv, D, prompts, per_prompt, own, hq):
     (64, 1, 16, [640], 9, [7]),              # 144 rows: two tiles
     (128, 2, 24, [4100], 12, [3, 90]),       # 288 rows: two CTAs of two tiles
 ])
-def test_attend_shared_against_64_bits(kv, fmt, io, D, Hkv, G, prompts, per_prompt, own):
+@pytest.mark.parametrize("way", [0, 1, 2])  # the one that the sizes choose, and both others whatever they are
+def test_attend_shared_against_64_bits(kv, fmt, io, D, Hkv, G, prompts, per_prompt, own, way):
     if fmt == "f16" and io == "f32":  # a bit-copy cache takes its own type; its queries may be f32
         cache, seqs = family(kv, fmt, "f16", Hkv, D, prompts, per_prompt, own, Hkv * G)
     else:
         cache, seqs = family(kv, fmt, io, Hkv, D, prompts, per_prompt, own, Hkv * G)
+    cache.profile(False, shared_way=way)
     q = rows(5, (len(seqs), Hkv * G, 1, D), io, scale=1.3)
     out = cache.attend_shared(seqs, q)
     cache.check()
@@ -279,7 +281,8 @@ def test_attend_shared_against_64_bits(kv, fmt, io, D, Hkv, G, prompts, per_prom
 
 
 @pytest.mark.parametrize("fmt,io", FORMATS)
-def test_attend_shared_over_a_mixed_batch(kv, fmt, io):
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_attend_shared_over_a_mixed_batch(kv, fmt, io, way):
     # neighbours that share much, little and nothing, a trimmed sequence, branches of branches, an order that is not that of
     # the sequence ids
     Hkv, D, G = 2, 128, 4
@@ -297,6 +300,7 @@ def test_attend_shared_over_a_mixed_batch(kv, fmt, io):
     cache.trim(gone[0], 300)
     batch = [more[1], b, more[0], lone, deep[2], deep[0], kids[0], deep[1], a, kids[3], kids[1], gone[1], cut]
     q = rows(9, (len(batch), Hkv * G, 1, D), io)
+    cache.profile(False, shared_way=way)
     out = cache.attend_shared(batch, q)
     cache.check()
     ref, size = reference(cache, batch, q)
@@ -313,9 +317,11 @@ def test_attend_shared_over_a_mixed_batch(kv, fmt, io):
 
 
 @pytest.mark.parametrize("fmt,io,D", [("f16", "f16", 128), ("bf16", "bf16", 64), ("q8_1", "bf16", 128), ("f32", "f32", 64)])
-def test_attend_shared_strides_rope_scale_and_quantised_result(kv, fmt, io, D):
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_attend_shared_strides_rope_scale_and_quantised_result(kv, fmt, io, D, way):
     Hkv, G = 2, 4
     cache, seqs = family(kv, fmt, io, Hkv, D, [1300], 6, [5, 70], Hkv * G)
+    cache.profile(False, shared_way=way)
     n, Hq = len(seqs), Hkv * G
     qkv = rows(5, (n, (Hq + 3) * D), io)  # the query heads of a fused projection: rows of a wider matrix
     q = qkv[:, D:D + Hq * D].unflatten(1, (Hq, 1, D))
@@ -325,7 +331,7 @@ def test_attend_shared_strides_rope_scale_and_quantised_result(kv, fmt, io, D):
     wide = torch.full((n, 2 * Hq, 1, D), 7.0, dtype=q.dtype, device="cuda")
     cache.attend_shared(seqs, q, out=wide[:, ::2])
     assert torch.equal(wide[:, ::2], want) and bool((wide[:, 1::2] == 7.0).all())
-    # rows that are not 16-byte aligned: the CUDA-core kernel
+    # rows that are not 16-byte aligned: the decode kernels alone
     odd = torch.empty(n * Hq * D + 1, dtype=q.dtype, device="cuda")[1:].view(n, Hq, 1, D)
     odd.copy_(dense)
     ref, size = reference(cache, seqs, q)
@@ -354,9 +360,11 @@ def test_attend_shared_strides_rope_scale_and_quantised_result(kv, fmt, io, D):
     cache.close()
 
 
-def test_attend_shared_more_than_256_sequences(kv):
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_attend_shared_more_than_256_sequences(kv, way):
     Hkv, D, G, n = 1, 64, 2, 300
     cache, seqs = family(kv, "f16", "f16", Hkv, D, [640], n, [3], Hkv * G)
+    cache.profile(False, shared_way=way)
     q = rows(5, (n, Hkv * G, 1, D), "f16")
     cos, sin = rows(21, (n, 1, D), "f16"), rows(22, (n, 1, D), "f16")
     ref, size = reference(cache, seqs, kv.rope(q, cos, sin))
@@ -369,10 +377,12 @@ def test_attend_shared_more_than_256_sequences(kv):
     cache.close()
 
 
-def test_attend_shared_in_a_small_workspace(kv):
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_attend_shared_in_a_small_workspace(kv, way):
     # a cache that announced one query head per kv head: the partials of the natural split do not fit, longer runs do
     Hkv, D, G = 2, 128, 16
     cache = kv.KvCache("f16", Hkv, D, max_seqs=34, max_seq_tokens=9000, max_q_heads=Hkv)
+    cache.profile(False, shared_way=way)
     parent = cache.new_seq()
     add(cache, [parent], 1, 8000, "f16")
     seqs = cache.fork_shared([parent] * 32)
@@ -385,10 +395,12 @@ def test_attend_shared_in_a_small_workspace(kv):
     cache.close()
 
 
-def test_attend_shared_peaked_scores(kv):
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_attend_shared_peaked_scores(kv, way):
     # weights that sit on single keys of the shared pages, of the own ones, and maxima that rise page by page
     Hkv, D, G = 1, 128, 4
     cache = kv.KvCache("f16", Hkv, D, max_seqs=6, max_seq_tokens=1024, max_q_heads=G)
+    cache.profile(False, shared_way=way)
     parent = cache.new_seq()
     k, v = rows(1, (1, Hkv, 640, D), "f16"), rows(2, (1, Hkv, 640, D), "f16")
     k *= torch.linspace(0.1, 12.0, 640, device="cuda").half()[None, None, :, None]

@@ -426,11 +426,12 @@ class KvCache:
     def check(self):
         _ck(lib().b200kv_check(self._h, _stream()))
 
-    def profile(self, enable=True, force_simt=False, kivi_cuda_core=False, stall_next_decode=False):
+    def profile(self, enable=True, force_simt=False, kivi_cuda_core=False, stall_next_decode=False, shared_way=0):
         """Timing records on / off and the test hooks of b200kv_profile (stall_next_decode: one CTA of the next decode
-        launch gives up on a copy nobody issued, after 1 ms)."""
+        launch gives up on a copy nobody issued, after 1 ms; shared_way: 1 or 2 for one way of attend_shared whatever the
+        sizes, 0 for the way that they choose)."""
         _ck(lib().b200kv_profile(self._h, int(bool(enable)) | (2 if force_simt else 0) | (4 if kivi_cuda_core else 0) |
-                                 (8 if stall_next_decode else 0)))
+                                 (8 if stall_next_decode else 0) | (16 * shared_way)))
 
     def profile_read(self, max_records=65536):
         """[(kernel name, milliseconds)] of the launches recorded since the last read."""

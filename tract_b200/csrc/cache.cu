@@ -922,6 +922,7 @@ int b200kv_profile(b200kv_cache* c, int32_t enable) {
     c->prof_on = (enable & 1) != 0;
     c->force_simt = (enable & 2) != 0;
     c->kivi_cuda_core = (enable & 4) != 0;
+    c->shared_way = (enable & 32) ? 2 : (enable & 16) ? 1 : 0;
     if (enable & 8) c->stall_next_decode = true;  // consumed by the next decode launch
     return B200KV_OK;
 }

@@ -99,6 +99,7 @@ struct b200kv_cache {
     // optional per-launch timing (the analogue of tract-cuda's event pairs around every launch,
     // cuda/src/context.rs:364-453): off by default
     bool kivi_cuda_core = false;  // test hook: KIVI decode through the CUDA-core kernel alone
+    int shared_way = 0;  // test hook: 0 chosen by the sizes, 1 and 2 the two ways of attention over shared pages whatever the sizes
     bool force_simt = false;  // test hook: route decode through the CUDA-core kernel even where the tensor-core one applies
     bool prof_on = false;
     struct ProfRec {
@@ -172,6 +173,7 @@ struct QueryRope {  // what a decode call may fold in at its two ends
     void* act_scratch; // the result also (or only) as the quantised activation of a W4A8 GEMM, or null
 };
 // pages of each sequence that a call walks -> pages per run
+int decode_ctas_per_sm(const b200kv_cache* c, bool use_mma);
 int64_t pages_per_split(const b200kv_cache* c, const int64_t* pages, int n_seqs, bool use_mma, int nz);
 int64_t decode_pages_per_split(const b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int64_t window, bool use_mma, int nz);
 int launch_decode(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q,

@@ -470,8 +470,8 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     if (warp == 0) tmem_dealloc(tmem, COLS_PER_TILE * 2);
 }
 
-// ---- the same on the CUDA cores: f32 queries or pages, and 16-bit queries whose rows are not 16-byte aligned -------------
-// A tile is 32 rows.  Per page: K and V as f32 in shared memory (read once for the 32 rows), S = Q K^T with 2 x 4 scores per
+// ---- the same on the CUDA cores, for f32 pages ---------------------------------------------------------------------------
+// A tile is 32 rows.  Per page: K and V in shared memory (read once for the 32 rows), S = Q K^T with 2 x 4 scores per
 // thread, the online softmax with expf (8 threads per row), O += P V with 2 rows x D / 16 channels per thread.  Bound by the
 // FMA pipe and the shared-memory reads that feed it: 4 D flops per row and key.
 constexpr int CR = 32;         // rows of a tile
@@ -484,7 +484,7 @@ struct CGeo {
 };
 
 template <int D>
-__global__ void __launch_bounds__(C_THREADS, 2) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb, int fmt) {
+__global__ void __launch_bounds__(C_THREADS, 2) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
     constexpr int LD = CGeo<D>::LD, PL = PAGE_TOKENS + 4, CPT = D / 16;
     extern __shared__ __align__(16) float csm[];
     float* q_s = csm;                     // [32][LD]
@@ -529,13 +529,9 @@ __global__ void __launch_bounds__(C_THREADS, 2) prefix_simt_kernel(const __grid_
         for (int x = 0; x < 2; x++) {
             const uint8_t* chunk = kc + x * p.chunk_bytes;
             float* dst = x ? v_s : k_s;
-            if (fmt == B200KV_FMT_F32) {
-                for (int u = tid; u < PAGE_TOKENS * (D / 4); u += C_THREADS) {
-                    const int t = u / (D / 4), c4 = u % (D / 4);
-                    *(float4*)(dst + t * LD + c4 * 4) = *(const float4*)(chunk + chunk_addr(B200KV_FMT_F32, D, x, t, c4 * 16));
-                }
-            } else {
-                for (int u = tid; u < PAGE_TOKENS * D; u += C_THREADS) dst[(u / D) * LD + u % D] = chunk_elem(chunk, fmt, D, x, u / D, u % D);
+            for (int u = tid; u < PAGE_TOKENS * (D / 4); u += C_THREADS) {
+                const int t = u / (D / 4), c4 = u % (D / 4);
+                *(float4*)(dst + t * LD + c4 * 4) = *(const float4*)(chunk + chunk_addr(B200KV_FMT_F32, D, x, t, c4 * 16));
             }
         }
         __syncthreads();
@@ -736,13 +732,53 @@ static cudaError_t launch_prefix_tc(int fmt, int D, bool one, const PrefixParams
     return D == 128 ? launch_prefix_tc_rows<128, PSRC_PAGES16>(one, p, pb, ctas, stream) : launch_prefix_tc_rows<64, PSRC_PAGES16>(one, p, pb, ctas, stream);
 }
 template <int D>
-static cudaError_t launch_prefix_simt(int fmt, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+static cudaError_t launch_prefix_simt(const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
     cudaError_t e = allow_shared_memory<prefix_simt_kernel<D>>(CGeo<D>::SMEM);
     if (e != cudaSuccess) return e;
-    return launch_after_predecessor(prefix_simt_kernel<D>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(C_THREADS), CGeo<D>::SMEM, stream, p, pb, fmt);
+    return launch_after_predecessor(prefix_simt_kernel<D>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(C_THREADS), CGeo<D>::SMEM, stream, p, pb);
 }
 
-constexpr int TOGETHER_ROWS = 32;
+// The three ways of a call, and what each takes in microseconds, fitted to grids of 2 to 64 sequences after 512 to 16384 tokens
+// and to 200 calls of random sizes: the choice is within 10% of the best of the three on all but a few of those (1.45 times at
+// worst), within 2% on average.
+//   ALONE      launch_decode: every sequence reads its pages from L2 or HBM, 8 (4) rows at a time.  No more to set up than
+//              regular attention, but each page is worked on n times.
+//   TOGETHER   one launch of the decode kernel, the shared pages being further work items: rows of several sequences fill the
+//              row tiles that a group of few heads leaves half empty, and the own pages need no launch of their own.  Each CTA
+//              of rows reads the pages again.
+//   APART      the shared pages through the kernels above, every row at once, the own pages beside them.
+// 32 heads over 8, f16 D = 128, alone / together / apart: 2 sequences after 1024 tokens 8.8 / 10.4 / 13.5; 8 after 4096
+// 18.9 / 16.3 / 17.0; 4 after 16384 28.0 / 22.7 / 24.4; 32 after 16384 176 / 148 / 30.
+enum Way { ALONE, TOGETHER, APART };
+struct WaySizes {
+    int fmt, D, Hkv, G, n_seqs, max_rows;
+    bool use_mma, tc;                       // the tensor-core forms of the decode kernel and of the kernel over shared pages
+    int64_t alone, together, apart, own;    // pages x row tiles, per kv head: 8 (4) rows of the decode kernels, XM .. of the others
+};
+static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
+    const bool quant = fmt_is_block_quant(z.fmt);
+    // a page against one row tile of a decode kernel, spread over the GPU: tensor cores 2.6 ns; CUDA cores by the page's bytes
+    // and the work of widening them, a single row three quarters of four
+    double unit = 2.6e-3;
+    if (!z.use_mma) unit = (z.fmt == B200KV_FMT_F32 ? 17e-3 : quant ? 9e-3 : 14e-3) * z.D / 128 * (z.G == 1 ? 0.75 : 1.0);
+    const double own = unit * (double)z.own * z.Hkv;
+    double alone = 6.5 + unit * (double)z.alone * z.Hkv;
+    const int64_t slots = 148 * decode_ctas_per_sm(c, z.use_mma);
+    // with more sequences than one CTA each can be resident, 16-bit pages go in several short rounds (44 sequences after 463
+    // tokens: 25, 36 of them: 14; 28 after 153, with 16 heads: 14)
+    const int64_t own_ctas = (int64_t)z.n_seqs * z.Hkv * ((z.G + (z.use_mma ? 7 : 3)) / (z.use_mma ? 8 : 4));
+    if (z.use_mma && !quant && own_ctas > slots) alone += std::min(10.0, 1.2 * (double)z.alone * z.Hkv / (double)own_ctas);
+    double together = 8.4 + 1.15 * unit * (double)z.together * z.Hkv + own, apart = 1e30;
+    // each sequence's own pages are CTAs of that launch, however few they are: many of them crowd out the shared pages (8 heads
+    // without groups after 4096 tokens: 16 sequences take 16, 32 of them 56)
+    if (own_ctas > slots / 2) together = 1e30;
+    if (z.tc)  // a page for all rows of a CTA, on 148 of them; two tiles of rows take 2.4 times as long as one
+        apart = (quant ? 15.0 : 13.0) + (quant ? 1.3 : 0.9) * (z.max_rows <= XM ? 1.0 : 2.4) * (double)z.apart * z.Hkv / 148 + own;
+    else if (z.fmt == B200KV_FMT_F32)  // whole rounds of 2 CTAs per SM
+        apart = 11.0 + (z.D == 128 ? 13.5 : 11.0) * (double)((z.apart * z.Hkv + 295) / 296) + own;
+    if (apart < together && apart < alone) return APART;
+    return together < alone ? TOGETHER : ALONE;
+}
 
 // At most INLINE_BATCH sequences; `ends` as launch_decode takes it.
 static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q, const int64_t* qs, void* out,
@@ -780,9 +816,22 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
             if (r.n > 1 && r.pages > 0) most[i] = MAX_SPLITS / 2;
             own_pages[i] = (s.len + PAGE_TOKENS - 1) / PAGE_TOKENS - first[i] / PAGE_TOKENS;
         }
+    const int dec_rows = use_mma ? 8 : 4;
+    WaySizes z{fmt, D, Hkv, G, n_seqs, max_rows, use_mma, tc, 0, 0, 0, 0};
+    for (const Run& r : runs)
+        if (r.n > 1 && r.pages > 0) {
+            z.alone += (int64_t)r.n * nz * r.pages, z.together += (int64_t)((r.n * G + dec_rows - 1) / dec_rows) * r.pages;
+            z.apart += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * r.pages;
+        }
+    for (int64_t x : own_pages) z.own += x * nz;
+    z.alone += z.own;
+    const Way way = c->shared_way == 0 ? shared_way(c, z) : c->shared_way == 2 && (tc || fmt == B200KV_FMT_F32) ? APART : TOGETHER;
+    if (way == ALONE) return launch_decode(c, n_seqs, seqs, n_q_heads, q, qs, out, os, dtype, scale, stream, 0, &ends);
+    const bool together = way == TOGETHER;
+    if (together) rows_cta = nz * dec_rows;
     // The own pages run beside the shared ones, on the SMs that these leave: each gets its share of the work (in microseconds of
     // an SM per page and head: 1.0 to 1.2 for a tile pair, 0.75 for 32 KB of an own page at the copy rate).
-    if (tc) {
+    if (tc && !together) {
         int64_t own = 0, shared = 0;
         for (int i = 0; i < n_seqs; i++) own += own_pages[i];
         for (const Run& r : runs)
@@ -790,10 +839,6 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
         const double own_us = (double)own * (2.0 * c->L.chunk_bytes / 32768.0) * 0.75, shared_us = (double)shared * 1.1;
         slots = std::max<int64_t>(slots / 4, (int64_t)(slots * shared_us / (shared_us + own_us)));
     }
-    // Few rows: the shared pages go through the decode kernel as further work items, eight (four) rows at a time, in one launch
-    // with the own pages.  Each CTA of rows reads the pages again, from L2.
-    const bool together = max_rows <= TOGETHER_ROWS;
-    if (together) rows_cta = nz * (use_mma ? 8 : 4);
     std::vector<int64_t> all_pages = own_pages;
     if (together)
         for (const Run& r : runs)
@@ -841,9 +886,8 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
         if ((size_t)n_rec * (D + 2) * sizeof(float) <= c->ws_bytes) break;  // sized once, at create: longer runs where it is small
         bool longest = run_pages >= max_pages;
         for (int i = 0; i < n_seqs; i++) longest &= own_pages[i] <= own_chunk;
-        if (longest)
-            return fail("%d sequences x %d query heads need %zu bytes of split partials, the workspace holds %zu: create the cache "
-                        "with max_q_heads >= %d", n_seqs, n_q_heads, (size_t)n_rec * (D + 2) * sizeof(float), c->ws_bytes, n_q_heads);
+        if (longest)  // the partials of the shared pages beside those of the own ones do not fit: regular attention needs half of them
+            return launch_decode(c, n_seqs, seqs, n_q_heads, q, qs, out, os, dtype, scale, stream, 0, &ends);
         run_pages += std::max<int64_t>(1, run_pages / 4);
         own_chunk += std::max<int64_t>(1, own_chunk / 4);
     }
@@ -861,7 +905,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     if (!together) {
         ProfScope ps(c, K_PREFIX, stream);
         e = tc ? launch_prefix_tc(fmt, D, one_tile, p, pb, ctas, stream)
-               : (D == 128 ? launch_prefix_simt<128>(fmt, p, pb, ctas, stream) : launch_prefix_simt<64>(fmt, p, pb, ctas, stream));
+               : (D == 128 ? launch_prefix_simt<128>(p, pb, ctas, stream) : launch_prefix_simt<64>(p, pb, ctas, stream));
     }
     if (e != cudaSuccess) return fail("shared-prefix launch failed: %s", cudaGetErrorString(e));
     if (together || n_items > 0) {
