@@ -1,5 +1,5 @@
 """Decode-loop driver for a Llama-shaped decoder built from the library's ops: per-layer paged KV caches, Q4_0 linear
-layers, RmsNorm, RoPE, SiLU gating, greedy argmax.
+layers, RmsNorm, RoPE, SiLU gating, greedy argmax or sampling; several continuations of one prompt share its pages.
 
 The caller of the hot path in the reference is examples/causal_llm/src/lib.rs:290-408 (prompt processing, then one
 token per step with the KV caches as model state) and cli/src/llm.rs:47-139 (the pp / tg benchmark loop).  Here the
@@ -107,6 +107,8 @@ class Decoder:
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
         self.cos_t, self.sin_t = z(B, sh.head_dim, dt=self.kv_dtype), z(B, sh.head_dim, dt=self.kv_dtype)
         self.lengths = [0] * n_seqs
+        self.shared = False  # some rows may share pages (branch): their attention reads the shared ones once
+        self.sampling = None  # greedy
         self.graphs = None
         if use_graphs:
             self._capture()
@@ -138,7 +140,10 @@ class Decoder:
         kv.q40_add_rms_norm_quantize(self.x, self.scratch, self.shape.eps, weight=self.final_norm, residual=self.proj if residual else None,
                                      x_out=self.x if residual else None)
         self.lm_head.gemm_quantized(self.B, self.logits, scratch=self.scratch)
-        kv.argmax(self.logits, out=self.tokens)
+        if self.sampling is None:
+            kv.argmax(self.logits, out=self.tokens)
+        else:
+            kv.sample(self.logits, out=self.tokens, **self.sampling)
 
     def _segments(self):
         """The launch sequences of one step that touch no cache: [head + pre(0)], [post(i) + pre(i+1)] ..., [post(last) + tail]."""
@@ -157,22 +162,62 @@ class Decoder:
             for seg in self._segments():  # one eager pass first: lazy initialisation happens outside the capture
                 seg()
             side.synchronize()
-            for seg in self._segments():
-                g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=side):
-                    seg()
-                self.graphs.append(g)
+            self.graphs = [self._captured(seg, side) for seg in self._segments()]
         torch.cuda.synchronize(self.dev)
         self.x.zero_(), self.tokens.zero_()
 
-    # ---- one decode step: `tokens` in, greedy next tokens out (both in self.tokens) --------------------
+    def _captured(self, segment, stream):
+        g = self.torch.cuda.CUDAGraph()
+        with self.torch.cuda.graph(g, stream=stream):
+            segment()
+        return g
+
+    def _choose_tokens_by(self, sampling):
+        self.sampling = sampling
+        if self.graphs:  # the choice is the end of the last segment
+            torch = self.torch
+            if sampling is not None:
+                kv.sample(self.logits, out=torch.empty_like(self.tokens), **sampling)  # lazy initialisation, outside the capture
+            torch.cuda.synchronize(self.dev)  # the graph that goes may still run
+            self.graphs[-1] = self._captured(self._segments()[-1], torch.cuda.Stream(device=self.dev))
+
+    # ---- how the next tokens are chosen ----------------------------------------------------------------
+    def set_sampling(self, temperature=1.0, top_k=None, top_p=None, min_p=None, seed=0):
+        """From now on steps and prompt passes draw their tokens (kv.sample): each setting is a number for every sequence or a
+        list of one per sequence, None leaves it off; a temperature of 0 takes the maximum.  The numbers behind the draws come
+        from a generator that starts at `seed`."""
+        torch = self.torch
+
+        def per_row(value, dtype):
+            if value is None:
+                return None
+            t = torch.as_tensor(value, dtype=dtype, device=self.dev)
+            assert t.dim() == 0 or t.shape == (self.B,)
+            return t.expand(self.B).clone()
+
+        self.draws = torch.Generator(device=self.dev).manual_seed(seed)
+        self._choose_tokens_by(dict(uniform=torch.zeros(self.B, dtype=torch.float32, device=self.dev), temperature=per_row(temperature, torch.float32),
+                                    top_k=per_row(top_k, torch.int32), top_p=per_row(top_p, torch.float32), min_p=per_row(min_p, torch.float32),
+                                    scratch=kv.sample_scratch(self.B, self.shape.vocab, self.dev)))
+
+    def set_greedy(self):
+        """Back to the first maximum of the logits, as a new decoder starts out."""
+        self._choose_tokens_by(None)
+
+    def _new_draws(self):
+        if self.sampling is not None:
+            self.sampling["uniform"].uniform_(generator=self.draws)
+
+    # ---- one decode step: `tokens` in, next tokens out (both in self.tokens) ---------------------------
     def step(self):
         run = (lambda i: self.graphs[i].replay()) if self.graphs else (lambda i, s=self._segments(): s[i]())
+        self._new_draws()
         run(0)
         for i, L in enumerate(self.layers):
             ids = self.seqs[i]
             L["cache"].append_rope(ids, self.k16, self.v16, self.cos_t.view(self.B, 1, -1), self.sin_t.view(self.B, 1, -1))
-            L["cache"].attend_q40(ids, self.q16, self.scratch, cos=self.cos_t, sin=self.sin_t)
+            attend = L["cache"].attend_shared if self.shared else L["cache"].attend_q40
+            attend(ids, self.q16, scratch=self.scratch, cos=self.cos_t, sin=self.sin_t)
             run(i + 1)
         self.pos += 1
         self.lengths = [n + 1 for n in self.lengths]
@@ -184,13 +229,49 @@ class Decoder:
         """Prompt pass: `prompt` is an int32 [B, S] tensor of token ids, all sequences S tokens long, appended after whatever
         the caches hold.  Runs every layer over all B * S rows (the GEMMs share each weight stage between 4 groups of 8
         rows), fills the caches, and leaves the greedy next token of every sequence in self.tokens."""
-        torch, sh, B = self.torch, self.shape, self.B
-        S = int(prompt.shape[1])
+        assert prompt.shape[0] == self.B
+        self._prompt_pass(prompt)
+
+    def prefill_shared(self, prompt):
+        """One prompt (int32, S token ids) for every sequence: runs the prompt pass once, after whatever sequence 0 holds, and
+        makes every sequence a continuation of it (what the others held is dropped).  Their pages are the same until they
+        diverge.  Leaves the next token of every sequence in self.tokens."""
+        self._prompt_pass(prompt.reshape(1, -1))
+        tokens = self.tokens.clone()  # every row has drawn its own
+        self.branch([0] * self.B)
+        self.tokens.copy_(tokens)
+
+    def branch(self, parents):
+        """Sequence i goes on from what sequence parents[i] holds (one index per sequence, any of them any number of times): the
+        re-ordering step of a beam search, or one sequence taken up several times.  Nothing but partly filled last pages is
+        copied; its next token, position and length go along.  Continuations of one sequence that stand next to each other in
+        the batch are attended to together (attend_shared)."""
+        parents = [int(p) for p in parents]
+        assert len(parents) == self.B and all(0 <= p < self.B for p in parents)
+        for i, L in enumerate(self.layers):
+            cache, old = L["cache"], self.seqs[i]
+            dropped = [old[p] for p in range(self.B) if p not in parents]
+            again = [b for b, p in enumerate(parents) if p in parents[:b]]  # the first continuation takes the sequence itself
+            new = [old[p] for p in parents]
+            if dropped:
+                cache.free_seqs(dropped)
+            for b, s in zip(again, cache.fork_shared([old[parents[b]] for b in again]) if again else []):
+                new[b] = s
+            self.seqs[i] = new
+        order = self.torch.tensor(parents, device=self.dev)
+        self.tokens.copy_(self.tokens[order]), self.pos.copy_(self.pos[order])
+        self.lengths = [self.lengths[p] for p in parents]
+        self.shared = self.shared or len(set(parents)) < self.B
+
+    def _prompt_pass(self, prompt):
+        """The prompt pass over the first B sequences: all of them, or one whose last row then stands for every sequence."""
+        torch, sh = self.torch, self.shape
+        B, S = int(prompt.shape[0]), int(prompt.shape[1])
         R = B * S
         dev, f32, kdt = self.dev, torch.float32, self.kv_dtype
         nq, nk = sh.n_q_heads * sh.head_dim, sh.n_kv_heads * sh.head_dim
         pos0 = self.lengths[0]
-        assert all(n == pos0 for n in self.lengths) and prompt.shape[0] == B
+        assert all(n == pos0 for n in self.lengths[:B])
         ids = prompt.to(dev, torch.int32).reshape(R).contiguous()
         x = kv.gather_rows(self.embed, ids)
         scratch = torch.empty(kv.Q40Linear.scratch_bytes(max(sh.hidden, sh.ffn, nq), R), dtype=torch.uint8, device=dev)
@@ -207,18 +288,20 @@ class Decoder:
             kv.q40_add_rms_norm_quantize(x, scratch, sh.eps, weight=L["attn_norm"], residual=proj if i else None, x_out=x if i else None)
             L["wqkv"].gemm_quantized(R, qkv16, scratch=scratch)
             kv.rope(q16, cos, sin, out=q16r)
-            L["cache"].append_rope(self.seqs[i], k16, v16, cos, sin)
-            L["cache"].attend(self.seqs[i], q16r, causal=True, out=attn16.permute(0, 2, 1, 3))
+            seqs = self.seqs[i][:B]
+            L["cache"].append_rope(seqs, k16, v16, cos, sin)
+            L["cache"].attend(seqs, q16r, causal=True, out=attn16.permute(0, 2, 1, 3))
             L["wo"].gemm(attn16.view(R, nq), proj, scratch=scratch)
             kv.q40_add_rms_norm_quantize(x, scratch, sh.eps, weight=L["ffn_norm"], residual=proj, x_out=x)
             L["wgu"].gemm_quantized(R, gate_up, scratch=scratch)
             kv.q40_silu_mul_quantize(gate_up[:, :sh.ffn], gate_up[:, sh.ffn:], scratch)
             L["wd"].gemm_quantized(R, proj, scratch=scratch)
         kv.add(x, proj, out=x)
-        kv.cast(x[S - 1::S], self.x)  # the last row of every sequence
+        kv.cast(x[S - 1::S].expand(self.B, -1), self.x)  # the last row of every sequence
+        self._new_draws()
         self._tail(residual=False)
-        self.pos += S
-        self.lengths = [n + S for n in self.lengths]
+        self.pos[:B] += S
+        self.lengths[:B] = [n + S for n in self.lengths[:B]]
 
     def reset(self):
         """Empties every cache (the sequences stay allocated) and moves the positions back to 0."""
@@ -227,6 +310,7 @@ class Decoder:
                 L["cache"].truncate(s, 0)
         self.pos.zero_()
         self.lengths = [0] * self.B
+        self.shared = False
 
     def truncate(self, n_tokens):
         """Rolls every sequence of every layer back to its first n_tokens cached tokens (the reference's `truncate`, used to
