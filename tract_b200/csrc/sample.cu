@@ -275,9 +275,12 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
 
     // ---- 1. the maximum, the slice onto the chip ----
     const RowSettings s = row_settings(p, row);
-    // Bins of log2(1 / w), 28 octaves deep, or for top-p as deep as its cut can lie: what is deeper than log2(n / (1 - p)) has, all
-    // of it together, less than 1 - p of the maximum's weight.
-    const float octaves = s.use_p && !s.use_k ? fminf(28.f, log2f((float)p.n / (1.f - s.p)) + 1.f) : 28.f;
+    // Bins of log2(1 / w), 28 octaves deep.  For top-p as deep as its cut can lie: what is deeper than log2(n / (1 - p)) has, all
+    // of it together, less than 1 - p of the maximum's weight.  For top-k at least 30 below the maximum, where the likeliest few
+    // hundred logits of a vocabulary lie: a cut below the bins takes the slow way (100 rows of 16000 logits, up to 200 of each:
+    // 40 us when one row in the batch does, 14 when none does).
+    const float octaves = s.use_k ? fminf(fmaxf(28.f, 30.f * 1.4426950408889634f / s.t), 96.f)
+                        : s.use_p ? fminf(28.f, log2f((float)p.n / (1.f - s.p)) + 1.f) : 28.f;
     const float per_octave = (float)(SP_BINS - 1) / octaves;
     float zscale = 1.4426950408889634f / s.t * per_octave;
     if (tid == 0 && !s.greedy) sh.t_unit = (double)SP_TABLE * 1.4426950408889634074 / (double)s.t;  // one division for all
@@ -892,20 +895,23 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
 
 // How a launch is cut: up to eight CTAs per row (of at least 1024 logits each).
 //   every CTA has an SM of its own           1024 threads, the slices on the chip
-//   two fit an SM                            512 threads, the slices on the chip
+//   up to three to an SM                     512 threads, the slices on the chip; two are resident
 //   more                                     256 threads, four per SM, that read their slice again from L2 where they need it: twice
 //                                            as many rows are in flight, and the exchanges of one hide behind the work of the others
-// Measured on rows of 128256 f32 logits with mixed settings: @@MEASURED@@
+// Measured on rows of 128256 f32 logits, top-p 0.9 (us for 1024 / 512 / 256 threads): 8 rows 24.8 / 26.7 / 35.3; 15 rows 25.5 /
+// 31.0; 16 rows 36.6 / 30.8; 37 rows 59.6 / 48.0 / 57.8; 48 rows - / 56.1 / 59.9; 64 rows 94 / 65 / 63; 256 rows 321 / 223 / 193.
 struct SampleCut {
     int c, slice, threads;  // CTAs per row, logits per CTA (the next slice starts on a 16-byte boundary when the row does)
 };
+// CTAs that get an SM of their own: the SMs of a processing cluster that are left over hold no whole cluster.
+static int sample_alone(int c) { return c == 8 ? 120 : c == 4 ? 128 : 148; }
 static SampleCut sample_cut(int64_t rows, int32_t n) {
     SampleCut k{1, 0, 1024};
-    while (k.c < SP_CLUSTER && n >= 2 * k.c * 1024 && (n > k.c * SP_SLICE || rows * k.c * 2 <= 148)) k.c *= 2;
+    while (k.c < SP_CLUSTER && n >= 2 * k.c * 1024 && (n > k.c * SP_SLICE || rows * k.c * 2 <= sample_alone(k.c * 2))) k.c *= 2;
     if (n > MAX_ON_CHIP) k.c = SP_CLUSTER;
     k.slice = ((n + k.c - 1) / k.c + 7) / 8 * 8;
     const bool two_fit = k.slice <= SP_SLICE;
-    if (n <= MAX_ON_CHIP && rows * k.c > 148) k.threads = two_fit && rows * k.c <= 2 * 148 ? 512 : 256;
+    if (n <= MAX_ON_CHIP && rows * k.c > sample_alone(k.c)) k.threads = two_fit && rows * k.c <= 3 * 148 ? 512 : 256;
     return k;
 }
 
