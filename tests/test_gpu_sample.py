@@ -271,3 +271,33 @@ def test_refusals(kv):
         kv.sample(x, None)
     with pytest.raises(kv.B200KvError, match="dtype"):
         kv.sample(x.double(), u)
+
+
+def test_rows_past_two_to_the_31st_logit(kv):
+    # rows of a wide matrix: the last ones begin 2^31 elements and more behind the first
+    n, stride, rows = 1000, 2 ** 28, 9
+    wide = torch.zeros(rows * stride - (stride - n), dtype=torch.bfloat16, device="cuda").as_strided((rows, n), (stride, 1))
+    x, g = model_logits(77, rows, n, "bf16")
+    wide.copy_(x)
+    check(kv, wide, g.random(rows), 0.5 + g.random(rows), np.full(rows, 50, np.int32), np.full(rows, 0.9, np.float32), None)
+
+
+def test_two_graphs_of_one_decode_loop(kv):
+    # captured with buffers of their own, replayed in turn with new logits and numbers
+    x, g = model_logits(5, 6, 50257)
+    y, _ = model_logits(6, 6, 50257)
+    u = torch.from_numpy(g.random((4, 6)).astype(np.float32)).cuda()
+    k = torch.full((6,), 40, dtype=torch.int32, device="cuda")
+    want = [[kv.sample(t, u[j], top_k=k) for t in (x, y)] for j in range(4)]
+    outs, uu, graphs = [torch.empty(6, dtype=torch.int32, device="cuda") for _ in range(2)], torch.zeros(6, device="cuda"), []
+    torch.cuda.synchronize()
+    for t, out in zip((x, y), outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kv.sample(t, uu, top_k=k, out=out)
+        graphs.append(graph)
+    for j in (2, 0, 3, 1):
+        uu.copy_(u[j])
+        for graph in graphs:
+            graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[j]))

@@ -489,3 +489,78 @@ def test_many_steps_of_branching(kv):
     cache.free_seqs(beams)
     assert cache.free_pages() == total
     cache.close(), lone.close()
+
+
+@pytest.mark.parametrize("way", [0, 1, 2])
+@pytest.mark.parametrize("fmt,io,D", [("f16", "f16", 128), ("q8_1", "bf16", 64), ("f32", "f32", 128)])
+def test_attend_shared_captured_and_replayed(kv, fmt, io, D, way):
+    # two graphs over one cache, replayed one after the other with new queries each time
+    Hkv, G = 2, 4
+    cache, seqs = family(kv, fmt, io, Hkv, D, [700], 6, [5, 70], Hkv * G)
+    cache.profile(False, shared_way=way)
+    qs = [rows(5 + j, (6, Hkv * G, 1, D), io) for j in range(4)]
+    want = [cache.attend_shared(seqs, q) for q in qs]
+    half = [cache.attend_shared(seqs[:3], q[:3]) for q in qs]
+    q, out, part = qs[0].clone(), torch.empty_like(qs[0]), torch.empty_like(qs[0][:3])
+    side = torch.cuda.Stream()
+    graphs = []
+    torch.cuda.synchronize()
+    for call in (lambda: cache.attend_shared(seqs, q, out=out), lambda: cache.attend_shared(seqs[:3], q[:3], out=part)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            call()
+        graphs.append(g)
+    for j in (3, 1, 2, 0):
+        q.copy_(qs[j])
+        for g in graphs:
+            g.replay()
+        assert torch.equal(out, want[j]) and torch.equal(part, half[j])
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("way", [0, 1, 2])
+@pytest.mark.parametrize("fmt,io", [("f16", "f16"), ("q4_0", "f16"), ("f32", "f32")])
+def test_attend_shared_many_calls_in_flight(kv, fmt, io, way):
+    # the own pages run beside the shared ones, the next call's kernels are scheduled before this one has ended: 60 calls of two
+    # batches without a synchronisation give the bits of the first, on either of two streams
+    Hkv, G, D = 4, 4, 128
+    cache, seqs = family(kv, fmt, io, Hkv, D, [1500, 200], 12, [3, 130, 64, 1], Hkv * G)
+    cache.profile(False, shared_way=way)
+    a, b = rows(5, (24, Hkv * G, 1, D), io), rows(6, (9, Hkv * G, 1, D), io)
+    batches = [(seqs, a), (seqs[4:13], b)]
+    want = [cache.attend_shared(*x) for x in batches]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            got = [cache.attend_shared(*batches[i % 2]) for i in range(60)]
+        stream.synchronize()
+        assert all(torch.equal(x, want[i % 2]) for i, x in enumerate(got))
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("fmt,io", [("f16", "f16"), ("f32", "f32")])
+def test_pages_past_four_gigabytes(kv, fmt, io):
+    # a filler takes the first pages of the pool: what is shared, copied and read lies behind 2^32 bytes
+    Hkv, G, D = 8, 4, 128
+    size = 4 if fmt == "f32" else 2
+    fill = (2 ** 32 // (2 * Hkv * D * size) + 63) // 64 * 64
+    cache = kv.KvCache(fmt, Hkv, D, max_seqs=8, max_seq_tokens=fill, pool_tokens=fill + 8 * 640, max_q_heads=Hkv * G)
+    filler = cache.new_seq()
+    one = rows(1, (1, Hkv, 1, D), io)
+    for at in range(0, fill, 2 ** 18):
+        wide = one.expand(1, Hkv, min(2 ** 18, fill - at), D)
+        cache.append([filler], wide, wide)
+    parent = cache.new_seq()
+    add(cache, [parent], 3, 400, io)
+    seqs = cache.fork_shared([parent] * 4)
+    add(cache, seqs, 5, 30, io)
+    q = rows(7, (4, Hkv * G, 1, D), io)
+    ref, size = reference(cache, seqs, q)
+    for way in (0, 1, 2):
+        cache.profile(False, shared_way=way)
+        assert_close(cache.attend_shared(seqs, q), ref, size, io)
+    cache.check()
+    cache.close()

@@ -389,7 +389,7 @@ class KvCache:
         quantised activation of a Q40Linear, as in attend_q40 (`out` stays unwritten then unless it is given)."""
         import torch
 
-        assert q.dim() == 4 and q.shape[0] == len(seqs) and q.shape[2] == 1 and q.shape[3] == self.head_dim
+        assert q.dim() == 4 and q.shape[0] == len(seqs) and q.shape[2] == 1 and q.shape[3] == self.head_dim and q.is_cuda
         stride = 0
         if cos is not None:
             cos, sin = cos.reshape(len(seqs), -1), sin.reshape(len(seqs), -1)
@@ -411,7 +411,7 @@ class KvCache:
         """A zero-argument callable that runs attend_shared(seqs, q, out=out) with every argument marshalled once, here (see
         prepared_step).  The tensors must stay alive and in place; the current CUDA stream is looked up at every call."""
         assert q.dim() == 4 and q.shape[0] == len(seqs) and q.shape[2] == 1 and q.shape[3] == self.head_dim
-        assert out.shape == q.shape and out.dtype == q.dtype
+        assert out.shape == q.shape and out.dtype == q.dtype and q.is_cuda and out.is_cuda
         L, h, n, ids = lib(), self._h, len(seqs), _ids(seqs)
         qs, os_, qp, op = _strides(q, 3), _strides(out, 3), C.c_void_p(q.data_ptr()), C.c_void_p(out.data_ptr())
         hq, dt, sc = int(q.shape[1]), _dtype_code(q), C.c_float(scale or 0.0)

@@ -73,8 +73,11 @@ struct XGeo {
 // of prefill_tc.cu and attn_tc.cu; there are no masks (every row sees every shared page whole) and the rows come from different
 // sequences.  The result is a run's partial (m, l, O) in f32 for the combine pass.
 // Bound: a page and kv head is 32 KB of f16, 1340 cycles of an SM's share of HBM at the copy rate; its products for 128 rows
-// take 640 to 900 cycles of the tensor pipe, but one pipeline needs 3400 cycles from a page to the next (product, softmax,
-// product, each waiting for the one before).  Two pipelines per CTA therefore: up to 128 rows they take the pages in turn.
+// take 640 to 900 cycles of the tensor pipe, but one pipeline needs 2200 cycles from a page to the next (product, softmax,
+// product, each waiting for the one before; 3500 over int8 pages, whose converter warps share the issue slots with the softmax).
+// Two pipelines per CTA therefore: up to 128 rows they take the pages in turn, one every 1100 (1750) cycles.
+// Measured: 128 rows per kv head, 8 of them, after 32768 tokens: f16 27 us for this kernel (134 MB, 5.0 TB/s), 43 for the call;
+// int8 35 and 51, of which the conversion is 9.  4 us go before the first page (TMEM, barriers, query tiles), 5 after the last.
 // A CTA has a run of pages; the two CTAs of a cluster have neighbouring runs and join (m, l, O) through distributed shared
 // memory, each for half of the channels, before a partial is written: half of the partials' traffic and workspace, which
 // otherwise limits the runs to fewer than the GPU has SMs.
@@ -132,7 +135,6 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     if (warp == 0) tmem_alloc(tmem_slot, COLS_PER_TILE * 2);
     cluster.barrier_arrive();  // every CTA of the cluster runs before one writes into the other's shared memory
     grid_dependency_wait();    // the append before this launch has written its pages, and whoever made q is done
-    grid_launch_dependents();  // the next kernel may be scheduled; it waits for this grid before it reads the partials
 
     const int qt = min(tid / X_SM_THREADS, 1), w4 = (tid % X_SM_THREADS) >> 5;  // pipeline, lane quarter
     const int row = w4 * 32 + lane;
@@ -144,6 +146,9 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     const int mma_bf16 = RAW ? 0 : is_bf16;  // type of the tensor-core operands (Q, K, V, P)
 
     __syncthreads();  // the barriers are there: the copy warp starts, the others fetch Q meanwhile
+    // The next kernel may be scheduled; it waits for this grid before it reads the partials.  Not before the TMEM is allocated: a
+    // later kernel that got hold of the SM's columns first would wait for this one, and this one for the columns.
+    grid_launch_dependents();
     const int role = warp - 2 * (X_SM_THREADS / 32);  // 0, 1: MMAs of that pipeline; above: copies and conversion; below 0: softmax
     // ---- Q tiles -> shared memory, K-major with the 128-byte swizzle; neighbouring threads fetch neighbouring units of a row ----
     if (is_softmax) {
