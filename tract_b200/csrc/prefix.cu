@@ -15,6 +15,7 @@
 
 #include "attn_convert.cuh"
 #include "decode_common.h"
+#include "f32x2.cuh"
 #include "q40_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -476,145 +477,181 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
 }
 
 // ---- the same on the CUDA cores, for f32 pages ---------------------------------------------------------------------------
-// A tile is 32 rows.  Per page: K and V in shared memory (read once for the 32 rows), S = Q K^T with 2 x 4 scores per
-// thread, the online softmax with expf (8 threads per row), O += P V with 2 rows x D / 16 channels per thread.  Bound by the
-// FMA pipe and the shared-memory reads that feed it: 4 D flops per row and key.
-constexpr int CR = 32;         // rows of a tile
-constexpr int C_THREADS = 256;
-
-template <int D>
+// A tile is 128 rows, or 64 for fewer.  Per page S = Q K^T with 4 x 4 scores per thread, the online softmax with expf (4 threads
+// per row), O += P V with 4 rows x D / 16 channels per thread, all products as packed pairs.  The chunks are used as they lie in the
+// page: two bulk copies, each on its way while the other operand's product runs.
+// Bound by the FMA pipe -- 4 D flops per row and key -- and the 16-byte shared-memory reads that feed it, which a warp takes two to
+// four cycles for: a page takes 17 us for 128 rows (FMA pipe alone: 8.6) and 8 for 64.  Scores and outputs of 8 x 4 or 8 x 8 a thread
+// read less and left too few warps or registers: the same times.
+template <int D, int ROWS>
 struct CGeo {
-    static constexpr int LD = D + 4;  // row pitch in floats: 16-byte aligned rows, successive rows 4 banks apart
-    static constexpr size_t SMEM = ((size_t)CR * LD + 2 * (size_t)PAGE_TOKENS * LD + (size_t)CR * (PAGE_TOKENS + 4) + 3 * CR) * 4;
+    static constexpr int THREADS = 4 * ROWS;
+    static constexpr int LD = D + 4;             // pitch of the query rows in floats: 16-byte aligned, successive rows 4 banks apart
+    static constexpr int PL = PAGE_TOKENS + 16;  // the same of the scores, 16 banks apart
+    static constexpr size_t SMEM = (2 * (size_t)PAGE_TOKENS * D + (size_t)ROWS * (LD + PL) + 3 * ROWS) * 4 + 32;
+    static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
 };
 
-template <int D>
-__global__ void __launch_bounds__(C_THREADS, 2) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
-    constexpr int LD = CGeo<D>::LD, PL = PAGE_TOKENS + 4, CPT = D / 16;
+template <int D, int ROWS>
+__global__ void __launch_bounds__(4 * ROWS, 1) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
+    using GEO = CGeo<D, ROWS>;
+    constexpr int LD = GEO::LD, PL = GEO::PL, CPT = D / 16;
     extern __shared__ __align__(16) float csm[];
-    float* q_s = csm;                     // [32][LD]
-    float* k_s = q_s + CR * LD;           // [64][LD]
-    float* v_s = k_s + PAGE_TOKENS * LD;  // [64][LD]
-    float* p_s = v_s + PAGE_TOKENS * LD;  // [32][PL] scores, then weights
-    float* m_s = p_s + CR * PL;           // [32] running maximum
-    float* l_s = m_s + CR;                // [32] running sum
-    float* a_s = l_s + CR;                // [32] factor of this page's rescale
+    float* k_s = csm;                     // the chunks as they lie in the page: planes of 32 channels, [64 tokens][8 units of 4], the
+    float* v_s = k_s + PAGE_TOKENS * D;   //   units of a token in the order unit ^ token % 8
+    float* q_s = v_s + PAGE_TOKENS * D;   // [ROWS][LD]
+    float* p_s = q_s + ROWS * LD;         // [ROWS][PL] scores, then weights
+    float* m_s = p_s + ROWS * PL;         // [ROWS] running maximum
+    float* l_s = m_s + ROWS;              // [ROWS] running sum
+    float* a_s = l_s + ROWS;              // [ROWS] factor of this page's rescale
+    uint64_t* bars = (uint64_t*)(a_s + ROWS);  // K, V have landed
+    volatile int* fail_s = (volatile int*)(bars + 2);
     const DecodeParams& dp = p.d;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int tid = threadIdx.x;
     const int kvh = blockIdx.y;
     const PrefixGroup grp = prefix_group_of(pb, blockIdx.x);
     const int split = (blockIdx.x - grp.cta0) / grp.tiles, tile = (blockIdx.x - grp.cta0) % grp.tiles;
     int page0, n_pages;
     prefix_run(grp, grp.splits, split, &page0, &n_pages);
-    const int n_rows = grp.n_seqs * dp.G, row0 = tile * CR;
-    grid_dependency_wait();
-    grid_launch_dependents();
-    for (int i = tid; i < CR * D; i += C_THREADS) {
-        const int r = i / D, ch = i % D;
-        float v = 0.f;
-        if (row0 + r < n_rows) v = load_query(dp, D, grp.b0 + (row0 + r) / dp.G, kvh * dp.G + (row0 + r) % dp.G, ch);
-        q_s[r * LD + ch] = v;
-    }
-    if (tid < CR) m_s[tid] = -INFINITY, l_s[tid] = 0.f;
-    float acc[2][CPT];
-#pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int e = 0; e < CPT; e++) acc[r][e] = 0.f;
+    const int n_rows = grp.n_seqs * dp.G, row0 = tile * ROWS;
     const int32_t* pages = dp.table + (int64_t)grp.trow * dp.max_pages_per_seq + page0;
-
-    for (int i = 0; i < n_pages; i++) {
+    auto fetch = [&](int i, int x) {  // thread 0: K (x = 0) or V of page i of the run
+        if (i >= n_pages) return;
         int32_t pg = pages[i];
         if (pg < 0 || pg >= dp.n_pages) {
-            if (tid == 0) atomicOr(dp.status, STATUS_PAGE_OOB);
+            atomicOr(dp.status, STATUS_PAGE_OOB);
             pg = 0;
         }
-        const uint8_t* kc = dp.pool + (int64_t)pg * dp.page_bytes + (int64_t)kvh * (2 * p.chunk_bytes);
-        __syncthreads();  // the page before has been used (and q, m, l are there)
-        for (int x = 0; x < 2; x++) {
-            const uint8_t* chunk = kc + x * p.chunk_bytes;
-            float* dst = x ? v_s : k_s;
-            for (int u = tid; u < PAGE_TOKENS * (D / 4); u += C_THREADS) {
-                const int t = u / (D / 4), c4 = u % (D / 4);
-                *(float4*)(dst + t * LD + c4 * 4) = *(const float4*)(chunk + chunk_addr(B200KV_FMT_F32, D, x, t, c4 * 16));
-            }
+        constexpr uint32_t BYTES = PAGE_TOKENS * D * 4;
+        mbar_expect_tx(&bars[x], BYTES);
+        bulk_g2s(x ? v_s : k_s, dp.pool + (int64_t)pg * dp.page_bytes + (int64_t)kvh * (2 * p.chunk_bytes) + x * p.chunk_bytes, BYTES, &bars[x]);
+    };
+    if (tid == 0) {
+        mbar_init(&bars[0], 1), mbar_init(&bars[1], 1);
+        *fail_s = 0;
+        mbar_fence_init();
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (tid == 0) fetch(0, 0), fetch(0, 1);
+    for (int i0 = tid; i0 < ROWS * D; i0 += 8 * GEO::THREADS) {  // eight on their way before the first is stored
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int r = (i0 + j * GEO::THREADS) / D, ch = (i0 + j * GEO::THREADS) % D;
+            v[j] = row0 + r < n_rows ? load_query(dp, D, grp.b0 + (row0 + r) / dp.G, kvh * dp.G + (row0 + r) % dp.G, ch) : 0.f;
         }
-        __syncthreads();
-        {  // scores: rows 2 ty + {0, 1}, keys tx + 16 {0 .. 3}
-            float s[2][4] = {};
-#pragma unroll 4
+#pragma unroll
+        for (int j = 0; j < 8; j++) q_s[(i0 + j * GEO::THREADS) / D * LD + (i0 + j * GEO::THREADS) % D] = v[j];
+    }
+    if (tid < ROWS) m_s[tid] = -INFINITY, l_s[tid] = 0.f;
+    const int tx = tid & 15, ty = tid >> 4;  // rows ty + (ROWS / 4) {0 .. 3}
+    uint64_t acc[4][CPT / 2] = {};           // their outputs, pairs of channels
+    __syncthreads();          // the queries are there, and the barriers
+
+    for (int i = 0; i < n_pages; i++) {
+        wait_or_fail(&bars[0], i & 1, fail_s);
+        {  // scores against keys tx + 16 {0 .. 3}
+            uint64_t s[4][4] = {};  // the sums over even and over odd channels
+#pragma unroll 2
             for (int c = 0; c < D; c += 4) {
-                float4 qv[2], kv[4];
+                ulonglong2 qv[4], kv[4];
 #pragma unroll
-                for (int r = 0; r < 2; r++) qv[r] = *(const float4*)(q_s + (2 * ty + r) * LD + c);
+                for (int r = 0; r < 4; r++) qv[r] = *(const ulonglong2*)(q_s + (ty + ROWS / 4 * r) * LD + c);
 #pragma unroll
-                for (int k = 0; k < 4; k++) kv[k] = *(const float4*)(k_s + (tx + 16 * k) * LD + c);
+                for (int k = 0; k < 4; k++) kv[k] = *(const ulonglong2*)(k_s + (c >> 5) * (PAGE_TOKENS * 32) + (tx + 16 * k) * 32 + ((c & 31) ^ ((tx & 7) << 2)));
 #pragma unroll
-                for (int r = 0; r < 2; r++)
+                for (int r = 0; r < 4; r++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        s[r][k] = fmaf(qv[r].x, kv[k].x, s[r][k]), s[r][k] = fmaf(qv[r].y, kv[k].y, s[r][k]);
-                        s[r][k] = fmaf(qv[r].z, kv[k].z, s[r][k]), s[r][k] = fmaf(qv[r].w, kv[k].w, s[r][k]);
-                    }
+                    for (int k = 0; k < 4; k++) s[r][k] = f2_fma(qv[r].y, kv[k].y, f2_fma(qv[r].x, kv[k].x, s[r][k]));
             }
 #pragma unroll
-            for (int r = 0; r < 2; r++)
+            for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) p_s[(2 * ty + r) * PL + tx + 16 * k] = s[r][k] * dp.scale;
+                for (int k = 0; k < 4; k++) {
+                    const float2 x = f2_unpack(s[r][k]);
+                    p_s[(ty + ROWS / 4 * r) * PL + tx + 16 * k] = (x.x + x.y) * dp.scale;
+                }
         }
         __syncthreads();
-        {  // softmax of the page: threads 8 r .. 8 r + 7 own row r
-            const int r = tid >> 3, part = tid & 7;
-            float x[8], mx = -INFINITY;
+        if (tid == 0) fetch(i + 1, 0);
+        {  // softmax of the page: four neighbouring threads own a row, quads of keys in turn
+            const int r = tid >> 2, part = tid & 3;
+            float4 x[4];
+            float mx = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = p_s[r * PL + part + 8 * e], mx = fmaxf(mx, x[e]);
+            for (int e = 0; e < 4; e++) {
+                x[e] = *(const float4*)(p_s + r * PL + 4 * (part + 4 * e));
+                mx = fmaxf(mx, fmaxf(fmaxf(x[e].x, x[e].y), fmaxf(x[e].z, x[e].w)));
+            }
 #pragma unroll
-            for (int o = 4; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            for (int o = 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             const float m_old = m_s[r], m_new = fmaxf(m_old, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
             float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float w = expf(x[e] - m_use);
-                p_s[r * PL + part + 8 * e] = w;
-                sum += w;
+            for (int e = 0; e < 4; e++) {
+                const float4 w = make_float4(expf(x[e].x - m_use), expf(x[e].y - m_use), expf(x[e].z - m_use), expf(x[e].w - m_use));
+                *(float4*)(p_s + r * PL + 4 * (part + 4 * e)) = w;
+                sum += (w.x + w.y) + (w.z + w.w);
             }
 #pragma unroll
-            for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            for (int o = 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             __syncwarp();  // every lane has read the old maximum of its row
             if (part == 0) {
                 const float a = expf(m_old - m_use);
                 a_s[r] = a, m_s[r] = m_new, l_s[r] = fmaf(l_s[r], a, sum);
             }
         }
+        wait_or_fail(&bars[1], i & 1, fail_s);
         __syncthreads();
-        {  // values: rows 2 ty + {0, 1}, channels tx * 4 + 64 j .. + 3
-            const float a0 = a_s[2 * ty], a1 = a_s[2 * ty + 1];
+        {  // values: channels tx * 4 + 64 j .. + 3
 #pragma unroll
-            for (int e = 0; e < CPT; e++) acc[0][e] *= a0, acc[1][e] *= a1;
-#pragma unroll 4
-            for (int t = 0; t < PAGE_TOKENS; t++) {
-                const float p0 = p_s[(2 * ty) * PL + t], p1 = p_s[(2 * ty + 1) * PL + t];
+            for (int r = 0; r < 4; r++) {
+                const float a = a_s[ty + ROWS / 4 * r];
 #pragma unroll
-                for (int j = 0; j < CPT / 4; j++) {
-                    const float4 v = *(const float4*)(v_s + t * LD + tx * 4 + 64 * j);
-                    acc[0][4 * j] = fmaf(p0, v.x, acc[0][4 * j]), acc[0][4 * j + 1] = fmaf(p0, v.y, acc[0][4 * j + 1]);
-                    acc[0][4 * j + 2] = fmaf(p0, v.z, acc[0][4 * j + 2]), acc[0][4 * j + 3] = fmaf(p0, v.w, acc[0][4 * j + 3]);
-                    acc[1][4 * j] = fmaf(p1, v.x, acc[1][4 * j]), acc[1][4 * j + 1] = fmaf(p1, v.y, acc[1][4 * j + 1]);
-                    acc[1][4 * j + 2] = fmaf(p1, v.z, acc[1][4 * j + 2]), acc[1][4 * j + 3] = fmaf(p1, v.w, acc[1][4 * j + 3]);
-                }
+                for (int e = 0; e < CPT / 2; e++) acc[r][e] = f2_mul(acc[r][e], f2_pack(a, a));
+            }
+#pragma unroll 1
+            for (int t = 0; t < PAGE_TOKENS; t += 4) {
+                float4 w[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) w[r] = *(const float4*)(p_s + (ty + ROWS / 4 * r) * PL + t);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int j = 0; j < CPT / 4; j++) {
+                        const int c = tx * 4 + 64 * j;
+                        const ulonglong2 v = *(const ulonglong2*)(v_s + (c >> 5) * (PAGE_TOKENS * 32) + (t + k) * 32 + ((c & 31) ^ (((t & 4) + k) << 2)));
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const float x = k == 0 ? w[r].x : k == 1 ? w[r].y : k == 2 ? w[r].z : w[r].w;
+                            acc[r][2 * j] = f2_fma(f2_pack(x, x), v.x, acc[r][2 * j]), acc[r][2 * j + 1] = f2_fma(f2_pack(x, x), v.y, acc[r][2 * j + 1]);
+                        }
+                    }
             }
         }
+        __syncthreads();
+        if (tid == 0) fetch(i + 1, 1);
     }
     __syncthreads();
+    if (*fail_s) {  // an empty partial, once the copies in flight have landed
+        if (tid == 0) atomicOr(dp.status, STATUS_WAIT_EXPIRED);
+        if (tid < ROWS) m_s[tid] = -INFINITY, l_s[tid] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int my_row = row0 + 2 * ty + r;
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int e = 0; e < CPT / 2; e++) acc[r][e] = 0ull;
+        __nanosleep(200000);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int row = ty + ROWS / 4 * r, my_row = row0 + row;
         if (my_row >= n_rows) continue;
         const int64_t rec = (int64_t)grp.base + ((int64_t)split * dp.Hkv + kvh) * n_rows + my_row;
 #pragma unroll
-        for (int j = 0; j < CPT / 4; j++)
-            *(float4*)(dp.part_o + rec * D + tx * 4 + 64 * j) = make_float4(acc[r][4 * j], acc[r][4 * j + 1], acc[r][4 * j + 2], acc[r][4 * j + 3]);
-        if (tx == 0) *(float2*)(dp.part_ml + rec * 2) = make_float2(m_s[2 * ty + r], l_s[2 * ty + r]);
+        for (int j = 0; j < CPT / 4; j++) *(ulonglong2*)(dp.part_o + rec * D + tx * 4 + 64 * j) = make_ulonglong2(acc[r][2 * j], acc[r][2 * j + 1]);
+        if (tx == 0) *(float2*)(dp.part_ml + rec * 2) = make_float2(m_s[row], l_s[row]);
     }
 }
 
@@ -736,16 +773,20 @@ static cudaError_t launch_prefix_tc(int fmt, int D, bool one, const PrefixParams
     if (fmt == B200KV_FMT_Q4_0) return D == 128 ? launch_prefix_tc_rows<128, PSRC_Q4>(one, p, pb, ctas, stream) : launch_prefix_tc_rows<64, PSRC_Q4>(one, p, pb, ctas, stream);
     return D == 128 ? launch_prefix_tc_rows<128, PSRC_PAGES16>(one, p, pb, ctas, stream) : launch_prefix_tc_rows<64, PSRC_PAGES16>(one, p, pb, ctas, stream);
 }
-template <int D>
-static cudaError_t launch_prefix_simt(const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
-    cudaError_t e = allow_shared_memory<prefix_simt_kernel<D>>(CGeo<D>::SMEM);
+template <int D, int ROWS>
+static cudaError_t launch_prefix_simt_t(const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    using GEO = CGeo<D, ROWS>;
+    cudaError_t e = allow_shared_memory<prefix_simt_kernel<D, ROWS>>(GEO::SMEM);
     if (e != cudaSuccess) return e;
-    return launch_after_predecessor(prefix_simt_kernel<D>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(C_THREADS), CGeo<D>::SMEM, stream, p, pb);
+    return launch_after_predecessor(prefix_simt_kernel<D, ROWS>, dim3((unsigned)ctas, (unsigned)p.d.Hkv), dim3(GEO::THREADS), GEO::SMEM, stream, p, pb);
+}
+static cudaError_t launch_prefix_simt(int D, int rows_cta, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
+    if (rows_cta > 64) return D == 128 ? launch_prefix_simt_t<128, 128>(p, pb, ctas, stream) : launch_prefix_simt_t<64, 128>(p, pb, ctas, stream);
+    return D == 128 ? launch_prefix_simt_t<128, 64>(p, pb, ctas, stream) : launch_prefix_simt_t<64, 64>(p, pb, ctas, stream);
 }
 
 // The three ways of a call, and what each takes in microseconds, fitted to grids of 2 to 64 sequences after 512 to 16384 tokens
-// and to 200 calls of random sizes: the choice is within 10% of the best of the three on all but a few of those (1.45 times at
-// worst), within 2% on average.
+// and to some hundred calls of random sizes: the choice is within 10% of the best of the three on 19 of 20 (1.5 times at worst).
 //   ALONE      launch_decode: every sequence reads its pages from L2 or HBM, 8 (4) rows at a time.  No more to set up than
 //              regular attention, but each page is worked on n times.
 //   TOGETHER   one launch of the decode kernel, the shared pages being further work items: rows of several sequences fill the
@@ -779,8 +820,9 @@ static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
     if (own_ctas > slots / 2) together = 1e30;
     if (z.tc)  // a page for all rows of a CTA, on 148 of them; two tiles of rows take 2.4 times as long as one
         apart = (quant ? 15.0 : 13.0) + (quant ? 1.3 : 0.9) * (z.max_rows <= XM ? 1.0 : 2.4) * (double)z.apart * z.Hkv / 148 + own;
-    else if (z.fmt == B200KV_FMT_F32)  // whole rounds of 2 CTAs per SM
-        apart = 11.0 + (z.D == 128 ? 13.5 : 11.0) * (double)((z.apart * z.Hkv + 295) / 296) + own;
+    else if (z.fmt == B200KV_FMT_F32)  // a page and tile, in whole rounds of a CTA per SM; then the own pages, which find no room beside them
+        apart = 8.0 + (z.max_rows <= 64 ? 8.0 : 17.0) * (z.D == 128 ? 1.0 : 0.6) * (double)((z.apart * z.Hkv + 147) / 148) +
+                7.0 * (double)own_ctas / 148;
     if (apart < together && apart < alone) return APART;
     return together < alone ? TOGETHER : ALONE;
 }
@@ -806,8 +848,8 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
         if (r.n > 1 && r.pages > 0) max_rows = std::max(max_rows, r.n * G), max_pages = std::max(max_pages, r.pages);
     const bool one_tile = max_rows <= XM;
     const int cluster = tc ? X_CLUSTER : 1;                  // CTAs that write one partial
-    int rows_cta = tc ? (one_tile ? XM : 2 * XM) : CR;
-    int64_t slots = tc ? 148 / X_CLUSTER : 148 * 2;          // resident CTAs, or clusters
+    int rows_cta = tc ? (one_tile ? XM : 2 * XM) : (max_rows > 64 ? 128 : 64);
+    int64_t slots = tc ? 148 / X_CLUSTER : 148;              // resident CTAs, or clusters
 
     // ---- the own pages of every sequence: as launch_decode cuts them, starting behind the shared ones ----
     const bool use_mma = decode_mma_supported(fmt, D, dtype) && !c->force_simt;
@@ -882,7 +924,9 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
             PrefixGroup& g = pb.g[pb.n++];
             g.trow = seqs[r.b0], g.n_pages = r.pages, g.b0 = r.b0, g.n_seqs = r.n;
             g.tiles = (rows + rows_cta - 1) / rows_cta;
-            g.splits = (int)std::min<int64_t>(MAX_SPLITS / 2, (r.pages + run_pages - 1) / run_pages);
+            int own_splits = 0;  // a row joins at most MAX_SPLITS partials
+            for (int i = r.b0; i < r.b0 + r.n; i++) own_splits = std::max(own_splits, ib.ent[i].w);
+            g.splits = (int)std::min<int64_t>(MAX_SPLITS - own_splits, (r.pages + run_pages - 1) / run_pages);
             g.cta0 = ctas, g.base = (int32_t)n_rec;
             for (int i = 0; i < r.n; i++) sb.pre[r.b0 + i] = make_int4(g.base, g.splits, rows, i * G);
             ctas += g.tiles * g.splits * (together ? 1 : cluster);
@@ -910,7 +954,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     if (!together) {
         ProfScope ps(c, K_PREFIX, stream);
         e = tc ? launch_prefix_tc(fmt, D, one_tile, p, pb, ctas, stream)
-               : (D == 128 ? launch_prefix_simt<128>(p, pb, ctas, stream) : launch_prefix_simt<64>(p, pb, ctas, stream));
+               : launch_prefix_simt(D, rows_cta, p, pb, ctas, stream);
     }
     if (e != cudaSuccess) return fail("shared-prefix launch failed: %s", cudaGetErrorString(e));
     if (together || n_items > 0) {
