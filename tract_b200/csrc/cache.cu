@@ -62,11 +62,12 @@ int64_t workspace_records(const b200kv_config& cfg) {
 int validate_seqs(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs) {
     if (!c) return fail("null cache");
     if (n_seqs <= 0 || !seqs) return fail("need at least one sequence");
+    c->call++;
     for (int i = 0; i < n_seqs; i++) {
         int s = seqs[i];
         if (s < 0 || s >= (int)c->seqs.size() || !c->seqs[s].live) return fail("sequence %d is not live", s);
-        for (int j = 0; j < i; j++)
-            if (seqs[j] == s) return fail("sequence %d appears twice in one call", s);
+        if (c->named_in[s] == c->call) return fail("sequence %d appears twice in one call", s);
+        c->named_in[s] = c->call;
     }
     return B200KV_OK;
 }
@@ -511,6 +512,7 @@ int b200kv_create(const b200kv_config* cfg, b200kv_cache** out) {
     // every live sequence may hold one partly filled page
     c->n_pages = (cfg->pool_tokens + PAGE_TOKENS - 1) / PAGE_TOKENS + cfg->max_seqs;
     c->seqs.resize(cfg->max_seqs);
+    c->named_in.assign((size_t)cfg->max_seqs, 0);
     auto cleanup = [&](int rc) {
         b200kv_destroy(c);
         return rc;

@@ -91,6 +91,8 @@ struct b200kv_cache {
     std::vector<int32_t> free_pages;
     std::vector<int32_t> page_refs;  // sequences that hold each page (b200kv_fork_shared): it goes back to the pool with the last of them
     std::vector<b200kv::SeqState> seqs;
+    std::vector<uint64_t> named_in;  // the last call that named each sequence: one that comes twice is found without looking at every pair
+    uint64_t call = 0;
     b200kv::Staging st;
     uint8_t* ws = nullptr;  // split-KV partials: allocated once at create, never grown
     size_t ws_bytes = 0;

@@ -801,12 +801,15 @@ struct WaySizes {
     bool use_mma, tc;                       // the tensor-core forms of the decode kernel and of the kernel over shared pages
     int64_t alone, together, apart, own;    // pages x row tiles, per kv head: 8 (4) rows of the decode kernels, XM .. of the others
 };
+// A page against one row tile of a decode kernel, spread over the GPU: tensor cores 2.6 ns; CUDA cores by the page's bytes and the
+// work of widening them, a single row three quarters of four.
+static double decode_unit(int fmt, int D, int G, bool use_mma) {
+    if (use_mma) return 2.6e-3;
+    return (fmt == B200KV_FMT_F32 ? 17e-3 : fmt_is_block_quant(fmt) ? 9e-3 : 14e-3) * D / 128 * (G == 1 ? 0.75 : 1.0);
+}
 static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
     const bool quant = fmt_is_block_quant(z.fmt);
-    // a page against one row tile of a decode kernel, spread over the GPU: tensor cores 2.6 ns; CUDA cores by the page's bytes
-    // and the work of widening them, a single row three quarters of four
-    double unit = 2.6e-3;
-    if (!z.use_mma) unit = (z.fmt == B200KV_FMT_F32 ? 17e-3 : quant ? 9e-3 : 14e-3) * z.D / 128 * (z.G == 1 ? 0.75 : 1.0);
+    const double unit = decode_unit(z.fmt, z.D, z.G, z.use_mma);
     const double own = unit * (double)z.own * z.Hkv;
     double alone = 6.5 + unit * (double)z.alone * z.Hkv;
     const int64_t slots = 148 * decode_ctas_per_sm(c, z.use_mma);
@@ -876,14 +879,16 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     if (way == ALONE) return launch_decode(c, n_seqs, seqs, n_q_heads, q, qs, out, os, dtype, scale, stream, 0, &ends);
     const bool together = way == TOGETHER;
     if (together) rows_cta = nz * dec_rows;
-    // The own pages run beside the shared ones, on the SMs that these leave: each gets its share of the work (in microseconds of
-    // an SM per page and head: 1.0 to 1.2 for a tile pair, 0.75 for 32 KB of an own page at the copy rate).
+    // The own pages run beside the shared ones, on the SMs that these leave: each gets its share of the work, in microseconds of
+    // an SM per page and head: 1.0 to 1.2 for a tile pair; for an own page 0.75 for each 32 KB at the copy rate, or what the decode
+    // kernel takes (15 sequences of 7 heads with up to 300 4-bit tokens of D = 64: 23.2 us when this took the bytes alone, 18.8 now).
     if (tc && !together) {
         int64_t own = 0, shared = 0;
         for (int i = 0; i < n_seqs; i++) own += own_pages[i];
         for (const Run& r : runs)
             if (r.n > 1 && r.pages > 0) shared += (int64_t)((r.n * G + rows_cta - 1) / rows_cta) * r.pages;
-        const double own_us = (double)own * (2.0 * c->L.chunk_bytes / 32768.0) * 0.75, shared_us = (double)shared * 1.1;
+        const double page_us = std::max(2.0 * c->L.chunk_bytes / 32768.0 * 0.75, decode_unit(fmt, D, G, use_mma) * 148 * nz);
+        const double own_us = (double)own * page_us, shared_us = (double)shared * 1.1;
         slots = std::max<int64_t>(slots / 4, (int64_t)(slots * shared_us / (shared_us + own_us)));
     }
     std::vector<int64_t> all_pages = own_pages;
