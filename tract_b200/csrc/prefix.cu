@@ -819,8 +819,10 @@ static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
     if (z.use_mma && !quant && own_ctas > slots) alone += std::min(10.0, 1.2 * (double)z.alone * z.Hkv / (double)own_ctas);
     double together = 8.4 + 1.15 * unit * (double)z.together * z.Hkv + own, apart = 1e30;
     // each sequence's own pages are CTAs of that launch, however few they are: many of them crowd out the shared pages (8 heads
-    // without groups after 4096 tokens: 16 sequences take 16, 32 of them 56)
-    if (own_ctas > slots / 2) together = 1e30;
+    // without groups after 4096 tokens: 16 sequences take 16, 32 of them 56), until they are too many to be resident together and
+    // all CTAs become short (48 sequences after 1024: 20)
+    if (own_ctas > slots) together *= 1.6;
+    else if (own_ctas > slots / 2) together = 1e30;
     if (z.tc)  // a page for all rows of a CTA, on 148 of them; two tiles of rows take 2.4 times as long as one
         apart = (quant ? 15.0 : 13.0) + (quant ? 1.3 : 0.9) * (z.max_rows <= XM ? 1.0 : 2.4) * (double)z.apart * z.Hkv / 148 + own;
     else if (z.fmt == B200KV_FMT_F32)  // a page and tile, in whole rounds of a CTA per SM; then the own pages, which find no room beside them
