@@ -477,23 +477,24 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
 }
 
 // ---- the same on the CUDA cores, for f32 pages ---------------------------------------------------------------------------
-// A tile is 128 rows, or 64 for fewer.  Per page S = Q K^T with 4 x 4 scores per thread, the online softmax with expf (4 threads
-// per row), O += P V with 4 rows x D / 16 channels per thread, all products as packed pairs.  The chunks are used as they lie in the
-// page: two bulk copies, each on its way while the other operand's product runs.
+// A tile is 128 rows, or 64 or 32 for fewer.  Per page S = Q K^T with 4 x 4 scores per thread, the online softmax with expf (4
+// threads per row), O += P V with 4 rows x D / 16 channels per thread, all products as packed pairs.  The chunks are used as they
+// lie in the page: two bulk copies, each on its way while the other operand's product runs.
 // Bound by the FMA pipe -- 4 D flops per row and key -- and the 16-byte shared-memory reads that feed it, which a warp takes two to
-// four cycles for: a page takes 17 us for 128 rows (FMA pipe alone: 8.6) and 8 for 64.  Scores and outputs of 8 x 4 or 8 x 8 a thread
-// read less and left too few warps or registers: the same times.
+// four cycles for: a page takes 17 us for 128 rows (FMA pipe alone: 8.6), 8 for 64, 9.5 for two CTAs of 32.  Scores and outputs of
+// 8 x 4 or 8 x 8 a thread read less and left too few warps or registers: the same times.  Measured, D = 128: 16 heads of their own,
+// 16 sequences after 8192 tokens 76 us (one tile of 64 rows: 129, regular attention 402); 32 heads over 8, 64 sequences 266 (959).
 template <int D, int ROWS>
 struct CGeo {
-    static constexpr int THREADS = 4 * ROWS;
+    static constexpr int THREADS = 4 * ROWS, CTAS = ROWS <= 32 ? 2 : 1;  // per SM
     static constexpr int LD = D + 4;             // pitch of the query rows in floats: 16-byte aligned, successive rows 4 banks apart
     static constexpr int PL = PAGE_TOKENS + 16;  // the same of the scores, 16 banks apart
     static constexpr size_t SMEM = (2 * (size_t)PAGE_TOKENS * D + (size_t)ROWS * (LD + PL) + 3 * ROWS) * 4 + 32;
-    static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
+    static_assert(CTAS * (SMEM + 1024) <= 227 * 1024, "shared memory of an SM");
 };
 
 template <int D, int ROWS>
-__global__ void __launch_bounds__(4 * ROWS, 1) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
+__global__ void __launch_bounds__(4 * ROWS, ROWS <= 32 ? 2 : 1) prefix_simt_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__ PrefixBatch pb) {
     using GEO = CGeo<D, ROWS>;
     constexpr int LD = GEO::LD, PL = GEO::PL, CPT = D / 16;
     extern __shared__ __align__(16) float csm[];
@@ -782,7 +783,8 @@ static cudaError_t launch_prefix_simt_t(const PrefixParams& p, const PrefixBatch
 }
 static cudaError_t launch_prefix_simt(int D, int rows_cta, const PrefixParams& p, const PrefixBatch& pb, int ctas, cudaStream_t stream) {
     if (rows_cta > 64) return D == 128 ? launch_prefix_simt_t<128, 128>(p, pb, ctas, stream) : launch_prefix_simt_t<64, 128>(p, pb, ctas, stream);
-    return D == 128 ? launch_prefix_simt_t<128, 64>(p, pb, ctas, stream) : launch_prefix_simt_t<64, 64>(p, pb, ctas, stream);
+    if (rows_cta > 32) return D == 128 ? launch_prefix_simt_t<128, 64>(p, pb, ctas, stream) : launch_prefix_simt_t<64, 64>(p, pb, ctas, stream);
+    return D == 128 ? launch_prefix_simt_t<128, 32>(p, pb, ctas, stream) : launch_prefix_simt_t<64, 32>(p, pb, ctas, stream);
 }
 
 // The three ways of a call, and what each takes in microseconds, fitted to grids of 2 to 64 sequences after 512 to 16384 tokens
@@ -825,9 +827,11 @@ static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
     else if (own_ctas > slots / 2) together = 1e30;
     if (z.tc)  // a page for all rows of a CTA, on 148 of them; two tiles of rows take 2.4 times as long as one
         apart = (quant ? 15.0 : 13.0) + (quant ? 1.3 : 0.9) * (z.max_rows <= XM ? 1.0 : 2.4) * (double)z.apart * z.Hkv / 148 + own;
-    else if (z.fmt == B200KV_FMT_F32)  // a page and tile, in whole rounds of a CTA per SM; then the own pages, which find no room beside them
-        apart = 8.0 + (z.max_rows <= 64 ? 8.0 : 17.0) * (z.D == 128 ? 1.0 : 0.6) * (double)((z.apart * z.Hkv + 147) / 148) +
+    else if (z.fmt == B200KV_FMT_F32) {  // a page and tile, in whole rounds of the resident CTAs; then the own pages, which find no room beside them
+        const int64_t resident = z.max_rows <= 32 ? 2 * 148 : 148;
+        apart = 8.0 + (z.max_rows <= 32 ? 9.5 : z.max_rows <= 64 ? 8.0 : 17.0) * (z.D == 128 ? 1.0 : 0.6) * (double)((z.apart * z.Hkv + resident - 1) / resident) +
                 7.0 * (double)own_ctas / 148;
+    }
     if (apart < together && apart < alone) return APART;
     return together < alone ? TOGETHER : ALONE;
 }
@@ -853,8 +857,8 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
         if (r.n > 1 && r.pages > 0) max_rows = std::max(max_rows, r.n * G), max_pages = std::max(max_pages, r.pages);
     const bool one_tile = max_rows <= XM;
     const int cluster = tc ? X_CLUSTER : 1;                  // CTAs that write one partial
-    int rows_cta = tc ? (one_tile ? XM : 2 * XM) : (max_rows > 64 ? 128 : 64);
-    int64_t slots = tc ? 148 / X_CLUSTER : 148;              // resident CTAs, or clusters
+    int rows_cta = tc ? (one_tile ? XM : 2 * XM) : (max_rows > 64 ? 128 : max_rows > 32 ? 64 : 32);
+    int64_t slots = tc ? 148 / X_CLUSTER : rows_cta == 32 ? 2 * 148 : 148;  // resident CTAs, or clusters
 
     // ---- the own pages of every sequence: as launch_decode cuts them, starting behind the shared ones ----
     const bool use_mma = decode_mma_supported(fmt, D, dtype) && !c->force_simt;
