@@ -887,7 +887,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     if (together) rows_cta = nz * dec_rows;
     // The own pages run beside the shared ones, on the SMs that these leave: each gets its share of the work, in microseconds of
     // an SM per page and head: 1.0 to 1.2 for a tile pair; for an own page 0.75 for each 32 KB at the copy rate, or what the decode
-    // kernel takes (15 sequences of 7 heads with up to 300 4-bit tokens of D = 64: 23.2 us when this took the bytes alone, 18.8 now).
+    // kernel takes (15 sequences of 7 heads a group with up to 200 own 4-bit tokens of D = 64: 23.2 us when this took the bytes alone, 18.8 now).
     if (tc && !together) {
         int64_t own = 0, shared = 0;
         for (int i = 0; i < n_seqs; i++) own += own_pages[i];
