@@ -564,3 +564,69 @@ def test_pages_past_four_gigabytes(kv, fmt, io):
         assert_close(cache.attend_shared(seqs, q), ref, size, io)
     cache.check()
     cache.close()
+
+
+def test_children_of_empty_and_trimmed_parents(kv):
+    Hkv, G, D = 2, 4, 128
+    cache = kv.KvCache("f16", Hkv, D, max_seqs=12, max_seq_tokens=1024, max_q_heads=Hkv * G)
+    empty, cut = cache.new_seq(), cache.new_seq()
+    add(cache, [cut], 1, 700, "f16")
+    cache.trim(cut, 250)
+    kids = cache.fork_shared([empty, cut, empty, cut, cut])
+    assert [cache.seq_len(s) for s in kids] == [0, 700, 0, 700, 700]
+    add(cache, kids, 3, 70, "f16")
+    q = rows(5, (5, Hkv * G, 1, D), "f16")
+    for way in (0, 1, 2):
+        cache.profile(False, shared_way=way)
+        got = cache.attend_shared(kids, q)
+        for i in (0, 2):  # nothing shared
+            ref, size = reference(cache, [kids[i]], q[i:i + 1])
+            assert_close(got[i:i + 1], ref, size, "f16")
+        assert torch.equal(got, cache.attend(kids, q))  # the front of a trimmed sequence is gone: regular attention
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("fmt,io", [("f16", "f16"), ("q8_1", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_truncated_children_share_what_is_left(kv, fmt, io, way):
+    # rolled back to different lengths, into pages that the others hold, and then on again: all in one call, twice
+    Hkv, G, D = 2, 4, 128
+    cache = kv.KvCache(fmt, Hkv, D, max_seqs=12, max_seq_tokens=1024, max_q_heads=Hkv * G)
+    parent = cache.new_seq()
+    add(cache, [parent], 1, 640, io)
+    kids = cache.fork_shared([parent] * 6)
+    for s, n in zip(kids, (640, 639, 321, 320, 64, 1)):
+        cache.truncate(s, n)
+    cache.profile(False, shared_way=way)
+    batch = [parent] + kids
+    for step in range(2):
+        q = rows(5 + step, (7, Hkv * G, 1, D), io)
+        ref, size = reference(cache, batch, q)
+        assert_close(cache.attend_shared(batch, q), ref, size, io)
+        add(cache, batch, 7 + 2 * step, 3, io)
+    q = rows(9, (7, Hkv * G, 1, D), io)
+    ref, size = reference(cache, batch, q)
+    assert_close(cache.attend_shared(batch, q), ref, size, io)
+    assert [cache.seq_len(s) for s in batch] == [646, 646, 645, 327, 326, 70, 7]
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_quantised_result_of_130_sequences(kv, way):
+    # from 128 rows on the activation is laid out in tiles
+    Hkv, G, D, n = 2, 2, 64, 130
+    cache, seqs = family(kv, "f16", "f16", Hkv, D, [200], n, [3, 1], Hkv * G)
+    cache.profile(False, shared_way=way)
+    q = rows(5, (n, Hkv * G, 1, D), "f16")
+    blocks = torch.randint(0, 256, (128, Hkv * G * D // 32, 18), dtype=torch.uint8, device="cuda")
+    blocks[:, :, :2] = torch.full((128, Hkv * G * D // 32), 0.01, device="cuda").half().view(torch.uint8).reshape(128, -1, 2)
+    lin = kv.Q40Linear(blocks, max_m=n)
+    out, scratch = torch.empty_like(q), torch.empty_like(lin.scratch)
+    cache.attend_shared(seqs, q, scratch=scratch, out=out)
+    got = lin.gemm_quantized(n, scratch=scratch)
+    assert torch.equal(got, lin.gemm(out.reshape(n, -1)))
+    lin.check(scratch)
+    cache.check()
+    cache.close()
