@@ -630,3 +630,43 @@ def test_quantised_result_of_130_sequences(kv, way):
     lin.check(scratch)
     cache.check()
     cache.close()
+
+
+@pytest.mark.parametrize("fmt,io,D", [("f16", "f16", 128), ("bf16", "bf16", 64), ("q8_1", "f16", 128), ("f32", "f32", 64)])
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_what_lies_beyond_the_tokens_and_in_other_rows_stays_out(kv, fmt, io, D, way):
+    # pages that held NaN and infinities before; a neighbour whose own keys, values or query are not numbers
+    Hkv, G = 2, 4
+    cache = kv.KvCache(fmt, Hkv, D, max_seqs=8, max_seq_tokens=1024, max_q_heads=Hkv * G, pool_tokens=1024)
+    cache.profile(False, shared_way=way)
+    dirty = cache.new_seq()
+    bad = torch.full((1, Hkv, 1000, D), float("nan"), dtype=rows(1, (1,), io).dtype, device="cuda")
+    if fmt != "q8_1":
+        cache.append([dirty], bad, bad)
+        bad.fill_(float("inf"))
+        cache.truncate(dirty, 500)
+    cache.append([dirty], bad[:, :, :500], bad[:, :, :500])
+    cache.free_seq(dirty)
+    parent = cache.new_seq()
+    add(cache, [parent], 3, 330, io)
+    kids = cache.fork_shared([parent] * 4)
+    add(cache, kids, 5, 7, io)
+    q = rows(7, (4, Hkv * G, 1, D), io)
+    ref, size = reference(cache, kids, q)
+    assert_close(cache.attend_shared(kids, q), ref, size, io)
+    # one neighbour's query, then its newest token
+    spoilt = q.clone()
+    spoilt[1, 3] = float("inf")
+    got = cache.attend_shared(kids, spoilt)
+    others = [i for i in range(4) if i != 1]
+    assert_close(got[others], ref[others], size[others], io)
+    heads = [h for h in range(Hkv * G) if h != 3]
+    assert_close(got[1, heads], ref[1, heads], size[1, heads], io)
+    assert bool(got[1, 3].isnan().all())
+    if fmt != "q8_1":
+        add_bad = bad[:, :, :1]
+        cache.append([kids[1]], add_bad, add_bad)
+        got = cache.attend_shared(kids, q)
+        assert_close(got[others], ref[others], size[others], io)
+    cache.check()
+    cache.close()
