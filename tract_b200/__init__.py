@@ -126,14 +126,29 @@ def _strides(t, n):
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] != 1:
         raise B200KvError("the innermost (head_dim) axis must be contiguous")
-    return (_I64x3 if n == 3 else _I64x2 if n == 2 else C.c_int64 * n)(*st[:n])
+    if n == 3:
+        return _I64x3(st[0], st[1], st[2])
+    return (_I64x2 if n == 2 else C.c_int64 * n)(*st[:n])
+
+
+_raw_of = None
+
+
+def _raw_stream():
+    """The current CUDA stream as an integer, for entries whose argument types are declared above."""
+    global _raw_of
+    if _raw_of is None:
+        import torch
+
+        torch.cuda.current_device()  # initialises CUDA, and says so if it cannot
+        # the raw handle: building a torch.cuda.Stream object for it takes 3.5 us of each call, this 0.2
+        get, device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+        _raw_of = lambda: get(device())
+    return _raw_of()
 
 
 def _stream():
-    import torch
-
-    # the raw handle: building a torch.cuda.Stream object for it takes 3.5 us of each call, this 0.3
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    return C.c_void_p(_raw_stream())
 
 
 def _ids(seqs):
@@ -197,10 +212,11 @@ class KvCache:
     # -- hot path --
     def append(self, seqs, k_new, v_new=None):
         """k_new / v_new: [n_seqs, Hkv, S, D] CUDA tensors."""
-        assert k_new.dim() == 4 and k_new.shape[0] == len(seqs)
-        _ck(lib().b200kv_append(self._h, len(seqs), _ids(seqs), k_new.shape[2], k_new.data_ptr(), _strides(k_new, 3),
+        n, shape = len(seqs), k_new.shape
+        assert len(shape) == 4 and shape[0] == n
+        _ck(lib().b200kv_append(self._h, n, _ids(seqs), shape[2], k_new.data_ptr(), _strides(k_new, 3),
                                 v_new.data_ptr() if v_new is not None else None,
-                                _strides(v_new, 3) if v_new is not None else None, _dtype_code(k_new), _stream()))
+                                _strides(v_new, 3) if v_new is not None else None, _dtype_code(k_new), _raw_stream()))
 
     def append_rope(self, seqs, k_new, v_new, cos, sin):
         """append() with ApplyRope fused on the key side; cos / sin: [n_seqs or 1, S, D] of k_new's dtype."""
@@ -380,8 +396,8 @@ class KvCache:
         pages and gets a copy of the partly filled last one."""
         n = len(seqs)
         out = (C.c_int32 * max(n, 1))()
-        _ck(lib().b200kv_fork_shared(self._h, n, _ids(seqs), out, _stream()))
-        return list(out[:n])
+        _ck(lib().b200kv_fork_shared(self._h, n, _ids(seqs), out, _raw_stream()))
+        return out[:n]
 
     def attend_shared(self, seqs, q, cos=None, sin=None, scratch=None, scale=None, out=None):
         """Decode attention (q: [n_seqs, Hq, 1, D]) in which the pages that neighbours of the batch share (fork_shared) are
@@ -389,22 +405,25 @@ class KvCache:
         quantised activation of a Q40Linear, as in attend_q40 (`out` stays unwritten then unless it is given)."""
         import torch
 
-        assert q.dim() == 4 and q.shape[0] == len(seqs) and q.shape[2] == 1 and q.shape[3] == self.head_dim and q.is_cuda
+        n, shape = len(seqs), q.shape
+        assert len(shape) == 4 and shape[0] == n and shape[2] == 1 and shape[3] == self.head_dim and q.is_cuda
+        cos_p = sin_p = scratch_p = out_p = out_strides = None
         stride = 0
         if cos is not None:
-            cos, sin = cos.reshape(len(seqs), -1), sin.reshape(len(seqs), -1)
+            cos, sin = cos.reshape(n, -1), sin.reshape(n, -1)
             assert cos.dtype == q.dtype and sin.dtype == q.dtype and cos.stride(1) == 1 and sin.stride(1) == 1
-            assert cos.stride(0) == sin.stride(0) and cos.shape[1] == q.shape[3]
-            stride = cos.stride(0)
+            assert cos.stride(0) == sin.stride(0) and cos.shape[1] == shape[3]
+            cos_p, sin_p, stride = cos.data_ptr(), sin.data_ptr(), cos.stride(0)
         if scratch is not None:
-            assert scratch.numel() >= Q40Linear.scratch_bytes(q.shape[1] * q.shape[3], len(seqs))
+            assert scratch.numel() >= Q40Linear.scratch_bytes(shape[1] * shape[3], n)
+            scratch_p = scratch.data_ptr()
         elif out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        assert out is None or (out.shape == q.shape and out.dtype == q.dtype)
-        _ck(lib().b200kv_attend_shared(self._h, len(seqs), _ids(seqs), q.shape[1], q.data_ptr(), _strides(q, 3),
-                                       cos.data_ptr() if cos is not None else None, sin.data_ptr() if sin is not None else None, stride,
-                                       out.data_ptr() if out is not None else None, _strides(out, 3) if out is not None else None,
-                                       scratch.data_ptr() if scratch is not None else None, _dtype_code(q), float(scale or 0.0), _stream()))
+        if out is not None:
+            assert out.shape == shape and out.dtype == q.dtype
+            out_p, out_strides = out.data_ptr(), _strides(out, 3)
+        _ck(lib().b200kv_attend_shared(self._h, n, _ids(seqs), shape[1], q.data_ptr(), _strides(q, 3), cos_p, sin_p, stride, out_p, out_strides,
+                                       scratch_p, _dtype_code(q), scale or 0.0, _raw_stream()))
         return out
 
     def prepared_attend_shared(self, seqs, q, out, scale=None):
@@ -418,7 +437,7 @@ class KvCache:
         keep = (q, out, self)
 
         def call(_keep=keep):
-            if L.b200kv_attend_shared(h, n, ids, hq, qp, qs, None, None, 0, op, os_, None, dt, sc, _stream()) != 0:
+            if L.b200kv_attend_shared(h, n, ids, hq, qp, qs, None, None, 0, op, os_, None, dt, sc, _raw_stream()) != 0:
                 raise B200KvError(L.b200kv_last_error().decode())
 
         return call
