@@ -59,3 +59,19 @@ def test_sampling_workspace_sizes(kv):
 def test_marshalling_of_sequence_ids(kv):
     assert list(kv._ids([3, 1])) == [3, 1] and list(kv._ids(np.array([3, 1]))) == [3, 1]
     assert list(kv._ids([np.int64(5)])) == [5] and list(kv._ids((2,))) == [2]
+    for ids in ([3, 1], np.array([3, 1]), (np.int64(3), 1), [3.0, 1.0]):
+        assert np.frombuffer(kv._id_bytes(ids), np.int32).tolist() == [3, 1]
+    assert kv._id_bytes([]) == b""
+    with pytest.raises(OverflowError):
+        kv._id_bytes([2 ** 31])
+
+
+def test_marshalling_of_strides(kv):
+    import torch
+
+    t = torch.empty((2, 3, 5, 8))
+    assert np.frombuffer(kv._stride_bytes(t), np.int64).tolist() == [120, 40, 8] == list(kv._strides(t, 3))
+    assert np.frombuffer(kv._stride_bytes(t[:, ::2].expand(2, 2, 5, 8)), np.int64).tolist() == [120, 80, 8]
+    with pytest.raises(kv.B200KvError, match="contiguous"):
+        kv._stride_bytes(t.transpose(2, 3))
+    assert np.frombuffer(kv._stride_bytes(t[..., :1]), np.int64).tolist() == [120, 40, 8]
