@@ -670,3 +670,33 @@ def test_what_lies_beyond_the_tokens_and_in_other_rows_stays_out(kv, fmt, io, D,
         assert_close(got[others], ref[others], size[others], io)
     cache.check()
     cache.close()
+
+
+@pytest.mark.parametrize("way,kernels", [(1, {"decode", "combine"}), (2, {"prefix", "decode", "combine"})])
+def test_timed_launches(kv, way, kernels):
+    # an event pair around every launch stands between those that otherwise overlap: the same bits, and the records say what ran
+    cache, seqs = family(kv, "f16", "f16", 2, 128, [700], 6, [5, 70], 8)
+    q = rows(5, (6, 8, 1, 128), "f16")
+    cache.profile(False, shared_way=way)
+    want = cache.attend_shared(seqs, q)
+    cache.profile(True, shared_way=way)
+    assert torch.equal(cache.attend_shared(seqs, q), want)
+    cache.fork_shared(seqs[:1])
+    names = [name for name, ms in cache.profile_read() if ms > 0]
+    assert set(names) == kernels | {"share"}
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("fmt,io,D", [("f16", "f16", 64), ("q8_1", "f16", 128), ("f32", "f32", 64)])
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_thousands_of_rows_share_a_page(kv, fmt, io, D, way):
+    n, G = 200, 40
+    cache, seqs = family(kv, fmt, io, 1, D, [330], n, [2, 1], G)
+    cache.profile(False, shared_way=way)
+    q = rows(5, (n, G, 1, D), io)
+    out = cache.attend_shared(seqs, q)
+    ref, size = reference(cache, seqs, q)
+    assert_close(out, ref, size, io)
+    cache.check()
+    cache.close()
