@@ -376,23 +376,25 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
     };
     // exp((x - max) / T) = 2^(t / 256), t = (x - max) 256 log2 e / T = n + r, n whole: 2^(n / 256) from the table and the exponent,
     // 2^(r / 256) by its Taylor polynomial of degree 3 in r ln 2 / 256 (|r| <= 1/2: what is left out is below 1.5e-13), rounded
-    // to 44 fractional bits by adding 1.5 * 2^8.  Below 2^-46: 0.
+    // to 44 fractional bits by adding 1.5 * 2^8.  What lies below 2^-46.5 (it would round to 0), -inf, a NaN and
+    // the fill of a slice have no weight, by comparison: what they give in the sums is not used.
     const double t_top = -(double)x_top * t_unit;
-    const float x_floor = __double2float_rd((double)x_top - 46.5 * 0.69314718055994530942 * (double)t_used);  // 2^-46.5 rounds to 0
+    const float x_floor = __double2float_ru((double)x_top - 46.5 * 0.69314718055994530942 * (double)t_used);  // always finite
     constexpr double L = 0.69314718055994530942 / SP_TABLE;
     double taylor1 = L, taylor2 = L * L / 2.0, taylor3 = L * L * L / 6.0;
     asm volatile("" : "+d"(taylor1), "+d"(taylor2), "+d"(taylor3));  // in registers: two moves per use otherwise
     auto weight = [&](float x) -> u64 {
         constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52
-        const double t = fma((double)fmaxf(x, x_floor), t_unit, t_top);
+        const double t = fma((double)x, t_unit, t_top);
         const double biased = t + MAGIC, r = t - (biased - MAGIC);
-        const int n = max(__double2loint(biased), -64 * SP_TABLE);  // the next float below the maximum may be deeper than that
+        const int n = __double2loint(biased);
         double q = fma(r, taylor3, taylor2);
         q = fma(q, r, taylor1);
         q = fma(q, r, 1.0);
         const double tab = sh.exp2_table[n & (SP_TABLE - 1)];
         const double scaled = __hiloint2double(__double2hiint(tab) + ((n << 12) & 0xfff00000), __double2loint(tab));
-        return (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
+        const u64 w = (u64)(__double_as_longlong(fma(q, scaled, 384.0)) - __double_as_longlong(384.0));
+        return x >= x_floor ? w : 0ull;
     };
     // f(x, place in the slice) for every logit of the slice; the fill is -inf
     auto each = [&](auto f) {
