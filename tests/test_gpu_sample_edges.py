@@ -1,5 +1,5 @@
-"""sample() where an empty place of a row could decide a token: rows masked with the lowest f32.  Tokens are compared with the
-64-bit restatement of test_gpu_sample."""
+"""sample() where a rounding or an empty place of a row could decide a token: rows masked with the lowest f32, logits at the borders of
+the histogram's bins.  Tokens are compared with the 64-bit restatement of test_gpu_sample."""
 import numpy as np
 import pytest
 
@@ -47,3 +47,59 @@ def test_the_two_lowest_values(kv, temperature, mode):
     x[2, ::2] = above
     x[2, 1::4] = -np.inf
     checked(kv, torch.from_numpy(x).cuda(), [0.3, 0.6, 0.97], **all_of(3, t=temperature, **mode))
+
+
+def bins_of(difference, zscale):
+    """Bins of the depth difference * zscale, rounded to the nearest whole number after the product was rounded (as the kernel's rule
+    has it), and from the unrounded product."""
+    rounded = (difference * zscale).astype(f32).astype(np.float64) + 2.0 ** 23
+    exact = difference.astype(np.longdouble) * zscale.astype(np.longdouble) + 2 ** 23
+    return rounded.astype(f32).view(np.uint32) & 1023, exact.astype(f32).view(np.uint32) & 1023
+
+
+def zscale_of(t):
+    """Bins per unit of the logits: 1023 bins over 28 octaves."""
+    return f32(f32(1.4426950408889634) / f32(t)) * f32(f32(1023) / f32(28))
+
+
+@pytest.mark.parametrize("n,copies", [(1000, 1), (9000, 1), (1000, 12)])
+def test_logits_at_the_border_of_a_bin(kv, n, copies):
+    # Two logits, the second at a depth whose product with the bins per unit lies next to k + 1/2: where it is counted, it has
+    # to be found.  p and n ask for the deepest bins (log2(n / (1 - p)) > 28).
+    lo, hi = (np.array([v], f32).view(np.uint32)[0] for v in (4.0, 10.0))
+    depth = np.random.default_rng(1).integers(lo, hi, 4_000_000).astype(np.uint32).view(f32)
+    depth = np.concatenate([np.array([0x4102120A], np.uint32).view(f32), depth])
+    a, b = bins_of(depth, zscale_of(1.0))
+    depth = depth[a != b][:40]
+    assert len(depth) == 40 and depth[0] == f32(8.129404)
+    rows = len(depth)
+    g = np.random.default_rng(2)
+    for neighbour in (False, True):  # alone; beside one that lies in the middle of the bin which the other rule names
+        x = np.full((rows, n), -np.inf, f32)
+        x[:, 0] = 0
+        x[np.arange(rows), g.integers(1, n // 2, rows)] = -depth
+        if neighbour:
+            x[np.arange(rows), g.integers(n // 2, n, rows)] = -(b[a != b][:rows].astype(np.float64) / float(zscale_of(1.0))).astype(f32)
+        u = 1 - np.exp(-depth) * g.uniform(0.2, 0.8, rows)
+        checked(kv, torch.from_numpy(x).cuda().repeat(copies, 1), np.tile(u, copies), **all_of(rows * copies, p=0.999999))
+
+
+@pytest.mark.parametrize("copies", [1, 20])
+def test_equal_logits_at_the_border_of_a_bin(kv, copies):
+    # fifty equal bf16 logits at such a depth: all of them or none
+    values = (np.arange(0x4080, 0x4120, dtype=np.uint32) << 16).view(f32)
+    g = np.random.default_rng(2)
+    found = []
+    while len(found) < 24:
+        t = f32(g.uniform(0.7, 2))
+        a, b = bins_of(values, zscale_of(t))
+        found += [(t, v) for v in values[(a != b) & (values / t < 9)]]
+    rows, n = len(found), 1000
+    t, v = (np.array(c, f32) for c in zip(*found))
+    x = np.full((rows, n), -np.inf, f32)
+    x[:, 500] = 0
+    for r in range(rows):
+        x[r, g.permutation(np.r_[0:500, 501:n])[:50]] = -v[r]
+    u = 1 - 50 * np.exp(-v / t) / (1 + 50 * np.exp(-v / t)) * g.uniform(0.1, 0.9, rows)
+    logits = torch.from_numpy(x).cuda().to(torch.bfloat16).repeat(copies, 1)
+    checked(kv, logits, np.tile(u, copies), np.tile(t, copies), **all_of(rows * copies, p=0.999999))

@@ -371,9 +371,11 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
 
     // ---- weights ----
     // the last bin takes everything that is deeper; monotone in x
-    auto z_bin = [&](float x) -> uint32_t {  // rounded to the nearest whole number
-        return __float_as_uint(fminf((x_top - x) * zscale, (float)(SP_BINS - 1)) + 8388608.f) & (SP_BINS - 1);
-    };
+    // (by its own rounded product wherever it is asked for: one that a sum took in unrounded would put a few logits next to a border
+    // into the other bin)
+    auto depth = [&](float x) -> float { return __fmul_rn(x_top - x, zscale); };
+    auto rounded = [](float z) -> float { return __fadd_rn(z, 8388608.f); };  // to the nearest whole number, in the low bits
+    auto z_bin = [&](float x) -> uint32_t { return __float_as_uint(rounded(fminf(depth(x), (float)(SP_BINS - 1)))) & (SP_BINS - 1); };
     // exp((x - max) / T) = 2^(t / 256), t = (x - max) 256 log2 e / T = n + r, n whole: 2^(n / 256) from the table and the exponent,
     // 2^(r / 256) by its Taylor polynomial of degree 3 in r ln 2 / 256 (|r| <= 1/2: what is left out is below 1.5e-13), rounded
     // to 44 fractional bits by adding 1.5 * 2^8.  What lies below 2^-46.5 (it would round to 0), -inf, a NaN and
@@ -763,8 +765,8 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
         }
         if (!s.use_k && !s.use_m && top.bin < SP_BINS - 1) {
             // top-p alone: the tokens of the bin, in every CTA
-            const float in_bin = 8388608.f + (float)top.bin;  // what z_bin rounds them to
-            if (gather(true, [&](float x) { return (x_top - x) * zscale + 8388608.f == in_bin; })) {
+            const float in_bin = 8388608.f + (float)top.bin;  // z_bin(x) == top.bin, which is not the last bin
+            if (gather(true, [&](float x) { return rounded(depth(x)) == in_bin; })) {
                 for (int i = tid; i < C * cap; i += T)
                     if ((i & (cap - 1)) < (int)sh.part[i >> cap_bits]) weights[i] = weight(logit_of(sh.list[i]));
                 __syncthreads();
