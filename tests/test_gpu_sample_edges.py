@@ -1,9 +1,9 @@
 """sample() where a rounding or an empty place of a row could decide a token: rows masked with the lowest f32, logits at the borders of
-the histogram's bins.  Tokens are compared with the 64-bit restatement of test_gpu_sample."""
+the histogram's bins, lists that every CTA of a row fills.  Tokens are compared with the 64-bit restatement of test_gpu_sample."""
 import numpy as np
 import pytest
 
-from test_gpu_sample import checked, kv  # noqa: F401 (kv is a fixture)
+from test_gpu_sample import checked, kv, model_logits  # noqa: F401 (kv is a fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -103,3 +103,19 @@ def test_equal_logits_at_the_border_of_a_bin(kv, copies):
     u = 1 - 50 * np.exp(-v / t) / (1 + 50 * np.exp(-v / t)) * g.uniform(0.1, 0.9, rows)
     logits = torch.from_numpy(x).cuda().to(torch.bfloat16).repeat(copies, 1)
     checked(kv, logits, np.tile(u, copies), np.tile(t, copies), **all_of(rows * copies, p=0.999999))
+
+
+@pytest.mark.parametrize("rows,n", [(15, 8192), (30, 4096), (60, 2048), (9, 8200), (100, 60000)])
+def test_lists_that_every_cta_of_a_row_fills(kv, rows, n):
+    # short slices, where the CTAs of a row run apart the most, and up to 100 candidates in each: the same token every time, the
+    # right one at first
+    x, g = model_logits(rows + n, rows, n)
+    u, t = g.random(rows), 0.5 + g.random(rows)
+    dev = lambda a, dt=torch.float32: torch.as_tensor(a, dtype=dt, device="cuda")
+    for k, p in ((2, 1.0), (199, 0.9), (700, 1.0)):
+        want = torch.from_numpy(checked(kv, x, u, t, **all_of(rows, k=k, p=p))).cuda()
+        args = dict(temperature=dev(t), top_k=dev(np.full(rows, k), torch.int32), top_p=dev(np.full(rows, p)))
+        outs = [torch.empty(rows, dtype=torch.int32, device="cuda") for _ in range(300)]
+        for out in outs:  # one after the other without a pause
+            kv.sample(x, dev(u), out=out, **args)
+        assert bool((torch.stack(outs) == want).all())

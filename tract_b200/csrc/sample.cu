@@ -124,7 +124,8 @@ struct RowShared {
     uint32_t hist[4][SP_BINS];     // limbs of the masses; counts
     u64 list[SP_LIST];             // gathered tokens
     double exp2_table[SP_TABLE];   // 2^(j / SP_TABLE)
-    // written by the other CTAs of the cluster
+    // written by the other CTAs of the cluster.  This CTA writes none of them itself while they may: a CTA that is ahead may have
+    // written what it gathered before this one has left the search (last, pick_w and list are its own once nobody else writes them)
     float x_max[SP_CLUSTER];
     u64 x_w[SP_CLUSTER];
     u64 last, pick_w;                // the last kept token, and the kept mass
@@ -520,10 +521,6 @@ __global__ void __launch_bounds__(T, 1024 / T) sample_kernel(SampleParams p) {
 #pragma unroll
                     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
                     if (lane == 0) sh.before_w[warp] = v;
-                }
-                if (counts) {  // its tokens up to the end of the bin
-                    const uint32_t v = __reduce_add_sync(0xffffffffu, (lane < run ? sh.run_n[warp][lane] : 0u) + (lane <= bin ? sh.bin_n[warp][lane] : 0u));
-                    if (lane == 0) sh.part[warp] = v;
                 }
             } else if (warp == 0 && lane == 0) {
                 sh.hit = Hit{0xffffffffu, 0, 0, 0, 0, all};  // in every CTA alike
