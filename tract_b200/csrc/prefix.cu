@@ -34,6 +34,10 @@ constexpr int X_XCHG = 8;          // per tile and page parity: one flag per sof
 // f16 weights skip the remainder product of a page once sqrt(64) x the largest weight of the page is below this fraction of
 // the running sum, for every row of the tile (see prefill_tc.cu)
 constexpr float X_SKIP_FRACTION = 0.125f;
+// Weights are 2^(s sl2 - m) with one rounding, while m is a rounded s sl2: at the maximum the exponent is off 0 by half a step
+// of m.  From this |m| on (a step of 2) the products are rounded first, as m was: otherwise the weights of a page leave the range
+// of f16 from 2^27 on, that of bf16 from 2^31 on.
+constexpr float X_FAR = 16777216.f;
 enum { PSRC_PAGES16 = 0, PSRC_Q8 = 1, PSRC_Q4 = 2 };
 
 constexpr int X_CLUSTER = 2;  // CTAs that join their runs before a partial leaves the chip
@@ -346,11 +350,12 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
             tmem_ld_wait();
             const float tmax = row_max64(sr) * sl2;
             int* flags = (int*)(xchg + (2 * qt + (i & 1)) * X_XCHG);
-            // Two questions per row, one reduction per warp.  Bit 0: the page needs its remainder product (see X_SKIP_FRACTION;
+            // Three questions per row, one reduction per warp.  Bit 0: the page needs its remainder product (see X_SKIP_FRACTION;
             // the first one always).  Bit 1: the reference maximum is exceeded by more than 2^8 (or was -inf until now): O is rescaled.
+            // Bit 2: see X_FAR.
             const bool mine = adaptive && (i == 0 || !(tmax - m_ref + 3.f <= log_thresh));
             const bool raise = tmax > m_ref + 8.f || (m_ref == -INFINITY && tmax > -INFINITY);
-            const uint32_t votes = __reduce_or_sync(0xffffffffu, (mine ? 1u : 0u) | (raise && i > 0 ? 2u : 0u));
+            const uint32_t votes = __reduce_or_sync(0xffffffffu, (mine ? 1u : 0u) | (raise && i > 0 ? 2u : 0u) | (fabsf(tmax) > X_FAR ? 4u : 0u));
             const bool two = !adaptive || (votes & 1u);
             if (adaptive && lane == 0) flags[w4] = two ? 1 : 0;
             float alpha = 1.f;
@@ -359,27 +364,45 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                 m_ref = tmax;
                 l_run *= alpha;
             }
-            if (votes & 2u) {
-                // O must hold every page before this one: see prefill_tc.cu for why the wait on barrier (i - 1) & 1 cannot
-                // mistake the completion of P.V(i - 3) or P.V(i + 1) for that of P.V(i - 1)
-                wait_or_fail(&bar_o[2 * qt + ((i - 1) & 1)], (uint32_t)(((i - 1) >> 1) & 1), fail_s);
-                tc_fence_after();
+            if (votes & 6u) {
+                if (votes & 2u) {
+                    // O must hold every page before this one: see prefill_tc.cu for why the wait on barrier (i - 1) & 1 cannot
+                    // mistake the completion of P.V(i - 3) or P.V(i + 1) for that of P.V(i - 1)
+                    wait_or_fail(&bar_o[2 * qt + ((i - 1) & 1)], (uint32_t)(((i - 1) >> 1) & 1), fail_s);
+                    tc_fence_after();
 #pragma unroll
-                for (int cc = 0; cc < D / 16; cc++) {
-                    uint32_t orow[16];
-                    tmem_ld16(lane_base + COL_O + cc * 16, orow);
+                    for (int cc = 0; cc < D / 16; cc++) {
+                        uint32_t orow[16];
+                        tmem_ld16(lane_base + COL_O + cc * 16, orow);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int c = 0; c < 16; c++) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
+                        tmem_st16(lane_base + COL_O + cc * 16, orow);
+                    }
+                }
+                if (votes & 4u) {  // (through TMEM: 64 products in registers would cost the common page spills)
+#pragma unroll 1
+                    for (int cc = 0; cc < 4; cc++) {
+                        uint32_t x[16];
+                        tmem_ld16(sbuf + cc * 16, x);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int c = 0; c < 16; c++) x[c] = __float_as_uint(__fmul_rn(__uint_as_float(x[c]), sl2));
+                        tmem_st16(sbuf + cc * 16, x);
+                    }
+                    tmem_st_wait();
+                    tmem_ld32(sbuf, sr);
+                    tmem_ld32(sbuf + 32, sr + 32);
                     tmem_ld_wait();
-#pragma unroll
-                    for (int c = 0; c < 16; c++) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
-                    tmem_st16(lane_base + COL_O + cc * 16, orow);
                 }
             }
             const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            const float unit = (votes & 4u) ? 1.f : sl2;
             uint32_t pr[32], pr2[32];
             float page_sum;
-            if (mma_bf16) page_sum = softmax_exps<2>(sr, sl2, m_use, pr, pr2);
-            else if (two) page_sum = softmax_exps<1>(sr, sl2, m_use, pr, pr2);
-            else page_sum = softmax_exps<0>(sr, sl2, m_use, pr, pr2);
+            if (mma_bf16) page_sum = softmax_exps<2>(sr, unit, m_use, pr, pr2);
+            else if (two) page_sum = softmax_exps<1>(sr, unit, m_use, pr, pr2);
+            else page_sum = softmax_exps<0>(sr, unit, m_use, pr, pr2);
             tmem_st32(sbuf + 32, pr2);
             tmem_st32(sbuf, pr);
             l_run += page_sum;
