@@ -1,7 +1,7 @@
-"""attend_shared where its ways could part: scores far from 0."""
+"""attend_shared where its ways could part: scores far from 0, the range of bf16 queries over quantised pages."""
 import pytest
 
-from test_gpu_share import assert_close, kv, reference, rows  # noqa: F401 (kv is a fixture)
+from test_gpu_share import assert_close, family, kv, reference, rows  # noqa: F401 (kv is a fixture)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -29,5 +29,34 @@ def test_scores_far_from_zero(kv, fmt, io, size, D, way):
         ref, weight = reference(cache, seqs, queries)
         assert_close(cache.attend_shared(seqs, queries), ref, weight, io)
         cache.free_seqs([parent, *seqs])
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("fmt", ["q8_1", "q4_0"])
+@pytest.mark.parametrize("D,own,way", [(64, [5, 70], 1), (64, [5, 70], 2), (64, [0], 2), (128, [0], 2)])
+def test_bf16_queries_of_any_magnitude_over_quantised_pages(kv, fmt, D, own, way):
+    # the scale of the call brings the scores back, so that the bound of the ordinary magnitudes holds for all of them.  (At
+    # head_dim 128 nothing goes through the decode kernel, which takes f16 queries over such pages.)
+    cache, seqs = family(kv, fmt, "bf16", 2, D, [640], 6, own, 14)
+    cache.profile(False, shared_way=way)
+    q = rows(5, (6, 14, 1, D), "bf16", scale=1.3)
+    for size in (1e6, 1e20, 1e35, 1e-7, 1e-20, 1e-35):
+        far = (q.float() * size).bfloat16()
+        scale = D ** -0.5 / size
+        ref, weight = reference(cache, seqs, far, scale=scale)
+        assert_close(cache.attend_shared(seqs, far, scale=scale), ref, weight, "bf16")
+    # one channel far above the others, one row far above its neighbours; a row of zeros
+    mixed = q.clone()
+    mixed[:, :, :, 3] *= 300.0
+    mixed[2] *= 2.0 ** 40
+    mixed[4, 1] = 0
+    ref, weight = reference(cache, seqs, mixed, scale=2.0 ** -10)
+    out = cache.attend_shared(seqs, mixed, scale=2.0 ** -10)
+    others = [0, 1, 3, 4, 5]
+    assert_close(out[others], ref[others], weight[others], "bf16")
+    assert torch.isfinite(out).all()  # (row 2 sees one key alone or a tie)
+    # ordinary magnitudes keep their bits when the power of two is another one
+    assert torch.equal(cache.attend_shared(seqs, q, scale=0.125), cache.attend_shared(seqs, q * 2, scale=0.0625))
     cache.check()
     cache.close()

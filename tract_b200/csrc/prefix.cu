@@ -66,7 +66,8 @@ struct XGeo {
     // what the other parts send of the columns that a CTA joins: over the operand rings, which are done with by then
     static constexpr size_t JOIN = (size_t)(PARTS - 1) * ROWS * (D / X_CLUSTER) * 4 + (size_t)ROWS * (D / X_CLUSTER / 4 + 1) * 16;
     static constexpr size_t RINGS = (size_t)NK * KSTAGE + (size_t)NV * CHUNK + (size_t)NR * RAW_STAGE;
-    static constexpr size_t SMEM = (size_t)ROWS * D * 2 + RINGS + N_BARS * 8 + 32 + 4 * X_XCHG * 4 + ML_BYTES;
+    static constexpr int UNIT_BYTES = RAW ? ROWS * 4 : 0;
+    static constexpr size_t SMEM = (size_t)ROWS * D * 2 + RINGS + N_BARS * 8 + 32 + 4 * X_XCHG * 4 + ML_BYTES + UNIT_BYTES;
     static_assert(COL_S + 128 <= COLS_PER_TILE && JOIN <= RINGS && SMEM <= 227 * 1024, "TMEM columns and shared memory of an SM");
 };
 
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     volatile int* fail_s = (volatile int*)(tmem_slot + 1);
     float* xchg = (float*)(tmem_slot + 4);                  // [2][2 parities][X_XCHG]
     float2* ml_s = (float2*)(xchg + 4 * X_XCHG);            // [PARTS][ROWS] (m, l) of every part of the cluster
+    float* unit_s = (float*)(ml_s + PARTS * ROWS);          // RAW: [ROWS] what a step of 1 of a bf16 query's f16 operand stands for
     float4* join_s = (float4*)k_ring;                       // [PARTS - 1][D / X_CLUSTER / 4][ROWS]
 
     const DecodeParams& dp = p.d;
@@ -162,9 +164,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
             const int r = x / UNITS, uu = x % UNITS, in_tile = r % XM;
             return (uint4*)(q_s + (r / XM) * QBYTES + (uu / 8) * (XM * 128) + in_tile * 128 + (((uu % 8) ^ (in_tile & 7)) << 4));
         };
-        if (dp.q_cos || (RAW && is_bf16)) {
-            // the rotated value is rounded to the query's type, as a separate rope kernel would store it; over converted
-            // pages a bf16 query becomes f16 (every bf16 value is an f16 value, short of its range)
+        if (dp.q_cos) {  // the rotated value is rounded to the query's type, as a separate rope kernel would store it
 #pragma unroll 1
             for (int x = tid; x < ROWS * UNITS; x += 2 * X_SM_THREADS) {
                 const int g_row = tile * ROWS + x / UNITS, b = grp.b0 + g_row / dp.G, head = kvh * dp.G + g_row % dp.G;
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const float a = load_query(dp, D, b, head, (x % UNITS) * 8 + 2 * j), c = load_query(dp, D, b, head, (x % UNITS) * 8 + 2 * j + 1);
-                        if (mma_bf16) {
+                        if (is_bf16) {
                             const __nv_bfloat162 h = __floats2bfloat162_rn(a, c);
                             w[j] = *(const uint32_t*)&h;
                         } else {
@@ -197,6 +197,30 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                 }
 #pragma unroll
                 for (int i = 0; i < BATCH; i++) *place(x0 + i * 2 * X_SM_THREADS) = w[i];
+            }
+        }
+        // Over converted pages a bf16 row becomes f16 times a power of two that brings its largest magnitude to 2^14 .. 2^15: what
+        // lies within 2^28 of that stays exact (bf16 has fewer bits), the rest is off by at most 2^-39 of it.  The scale of the
+        // row's scores takes the power back.  A thread has the units that it stored, UNITS neighbouring lanes a row.
+        if (RAW && is_bf16) {
+#pragma unroll 1
+            for (int x = tid; x < ROWS * UNITS; x += 2 * X_SM_THREADS) {
+                const uint4 b = *place(x);
+                uint32_t w[4] = {b.x, b.y, b.z, b.w};
+                float big = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xffff0000u))));
+#pragma unroll
+                for (int o = UNITS / 2; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const int e = max((int)(__float_as_uint(big) >> 23) - 127, -100);  // (both powers stay normal)
+                const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+                if (x % UNITS == 0) unit_s[x / UNITS] = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const __half2 h = __floats2half2_rn(__uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xffff0000u) * up);
+                    w[j] = *(const uint32_t*)&h;
+                }
+                *place(x) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
         fence_async_proxy();  // generic-proxy writes -> visible to the tensor core
@@ -337,7 +361,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     } else {
         // ================= softmax threads =================
         const bool adaptive = !mma_bf16;
-        const float sl2 = dp.scale * 1.4426950408889634f;  // scores enter the exponent in log2 units
+        const float sl2 = dp.scale * 1.4426950408889634f * (RAW && is_bf16 ? unit_s[cta_row] : 1.f);  // scores enter the exponent in log2 units
         float log_thresh = -INFINITY;
         const int n = pages_of(qt);
         for (int i = 0; i < n; i++) {
