@@ -443,6 +443,10 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
 
     // ---- join the parts of the cluster: (m, l) to both CTAs, then each CTA's half of the channels ----
     const int part = ALT ? 2 * rank + qt : rank;
+    // A CTA that gave up lets copies and products that may still be in flight end first: its rings take the other CTA's part next.
+    // (Whoever gave up has set the flag and waits here; nobody is past the barriers below before.)
+    if (*fail_s)
+        for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 200000ull;) __nanosleep(10000);
     cluster.barrier_wait();
     if (is_softmax)
 #pragma unroll
@@ -515,11 +519,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     }
     tc_fence_before();
     __syncthreads();
-    if (*fail_s) {
-        if (tid == 0) atomicOr(dp.status, STATUS_WAIT_EXPIRED);
-        __nanosleep(200000);  // give copies that may still be in flight time to land before the CTA's memory is released
-        __syncthreads();
-    }
+    if (*fail_s && tid == 0) atomicOr(dp.status, STATUS_WAIT_EXPIRED);
     if (warp == 0) tmem_dealloc(tmem, COLS_PER_TILE * 2);
 }
 
