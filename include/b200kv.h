@@ -369,9 +369,9 @@ int b200kv_cast(const void* src, int64_t src_stride, int32_t src_dtype, void* ds
  * `enable` is a bit set: bit 0 turns the timing on; bit 1 (a test hook) routes decode attention through the
  * CUDA-core kernel even where the tensor-core kernel applies (KIVI caches: through export + the generic kernel), so
  * the two can be checked against each other; bit 2 (a test hook) keeps KIVI decode attention on its CUDA-core
- * kernel alone; bit 3 (a test hook, consumed by the next decode launch of a non-KIVI cache) exercises the give-up path of
- * the bounded waits without any fault: one CTA of that launch issues no copies, its first wait runs out after 1 ms, it
- * sets the status word, publishes an empty partial and returns -- b200kv_check then reports the expired wait, the
+ * kernel alone; bit 3 (a test hook, consumed by the next decode attention of a non-KIVI cache, b200kv_attend_shared
+ * included) exercises the give-up path of the bounded waits without any fault: one CTA of the call's first launch issues no
+ * copies, its first wait runs out after 1 ms, it sets the status word, publishes an empty partial and returns -- b200kv_check then reports the expired wait, the
  * output of that call is not meaningful, and the cache is usable as before; bits 4 and 5 (test hooks) take one way of
  * b200kv_attend_shared whatever the sizes: the shared pages as work items of the decode kernel, or through the kernels that
  * meet all rows at once (where they take the format). */

@@ -1,4 +1,5 @@
-"""attend_shared where its ways could part: scores far from 0, the range of bf16 queries over quantised pages."""
+"""attend_shared where its ways could part: scores far from 0, the range of bf16 queries over quantised pages;
+waits that run out."""
 import pytest
 
 from test_gpu_share import assert_close, family, kv, reference, rows  # noqa: F401 (kv is a fixture)
@@ -58,5 +59,31 @@ def test_bf16_queries_of_any_magnitude_over_quantised_pages(kv, fmt, D, own, way
     assert torch.isfinite(out).all()  # (row 2 sees one key alone or a tie)
     # ordinary magnitudes keep their bits when the power of two is another one
     assert torch.equal(cache.attend_shared(seqs, q, scale=0.125), cache.attend_shared(seqs, q * 2, scale=0.0625))
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("fmt,io,D,n", [("f16", "f16", 128, 6), ("bf16", "bf16", 64, 6), ("q8_1", "f16", 128, 6), ("q4_0", "bf16", 64, 40), ("f16", "f16", 128, 40),
+                                        ("f32", "f32", 128, 6), ("f32", "f32", 64, 40)])
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_a_wait_that_runs_out_is_reported_and_the_cache_stays_usable(kv, fmt, io, D, n, way):
+    # one CTA of kv head 0 issues none of its copies and gives up after 1 ms: what the others hold is not touched by it
+    Hkv, G = 2, 4
+    cache, seqs = family(kv, fmt, io, Hkv, D, [1500], n, [5, 70, 130], Hkv * G)
+    cache.profile(False, shared_way=way)
+    q = rows(5, (n, Hkv * G, 1, D), io)
+    good = cache.attend_shared(seqs, q)
+    cache.check()
+    cache.profile(False, shared_way=way, stall_next_decode=True)
+    short = cache.attend_shared(seqs, q)  # about 1 ms longer; a run of pages is missing from some rows of kv head 0
+    with pytest.raises(kv.B200KvError, match="bounded wait expired"):
+        cache.check()
+    cache.check()  # reported once
+    assert torch.equal(short[:, G:], good[:, G:]) and torch.isfinite(short[:, :G]).all() and not torch.equal(short[:, :G], good[:, :G])
+    for _ in range(2):  # the hook is spent
+        assert torch.equal(cache.attend_shared(seqs, q), good)
+        cache.check()
+    ref, size = reference(cache, seqs, q)
+    assert_close(cache.attend(seqs, q), ref, size, io)
     cache.check()
     cache.close()

@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
     }
 
     const int32_t* pages = dp.table + (int64_t)grp.trow * dp.max_pages_per_seq + page0;
+    const int n_copy = (int)blockIdx.x == dp.stall_item && kvh == 0 ? 0 : n_pages;  // test hook, see DecodeParams
     auto page_src = [&](int32_t pg) {  // a page id outside the pool is reported and replaced, so that the barriers go on
         if (pg < 0 || pg >= dp.n_pages) {
             if (lane == 0) atomicOr(dp.status, STATUS_PAGE_OOB);
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
             const bool adaptive = !mma_bf16;
             auto issue_qk = [&](int i) {  // S(i) = Q . K^T of the pipeline's i-th page into buffer i & 1
                 const int j = page_at(t, i);
-                wait_or_fail(&full_k[j % NK], (uint32_t)((j / NK) & 1), fail_s);
+                wait_or_fail(&full_k[j % NK], (uint32_t)((j / NK) & 1), fail_s, dp.wait_ns);
                 tc_fence_after();
                 if (elect_one()) {
                     const uint64_t kd = k_desc + (uint64_t)(((j % NK) * KSTAGE) >> 4);
@@ -284,8 +285,8 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
             if (n > 1) issue_qk(1);
             for (int i = 0; i < n; i++) {
                 const int j = page_at(t, i);
-                wait_or_fail(&full_v[j % NV], (uint32_t)((j / NV) & 1), fail_s);
-                wait_or_fail(&bar_p[2 * t + (i & 1)], (uint32_t)((i >> 1) & 1), fail_s);
+                wait_or_fail(&full_v[j % NV], (uint32_t)((j / NV) & 1), fail_s, dp.wait_ns);
+                wait_or_fail(&bar_p[2 * t + (i & 1)], (uint32_t)((i >> 1) & 1), fail_s, dp.wait_ns);
                 tc_fence_after();
                 const int* flags = (const int*)(xchg + (2 * t + (i & 1)) * X_XCHG);
                 const bool two = !adaptive || __any_sync(0xffffffffu, flags[lane & 3] != 0);
@@ -307,16 +308,16 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
         } else if constexpr (!RAW) {
             // ================= the chunks of a 16-bit page are the operand tiles =================
             int32_t pg_next = n_pages > 0 ? pages[0] : 0;
-            for (int i = 0; i < n_pages; i++) {
+            for (int i = 0; i < n_copy; i++) {
                 const uint8_t* src = page_src(pg_next);
                 if (i + 1 < n_pages) pg_next = pages[i + 1];  // fetched one page ahead of its use
-                if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
+                if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s, dp.wait_ns);
                 if (elect_one()) {
                     mbar_expect_tx(&full_k[i % NK], CHUNK);
                     bulk_g2s(k_ring + (i % NK) * CHUNK, src, CHUNK, &full_k[i % NK]);
                 }
                 __syncwarp();
-                if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s);
+                if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s, dp.wait_ns);
                 if (elect_one()) {
                     mbar_expect_tx(&full_v[i % NV], CHUNK);
                     bulk_g2s(v_ring + (i % NV) * CHUNK, src + CHUNK, CHUNK, &full_v[i % NV]);
@@ -329,10 +330,10 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
             if (ft < 0) {
                 // ================= raw chunk pairs, for the converter warps =================
                 int32_t pg_next = n_pages > 0 ? pages[0] : 0;
-                for (int i = 0; i < n_pages; i++) {
+                for (int i = 0; i < n_copy; i++) {
                     const uint8_t* src = page_src(pg_next);
                     if (i + 1 < n_pages) pg_next = pages[i + 1];
-                    if (i >= NR) wait_or_fail(&free_raw[i % NR], (uint32_t)((i / NR - 1) & 1), fail_s);
+                    if (i >= NR) wait_or_fail(&free_raw[i % NR], (uint32_t)((i / NR - 1) & 1), fail_s, dp.wait_ns);
                     if (elect_one()) {
                         mbar_expect_tx(&full_raw[i % NR], 2 * p.chunk_bytes);
                         bulk_g2s(raw_ring + (i % NR) * GEO::RAW_STAGE, src, 2 * p.chunk_bytes, &full_raw[i % NR]);
@@ -344,13 +345,13 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                 // No warp waits for another one: each goes on with the next page as soon as its share of this one is written.
                 for (int i = 0; i < n_pages; i++) {
                     const uint8_t* raw = raw_ring + (i % NR) * GEO::RAW_STAGE;
-                    wait_or_fail(&full_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s);
-                    if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s);
+                    wait_or_fail(&full_raw[i % NR], (uint32_t)((i / NR) & 1), fail_s, dp.wait_ns);
+                    if (i >= NK) wait_or_fail(&free_k[i % NK], (uint32_t)((i / NK - 1) & 1), fail_s, dp.wait_ns);
                     convert_rows<FMT, D, 0, FT, true>(raw, k_ring + (i % NK) * KSTAGE, k_ring + (i % NK) * KSTAGE + CHUNK, PAGE_TOKENS, ft);
                     fence_async_proxy();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full_k[i % NK]);
-                    if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s);
+                    if (i >= NV) wait_or_fail(&free_v[i % NV], (uint32_t)((i / NV - 1) & 1), fail_s, dp.wait_ns);
                     convert_rows<FMT, D, 1, FT, true>(raw + p.chunk_bytes, v_ring + (i % NV) * CHUNK, nullptr, PAGE_TOKENS, ft);
                     fence_async_proxy();
                     __syncwarp();
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
         const int n = pages_of(qt);
         for (int i = 0; i < n; i++) {
             const uint32_t sbuf = lane_base + COL_S + 64 * (i & 1);
-            wait_or_fail(&bar_s[2 * qt + (i & 1)], (uint32_t)((i >> 1) & 1), fail_s);
+            wait_or_fail(&bar_s[2 * qt + (i & 1)], (uint32_t)((i >> 1) & 1), fail_s, dp.wait_ns);
             tc_fence_after();
             uint32_t sr[64];
             tmem_ld32(sbuf, sr);
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
                 if (votes & 2u) {
                     // O must hold every page before this one: see prefill_tc.cu for why the wait on barrier (i - 1) & 1 cannot
                     // mistake the completion of P.V(i - 3) or P.V(i + 1) for that of P.V(i - 1)
-                    wait_or_fail(&bar_o[2 * qt + ((i - 1) & 1)], (uint32_t)(((i - 1) >> 1) & 1), fail_s);
+                    wait_or_fail(&bar_o[2 * qt + ((i - 1) & 1)], (uint32_t)(((i - 1) >> 1) & 1), fail_s, dp.wait_ns);
                     tc_fence_after();
 #pragma unroll
                     for (int cc = 0; cc < D / 16; cc++) {
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(XGeo<ALT, D, SRC>::THREADS, 1) __cluster_dims_
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_p[2 * qt + (i & 1)]);
         }
-        if (n > 0) wait_or_fail(&bar_o[2 * qt + ((n - 1) & 1)], (uint32_t)(((n - 1) >> 1) & 1), fail_s);
+        if (n > 0) wait_or_fail(&bar_o[2 * qt + ((n - 1) & 1)], (uint32_t)(((n - 1) >> 1) & 1), fail_s, dp.wait_ns);
         tc_fence_after();
         if (n == 0 || *fail_s) m_ref = -INFINITY, l_run = 0.f;  // no pages, or a CTA that gave up: an empty partial
     }
@@ -563,8 +564,9 @@ __global__ void __launch_bounds__(4 * ROWS, ROWS <= 32 ? 2 : 1) prefix_simt_kern
     prefix_run(grp, grp.splits, split, &page0, &n_pages);
     const int n_rows = grp.n_seqs * dp.G, row0 = tile * ROWS;
     const int32_t* pages = dp.table + (int64_t)grp.trow * dp.max_pages_per_seq + page0;
+    const int n_copy = (int)blockIdx.x == dp.stall_item && kvh == 0 ? 0 : n_pages;  // test hook, see DecodeParams
     auto fetch = [&](int i, int x) {  // thread 0: K (x = 0) or V of page i of the run
-        if (i >= n_pages) return;
+        if (i >= n_copy) return;
         int32_t pg = pages[i];
         if (pg < 0 || pg >= dp.n_pages) {
             atomicOr(dp.status, STATUS_PAGE_OOB);
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(4 * ROWS, ROWS <= 32 ? 2 : 1) prefix_simt_kern
     __syncthreads();          // the queries are there, and the barriers
 
     for (int i = 0; i < n_pages; i++) {
-        wait_or_fail(&bars[0], i & 1, fail_s);
+        wait_or_fail(&bars[0], i & 1, fail_s, dp.wait_ns);
         {  // scores against keys tx + 16 {0 .. 3}
             uint64_t s[4][4] = {};  // the sums over even and over odd channels
 #pragma unroll 2
@@ -650,7 +652,7 @@ __global__ void __launch_bounds__(4 * ROWS, ROWS <= 32 ? 2 : 1) prefix_simt_kern
                 a_s[r] = a, m_s[r] = m_new, l_s[r] = fmaf(l_s[r], a, sum);
             }
         }
-        wait_or_fail(&bars[1], i & 1, fail_s);
+        wait_or_fail(&bars[1], i & 1, fail_s, dp.wait_ns);
         __syncthreads();
         {  // values: channels tx * 4 + 64 j .. + 3
 #pragma unroll
@@ -1007,6 +1009,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     dp.part_o = (float*)c->ws, dp.part_ml = dp.part_o + n_rec * D;
     dp.page_bytes = c->L.page_bytes, dp.n_pages = (int32_t)c->n_pages, dp.max_pages_per_seq = c->max_pages_per_seq;
     dp.Hkv = Hkv, dp.G = G, dp.dtype = dtype, dp.scale = scale, dp.wait_ns = c->wait_ns;
+    if (c->stall_next_decode) dp.stall_item = 0, dp.wait_ns = 1000000, c->stall_next_decode = false;  // one call, 1 ms
     p.chunk_bytes = c->L.chunk_bytes, p.skip_fraction = X_SKIP_FRACTION;
     cudaError_t e = cudaSuccess;
     if (!together) {
@@ -1018,6 +1021,7 @@ static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, i
     if (together || n_items > 0) {
         ProfScope ps(c, K_DECODE, stream);
         dp.beside = !together;
+        if (!together) dp.stall_item = -1;  // the launch before took the hook
         const PrefixBatch* with = together ? &pb : nullptr;
         const int more = together ? ctas - n_items : 0;
         if ((use_mma ? launch_decode_mma(fmt, dp, n_items, stream, &ib, with, more) : launch_decode_simt(fmt, D, dp, n_items, stream, &ib, with, more)) != B200KV_OK)

@@ -209,8 +209,8 @@ __device__ inline bool mbar_test(uint64_t* bar, uint32_t parity) {  // one look,
         : "memory");
     return ok != 0;
 }
-// Waits for a barrier phase unless the CTA has already failed; gives up after ~1 s and marks the CTA failed.
-__device__ inline void wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* fail) {
+// Waits for a barrier phase unless the CTA has already failed; gives up after limit_ns and marks the CTA failed.
+__device__ inline void wait_or_fail(uint64_t* bar, uint32_t parity, volatile int* fail, uint64_t limit_ns = 1000000000ull) {
     if (mbar_try_wait(bar, parity)) return;
     const uint64_t t0 = globaltimer_ns();
     for (;;) {
@@ -218,7 +218,7 @@ __device__ inline void wait_or_fail(uint64_t* bar, uint32_t parity, volatile int
 #pragma unroll 1
         for (int i = 0; i < 32; i++)
             if (mbar_try_wait(bar, parity)) return;
-        if (globaltimer_ns() - t0 > 1000000000ull) {
+        if (globaltimer_ns() - t0 > limit_ns) {
             *fail = 1;
             return;
         }
