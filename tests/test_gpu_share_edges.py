@@ -1,5 +1,5 @@
 """attend_shared where its ways could part: scores far from 0, the range of bf16 queries over quantised pages;
-waits that run out."""
+waits that run out; refusals."""
 import pytest
 
 from test_gpu_share import assert_close, family, kv, reference, rows  # noqa: F401 (kv is a fixture)
@@ -85,5 +85,22 @@ def test_a_wait_that_runs_out_is_reported_and_the_cache_stays_usable(kv, fmt, io
         cache.check()
     ref, size = reference(cache, seqs, q)
     assert_close(cache.attend(seqs, q), ref, size, io)
+    cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("way", [0, 1, 2])
+def test_a_batch_with_an_empty_sequence_is_refused_whole(kv, way):
+    # more than 256 sequences are served in parts: nothing of the first part is written when a later one holds the empty sequence
+    n = 280
+    cache, seqs = family(kv, "f16", "f16", 1, 64, [130], n, [3], 2)
+    cache.profile(False, shared_way=way)
+    empty = cache.new_seq()
+    q, out = rows(5, (n + 1, 2, 1, 64), "f16"), torch.full((n + 1, 2, 1, 64), 3.25, dtype=torch.float16, device="cuda")
+    for at in (n, 256, 255, 0):
+        with pytest.raises(kv.B200KvError, match="is empty"):
+            cache.attend_shared(seqs[:at] + [empty] + seqs[at:], q, out=out)
+    torch.cuda.synchronize()
+    assert bool((out == 3.25).all())
     cache.check()
     cache.close()

@@ -889,8 +889,6 @@ static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
 static int launch_shared(b200kv_cache* c, int32_t n_seqs, const int32_t* seqs, int32_t n_q_heads, const void* q, const int64_t* qs, void* out,
                          const int64_t* os, int32_t dtype, float scale, cudaStream_t stream, const QueryRope& ends) {
     const int Hkv = c->L.Hkv, D = c->L.D, G = n_q_heads / Hkv;
-    for (int i = 0; i < n_seqs; i++)
-        if (c->seqs[seqs[i]].len <= 0) return fail("sequence %d is empty: nothing to attend to", seqs[i]);
     std::vector<Run> runs = shared_runs(c, n_seqs, seqs);
     bool any = false;
     for (const Run& r : runs) any |= r.n > 1 && r.pages > 0;
@@ -1057,6 +1055,8 @@ extern "C" int b200kv_attend_shared(b200kv_cache* c, int32_t n_seqs, const int32
     if (n_q_heads <= 0 || n_q_heads % c->L.Hkv != 0)
         return fail("n_q_heads (%d) must be a positive multiple of n_kv_heads (%d)", n_q_heads, c->L.Hkv);
     if (dtype < B200KV_F32 || dtype > B200KV_BF16) return fail("unknown dtype %d", dtype);
+    for (int i = 0; i < n_seqs; i++)
+        if (c->seqs[seqs[i]].len <= 0) return fail("sequence %d is empty: nothing to attend to", seqs[i]);
     if (scale <= 0.f) scale = 1.0f / sqrtf((float)c->L.D);
     cudaStream_t stream = (cudaStream_t)stream_;
     DeviceGuard guard(c->cfg.device);
