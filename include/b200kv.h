@@ -230,8 +230,12 @@ int b200kv_fork(b200kv_cache* cache, int32_t seq, int32_t* new_seq_out, void* st
 int b200kv_fork_shared(b200kv_cache* cache, int32_t n, const int32_t* seqs, int32_t* new_seqs_out, void* stream);
 
 /* Decode attention of a batch whose sequences share their beginning (b200kv_fork_shared): what b200kv_attend with
- * n_new = 1 gives, up to the order of its sums, but the pages that neighbours of the batch share are read once for all of
- * them.  Neighbours: sequences of one prompt stand next to each other in `seqs`; a batch may hold several prompts, and
+ * n_new = 1 gives, but the pages that neighbours of the batch share are read once for all of them.  With f32 queries the two
+ * differ in the order of their sums.  With 16-bit queries the operands of the shared pages are 16-bit too, whatever head_dim:
+ * weights (with the remainder of their rounding where a page carries more than an eighth of a row) and dequantised values,
+ * each off by at most half a step of f16, so that a result is off by its own rounding and 2^-10 of the weighted sum of
+ * |value| at most; dequantised keys and values beyond 65504 leave that range.  Which way a call takes follows from its sizes.
+ * Where nothing is shared it is b200kv_attend, bit for bit.  Neighbours: sequences of one prompt stand next to each other in `seqs`; a batch may hold several prompts, and
  * sequences that share nothing.  q, out: [n_seqs, n_q_heads, 1, D].
  * cos / sin (both or none): ApplyRope folded into the query load, as in b200kv_attend_rope.  scratch (may be null): the
  * result as the quantised activation of a W4A8 GEMM, as in b200kv_attend_q40; `out` may then be null.

@@ -1,5 +1,5 @@
 """attend_shared where its ways could part: scores far from 0, the range of bf16 queries over quantised pages;
-waits that run out; refusals."""
+the distance from regular attention; waits that run out; refusals."""
 import pytest
 
 from test_gpu_share import assert_close, family, kv, reference, rows  # noqa: F401 (kv is a fixture)
@@ -60,6 +60,29 @@ def test_bf16_queries_of_any_magnitude_over_quantised_pages(kv, fmt, D, own, way
     # ordinary magnitudes keep their bits when the power of two is another one
     assert torch.equal(cache.attend_shared(seqs, q, scale=0.125), cache.attend_shared(seqs, q * 2, scale=0.0625))
     cache.check()
+    cache.close()
+
+
+@pytest.mark.parametrize("fmt,io", [("f16", "f16"), ("bf16", "bf16"), ("q8_1", "f16"), ("q8_1", "bf16"), ("q4_0", "f16"), ("q8_1", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("way", [1, 2])
+def test_distance_from_regular_attention(kv, fmt, io, D, way):
+    # Both are off from the exact result by no more than assert_close allows, of which half a step of the result and two of the
+    # weights and values are counted twice here; a flat row (many weights of the same size) beside peaked ones.
+    cache, seqs = family(kv, fmt, io, 2, D, [1300], 8, [5, 70], 8)
+    q = rows(5, (8, 8, 1, D), io, scale=1.3)
+    q[0] = 0
+    q[1] *= 4
+    want = cache.attend(seqs, q)
+    cache.profile(False, shared_way=way)
+    got = cache.attend_shared(seqs, q)
+    cache.check()
+    ref, size = reference(cache, seqs, q)
+    if io == "f32":
+        bound = 2 * (2.0 ** -24 * ref.abs() + 2.0 ** -17 * size)
+    else:
+        bound = torch.finfo(got.dtype).eps * ref.abs() + 2 * (2.0 ** -10 + 2.0 ** -15) * size
+    assert bool(((got.double() - want.double()).abs() <= bound).all())
     cache.close()
 
 
