@@ -81,7 +81,9 @@ class Decoder:
                 attn_norm=norm_weight(f"l{i}.attn_norm"), ffn_norm=norm_weight(f"l{i}.ffn_norm"),
                 wqkv=linear(f"l{i}.wqkv", qkv_rows, sh.hidden), wo=linear(f"l{i}.wo", sh.hidden, sh.n_q_heads * sh.head_dim),
                 wgu=linear_rows([f"l{i}.wg", f"l{i}.wu"], sh.ffn, sh.hidden), wd=linear(f"l{i}.wd", sh.hidden, sh.ffn),
-                cache=kv.KvCache(kv_format, sh.n_kv_heads, sh.head_dim, max_seqs=n_seqs, max_seq_tokens=max_tokens)))
+                # (branch() makes the new continuations before it lets go of what nobody goes on from)
+                cache=kv.KvCache(kv_format, sh.n_kv_heads, sh.head_dim, max_seqs=2 * n_seqs - 1, max_seq_tokens=max_tokens,
+                                 pool_tokens=n_seqs * max_tokens)))
         self.final_norm = norm_weight("final_norm")
         self.lm_head = linear("lm_head", sh.vocab, sh.hidden)
         self.embed = (weights["embed"] if weights is not None else torch.randn((sh.vocab, sh.hidden), generator=gen, device=dev)).to(dev, torch.float32)
@@ -244,19 +246,26 @@ class Decoder:
     def branch(self, parents):
         """Sequence i goes on from what sequence parents[i] holds (one index per sequence, any of them any number of times): the
         re-ordering step of a beam search, or one sequence taken up several times.  Nothing but partly filled last pages is
-        copied; its next token, position and length go along.  Continuations of one sequence that stand next to each other in
-        the batch are attended to together (attend_shared)."""
+        copied; its next token, position and length go along.  Where a cache lacks the pages nothing changes.  Continuations of one
+        sequence that stand next to each other in the batch are attended to together (attend_shared)."""
         parents = [int(p) for p in parents]
         assert len(parents) == self.B and all(0 <= p < self.B for p in parents)
+        again = [b for b, p in enumerate(parents) if p in parents[:b]]  # the first continuation takes the sequence itself
+        forked = []
+        try:
+            for i, L in enumerate(self.layers):
+                forked.append(L["cache"].fork_shared([self.seqs[i][parents[b]] for b in again]) if again else [])
+        except kv.B200KvError:  # a layer without the pages: the others give theirs back, nothing has changed
+            for L, new in zip(self.layers, forked):
+                L["cache"].free_seqs(new)
+            raise
         for i, L in enumerate(self.layers):
-            cache, old = L["cache"], self.seqs[i]
-            dropped = [old[p] for p in range(self.B) if p not in parents]
-            again = [b for b, p in enumerate(parents) if p in parents[:b]]  # the first continuation takes the sequence itself
+            old = self.seqs[i]
             new = [old[p] for p in parents]
-            if dropped:
-                cache.free_seqs(dropped)
-            for b, s in zip(again, cache.fork_shared([old[parents[b]] for b in again]) if again else []):
+            for b, s in zip(again, forked[i]):
                 new[b] = s
+            if again:
+                L["cache"].free_seqs([old[p] for p in range(self.B) if p not in parents])
             self.seqs[i] = new
         order = self.torch.tensor(parents, device=self.dev)
         self.tokens.copy_(self.tokens[order]), self.pos.copy_(self.pos[order])
