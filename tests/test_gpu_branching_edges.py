@@ -1,4 +1,4 @@
-"""The decode loop's branch() where a layer refuses it."""
+"""The decode loop's branch() and set_sampling() where they are refused."""
 import numpy as np
 import pytest
 
@@ -42,6 +42,23 @@ def test_a_refused_branch_changes_nothing(use_graphs):
                 d.branch(parents)
             d.step()
         assert torch.equal(dec.logits, twin.logits) and torch.equal(dec.tokens, twin.tokens)
+    for d in (dec, twin):
+        d.check()
+        d.close()
+
+
+def test_refused_settings_leave_the_draws_alone():
+    dec, twin = (small(4, max_tokens=64, kv_format="f16", seed=22, use_graphs=True) for _ in range(2))
+    prompt = torch.from_numpy(np.random.default_rng(5).integers(0, 640, (4, 9)).astype(np.int32))
+    for d in (dec, twin):
+        d.set_sampling(temperature=1.5, seed=6)
+        d.prefill(prompt)
+    for _ in range(3):
+        with pytest.raises(AssertionError):
+            dec.set_sampling(temperature=[1.0, 1.0], seed=6)  # two settings for four sequences
+        for d in (dec, twin):
+            d.step()
+        assert torch.equal(dec.sampling["uniform"], twin.sampling["uniform"]) and torch.equal(dec.tokens, twin.tokens)
     for d in (dec, twin):
         d.check()
         d.close()

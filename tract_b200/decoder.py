@@ -197,10 +197,11 @@ class Decoder:
             assert t.dim() == 0 or t.shape == (self.B,)
             return t.expand(self.B).clone()
 
-        self.draws = torch.Generator(device=self.dev).manual_seed(seed)
-        self._choose_tokens_by(dict(uniform=torch.zeros(self.B, dtype=torch.float32, device=self.dev), temperature=per_row(temperature, torch.float32),
-                                    top_k=per_row(top_k, torch.int32), top_p=per_row(top_p, torch.float32), min_p=per_row(min_p, torch.float32),
-                                    scratch=kv.sample_scratch(self.B, self.shape.vocab, self.dev)))
+        settings = dict(uniform=torch.zeros(self.B, dtype=torch.float32, device=self.dev), temperature=per_row(temperature, torch.float32),
+                        top_k=per_row(top_k, torch.int32), top_p=per_row(top_p, torch.float32), min_p=per_row(min_p, torch.float32),
+                        scratch=kv.sample_scratch(self.B, self.shape.vocab, self.dev))
+        self.draws = torch.Generator(device=self.dev).manual_seed(seed)  # (what is refused has been by now)
+        self._choose_tokens_by(settings)
 
     def set_greedy(self):
         """Back to the first maximum of the logits, as a new decoder starts out."""
