@@ -81,7 +81,9 @@ struct XGeo {
 // Bound: a page and kv head is 32 KB of f16, 1340 cycles of an SM's share of HBM at the copy rate; its products for 128 rows
 // take 640 to 900 cycles of the tensor pipe, but one pipeline needs 2200 cycles from a page to the next (product, softmax,
 // product, each waiting for the one before; 3500 over int8 pages, whose converter warps share the issue slots with the softmax).
-// Two pipelines per CTA therefore: up to 128 rows they take the pages in turn, one every 1100 (1750) cycles.
+// Two pipelines per CTA therefore: up to 128 rows they take the pages in turn, one every 1100 (1750) cycles; above that they are two
+// tiles, each of which meets every page, at the pace of one pipeline.  Measured without own pages, 8 heads, from 16384 to 32768
+// tokens: 0.83 us a page and CTA with one tile (the copy rate), 1.24 with two; int8 0.92 and 1.61.
 // Measured: 128 rows per kv head, 8 of them, after 32768 tokens: f16 27 us for this kernel (134 MB, 5.0 TB/s), 43 for the call;
 // int8 35 and 51, of which the conversion is 9.  4 us go before the first page (TMEM, barriers, query tiles), 5 after the last.
 // A CTA has a run of pages; the two CTAs of a cluster have neighbouring runs and join (m, l, O) through distributed shared
@@ -837,7 +839,8 @@ static cudaError_t launch_prefix_simt(int D, int rows_cta, const PrefixParams& p
 }
 
 // The three ways of a call, and what each takes in microseconds, fitted to grids of 2 to 64 sequences after 512 to 16384 tokens
-// and to some hundred calls of random sizes: the choice is within 10% of the best of the three on 19 of 20 (1.5 times at worst).
+// and to some hundred calls of random sizes.  Of 196 calls, 160 of them of random sizes, the choice is within 10% of the best of the
+// three for 186, the median the best itself; at worst 1.5 times (2 f32 sequences of 16 heads of their own after 748 tokens: 17.3, alone 11.4).
 //   ALONE      launch_decode: every sequence reads its pages from L2 or HBM, 8 (4) rows at a time.  No more to set up than
 //              regular attention, but each page is worked on n times.
 //   TOGETHER   one launch of the decode kernel, the shared pages being further work items: rows of several sequences fill the
@@ -874,7 +877,8 @@ static Way shared_way(const b200kv_cache* c, const WaySizes& z) {
     // all CTAs become short (48 sequences after 1024: 20)
     if (own_ctas > slots) together *= 1.6;
     else if (own_ctas > slots / 2) together = 1e30;
-    if (z.tc)  // a page for all rows of a CTA, on 148 of them; two tiles of rows take 2.4 times as long as one
+    if (z.tc)  // a page for all rows of a CTA, on 148 of them; 2.4 is fitted to whole calls with two tiles of rows (larger query tiles and
+               // joins, and pages at 1.5 to 1.75 times the pace of one tile)
         apart = (quant ? 15.0 : 13.0) + (quant ? 1.3 : 0.9) * (z.max_rows <= XM ? 1.0 : 2.4) * (double)z.apart * z.Hkv / 148 + own;
     else if (z.fmt == B200KV_FMT_F32) {  // a page and tile, in whole rounds of the resident CTAs; then the own pages, which find no room beside them
         const int64_t resident = z.max_rows <= 32 ? 2 * 148 : 148;
