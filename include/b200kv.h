@@ -233,11 +233,11 @@ int b200kv_fork_shared(b200kv_cache* cache, int32_t n, const int32_t* seqs, int3
  * n_new = 1 gives, but the pages that neighbours of the batch share are read once for all of them.  With f32 queries the two
  * differ in the order of their sums.  With 16-bit queries the operands of the shared pages are 16-bit too, whatever head_dim:
  * weights (with the remainder of their rounding where a page carries more than an eighth of a row) and dequantised values,
- * each off by at most half a step of f16, so that a result is off by its own rounding and 2^-10 of the weighted sum of
- * |value| at most; dequantised keys and values beyond 65504 leave that range (and so do, at head_dim 128, bf16 queries over
- * quantised pages that are not shared, as in b200kv_attend).  Which way a call takes follows from its sizes.
- * Where nothing is shared it is b200kv_attend, bit for bit.  Neighbours: sequences of one prompt stand next to each other in `seqs`; a batch may hold several prompts, and
- * sequences that share nothing.  q, out: [n_seqs, n_q_heads, 1, D].
+ * each off by at most half a step of f16, so that a result is off by its own rounding and about 2^-10 of the weighted sum of
+ * |value|; dequantised keys and values beyond 65504 leave that range (and so do, at head_dim 128, bf16 queries over quantised
+ * pages that are not shared, as in b200kv_attend).  Which way a call takes follows from its sizes.  Where nothing is shared it
+ * is b200kv_attend, bit for bit.  Neighbours: sequences of one prompt stand next to each other in `seqs`; a batch may hold
+ * several prompts, and sequences that share nothing.  q, out: [n_seqs, n_q_heads, 1, D].
  * cos / sin (both or none): ApplyRope folded into the query load, as in b200kv_attend_rope.  scratch (may be null): the
  * result as the quantised activation of a W4A8 GEMM, as in b200kv_attend_q40; `out` may then be null.
  * Batches of more than 256 sequences are served 256 at a time, and without sharing where `scratch` is given.  Not for the
